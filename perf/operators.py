@@ -346,8 +346,9 @@ def _own_dispatch(s, c, core, stream):
     shape = (cap, cols) if c["target"] == "row" else (cols, cap)
     x = _kept(s, "x", shape, s["x"].dtype)
     core.gather_rows_device(0, CODES[c["type"]], s["x"].data_ptr(), n, cols, s["x"].shape[1],
-                            LAYOUTS[c["source"]], k, order.data_ptr(), cap, x.data_ptr(),
-                            shape[1], LAYOUTS[c["target"]], stream=stream)
+                            LAYOUTS[c["source"]], k, e, offsets.data_ptr(), order.data_ptr(),
+                            slots.data_ptr(), cap, x.data_ptr(), shape[1],
+                            LAYOUTS[c["target"]], stream=stream)
     return {"offsets": offsets, "counts": counts, "order": order, "slots": slots, "x": x}
 
 
