@@ -381,6 +381,95 @@ int32_t macboost_cli_dataset(const char *data_path, int32_t format, const char *
 int32_t macboost_predict_dataset(void *handle, void *dataset, int32_t kind,
                                  const int32_t *devices, int32_t ndev, void *out, char **err);
 
+/* ---- rows routed among several models (additive) ------------------------ */
+
+/* The steps between a gate and several models that score each row together:
+ * choose k models a row, sort the rows by model, gather every model's rows
+ * into a segment that macboost_predict_device takes, and combine the models'
+ * outputs -- and the gradients of these steps, which are what a booster of the
+ * gate (dlogits) and of the models (dy) fits next.  Every array is device
+ * memory on `device`; the calls are enqueued on `stream` (a cudaStream_t; NULL
+ * = legacy default stream), return before the work completes and allocate
+ * nothing.  Results do not depend on timing: no sum's order does.
+ * `dtype` is one of MACBOOST_F32 / BF16 / F16; arrays are aligned to their
+ * values (16-byte aligned rows move fastest).  Sums are held in float32 and
+ * rounded once. */
+enum { MACBOOST_F32 = 0, MACBOOST_BF16 = 1, MACBOOST_F16 = 2 };
+enum { MACBOOST_ROUTE_CHOSEN = 0, MACBOOST_ROUTE_ALL = 1 };
+
+/* Choose k of `experts` models (at most 1024; k at most 32) for each row of
+ * float32 gate logits (rows x experts, stride ld).  ids (rows x k int32): the k
+ * largest in descending order, equal ones by ascending index; -inf and NaN
+ * logits are never chosen, and a row that runs out of others gets -1 with
+ * weight 0.  weights (rows x k float32): softmax over the chosen
+ * (MACBOOST_ROUTE_CHOSEN) or the full softmax at the chosen
+ * (MACBOOST_ROUTE_ALL). */
+int32_t macboost_route_device(int32_t device, const float *logits, int64_t rows, int64_t experts,
+                              int64_t ld, int64_t k, int32_t norm, int32_t *ids, float *weights,
+                              void *stream, char **err);
+
+/* Gradient of macboost_route_device: dlogits (rows x experts, stride ld_d) from
+ * dweights (rows x k), the call's logits, ids and weights.  Entries of dweights
+ * beside an id of -1 are not read. */
+int32_t macboost_route_grad_device(int32_t device, const float *logits, int64_t rows,
+                                   int64_t experts, int64_t ld, int64_t k, int32_t norm,
+                                   const int32_t *ids, const float *weights,
+                                   const float *dweights, float *dlogits, int64_t ld_d,
+                                   void *stream, char **err);
+
+/* Bytes of device workspace that macboost_sort_rows_device needs (0 for few
+ * rows; -1 for arguments it refuses). */
+int64_t macboost_sort_rows_workspace(int64_t rows, int64_t k, int64_t experts);
+
+/* Sort the entries n * k + j of ids (rows x k int32, from macboost_route_device
+ * or the caller's own segments) by model.  Model e's entries, ascending, take
+ * the slots offsets[e] .. offsets[e] + counts[e] - 1; offsets[e] (int64,
+ * experts + 1 of them, the last one the end) is a multiple of `align` (1...1024;
+ * 4 keeps every segment of a 16-byte aligned feature-major matrix 16-byte
+ * aligned).  order[slot] is the entry, -1 for a slot without one, over all
+ * rows * k + experts * (align - 1) slots; slots[entry] is the slot, -1 for an id
+ * outside 0 .. experts - 1, which is left out.  workspace:
+ * macboost_sort_rows_workspace bytes, 4-byte aligned, free again when the call's
+ * work is done. */
+int32_t macboost_sort_rows_device(int32_t device, const int32_t *ids, int64_t rows, int64_t k,
+                                  int64_t experts, int64_t align, int64_t *offsets,
+                                  int32_t *counts, int32_t *order, int32_t *slots,
+                                  void *workspace, int64_t workspace_bytes, void *stream,
+                                  char **err);
+
+/* out[slot] = x[order[slot] / k] for all `capacity` slots of a sort's plan, zeros
+ * where order is -1.  x is rows x cols in `layout` (MACBOOST_LAYOUT_*, stride
+ * ld), out capacity x cols in `layout_out` (stride ld_out); feature-major means
+ * x[f * ld + i].  Its gradient is macboost_combine_rows_device without weights. */
+int32_t macboost_gather_rows_device(int32_t device, int32_t dtype, const void *x, int64_t rows,
+                                    int64_t cols, int64_t ld, int32_t layout, int64_t k,
+                                    int64_t experts, const int64_t *offsets,
+                                    const int32_t *order, const int32_t *slots,
+                                    int64_t capacity, void *out, int64_t ld_out,
+                                    int32_t layout_out, void *stream, char **err);
+
+/* out[n] = sum over j of weights[n, j] * y[slots[n, j]] (weights NULL: ones).  y
+ * is capacity x cols, out rows x cols, both row-major.  An entry whose slot is
+ * outside 0 .. capacity - 1 adds nothing, whatever its weight; a row without
+ * entries is zero. */
+int32_t macboost_combine_rows_device(int32_t device, int32_t dtype, const void *y,
+                                     int64_t capacity, int64_t cols, int64_t ld,
+                                     const int32_t *slots, const float *weights, int64_t rows,
+                                     int64_t k, void *out, int64_t ld_out, void *stream,
+                                     char **err);
+
+/* Gradient of macboost_combine_rows_device for dout (rows x cols): dy[slot] =
+ * weights * dout (capacity x cols, zeros in slots whose order is -1) and, unless
+ * dweights is NULL, dweights[n, j] = <dout[n], y[slot]> (0 for an entry that was
+ * left out). */
+int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const void *y,
+                                          int64_t capacity, int64_t cols, int64_t ld,
+                                          const int32_t *order, const int32_t *slots,
+                                          const float *weights, int64_t rows, int64_t k,
+                                          const void *dout, int64_t ld_dout, void *dy,
+                                          int64_t ld_dy, float *dweights, void *stream,
+                                          char **err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,8 @@ import numpy as np
 
 KIND_PREDICT, KIND_RAW, KIND_PROBA, KIND_LEAF, KIND_CLI = 0, 1, 2, 3, 4
 LAYOUT_FEATURE_MAJOR, LAYOUT_ROW_MAJOR = 0, 1
+F32, BF16, F16 = 0, 1, 2
+ROUTE_CHOSEN, ROUTE_ALL = 0, 1
 FORMATS = {"csv": 0, "tsv": 0, "libsvm": 1, "auto": 2}
 
 _PKG = Path(__file__).resolve().parent
@@ -110,6 +112,18 @@ def _configure(lib):
         "macboost_write_predictions": (I32, [P, I64, I64, ctypes.c_char_p, _c_char_pp]),
         "macboost_cli_predict": (I32, [P, ctypes.c_char_p, I32, I32, _i32_p, I32,
                                        ctypes.c_char_p, ctypes.POINTER(I64), _c_char_pp]),
+        "macboost_route_device": (I32, [I32, P, I64, I64, I64, I64, I32, P, P, P, _c_char_pp]),
+        "macboost_route_grad_device": (I32, [I32, P, I64, I64, I64, I64, I32, P, P, P, P, I64, P,
+                                             _c_char_pp]),
+        "macboost_sort_rows_workspace": (I64, [I64, I64, I64]),
+        "macboost_sort_rows_device": (I32, [I32, P, I64, I64, I64, I64, P, P, P, P, P, I64, P,
+                                            _c_char_pp]),
+        "macboost_gather_rows_device": (I32, [I32, I32, P, I64, I64, I64, I32, I64, I64, P, P, P,
+                                              I64, P, I64, I32, P, _c_char_pp]),
+        "macboost_combine_rows_device": (I32, [I32, I32, P, I64, I64, I64, P, P, I64, I64, P, I64,
+                                               P, _c_char_pp]),
+        "macboost_combine_rows_grad_device": (I32, [I32, I32, P, I64, I64, I64, P, P, P, I64, I64,
+                                                    P, I64, P, I64, P, P, _c_char_pp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -658,3 +672,79 @@ def predict_dataset(handle: _Handle, dataset: Dataset, kind: int = KIND_PREDICT,
                                      ctypes.byref(err)) != 0:
         raise MacBoostError(_take_error(err))
     return out
+
+
+# ---- rows routed among several models (device pointers, enqueued on `stream`) ----
+
+def _enqueue(fn, *args) -> None:
+    """One C call whose last argument is the error; 0 and None are null pointers."""
+    err = ctypes.c_char_p()
+    if fn(*args, ctypes.byref(err)) != 0:
+        raise MacBoostError(_take_error(err))
+
+
+def route_device(device: int, logits_ptr: int, rows: int, experts: int, ld: int, k: int,
+                 norm: int, ids_ptr: int, weights_ptr: int, stream: int = 0) -> None:
+    """The k best of each row's gate logits with their softmax weights (rows x k
+    int32 ids and float32 weights); norm ROUTE_CHOSEN or ROUTE_ALL."""
+    _enqueue(_lib.macboost_route_device, device, logits_ptr, rows, experts, ld, k, norm, ids_ptr,
+             weights_ptr, stream or None)
+
+
+def route_grad_device(device: int, logits_ptr: int, rows: int, experts: int, ld: int, k: int,
+                      norm: int, ids_ptr: int, weights_ptr: int, dweights_ptr: int,
+                      dlogits_ptr: int, ld_d: int, stream: int = 0) -> None:
+    """Gradient of route_device: dlogits (rows x experts) from dweights (rows x k)."""
+    _enqueue(_lib.macboost_route_grad_device, device, logits_ptr, rows, experts, ld, k, norm,
+             ids_ptr, weights_ptr, dweights_ptr, dlogits_ptr, ld_d, stream or None)
+
+
+def sort_rows_capacity(rows: int, k: int, experts: int, align: int = 1) -> int:
+    """Slots of a sorted plan: the length of `order` and the rows of gathered data."""
+    return rows * k + experts * (align - 1)
+
+
+def sort_rows_workspace(rows: int, k: int, experts: int) -> int:
+    """Bytes of device workspace for sort_rows_device."""
+    n = _lib.macboost_sort_rows_workspace(rows, k, experts)
+    if n < 0:
+        raise MacBoostError(f"cannot sort rows={rows}, k={k} among experts={experts}")
+    return n
+
+
+def sort_rows_device(device: int, ids_ptr: int, rows: int, k: int, experts: int, align: int,
+                     offsets_ptr: int, counts_ptr: int, order_ptr: int, slots_ptr: int,
+                     workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """Sort entries n * k + j by model: int64 offsets (experts + 1), int32 counts,
+    order (slot -> entry or -1) and slots (entry -> slot or -1)."""
+    _enqueue(_lib.macboost_sort_rows_device, device, ids_ptr, rows, k, experts, align,
+             offsets_ptr, counts_ptr, order_ptr, slots_ptr, workspace_ptr or None,
+             workspace_bytes, stream or None)
+
+
+def gather_rows_device(device: int, dtype: int, x_ptr: int, rows: int, cols: int, ld: int,
+                       layout: int, k: int, experts: int, offsets_ptr: int, order_ptr: int,
+                       slots_ptr: int, capacity: int, out_ptr: int, ld_out: int,
+                       layout_out: int, stream: int = 0) -> None:
+    """Each slot's row of x (zeros in empty slots), between any two LAYOUT_*."""
+    _enqueue(_lib.macboost_gather_rows_device, device, dtype, x_ptr, rows, cols, ld, layout, k,
+             experts, offsets_ptr, order_ptr, slots_ptr, capacity, out_ptr, ld_out, layout_out,
+             stream or None)
+
+
+def combine_rows_device(device: int, dtype: int, y_ptr: int, capacity: int, cols: int, ld: int,
+                        slots_ptr: int, weights_ptr: int | None, rows: int, k: int, out_ptr: int,
+                        ld_out: int, stream: int = 0) -> None:
+    """out[n] = sum over j of weights[n, j] * y[slots[n, j]] (weights 0/None: ones)."""
+    _enqueue(_lib.macboost_combine_rows_device, device, dtype, y_ptr, capacity, cols, ld,
+             slots_ptr, weights_ptr or None, rows, k, out_ptr, ld_out, stream or None)
+
+
+def combine_rows_grad_device(device: int, dtype: int, y_ptr: int, capacity: int, cols: int,
+                             ld: int, order_ptr: int, slots_ptr: int, weights_ptr: int | None,
+                             rows: int, k: int, dout_ptr: int, ld_dout: int, dy_ptr: int,
+                             ld_dy: int, dweights_ptr: int | None, stream: int = 0) -> None:
+    """Gradient of combine_rows_device: dy (capacity x cols) and dweights (rows x k)."""
+    _enqueue(_lib.macboost_combine_rows_grad_device, device, dtype, y_ptr, capacity, cols, ld,
+             order_ptr, slots_ptr, weights_ptr or None, rows, k, dout_ptr, ld_dout, dy_ptr,
+             ld_dy, dweights_ptr or None, stream or None)

@@ -14,6 +14,7 @@
 #include "../../include/macboost_c.h"
 #include "binned.h"
 #include "engine.h"
+#include "mixture.h"
 #include "table.h"
 
 namespace {
@@ -41,6 +42,16 @@ std::vector<int> default_devices() {
   }
   return d;
 }
+
+// The end of an entry point: its message, if it failed.
+int32_t finish(int rc, const std::string& msg, char** err) {
+  if (rc == 0) return 0;
+  set_error(err, msg);
+  return -1;
+}
+
+// k and experts as the launches take them; out of int's range they are refused all the same.
+int narrow(int64_t v) { return v < 0 || v > 2147483647 ? -1 : int(v); }
 
 constexpr const char* kNoTraining = "not supported by this inference engine";
 
@@ -588,6 +599,134 @@ int32_t macboost_predict_dataset(void* handle, void* ds, int32_t kind, const int
     return -1;
   }
   return 0;
+}
+
+int32_t macboost_route_device(int32_t device, const float* logits, int64_t rows, int64_t experts,
+                              int64_t ld, int64_t k, int32_t norm, int32_t* ids, float* weights,
+                              void* stream, char** err) {
+  mb::RouteArgs a{};
+  a.logits = logits;
+  a.rows = rows;
+  a.ld = ld;
+  a.experts = narrow(experts);
+  a.k = narrow(k);
+  a.norm = norm;
+  a.ids = ids;
+  a.weights = weights;
+  std::string e;
+  return finish(mb::route_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int32_t macboost_route_grad_device(int32_t device, const float* logits, int64_t rows,
+                                   int64_t experts, int64_t ld, int64_t k, int32_t norm,
+                                   const int32_t* ids, const float* weights,
+                                   const float* dweights, float* dlogits, int64_t ld_d,
+                                   void* stream, char** err) {
+  mb::RouteArgs a{};
+  a.logits = logits;
+  a.rows = rows;
+  a.ld = ld;
+  a.experts = narrow(experts);
+  a.k = narrow(k);
+  a.norm = norm;
+  a.ids = const_cast<int32_t*>(ids);
+  a.weights = const_cast<float*>(weights);
+  a.dweights = dweights;
+  a.dlogits = dlogits;
+  a.ld_d = ld_d;
+  std::string e;
+  return finish(mb::route_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int64_t macboost_sort_rows_workspace(int64_t rows, int64_t k, int64_t experts) {
+  return mb::sort_rows_workspace(rows, k, experts);
+}
+
+int32_t macboost_sort_rows_device(int32_t device, const int32_t* ids, int64_t rows, int64_t k,
+                                  int64_t experts, int64_t align, int64_t* offsets,
+                                  int32_t* counts, int32_t* order, int32_t* slots,
+                                  void* workspace, int64_t workspace_bytes, void* stream,
+                                  char** err) {
+  std::string e;
+  return finish(mb::sort_rows_device(device, ids, rows, k, experts, align, offsets, counts, order,
+                                     slots, workspace, workspace_bytes,
+                                     static_cast<cudaStream_t>(stream), e),
+                e, err);
+}
+
+int32_t macboost_gather_rows_device(int32_t device, int32_t dtype, const void* x, int64_t rows,
+                                    int64_t cols, int64_t ld, int32_t layout, int64_t k,
+                                    int64_t experts, const int64_t* offsets,
+                                    const int32_t* order, const int32_t* slots,
+                                    int64_t capacity, void* out, int64_t ld_out,
+                                    int32_t layout_out, void* stream, char** err) {
+  mb::GatherArgs a{};
+  a.x = x;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld = ld;
+  a.layout = layout;
+  a.k = narrow(k);
+  a.experts = narrow(experts);
+  a.offsets = reinterpret_cast<const long long*>(offsets);
+  a.order = order;
+  a.slots = slots;
+  a.capacity = capacity;
+  a.out = out;
+  a.ld_out = ld_out;
+  a.layout_out = layout_out;
+  a.dtype = dtype;
+  std::string e;
+  return finish(mb::gather_rows_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int32_t macboost_combine_rows_device(int32_t device, int32_t dtype, const void* y,
+                                     int64_t capacity, int64_t cols, int64_t ld,
+                                     const int32_t* slots, const float* weights, int64_t rows,
+                                     int64_t k, void* out, int64_t ld_out, void* stream,
+                                     char** err) {
+  mb::CombineArgs a{};
+  a.dtype = dtype;
+  a.y = y;
+  a.capacity = capacity;
+  a.cols = cols;
+  a.ld = ld;
+  a.slots = slots;
+  a.weights = weights;
+  a.rows = rows;
+  a.k = narrow(k);
+  a.out = out;
+  a.ld_out = ld_out;
+  std::string e;
+  return finish(mb::combine_rows_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const void* y,
+                                          int64_t capacity, int64_t cols, int64_t ld,
+                                          const int32_t* order, const int32_t* slots,
+                                          const float* weights, int64_t rows, int64_t k,
+                                          const void* dout, int64_t ld_dout, void* dy,
+                                          int64_t ld_dy, float* dweights, void* stream,
+                                          char** err) {
+  mb::CombineArgs a{};
+  a.dtype = dtype;
+  a.y = y;
+  a.capacity = capacity;
+  a.cols = cols;
+  a.ld = ld;
+  a.order = order;
+  a.slots = slots;
+  a.weights = weights;
+  a.rows = rows;
+  a.k = narrow(k);
+  a.dout = dout;
+  a.ld_dout = ld_dout;
+  a.dy = dy;
+  a.ld_dy = ld_dy;
+  a.dweights = dweights;
+  std::string e;
+  return finish(mb::combine_rows_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e,
+                err);
 }
 
 }  // extern "C"
