@@ -470,6 +470,50 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
                                           int64_t ld_dy, float *dweights, void *stream,
                                           char **err);
 
+/* ---- a softmax head over many classes (additive) ------------------------- */
+
+/* The cross entropy of softmax(h w^T): the layer trained on top of models'
+ * outputs (class margins, embeddings), without the rows x classes logits in
+ * memory.  h is rows x cols (stride ld_h), w classes x cols (stride ld_w), of
+ * `dtype` MACBOOST_F32 or MACBOOST_BF16; products and sums are float32 (float32
+ * inputs keep 24 bits in every product).  A constant column in h is a bias.
+ * Conventions as for the rows routed among models; `workspace` is device memory,
+ * 256-byte aligned, used until the call's work is done.  Rows that start on 16
+ * bytes are read in place, others are copied into the workspace first. */
+
+/* Bytes of workspace for macboost_head_loss_device, or for both calls when
+ * `grad` is non-zero; -1 for arguments they refuse.  `strided` non-zero: also
+ * when cols is a multiple of 8 but the rows of h or w do not start on 16 bytes
+ * (an odd stride or base). */
+int64_t macboost_head_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t classes,
+                                int32_t grad, int32_t strided);
+
+/* lse[n] = log sum over v of exp(<h[n], w[v]>); loss[n] = lse[n] - <h[n],
+ * w[labels[n]]>, or 0 for a label outside 0 .. classes - 1 (float32, rows). */
+int32_t macboost_head_loss_device(int32_t device, int32_t dtype, const void *h, int64_t rows,
+                                  int64_t cols, int64_t ld_h, const void *w, int64_t classes,
+                                  int64_t ld_w, const int32_t *labels, float *loss, float *lse,
+                                  void *workspace, int64_t workspace_bytes, void *stream,
+                                  char **err);
+
+/* Gradient of sum over n of dloss[n] * loss[n], from the lse of the loss call:
+ * dh (rows x cols) and dw (classes x cols), of `dtype`; either may be NULL.  With
+ * p = exp(<h[n], w[v]> - lse[n]) and g = dloss[n] * (p - [v = labels[n]]): dh = g w,
+ * dw = g^T h.  A row whose label is outside 0 .. classes - 1 has g = 0, whatever
+ * h, lse and dloss hold there.  g is formed for a piece of the classes at a
+ * time, in bfloat16 for bfloat16 inputs and in three bfloat16 terms (24 bits)
+ * for float32. */
+int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void *h, int64_t rows,
+                                  int64_t cols, int64_t ld_h, const void *w, int64_t classes,
+                                  int64_t ld_w, const int32_t *labels, const float *lse,
+                                  const float *dloss, void *dh, int64_t ld_dh, void *dw,
+                                  int64_t ld_dw, void *workspace, int64_t workspace_bytes,
+                                  void *stream, char **err);
+
+/* Synchronise `device` and report whether the last head call with this workspace
+ * gave up waiting (its outputs are then void). */
+int32_t macboost_head_check_device(int32_t device, const void *workspace, char **err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -124,6 +124,12 @@ def _configure(lib):
                                                P, _c_char_pp]),
         "macboost_combine_rows_grad_device": (I32, [I32, I32, P, I64, I64, I64, P, P, P, I64, I64,
                                                     P, I64, P, I64, P, P, _c_char_pp]),
+        "macboost_head_workspace": (I64, [I32, I64, I64, I64, I32, I32]),
+        "macboost_head_loss_device": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, P, P, P, P,
+                                            I64, P, _c_char_pp]),
+        "macboost_head_grad_device": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, P, P, P, P,
+                                            I64, P, I64, P, I64, P, _c_char_pp]),
+        "macboost_head_check_device": (I32, [I32, P, _c_char_pp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -748,3 +754,42 @@ def combine_rows_grad_device(device: int, dtype: int, y_ptr: int, capacity: int,
     _enqueue(_lib.macboost_combine_rows_grad_device, device, dtype, y_ptr, capacity, cols, ld,
              order_ptr, slots_ptr, weights_ptr or None, rows, k, dout_ptr, ld_dout, dy_ptr,
              ld_dy, dweights_ptr or None, stream or None)
+
+
+# ---- a softmax head over many classes (device pointers, enqueued on `stream`) ----
+
+def head_workspace(dtype: int, rows: int, cols: int, classes: int, grad: bool = False,
+                   strided: bool = False) -> int:
+    """Bytes of device workspace for head_loss_device (grad: and head_grad_device);
+    strided: rows of h or w may start off a 16-byte boundary."""
+    n = _lib.macboost_head_workspace(dtype, rows, cols, classes, int(grad), int(strided))
+    if n < 0:
+        raise MacBoostError(f"no head of dtype={dtype}, rows={rows}, cols={cols}, "
+                            f"classes={classes}")
+    return n
+
+
+def head_loss_device(device: int, dtype: int, h_ptr: int, rows: int, cols: int, ld_h: int,
+                     w_ptr: int, classes: int, ld_w: int, labels_ptr: int, loss_ptr: int,
+                     lse_ptr: int, workspace_ptr: int, workspace_bytes: int,
+                     stream: int = 0) -> None:
+    """Cross entropy of softmax(h w^T) and its log-sum-exp, float32 per row."""
+    _enqueue(_lib.macboost_head_loss_device, device, dtype, h_ptr, rows, cols, ld_h, w_ptr,
+             classes, ld_w, labels_ptr, loss_ptr, lse_ptr, workspace_ptr, workspace_bytes,
+             stream or None)
+
+
+def head_grad_device(device: int, dtype: int, h_ptr: int, rows: int, cols: int, ld_h: int,
+                     w_ptr: int, classes: int, ld_w: int, labels_ptr: int, lse_ptr: int,
+                     dloss_ptr: int, dh_ptr: int | None, ld_dh: int, dw_ptr: int | None,
+                     ld_dw: int, workspace_ptr: int, workspace_bytes: int,
+                     stream: int = 0) -> None:
+    """Gradients dh and dw (either may be 0/None) of sum(dloss * loss)."""
+    _enqueue(_lib.macboost_head_grad_device, device, dtype, h_ptr, rows, cols, ld_h, w_ptr,
+             classes, ld_w, labels_ptr, lse_ptr, dloss_ptr, dh_ptr or None, ld_dh,
+             dw_ptr or None, ld_dw, workspace_ptr, workspace_bytes, stream or None)
+
+
+def head_check_device(device: int, workspace_ptr: int) -> None:
+    """Synchronise and raise if the last head call with this workspace gave up waiting."""
+    _enqueue(_lib.macboost_head_check_device, device, workspace_ptr)

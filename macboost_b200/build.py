@@ -23,10 +23,10 @@ LIB = PKG / "libmacboostc.so"
 CLI = PKG / "macboost"          # the `macboost` command (C++ over the C ABI)
 
 CXX_SOURCES = ["model.cpp", "forest.cpp", "forest_codes.cpp", "shap.cpp", "engine.cpp",
-               "table.cpp", "binned.cpp", "mixture.cpp", "capi.cpp"]
+               "table.cpp", "binned.cpp", "mixture.cpp", "head.cpp", "capi.cpp"]
 CU_SOURCES = ["kernels.cu", "kernels_complete.cu", "kernels_complete_fixed.cu",
               "kernels_explicit.cu", "kernels_codes.cu", "kernels_shap.cu", "kernels_binned.cu",
-              "kernels_route.cu", "kernels_rows.cu", "noalloc.cu"]
+              "kernels_route.cu", "kernels_rows.cu", "kernels_head.cu", "noalloc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -14,6 +14,7 @@
 #include "../../include/macboost_c.h"
 #include "binned.h"
 #include "engine.h"
+#include "head.h"
 #include "mixture.h"
 #include "table.h"
 
@@ -727,6 +728,67 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
   std::string e;
   return finish(mb::combine_rows_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e,
                 err);
+}
+
+int64_t macboost_head_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t classes,
+                                int32_t grad, int32_t strided) {
+  return mb::head_workspace(dtype, rows, cols, classes, grad != 0, strided != 0);
+}
+
+int32_t macboost_head_loss_device(int32_t device, int32_t dtype, const void* h, int64_t rows,
+                                  int64_t cols, int64_t ld_h, const void* w, int64_t classes,
+                                  int64_t ld_w, const int32_t* labels, float* loss, float* lse,
+                                  void* workspace, int64_t workspace_bytes, void* stream,
+                                  char** err) {
+  mb::HeadArgs a;
+  a.dtype = dtype;
+  a.h = h;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld_h = ld_h;
+  a.w = w;
+  a.classes = classes;
+  a.ld_w = ld_w;
+  a.labels = labels;
+  a.loss = loss;
+  a.lse_out = lse;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  std::string e;
+  return finish(mb::head_loss_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void* h, int64_t rows,
+                                  int64_t cols, int64_t ld_h, const void* w, int64_t classes,
+                                  int64_t ld_w, const int32_t* labels, const float* lse,
+                                  const float* dloss, void* dh, int64_t ld_dh, void* dw,
+                                  int64_t ld_dw, void* workspace, int64_t workspace_bytes,
+                                  void* stream, char** err) {
+  mb::HeadArgs a;
+  a.dtype = dtype;
+  a.h = h;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld_h = ld_h;
+  a.w = w;
+  a.classes = classes;
+  a.ld_w = ld_w;
+  a.labels = labels;
+  a.lse = lse;
+  a.dloss = dloss;
+  a.dh = dh;
+  a.ld_dh = ld_dh;
+  a.dw = dw;
+  a.ld_dw = ld_dw;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  std::string e;
+  return finish(mb::head_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+}
+
+int32_t macboost_head_check_device(int32_t device, const void* workspace, char** err) {
+  std::string e;
+  return finish(mb::head_check_device(device, workspace, e), e, err);
 }
 
 }  // extern "C"

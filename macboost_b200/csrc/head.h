@@ -1,0 +1,116 @@
+// A softmax head: the cross entropy of softmax(h W^T) over many classes, and its
+// gradient, without the logits in memory.
+//
+//   l = h W^T (rows x classes),  lse_n = log sum_v exp(l_nv),
+//   loss_n = lse_n - l[n, label_n]           (0 for a label outside 0..classes-1)
+//   g = dloss_n (exp(l - lse_n) - [v = label_n])   (0 for such a row)
+//   dh = g W,  dW = g^T h
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+namespace mb {
+
+struct HeadArgs {
+  int dtype = 0;               // kF32 or kBF16
+  const void* h = nullptr;     // rows x cols, stride ld_h
+  int64_t rows = 0, cols = 0, ld_h = 0;
+  const void* w = nullptr;     // classes x cols, stride ld_w
+  int64_t classes = 0, ld_w = 0;
+  const int32_t* labels = nullptr;
+  float* loss = nullptr;       // forward outputs
+  float* lse_out = nullptr;
+  const float* lse = nullptr;  // gradient inputs
+  const float* dloss = nullptr;
+  void* dh = nullptr;          // either may be null
+  int64_t ld_dh = 0;
+  void* dw = nullptr;
+  int64_t ld_dw = 0;
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+
+int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad,
+                       bool strided);
+int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string& err);
+int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string& err);
+// Wait for `device` and report a wait of these kernels that ran out.
+int head_check_device(int device, const void* workspace, std::string& err);
+
+// ---- between head.cpp and kernels_head.cu ---------------------------------------
+
+constexpr int kHeadTileM = 128;      // accumulator rows a CTA (TMEM lanes)
+constexpr int kHeadTileN = 256;      // accumulator columns
+constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit values
+constexpr int kHeadPair = 2;         // CTAs that share a tile
+
+// One product C = A B^T over K, as tiles.  Operands are 16-bit values in `planes`
+// planes (the terms of a float32, or the value itself) behind tensor maps of
+// (inner, outer, plane).  a_mn / b_mn: the inner dimension is the tile's own (M or N),
+// not K.
+struct HeadJob {
+  CUtensorMap a, b;
+  int a_mn, b_mn;
+  int tiles_m, tiles_n, splits;      // splits: parts of K, each with its own output
+  int kblocks;                       // ceil(K / kHeadTileK)
+  int group;                         // tile rows walked together (L2 reuse)
+  int a_row0, b_row0;                // first outer coordinate of A and B (K-major) ...
+  int a_k0, b_k0;                    // ... and first K coordinate of each
+  // output of the plain epilogue: rows M x N
+  int M, N;
+  float* acc;                        // float32 sums, stride N, M * N apart per split
+  int acc_in, final;                 // add what acc holds; write out (else acc)
+  void* out;
+  long long ld_out;
+  int out_f32;
+};
+
+struct HeadRows {                    // what the logits' epilogues know of each row
+  const int* labels;
+  const float* lse;
+  const float* dloss;
+  float2* part;                      // forward: (max, sum) of each row and half tile
+  float* target;                     // forward: the label's logit
+  void* g;                           // gradient: planes x rows x ld_g of bfloat16
+  long long ld_g, plane_g;
+  int rows, classes, v0;             // v0: first class of this piece
+};
+
+struct HeadLaunch {
+  HeadJob job[2];
+  int jobs;
+  int pairs;                         // products of planes: 1, or 6 for float32
+  HeadRows r;
+  unsigned* status;
+  unsigned long long wait_ns;
+  int stall;                         // test hook: no copy is issued, so waits run out
+};
+
+enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2 };
+cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s);
+// Source rows (float32 or bfloat16) to planes of bfloat16 (3 or 1), stride ldp; rows
+// whose label (unless null) is none of the classes become zeros.
+cudaError_t launch_head_pack(int dtype, const void* src, int64_t rows, int64_t cols, int64_t ld,
+                             const int* labels, int64_t classes, void* dst, int64_t ldp,
+                             cudaStream_t s);
+cudaError_t launch_head_finish(const float2* part, const float* target, const int* labels,
+                               int64_t rows, int64_t classes, int64_t parts, float* loss,
+                               float* lse, cudaStream_t s);
+// out = (acc_in ? acc : 0) + sum of the splits' parts, to out or back to acc.
+struct HeadReduce {
+  const float* part;
+  int splits;
+  int64_t M, N;
+  float* acc;
+  int acc_in, final;
+  void* out;
+  int64_t ld_out;
+  int out_f32;
+};
+cudaError_t launch_head_reduce(const HeadReduce& a, cudaStream_t s);
+
+}  // namespace mb
