@@ -10,14 +10,16 @@
 //                 p_e = w_0 exp(l_e - l_{id 0}): choice 0 has the largest
 //                 probability, at least 1/E, so no sum over the row is taken again
 //
-// A row belongs to L lanes that hold V logits each in registers; a choice is a
-// local maximum, log2 L shuffles and the removal of the winner.  Rows of up to 64
-// logits (L <= 4) pass through shared memory, since a lane's own loads would touch
-// one 32-byte sector for every few values of a 4 E-byte row; wider rows are loaded
-// directly, 4 L consecutive bytes a row and instruction.
+// Three shapes.  Up to 16 logits: a lane a row, the number of logits a constant of the
+// kernel, so that a row is registers and a choice 5 E instructions.  Up to 64: L lanes
+// a row, a choice a local maximum and log2 L shuffles.  Both pass the logits through
+// shared memory, since a lane's own loads would touch one 32-byte sector for every few
+// values of a row.  Wider: a warp a row.  Each lane keeps the best two of its values
+// and two reductions name the winner, so a choice is about 20 instructions however wide
+// the row; only a lane that wins a third time looks through its values again.  Lane j
+// keeps choice j, and the exponentials, divisions and stores are one for all choices.
 #include <cuda_runtime.h>
 
-#include <climits>
 #include <cmath>
 
 #include "mixture.h"
@@ -44,45 +46,52 @@ __device__ __forceinline__ void each_value(int nr, int E, int lane, F f) {
   }
 }
 
-template <int L, int V>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteArgs a) {
-  constexpr bool kThrough = L <= 4;
+// Rows of L x V logits at most; E: their number when a lane has a row (L = 1), else 0.
+template <int L, int V, int E1>
+__global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
+    route_kernel(const RouteArgs a) {
   constexpr int R = 32 / L;             // rows a warp
-  __shared__ float tile[kThrough ? kWarps : 1][kThrough ? kTile : 1];
-  // the choices, written out together: R * k <= 512 since k <= E <= 16 L and k <= 32
-  __shared__ int s_id[kWarps][512];
-  __shared__ float s_e[kWarps][512];
+  __shared__ float tile[kWarps][E1 ? 32 * (E1 | 1) : kTile];
+  // the choices, written out together: k <= E1, else k <= min(16 L, 32)
+  constexpr int kChoices = E1 ? 32 * E1 : R * 32;
+  __shared__ int s_id[kWarps][kChoices];
+  __shared__ float s_e[kWarps][kChoices];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sub = lane % L, r = lane / L;
   const long long row0 = (long long)(blockIdx.x * (long long)kWarps + warp) * R;
   if (row0 >= a.rows) return;           // whole warps only: no block barrier below
   const int nr = int(a.rows - row0 < R ? a.rows - row0 : R);
-  const int E = a.experts, k = a.k;
-  float v[V];
-  if (kThrough) {
-    float* t = tile[warp];
-    const int sp = E | 1;
-    each_value(nr, E, lane, [&](int rr, int c) { t[rr * sp + c] = a.logits[(row0 + rr) * a.ld + c]; });
-    __syncwarp();
+  const int E = E1 ? E1 : a.experts, k = a.k;
+  float* t = tile[warp];
+  const int sp = E | 1;
+  if (E1 && nr == 32 && a.ld == E1) {
+    // a whole tile of adjacent rows: 32 E consecutive values
+    const float* p = a.logits + row0 * E1 + lane;
+    float u[E1 ? E1 : 1];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * L + sub;
-      v[i] = e < E && r < nr ? not_nan(t[r * sp + e]) : -INFINITY;
+    for (int i = 0; i < E1; ++i) u[i] = p[i * 32];
+#pragma unroll
+    for (int i = 0; i < E1; ++i) {
+      const int at = i * 32 + lane;
+      t[E1 % 2 ? at : at + at / (E1 ? E1 : 1)] = u[i];
     }
   } else {
-    const float* p = a.logits + (row0 + (r < nr ? r : 0)) * a.ld;
+    each_value(nr, E, lane, [&](int rr, int c) { t[rr * sp + c] = a.logits[(row0 + rr) * a.ld + c]; });
+  }
+  __syncwarp();
+  float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * L + sub;
-      v[i] = e < E && r < nr ? not_nan(p[e]) : -INFINITY;
-    }
+  for (int i = 0; i < V; ++i) {
+    const int e = i * L + sub;
+    v[i] = e < E && r < nr ? t[r * sp + e] : -INFINITY;
   }
   float top = 0.f, total = 0.f;
   for (int j = 0; j < k; ++j) {
-    float best = v[0];
+    // NaN is never greater, so it is never chosen
+    float best = -INFINITY;
     int at = 0;
 #pragma unroll
-    for (int i = 1; i < V; ++i)
+    for (int i = 0; i < V; ++i)
       if (v[i] > best) {
         best = v[i];
         at = i;
@@ -102,7 +111,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteArgs a) {
       top = found ? best : 0.f;
       if (a.norm == kRouteAll) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) total += expf(v[i] - top);
+        for (int i = 0; i < V; ++i) total += expf(not_nan(v[i]) - top);
 #pragma unroll
         for (int o = L / 2; o > 0; o /= 2) total += __shfl_xor_sync(~0u, total, o);
       }
@@ -113,18 +122,106 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteArgs a) {
       s_id[warp][r * k + j] = found ? id : -1;
       s_e[warp][r * k + j] = e;
     }
+    if (j + 1 < k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i * L + sub == id) v[i] = -INFINITY;
+      for (int i = 0; i < V; ++i)
+        if (i * L + sub == id) v[i] = -INFINITY;
+    }
   }
   // the group's lanes divide their row's choices by the same total
   __syncwarp();
   const float over = total > 0.f || total != total ? total : 1.f;
   for (int j = sub; j < k; j += L) s_e[warp][r * k + j] = s_e[warp][r * k + j] / over;
   __syncwarp();
+  int* ids = a.ids + row0 * k;
+  float* weights = a.weights + row0 * k;
   for (int i = lane; i < nr * k; i += 32) {
-    a.ids[row0 * k + i] = s_id[warp][i];
-    a.weights[row0 * k + i] = s_e[warp][i];
+    ids[i] = s_id[warp][i];
+    weights[i] = s_e[warp][i];
+  }
+}
+
+// Floats in the order of unsigned integers; -0 and 0 are equal, NaN is as -inf.
+__device__ __forceinline__ unsigned ordered(float v) {
+  const unsigned b = __float_as_uint(not_nan(v) + 0.f);
+  return b ^ (unsigned(int(b) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(unsigned u) {
+  return __uint_as_float(u ^ (unsigned(int(~u) >> 31) | 0x80000000u));
+}
+// exp(x) for a sum of terms up to 1: the argument's rounding, |x| 2^-24 of a term e^x,
+// is at most 2^-24 / e of the sum.
+__device__ __forceinline__ float exp_term(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
+// A warp a row of up to 32 V logits.
+template <int V>
+__global__ void __launch_bounds__(kWarps * 32) route_wide_kernel(const RouteArgs a) {
+  const int lane = threadIdx.x % 32;
+  const long long row = blockIdx.x * (long long)kWarps + threadIdx.x / 32;
+  if (row >= a.rows) return;
+  const int E = a.experts, k = a.k;
+  const float* p = a.logits + row * a.ld;
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * 32 + lane;
+    v[i] = e < E ? p[e] : -INFINITY;
+  }
+  const unsigned none = ordered(-INFINITY);
+  // the lane's best two as keys with their indexes, the lower index first among equals
+  unsigned k0 = none, k1 = none, i0 = 0, i1 = 0;
+  auto put = [&](unsigned x, unsigned i) {
+    const bool first = x > k0, second = x > k1;
+    k1 = first ? k0 : second ? x : k1;
+    i1 = first ? i0 : second ? i : i1;
+    k0 = first ? x : k0;
+    i0 = first ? i : i0;
+  };
+#pragma unroll
+  for (int i = 0; i < V; ++i) put(ordered(v[i]), i * 32 + lane);
+  unsigned mine = none, first = none;
+  int id = -1;
+  for (int j = 0; j < k; ++j) {
+    const unsigned most = __reduce_max_sync(~0u, k0);
+    if (most == none) break;            // nothing left to choose
+    if (j == 0) first = most;
+    const unsigned win = __reduce_min_sync(~0u, k0 == most ? i0 : ~0u);
+    if (lane == j) {
+      mine = most;
+      id = int(win);
+    }
+    const bool won = k0 == most && i0 == win;
+    k0 = won ? k1 : k0;
+    i0 = won ? i1 : i0;
+    k1 = won ? none : k1;
+    if (__any_sync(~0u, won && k0 == none) && won) {
+      // the best two behind the lane's last choice in (value, index) order
+      k0 = k1 = none;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const unsigned x = ordered(v[i]), at = i * 32 + lane;
+        if (x < most || (x == most && at > win)) put(x, at);
+      }
+    }
+  }
+  const float top = first == none ? 0.f : from_ordered(first);
+  const float e = expf(from_ordered(mine) - top);  // 0 where there is no choice
+  float total = 0.f;
+  if (a.norm == kRouteAll) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) total += exp_term(not_nan(v[i]) - top);
+  } else {
+    total = lane < k ? e : 0.f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(~0u, total, o);
+  if (lane < k) {
+    a.ids[row * k + lane] = id;
+    a.weights[row * k + lane] = e / (total > 0.f || total != total ? total : 1.f);
   }
 }
 
@@ -138,13 +235,14 @@ __device__ __forceinline__ void choice(const RouteArgs& a, long long row, int j,
   *dw = ok ? a.dweights[row * a.k + j] : 0.f;
 }
 
-// Rows of up to 64 logits: 32 rows a warp when E <= 16, 16 or 8 above, one lane a row,
-// through the warp's tile.
+// Rows of up to 64 logits: 32 rows a warp when E <= 16 (E1 = E), 16 or 8 above, one
+// lane a row, through the warp's tile.
+template <int E1>
 __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const RouteArgs a) {
-  __shared__ float tile[kWarps][kTile];
+  __shared__ float tile[kWarps][E1 ? 32 * (E1 | 1) : kTile];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int E = a.experts, k = a.k, sp = E | 1;
-  const int R = E <= 16 ? 32 : E <= 32 ? 16 : 8;
+  const int E = E1 ? E1 : a.experts, k = a.k, sp = E | 1;
+  const int R = E1 ? 32 : E <= 32 ? 16 : 8;
   const long long row0 = (long long)(blockIdx.x * (long long)kWarps + warp) * R;
   if (row0 >= a.rows) return;
   const int nr = int(a.rows - row0 < R ? a.rows - row0 : R);
@@ -169,9 +267,11 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const Ro
     }
     if (a.norm == kRouteAll && id0 >= 0) {
       const float l0 = mine[id0];
-      for (int e = 0; e < E; ++e) mine[e] = -mean * (w0 * expf(not_nan(mine[e]) - l0));
+#pragma unroll
+      for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = -mean * (w0 * expf(not_nan(mine[e]) - l0));
     } else {
-      for (int e = 0; e < E; ++e) mine[e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = 0.f;
     }
     for (int j = 0; j < k; ++j) {
       int id;
@@ -181,7 +281,17 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const Ro
     }
   }
   __syncwarp();
-  each_value(nr, E, lane, [&](int r, int c) { a.dlogits[(row0 + r) * a.ld_d + c] = t[r * sp + c]; });
+  if (E1 && nr == 32 && a.ld_d == E1) {
+    float* p = a.dlogits + row0 * E1 + lane;
+#pragma unroll
+    for (int i = 0; i < E1; ++i) {
+      const int at = i * 32 + lane;
+      p[i * 32] = t[E1 % 2 ? at : at + at / (E1 ? E1 : 1)];
+    }
+  } else {
+    each_value(nr, E, lane,
+               [&](int r, int c) { a.dlogits[(row0 + r) * a.ld_d + c] = t[r * sp + c]; });
+  }
 }
 
 // Wider rows: a warp a row, lane j holding choice j.  VEC: rows of both matrices are
@@ -223,43 +333,58 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteArgs
   if (id >= 0) d[id] = w * (dw - mean);
 }
 
-template <int L, int V>
-cudaError_t go(const RouteArgs& a, cudaStream_t s) {
-  const long long per = (long long)kWarps * (32 / L);
-  const long long blocks = (a.rows + per - 1) / per;
-  if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  route_kernel<L, V><<<unsigned(blocks), kWarps * 32, 0, s>>>(a);
+unsigned blocks_for(long long rows, int per) { return unsigned((rows + per - 1) / per); }
+
+template <int L, int V, int E1>
+cudaError_t go(const RouteArgs& a, bool grad, cudaStream_t s) {
+  // at least 32 rows a block and below 2^31 rows: the grid fits
+  const unsigned blocks = blocks_for(a.rows, kWarps * (32 / L));
+  if (grad) {
+    const int R = E1 ? 32 : a.experts <= 32 ? 16 : 8;
+    route_grad_narrow_kernel<E1><<<blocks_for(a.rows, kWarps * R), kWarps * 32, 0, s>>>(a);
+  } else {
+    route_kernel<L, V, E1><<<blocks, kWarps * 32, 0, s>>>(a);
+  }
   return cudaGetLastError();
+}
+
+template <int V>
+cudaError_t wide(const RouteArgs& a, cudaStream_t s) {
+  route_wide_kernel<V><<<blocks_for(a.rows, kWarps), kWarps * 32, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t narrow(const RouteArgs& a, bool grad, cudaStream_t s) {
+  switch (a.experts) {
+#define MB_ROUTE(E) case E: return go<1, E, E>(a, grad, s);
+    MB_ROUTE(1) MB_ROUTE(2) MB_ROUTE(3) MB_ROUTE(4) MB_ROUTE(5) MB_ROUTE(6) MB_ROUTE(7)
+    MB_ROUTE(8) MB_ROUTE(9) MB_ROUTE(10) MB_ROUTE(11) MB_ROUTE(12) MB_ROUTE(13) MB_ROUTE(14)
+    MB_ROUTE(15) MB_ROUTE(16)
+#undef MB_ROUTE
+    default: break;
+  }
+  return a.experts <= 32 ? go<2, 16, 0>(a, grad, s) : go<4, 16, 0>(a, grad, s);
 }
 
 }  // namespace
 
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t s) {
   const int E = a.experts;
-  if (E <= 4) return go<1, 4>(a, s);
-  if (E <= 8) return go<1, 8>(a, s);
-  if (E <= 16) return go<1, 16>(a, s);
-  if (E <= 32) return go<2, 16>(a, s);
-  if (E <= 64) return go<4, 16>(a, s);
-  if (E <= 128) return go<8, 16>(a, s);
-  if (E <= 256) return go<16, 16>(a, s);
-  if (E <= 512) return go<32, 16>(a, s);
-  return go<32, 32>(a, s);
+  if (E <= kStaged) return narrow(a, false, s);
+  if (E <= 128) return wide<4>(a, s);
+  if (E <= 256) return wide<8>(a, s);
+  if (E <= 512) return wide<16>(a, s);
+  return wide<32>(a, s);
 }
 
 cudaError_t launch_route_grad(const RouteArgs& a, cudaStream_t s) {
   const int E = a.experts;
-  const long long per = E > kStaged ? kWarps : kWarps * (E <= 16 ? 32 : E <= 32 ? 16 : 8);
-  const long long blocks = (a.rows + per - 1) / per;
-  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  if (E <= kStaged) return narrow(a, true, s);
   const auto bits = reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.dlogits);
-  const bool vec = bits % 16 == 0 && (a.ld | a.ld_d | E) % 4 == 0;
-  if (E <= kStaged)
-    route_grad_narrow_kernel<<<unsigned(blocks), kWarps * 32, 0, s>>>(a);
-  else if (vec)
-    route_grad_kernel<true><<<unsigned(blocks), kWarps * 32, 0, s>>>(a);
+  if (bits % 16 == 0 && (a.ld | a.ld_d | E) % 4 == 0)
+    route_grad_kernel<true><<<blocks_for(a.rows, kWarps), kWarps * 32, 0, s>>>(a);
   else
-    route_grad_kernel<false><<<unsigned(blocks), kWarps * 32, 0, s>>>(a);
+    route_grad_kernel<false><<<blocks_for(a.rows, kWarps), kWarps * 32, 0, s>>>(a);
   return cudaGetLastError();
 }
 
