@@ -108,6 +108,14 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad
   return p;
 }
 
+bool is_narrow(int64_t cols, int64_t classes) {
+  return cols <= kNarrowCols && classes <= kNarrowClasses;
+}
+// Its workspace: the status word, and a dw of each block.
+int64_t narrow_bytes(int64_t rows, int64_t cols, int64_t classes, bool grad) {
+  return 256 + (grad ? up(narrow_blocks(rows) * cols * classes * 4, 256) : 0);
+}
+
 // ---- tensor maps ----------------------------------------------------------------
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -145,6 +153,10 @@ int encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t 
     return fail(err, "cuTensorMapEncodeTiled failed with " + std::to_string(int(r)));
   return 0;
 }
+
+// Rows of a K-major box: all of a tile's, or the matrix's when it has fewer (in groups
+// of 8, a swizzle atom).
+int box_rows(int64_t rows, int tile) { return int(std::min<int64_t>(tile, up(rows, 8))); }
 
 // ---- checks ---------------------------------------------------------------------
 
@@ -186,10 +198,10 @@ int check(const HeadArgs& a, bool grad, std::string& err) {
   return 0;
 }
 
-int check_workspace(const HeadArgs& a, const Plan& p, std::string& err) {
-  if (a.workspace && a.workspace_bytes >= p.bytes) return 0;
+int check_workspace(const HeadArgs& a, int64_t need, std::string& err) {
+  if (a.workspace && a.workspace_bytes >= need) return 0;
   return fail(err, "workspace holds " + std::to_string(a.workspace ? a.workspace_bytes : 0) +
-                       " bytes, the head needs " + std::to_string(p.bytes));
+                       " bytes, the head needs " + std::to_string(need));
 }
 
 #define HEAD_CUDA(call, what)                                                     \
@@ -250,8 +262,12 @@ void settings(HeadLaunch& l, const HeadArgs& a, const Plan& p) {
 // The logits of classes v0 ... v0 + n - 1: A = h, B = w, both along cols.
 int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, int64_t v0, int64_t n,
                std::string& err) {
-  if (encode(&j.a, o.h, a.cols, a.rows, o.ld_h, p.planes, kHeadTileM, err) ||
-      encode(&j.b, o.w, a.cols, a.classes, o.ld_w, p.planes, kHeadTileN / kHeadPair, err))
+  j.M = int(a.rows);
+  j.N = int(n);
+  j.a_box = box_rows(a.rows, kHeadTileM);
+  j.b_box = box_rows(n, kHeadTileN / kHeadPair);
+  if (encode(&j.a, o.h, a.cols, a.rows, o.ld_h, p.planes, j.a_box, err) ||
+      encode(&j.b, o.w, a.cols, a.classes, o.ld_w, p.planes, j.b_box, err))
     return -1;
   j.tiles_m = int(parts(a.rows, kHeadPair * kHeadTileM));
   j.tiles_n = int(parts(n, kHeadTileN));
@@ -262,11 +278,22 @@ int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, 
   return 0;
 }
 
+int narrow(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string& err) {
+  if (check_workspace(a, narrow_bytes(a.rows, a.cols, a.classes, grad), err)) return -1;
+  if (use_device(device, err)) return -1;
+  Guard gd(device);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + 256);
+  HEAD_CUDA(launch_head_narrow(a, grad, part, narrow_blocks(a.rows), s), "narrow head launch");
+  g_kernel_launches.fetch_add(grad && a.dw ? 2 : 1, std::memory_order_relaxed);
+  return 0;
+}
+
 }  // namespace
 
 int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool strided) {
   std::string err;
   if (check_shape(dtype, rows, cols, classes, err)) return -1;
+  if (is_narrow(cols, classes)) return narrow_bytes(rows, cols, classes, grad);
   const bool pack = dtype == kF32 || strided || cols % 8 != 0;
   const int64_t loss = make_plan(dtype, rows, cols, classes, false, pack, pack, true, true).bytes;
   if (!grad) return loss;
@@ -281,9 +308,10 @@ int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, b
 int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string& err) {
   if (check(a, false, err)) return -1;
   if (a.rows == 0) return 0;
+  if (is_narrow(a.cols, a.classes)) return narrow(device, a, false, s, err);
   const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, false, !in_place(a.dtype, a.h, a.ld_h),
                            !in_place(a.dtype, a.w, a.ld_w), true, true);
-  if (check_workspace(a, p, err)) return -1;
+  if (check_workspace(a, p.bytes, err)) return -1;
   if (use_device(device, err)) return -1;
   Guard gd(device);
   char* base = static_cast<char*>(a.workspace);
@@ -320,9 +348,10 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
               "clearing dw");
     return 0;
   }
+  if (is_narrow(a.cols, a.classes)) return narrow(device, a, true, s, err);
   const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, true, !in_place(a.dtype, a.h, a.ld_h),
                            !in_place(a.dtype, a.w, a.ld_w), a.dh != nullptr, a.dw != nullptr);
-  if (check_workspace(a, p, err)) return -1;
+  if (check_workspace(a, p.bytes, err)) return -1;
   if (use_device(device, err)) return -1;
   Guard gd(device);
   char* base = static_cast<char*>(a.workspace);
@@ -354,7 +383,8 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
     int reds = 0;
     HeadJob dh{}, dw{};
     if (a.dh) {  // dh = g w: A = g along its classes, B = w's columns
-      if (encode(&dh.a, base + p.g, n, a.rows, p.ld_g, p.planes, kHeadTileM, err) ||
+      dh.a_box = box_rows(a.rows, kHeadTileM);
+      if (encode(&dh.a, base + p.g, n, a.rows, p.ld_g, p.planes, dh.a_box, err) ||
           encode(&dh.b, o.w, a.cols, a.classes, o.ld_w, p.planes, 64, err))
         return -1;
       dh.b_mn = 1;

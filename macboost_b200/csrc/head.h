@@ -60,8 +60,9 @@ struct HeadJob {
   int group;                         // tile rows walked together (L2 reuse)
   int a_row0, b_row0;                // first outer coordinate of A and B (K-major) ...
   int a_k0, b_k0;                    // ... and first K coordinate of each
-  // output of the plain epilogue: rows M x N
-  int M, N;
+  int a_box, b_box;                  // rows of a K-major operand's box
+  int M, N;                          // the product's rows and columns
+  // output of the plain epilogue
   float* acc;                        // float32 sums, stride N, M * N apart per split
   int acc_in, final;                 // add what acc holds; write out (else acc)
   void* out;
@@ -89,6 +90,15 @@ struct HeadLaunch {
   unsigned long long wait_ns;
   int stall;                         // test hook: no copy is issued, so waits run out
 };
+
+// A narrow head takes none of this: kernels of its own, in float32 (kernels_head.cu).
+constexpr int kNarrowCols = 64, kNarrowClasses = 32;
+// Blocks: enough to fill the GPU four times, one for 128 rows at most.
+inline int narrow_blocks(int64_t rows) {
+  const int64_t n = (rows + 127) / 128;
+  return int(n < 592 ? n : 592);
+}
+cudaError_t launch_head_narrow(const HeadArgs& h, bool grad, float* part, int blocks, cudaStream_t s);
 
 enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2 };
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s);

@@ -62,15 +62,18 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t rank) {
   asm volatile(
       "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
-      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(bar),
+      " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(bar),
       "r"(rank)
       : "memory");
 }
+// Without .acquire.cluster, which would make every wait a memory barrier: what the waits
+// order is the asynchronous copies, the products and tensor memory, by the rules of
+// mbarrier transactions, tcgen05.commit and the tcgen05 fences.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n .reg .pred p;\n"
-      " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -341,11 +344,29 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         walk.blocks(t, &k0, &k1);
         const int am = (t.m * kHeadPair + int(rank)) * kHeadTileM;
         const int bn = t.n * TN + int(rank) * (TN / kHeadPair);
+        // Boxes that lie outside the matrix are not fetched (what the shared memory holds
+        // there only reaches sums that are not used): a box that TMA has to fill with
+        // zeros is slower than one it reads.
+        auto bytes_a = [&](int m0) {
+          return q.a_mn ? min(kHeadTileM / 64, max(0, (q.M - m0 + 63) / 64)) * 8192
+                        : m0 < q.M ? q.a_box * 128 : 0;
+        };
+        auto bytes_b = [&](int n0) {
+          return q.b_mn ? min(TN / kHeadPair / 64, max(0, (q.N - n0 + 63) / 64)) * 8192
+                        : n0 < q.N ? q.b_box * 128 : 0;
+        };
+        const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
+        const uint32_t bytes = uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
+                                        bytes_b(n0 + TN / kHeadPair));
+        // Each tile starts at another K block: tiles that run together would read the same
+        // 128 bytes of every row, which are few of the memory's channels.
+        const int turn = (t.m + t.n) % (k1 - k0);
         for (int p = 6 - a.pairs; ok && p < 6; ++p)
-          for (int kb = k0; kb < k1; ++kb) {
+          for (int i = k0; i < k1; ++i) {
+            const int kb = i + turn < k1 ? i + turn : i + turn - (k1 - k0);
             ok = wait(empty + 8 * s, ph ^ 1);
             if (!ok) break;
-            if (rank == 0) bar_expect(full + 8 * s, kHeadPair * kStage);
+            if (rank == 0) bar_expect(full + 8 * s, bytes);
             const uint32_t sa = ring + s * kStage, sb = sa + kBytesA, bar = full + 8 * s;
             if (++s == kStages) {
               s = 0;
@@ -355,23 +376,23 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
             int pa = 0, pb = 0;
 #pragma unroll
-            for (int i = 0; i < 6; ++i)
-              if (i == p) {
-                pa = kPlaneA[i];
-                pb = kPlaneB[i];
+            for (int z = 0; z < 6; ++z)
+              if (z == p) {
+                pa = kPlaneA[z];
+                pb = kPlaneB[z];
               }
             if (q.a_mn) {
 #pragma unroll
               for (int i = 0; i < kHeadTileM / 64; ++i)
-                tma_load(sa + i * 8192, &q.a, q.a_row0 + am + 64 * i, ka, pa, bar);
-            } else {
+                if (am + 64 * i < q.M) tma_load(sa + i * 8192, &q.a, q.a_row0 + am + 64 * i, ka, pa, bar);
+            } else if (am < q.M) {
               tma_load(sa, &q.a, ka, q.a_row0 + am, pa, bar);
             }
             if (q.b_mn) {
 #pragma unroll
               for (int i = 0; i < TN / kHeadPair / 64; ++i)
-                tma_load(sb + i * 8192, &q.b, q.b_row0 + bn + 64 * i, kk, pb, bar);
-            } else {
+                if (bn + 64 * i < q.N) tma_load(sb + i * 8192, &q.b, q.b_row0 + bn + 64 * i, kk, pb, bar);
+            } else if (bn < q.N) {
               tma_load(sb, &q.b, kk, q.b_row0 + bn, pb, bar);
             }
           }
@@ -556,30 +577,44 @@ __global__ void __launch_bounds__(256)
 }
 
 // The (max, sum) parts of a row to its log-sum-exp and loss.  A block takes `per` rows
-// (a power of two, at most 32) with 256 / per threads each.
+// (a power of two, at most 32) with 256 / per threads each, eight parts at a time.
 __global__ void __launch_bounds__(256)
     head_finish_kernel(const float2* part, const float* target, const int* labels, long long rows,
                        int classes, int parts, float* loss, float* lse, int per) {
+  constexpr int BATCH = 8;
   __shared__ float2 mine[256];
   const int x = threadIdx.x % per, t = threadIdx.x / per, threads = 256 / per;
   const long long n = (long long)blockIdx.x * per + x;
   float m = -INFINITY, s = 0.f;
   // s exp(m - base), with an infinite m standing for 0 as in online()
-  auto term = [](float2 p, float base) {
-    return p.y == 0.f ? 0.f : p.y * expf((fabsf(p.x) == INFINITY ? 0.f : p.x) - base);
-  };
-  auto join = [&](float2 p) {
-    const float top = fmaxf(m, p.x), base = fabsf(top) == INFINITY ? 0.f : top;
-    s = term(make_float2(m, s), base) + term(p, base);
-    m = top;
+  auto term = [](float m, float s, float base) {
+    return s == 0.f ? 0.f : s * expf((fabsf(m) == INFINITY ? 0.f : m) - base);
   };
   if (n < rows)
-    for (int i = t; i < parts; i += threads) join(part[i * rows + n]);
+    for (int i = t; i < parts; i += threads * BATCH) {
+      float2 p[BATCH];
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
+        const int at = i + q * threads;
+        p[q] = at < parts ? part[at * rows + n] : make_float2(-INFINITY, 0.f);
+      }
+      float top = m;
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) top = fmaxf(top, p[q].x);
+      const float base = fabsf(top) == INFINITY ? 0.f : top;
+      s = term(m, s, base);
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) s += term(p[q].x, p[q].y, base);
+      m = top;
+    }
   mine[threadIdx.x] = make_float2(m, s);
   __syncthreads();
   for (int o = threads / 2; o > 0; o /= 2) {
     if (t < o) {
-      join(mine[threadIdx.x + o * per]);
+      const float2 p = mine[threadIdx.x + o * per];
+      const float top = fmaxf(m, p.x), base = fabsf(top) == INFINITY ? 0.f : top;
+      s = term(m, s, base) + term(p.x, p.y, base);
+      m = top;
       mine[threadIdx.x] = make_float2(m, s);
     }
     __syncthreads();
@@ -608,6 +643,289 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a) {
     static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
 }
 
+// ---- a narrow head --------------------------------------------------------------
+//
+// At most 64 columns and 32 classes (a calibration of class margins): the tensor
+// cores' tiles of 256 x 256 would be padding, and the bytes of h and dh bound the work.
+// A lane has a row in registers, the weights are 16-byte broadcasts from shared memory,
+// all in float32.  dw: lane c of a warp sums the products of class and four columns
+// number c (and c + 32 ...) over the warp's rows, block after block of rows, in
+// registers; blocks leave their sums for a last small kernel.
+
+constexpr int kNarrowWarps = 4;
+
+struct Narrow {
+  const void *h, *w;
+  long long rows, ld_h, ld_w;
+  int cols, classes;
+  const int* labels;
+  float *loss, *lse_out;
+  const float *lse, *dloss;
+  void* dh;
+  long long ld_dh;
+  float* part;             // gridDim.x x classes x cols, or null
+  unsigned* status;
+};
+
+template <class T>
+__device__ __forceinline__ float load_f(const T* p) {
+  return float(*p);
+}
+
+// Two float32 products and sums in one instruction.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pair(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+struct alignas(16) F4 {  // four adjacent floats of shared memory
+  F2 lo, hi;
+};
+
+template <class T, int DP, int VP, bool GRAD>
+__global__ void __launch_bounds__(kNarrowWarps * 32) head_narrow_kernel(const Narrow a) {
+  constexpr int Q = DP / 4;              // quads of columns
+  constexpr int PITCH = DP + 4;          // an odd number of 16 bytes: no bank conflicts
+  constexpr int GP = VP + 1;
+  constexpr int NC = (VP * Q + 31) / 32; // (class, quad) pairs a lane
+  extern __shared__ float4 shared4[];
+  float* w = reinterpret_cast<float*>(shared4);                      // VP x DP, zeros beyond
+  float* tiles = w + VP * DP;                                        // warps x 32 x PITCH
+  float* gs = tiles + kNarrowWarps * 32 * PITCH;                     // warps x 32 x GP
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  float* tile = tiles + warp * 32 * PITCH;
+  float* gt = gs + warp * 32 * GP;
+  const int D = a.cols, V = a.classes, nq = (D + 3) / 4;
+  const T* W = static_cast<const T*>(a.w);
+  for (int i = threadIdx.x; i < VP * DP; i += kNarrowWarps * 32) {
+    const int v = i / DP, d = i % DP;
+    w[i] = v < V && d < D ? load_f(W + v * a.ld_w + d) : 0.f;
+  }
+  for (int i = lane; i < 32 * PITCH; i += 32) tile[i] = 0.f;  // columns D .. stay zero
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;     // there is no wait to run out
+  __syncthreads();
+  const unsigned inv = ((1u << 20) + unsigned(D) - 1u) / unsigned(D);  // exact for i < 2,048
+  F4 acc[GRAD ? NC : 1];
+  int acc_v[GRAD ? NC : 1], acc_q[GRAD ? NC : 1];
+#pragma unroll
+  for (int c = 0; c < (GRAD ? NC : 1); ++c) {
+    acc[c].lo = acc[c].hi = pair(0.f, 0.f);
+    const int i = lane + 32 * c;
+    acc_v[c] = i < V * nq ? i / nq : 0;
+    acc_q[c] = i < V * nq ? i % nq : 0;
+  }
+  const long long step = (long long)gridDim.x * kNarrowWarps * 32;
+  // adjacent rows on 16 bytes: a warp's 32 are fetched ahead, while the ones before are
+  // worked on
+  constexpr int PER = 16 / int(sizeof(T)), AHEAD = DP / PER;
+  const bool dense = a.ld_h == D && (reinterpret_cast<uintptr_t>(a.h) & 15) == 0;
+  uint4 ahead[AHEAD];
+  auto fetch = [&](long long row0) {
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(a.h) + row0 * D);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (32 * j + lane < 32 / PER * D) ahead[j] = from[32 * j + lane];
+  };
+  {
+    const long long row0 = ((long long)blockIdx.x * kNarrowWarps + warp) * 32;
+    if (dense && row0 + 32 <= a.rows) fetch(row0);
+  }
+  for (long long row0 = ((long long)blockIdx.x * kNarrowWarps + warp) * 32; row0 < a.rows; row0 += step) {
+    const int nr = int(a.rows - row0 < 32 ? a.rows - row0 : 32);
+    const T* H = static_cast<const T*>(a.h) + row0 * a.ld_h;
+    const long long row = row0 + lane;
+    const bool there = lane < nr;
+    const int y = there ? a.labels[row] : -1;
+    const bool known = unsigned(y) < unsigned(V);
+    const float lse_in = GRAD && there ? a.lse[row] : 0.f, up = GRAD && known ? a.dloss[row] : 0.f;
+    __syncwarp();
+    if (dense && nr == 32) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (32 * j + lane < 32 / PER * D) {
+          const T* x = reinterpret_cast<const T*>(&ahead[j]);
+          const int i0 = (32 * j + lane) * PER;
+          int r = int((unsigned(i0) * inv) >> 20), c = i0 - r * D;
+#pragma unroll
+          for (int z = 0; z < PER; ++z) {
+            tile[r * PITCH + c] = load_f(x + z);
+            if (++c == D) {
+              c = 0;
+              ++r;
+            }
+          }
+        }
+      if (row0 + step + 32 <= a.rows) fetch(row0 + step);
+    } else {
+      for (int i = lane; i < nr * D; i += 32) {
+        const int r = int((unsigned(i) * inv) >> 20), c = i - r * D;
+        tile[r * PITCH + c] = load_f(H + r * a.ld_h + c);
+      }
+    }
+    __syncwarp();
+    // logits: VP independent chains, a quad of columns after the other
+    F2 x[VP];
+#pragma unroll
+    for (int v = 0; v < VP; ++v) x[v] = pair(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (q < nq) {
+        const F4 h = *reinterpret_cast<const F4*>(tile + lane * PITCH + 4 * q);
+#pragma unroll
+        for (int v = 0; v < VP; ++v) {
+          const F4 t = *reinterpret_cast<const F4*>(w + v * DP + 4 * q);
+          x[v] = fma2(h.hi, t.hi, fma2(h.lo, t.lo, x[v]));
+        }
+      }
+    float l[VP], m = -INFINITY, target = 0.f;
+#pragma unroll
+    for (int v = 0; v < VP; ++v) {
+      const float2 p = split(x[v]);
+      l[v] = v < V ? p.x + p.y : -INFINITY;
+      m = fmaxf(m, l[v]);
+      if (v == y) target = l[v];
+    }
+    if constexpr (!GRAD) {
+      const float base = fabsf(m) == INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < VP; ++v) s += exp2_approx((l[v] - base) * kLog2e);
+      const float lse = base + logf(s);
+      if (there) {
+        a.lse_out[row] = lse;
+        a.loss[row] = known ? lse - target : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < VP; ++v) {
+        const float p = exp2_approx((l[v] - lse_in) * kLog2e);
+        l[v] = known && v < V ? up * (v == y ? p - 1.f : p) : 0.f;
+        gt[lane * GP + v] = l[v];
+      }
+      if (a.part) {
+        // a row without a label adds nothing, whatever its h
+        if (!known)
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+            *reinterpret_cast<float4*>(tile + lane * PITCH + 4 * q) = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          if (32 * c < V * nq) {
+            const float *pg = gt + acc_v[c], *ph = tile + 4 * acc_q[c];
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+              const float g = pg[r * GP];
+              const F4 h = *reinterpret_cast<const F4*>(ph + r * PITCH);
+              const F2 gg = pair(g, g);
+              acc[c].lo = fma2(gg, h.lo, acc[c].lo);
+              acc[c].hi = fma2(gg, h.hi, acc[c].hi);
+            }
+          }
+        __syncwarp();
+      }
+      if (a.dh) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+          if (q < nq) {
+            F4 s;
+            s.lo = s.hi = pair(0.f, 0.f);
+#pragma unroll
+            for (int v = 0; v < VP; ++v) {
+              const F4 t = *reinterpret_cast<const F4*>(w + v * DP + 4 * q);
+              const F2 gg = pair(l[v], l[v]);
+              s.lo = fma2(gg, t.lo, s.lo);
+              s.hi = fma2(gg, t.hi, s.hi);
+            }
+            *reinterpret_cast<F4*>(tile + lane * PITCH + 4 * q) = s;
+          }
+        __syncwarp();
+        T* to = static_cast<T*>(a.dh) + row0 * a.ld_dh;
+#pragma unroll 4
+        for (int i = lane; i < nr * D; i += 32) {
+          const int r = int((unsigned(i) * inv) >> 20), c = i - r * D;
+          to[r * a.ld_dh + c] = T(tile[r * PITCH + c]);
+        }
+      }
+    }
+  }
+  if (GRAD && a.part) {
+    // the warps' sums, one after the other, in the tiles' place
+    float4* sums = reinterpret_cast<float4*>(tiles);
+    for (int k = 0; k < kNarrowWarps; ++k) {
+      __syncthreads();
+      if (warp == k) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float2 lo = split(acc[c].lo), hi = split(acc[c].hi);
+          float4 x = make_float4(lo.x, lo.y, hi.x, hi.y);
+          if (k > 0) {
+            const float4 o = sums[lane + 32 * c];
+            x = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+          }
+          sums[lane + 32 * c] = x;
+        }
+      }
+    }
+    __syncthreads();
+    const float* flat = reinterpret_cast<const float*>(sums);
+    for (int i = threadIdx.x; i < V * D; i += kNarrowWarps * 32)
+      a.part[(long long)blockIdx.x * V * D + i] = flat[i / D * (4 * nq) + i % D];
+  }
+}
+
+// dw from the blocks' sums, a warp a value.
+template <class T>
+__global__ void __launch_bounds__(256)
+    head_narrow_reduce_kernel(const float* part, int blocks, int classes, int cols, T* dw, long long ld) {
+  const int i = int(blockIdx.x) * 8 + int(threadIdx.x) / 32, lane = threadIdx.x % 32;
+  if (i >= classes * cols) return;
+  float v = 0.f;
+  for (int b = lane; b < blocks; b += 32) v += part[(long long)b * classes * cols + i];
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(~0u, v, o);
+  if (lane == 0) dw[i / cols * ld + i % cols] = T(v);
+}
+
+template <class T, int DP, int VP>
+cudaError_t narrow_of(const Narrow& a, bool grad, int blocks, cudaStream_t s) {
+  constexpr size_t smem = (VP * DP + kNarrowWarps * 32 * (DP + 4 + VP + 1)) * sizeof(float);
+  const auto k = grad ? head_narrow_kernel<T, DP, VP, true> : head_narrow_kernel<T, DP, VP, false>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  k<<<blocks, kNarrowWarps * 32, smem, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T, int DP>
+cudaError_t narrow_cols(const Narrow& a, bool grad, int blocks, cudaStream_t s) {
+  if (a.classes <= 4) return narrow_of<T, DP, 4>(a, grad, blocks, s);
+  if (a.classes <= 8) return narrow_of<T, DP, 8>(a, grad, blocks, s);
+  if (a.classes <= 12) return narrow_of<T, DP, 12>(a, grad, blocks, s);
+  if (a.classes <= 16) return narrow_of<T, DP, 16>(a, grad, blocks, s);
+  return narrow_of<T, DP, 32>(a, grad, blocks, s);
+}
+
+template <class T>
+cudaError_t narrow_type(const Narrow& a, bool grad, int blocks, cudaStream_t s) {
+  if (a.cols <= 16) return narrow_cols<T, 16>(a, grad, blocks, s);
+  if (a.cols <= 32) return narrow_cols<T, 32>(a, grad, blocks, s);
+  return narrow_cols<T, 64>(a, grad, blocks, s);
+}
+
 template <int EPI, int TN>
 cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
   constexpr int kStage = kHeadTileM * 128 + TN / kHeadPair * 128;
@@ -632,6 +950,37 @@ cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStrea
   return tile_n == 128 ? go<kHeadOut, 128>(a, s) : go<kHeadOut, 256>(a, s);
 }
 
+cudaError_t launch_head_narrow(const HeadArgs& h, bool grad, float* part, int blocks, cudaStream_t s) {
+  Narrow a{};
+  a.h = h.h;
+  a.w = h.w;
+  a.rows = h.rows;
+  a.ld_h = h.ld_h;
+  a.ld_w = h.ld_w;
+  a.cols = int(h.cols);
+  a.classes = int(h.classes);
+  a.labels = h.labels;
+  a.loss = h.loss;
+  a.lse_out = h.lse_out;
+  a.lse = h.lse;
+  a.dloss = h.dloss;
+  a.dh = h.dh;
+  a.ld_dh = h.ld_dh;
+  a.part = h.dw ? part : nullptr;
+  a.status = static_cast<unsigned*>(h.workspace);
+  cudaError_t e = h.dtype == kF32 ? narrow_type<float>(a, grad, blocks, s)
+                                  : narrow_type<__nv_bfloat16>(a, grad, blocks, s);
+  if (e != cudaSuccess || !grad || !h.dw) return e;
+  const unsigned n = unsigned((h.classes * h.cols + 7) / 8);
+  if (h.dtype == kF32)
+    head_narrow_reduce_kernel<float><<<n, 256, 0, s>>>(part, blocks, a.classes, a.cols,
+                                                       static_cast<float*>(h.dw), h.ld_dw);
+  else
+    head_narrow_reduce_kernel<__nv_bfloat16><<<n, 256, 0, s>>>(
+        part, blocks, a.classes, a.cols, static_cast<__nv_bfloat16*>(h.dw), h.ld_dw);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_head_pack(int dtype, const void* src, int64_t rows, int64_t cols, int64_t ld,
                              const int* labels, int64_t classes, void* dst, int64_t ldp,
                              cudaStream_t s) {
@@ -651,8 +1000,9 @@ cudaError_t launch_head_pack(int dtype, const void* src, int64_t rows, int64_t c
 cudaError_t launch_head_finish(const float2* part, const float* target, const int* labels,
                                int64_t rows, int64_t classes, int64_t parts, float* loss,
                                float* lse, cudaStream_t s) {
+  // rows a block: fewer when that leaves multiprocessors without one
   int per = 1;
-  while (per < 32 && per < rows) per *= 2;
+  while (per < 32 && rows / (2 * per) >= 2 * device_sms()) per *= 2;
   const long long blocks = (rows + per - 1) / per;
   head_finish_kernel<<<unsigned(blocks), 256, 0, s>>>(part, target, labels, rows, int(classes),
                                                       int(parts), loss, lse, per);
