@@ -43,7 +43,7 @@ struct Guard {
 // ---- the plan -------------------------------------------------------------------
 
 struct Plan {
-  int planes, pairs;
+  int planes;
   bool pack_h, pack_w;
   int64_t ldp;                        // stride of packed rows
   int64_t piece, pieces, ld_g;        // classes a piece, pieces, stride of g
@@ -59,21 +59,19 @@ bool in_place(int dtype, const void* p, int64_t ld) {
   return dtype == kBF16 && aligned(p, 16) && ld % 8 == 0;
 }
 
-int splits_for(int64_t tiles, int64_t kblocks, int dtype) {
-  // few tiles: parts of K until the pairs of CTAs are busy, 8 steps each at least
-  int64_t n = 1;
-  if (tiles < 37) n = std::min(parts(74, tiles), std::max<int64_t>(1, kblocks / 8));
-  // float32: sums of at most 2,048 products before they are rounded to nearest, since
-  // the tensor core truncates each step
-  if (dtype == kF32) n = std::max(n, parts(kblocks, 2048 / kHeadTileK));
-  return int(std::min<int64_t>(n, 4096));
+// Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
+// CTAs gets of `all` tile-blocks in total, so that they end together, and none shorter
+// than 8 blocks (float32: 2, of six products), so that the sums of parts stay few.
+int splits_for(int64_t kblocks, int64_t all, int dtype) {
+  const int64_t least = dtype == kF32 ? 2 : 8;
+  const int64_t most = std::max(least, all / 74);
+  return int(std::max<int64_t>(1, std::min(parts(kblocks, most), kblocks / least)));
 }
 
 Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool pack_h,
                bool pack_w, bool want_dh, bool want_dw) {
   Plan p{};
   p.planes = dtype == kF32 ? 3 : 1;
-  p.pairs = dtype == kF32 ? 6 : 1;
   p.pack_h = pack_h || grad;  // the gradient's copy has zeros in rows without a label
   p.pack_w = pack_w;
   p.ldp = up(cols, 8);
@@ -98,8 +96,10 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad
     const int64_t tm = kHeadPair * kHeadTileM, tn = parts(cols, p.tile_n);
     const int64_t dh_tiles = want_dh ? parts(rows, tm) * tn : 0;
     const int64_t dw_tiles = want_dw ? parts(p.piece, tm) * tn : 0;
-    p.dh_splits = splits_for(std::max<int64_t>(1, dh_tiles + dw_tiles), parts(p.piece, kHeadTileK), dtype);
-    p.dw_splits = splits_for(std::max<int64_t>(1, dh_tiles + dw_tiles), parts(rows, kHeadTileK), dtype);
+    const int64_t dh_blocks = parts(p.piece, kHeadTileK), dw_blocks = parts(rows, kHeadTileK);
+    const int64_t all = dh_tiles * dh_blocks + dw_tiles * dw_blocks;
+    p.dh_splits = splits_for(dh_blocks, all, dtype);
+    p.dw_splits = splits_for(dw_blocks, all, dtype);
     if (want_dh && p.pieces > 1) p.acc = take(rows * cols * 4);
     if (want_dh && p.dh_splits > 1) p.dh_part = take(p.dh_splits * rows * cols * 4);
     if (want_dw && p.dw_splits > 1) p.dw_part = take(p.dw_splits * p.piece * cols * 4);
@@ -114,6 +114,41 @@ bool is_narrow(int64_t cols, int64_t classes) {
 // Its workspace: the status word, and a dw of each block.
 int64_t narrow_bytes(int64_t rows, int64_t cols, int64_t classes, bool grad) {
   return 256 + (grad ? up(narrow_blocks(rows) * cols * classes * 4, 256) : 0);
+}
+
+int few_padded(int64_t rows) {
+  int n = 1;
+  while (n < rows) n *= 2;
+  return n;
+}
+bool is_few(int dtype, int64_t rows, int64_t cols) {
+  return rows <= (dtype == kF32 ? 16 : 4) && few_padded(rows) * int64_t(few_pitch(cols)) * 4 <= kFewSmem;
+}
+// Blocks of the first kernel (two a multiprocessor) and parts of the classes for dh (as
+// many as give every multiprocessor a few blocks); 148 multiprocessors whatever the GPU
+// has, since a workspace is sized before a device is named.
+struct FewPlan {
+  HeadFew f{};
+  int64_t part, target, g, dh_part, bytes;
+};
+FewPlan few_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad) {
+  FewPlan p{};
+  const int64_t nr = few_padded(rows), c = nr <= 4 ? 8 : 32 / nr;
+  p.f.blocks = int(std::min<int64_t>(296, parts(classes, 8 * c)));
+  const int64_t columns = parts(cols, dtype == kF32 ? 1024 : 2048);
+  p.f.chunks = int(std::max<int64_t>(1, std::min<int64_t>(592 / columns, classes / 64)));
+  int64_t at = 256;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  p.part = take(grad ? 0 : p.f.blocks * rows * 8);
+  p.target = take(grad ? 0 : rows * 4);
+  p.g = take(grad ? classes * nr * 4 : 0);
+  p.dh_part = take(grad ? p.f.chunks * rows * cols * 4 : 0);
+  p.bytes = at;
+  return p;
 }
 
 // ---- tensor maps ----------------------------------------------------------------
@@ -215,39 +250,50 @@ int check_workspace(const HeadArgs& a, int64_t need, std::string& err) {
 
 struct Operands {
   const void *h, *w;
-  int64_t ld_h, ld_w;
-  int64_t launches = 0;
+  int64_t ld_h, ld_w, launches;
 };
 
-// Status word cleared; operands packed where the plan says so.
+// Status word cleared; operands packed where the plan says so, in one launch.
 int operands(const HeadArgs& a, const Plan& p, bool grad, Operands* o, cudaStream_t s, std::string& err) {
   char* base = static_cast<char*>(a.workspace);
-  HEAD_CUDA(cudaMemsetAsync(base, 0, 4, s), "clearing the head's status word");
   o->h = a.h;
   o->ld_h = a.ld_h;
   o->w = a.w;
   o->ld_w = a.ld_w;
+  HeadPack h, w;
   if (p.pack_h) {
-    HEAD_CUDA(launch_head_pack(a.dtype, a.h, a.rows, a.cols, a.ld_h, grad ? a.labels : nullptr,
-                               a.classes, base + p.h, p.ldp, s),
-              "head pack launch");
-    o->h = base + p.h;
+    h.src = a.h;
+    h.rows = a.rows;
+    h.cols = a.cols;
+    h.ld = a.ld_h;
+    h.labels = grad ? a.labels : nullptr;
+    h.classes = a.classes;
+    h.dst = base + p.h;
+    h.ldp = p.ldp;
+    o->h = h.dst;
     o->ld_h = p.ldp;
-    ++o->launches;
   }
   if (p.pack_w) {
-    HEAD_CUDA(launch_head_pack(a.dtype, a.w, a.classes, a.cols, a.ld_w, nullptr, 0, base + p.w,
-                               p.ldp, s),
-              "head pack launch");
-    o->w = base + p.w;
+    w.src = a.w;
+    w.rows = a.classes;
+    w.cols = a.cols;
+    w.ld = a.ld_w;
+    w.dst = base + p.w;
+    w.ldp = p.ldp;
+    o->w = w.dst;
     o->ld_w = p.ldp;
-    ++o->launches;
   }
+  if (!p.pack_h && !p.pack_w) {
+    HEAD_CUDA(cudaMemsetAsync(base, 0, 4, s), "clearing the head's status word");
+    return 0;
+  }
+  HEAD_CUDA(launch_head_pack(a.dtype, h, w, reinterpret_cast<unsigned*>(base), s), "head pack launch");
+  o->launches = 1;
   return 0;
 }
 
-void settings(HeadLaunch& l, const HeadArgs& a, const Plan& p) {
-  l.pairs = p.pairs;
+void settings(HeadLaunch& l, const HeadArgs& a) {
+  l.f32 = a.dtype == kF32;
   l.status = static_cast<unsigned*>(a.workspace);
   l.wait_ns = kDefaultWaitNs;
   if (const char* s = std::getenv("MACBOOST_WAIT_LIMIT_US")) {
@@ -288,12 +334,43 @@ int narrow(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string
   return 0;
 }
 
+int few(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string& err) {
+  FewPlan p = few_plan(a.dtype, a.rows, a.cols, a.classes, grad);
+  if (check_workspace(a, p.bytes, err)) return -1;
+  if (use_device(device, err)) return -1;
+  Guard gd(device);
+  char* base = static_cast<char*>(a.workspace);
+  p.f.part = reinterpret_cast<float2*>(base + p.part);
+  p.f.target = reinterpret_cast<float*>(base + p.target);
+  p.f.g = reinterpret_cast<float*>(base + p.g);
+  p.f.dh_part = reinterpret_cast<float*>(base + p.dh_part);
+  HEAD_CUDA(launch_head_few(a, grad, p.f, s), "head launch");
+  if (!grad) {
+    HEAD_CUDA(launch_head_finish(p.f.part, p.f.target, a.labels, a.rows, a.classes, p.f.blocks, a.loss,
+                                 a.lse_out, s),
+              "head finish launch");
+    g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
+    return 0;
+  }
+  if (a.dh)
+    HEAD_CUDA(launch_head_reduce(HeadReduce{p.f.dh_part, p.f.chunks, a.rows, a.cols, nullptr, 0, 1, a.dh,
+                                            a.ld_dh, a.dtype == kF32},
+                                 s),
+              "head reduce launch");
+  g_kernel_launches.fetch_add(a.dh ? 3 : 1, std::memory_order_relaxed);
+  return 0;
+}
+
 }  // namespace
 
 int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool strided) {
   std::string err;
   if (check_shape(dtype, rows, cols, classes, err)) return -1;
   if (is_narrow(cols, classes)) return narrow_bytes(rows, cols, classes, grad);
+  if (is_few(dtype, rows, cols)) {
+    const int64_t loss = few_plan(dtype, rows, cols, classes, false).bytes;
+    return grad ? std::max(loss, few_plan(dtype, rows, cols, classes, true).bytes) : loss;
+  }
   const bool pack = dtype == kF32 || strided || cols % 8 != 0;
   const int64_t loss = make_plan(dtype, rows, cols, classes, false, pack, pack, true, true).bytes;
   if (!grad) return loss;
@@ -309,6 +386,7 @@ int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   if (check(a, false, err)) return -1;
   if (a.rows == 0) return 0;
   if (is_narrow(a.cols, a.classes)) return narrow(device, a, false, s, err);
+  if (is_few(a.dtype, a.rows, a.cols)) return few(device, a, false, s, err);
   const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, false, !in_place(a.dtype, a.h, a.ld_h),
                            !in_place(a.dtype, a.w, a.ld_w), true, true);
   if (check_workspace(a, p.bytes, err)) return -1;
@@ -318,7 +396,7 @@ int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   Operands o{};
   if (operands(a, p, false, &o, s, err)) return -1;
   HeadLaunch l{};
-  settings(l, a, p);
+  settings(l, a);
   l.jobs = 1;
   if (logits_job(l.job[0], a, p, o, 0, a.classes, err)) return -1;
   l.r.labels = a.labels;
@@ -349,6 +427,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
     return 0;
   }
   if (is_narrow(a.cols, a.classes)) return narrow(device, a, true, s, err);
+  if (is_few(a.dtype, a.rows, a.cols)) return few(device, a, true, s, err);
   const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, true, !in_place(a.dtype, a.h, a.ld_h),
                            !in_place(a.dtype, a.w, a.ld_w), a.dh != nullptr, a.dw != nullptr);
   if (check_workspace(a, p.bytes, err)) return -1;
@@ -363,7 +442,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, n = std::min(p.piece, a.classes - v0);
     HeadLaunch l{};
-    settings(l, a, p);
+    settings(l, a);
     l.jobs = 1;
     if (logits_job(l.job[0], a, p, o, v0, n, err)) return -1;
     l.r.labels = a.labels;
@@ -378,7 +457,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
     HEAD_CUDA(launch_head(kHeadG, kHeadTileN, l, s), "head launch");
 
     HeadLaunch q{};
-    settings(q, a, p);
+    settings(q, a);
     HeadReduce red[2]{};
     int reds = 0;
     HeadJob dh{}, dw{};

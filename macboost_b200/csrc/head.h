@@ -47,6 +47,7 @@ constexpr int kHeadTileM = 128;      // accumulator rows a CTA (TMEM lanes)
 constexpr int kHeadTileN = 256;      // accumulator columns
 constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit values
 constexpr int kHeadPair = 2;         // CTAs that share a tile
+constexpr int kHeadChunk = 4;        // float32: K blocks of one sum of the tensor core
 
 // One product C = A B^T over K, as tiles.  Operands are 16-bit values in `planes`
 // planes (the terms of a float32, or the value itself) behind tensor maps of
@@ -84,7 +85,7 @@ struct HeadRows {                    // what the logits' epilogues know of each 
 struct HeadLaunch {
   HeadJob job[2];
   int jobs;
-  int pairs;                         // products of planes: 1, or 6 for float32
+  int f32;                           // three planes an operand, six products
   HeadRows r;
   unsigned* status;
   unsigned long long wait_ns;
@@ -100,12 +101,37 @@ inline int narrow_blocks(int64_t rows) {
 }
 cudaError_t launch_head_narrow(const HeadArgs& h, bool grad, float* part, int blocks, cudaStream_t s);
 
+// Nor does a head of few rows, whose h fits in shared memory: float32 to 16 rows,
+// bfloat16 to 4.  Measured at 1,024 x 131,072 bfloat16, loss: 4 rows 61 us here and 72 us
+// on the tensor cores, 8 rows 105 and 72.
+constexpr int64_t kFewSmem = 128 * 1024;
+// Floats between its rows there: whole steps of 64 columns.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int few_pitch(long long cols) { return int((cols + 63) / 64 * 64); }
+struct HeadFew {
+  int blocks, chunks;                // of the first kernel; of the classes for dh
+  float2* part;
+  float* target;
+  float* g;
+  float* dh_part;
+};
+cudaError_t launch_head_few(const HeadArgs& h, bool grad, const HeadFew& f, cudaStream_t s);
+
 enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2 };
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s);
 // Source rows (float32 or bfloat16) to planes of bfloat16 (3 or 1), stride ldp; rows
 // whose label (unless null) is none of the classes become zeros.
-cudaError_t launch_head_pack(int dtype, const void* src, int64_t rows, int64_t cols, int64_t ld,
-                             const int* labels, int64_t classes, void* dst, int64_t ldp,
+struct HeadPack {
+  const void* src = nullptr;
+  long long rows = 0, cols = 0, ld = 0;
+  const int* labels = nullptr;
+  long long classes = 0;
+  void* dst = nullptr;
+  long long ldp = 0;
+};
+cudaError_t launch_head_pack(int dtype, const HeadPack& a, const HeadPack& b, unsigned* status,
                              cudaStream_t s);
 cudaError_t launch_head_finish(const float2* part, const float* target, const int* labels,
                                int64_t rows, int64_t classes, int64_t parts, float* loss,

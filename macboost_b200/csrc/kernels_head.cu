@@ -10,8 +10,10 @@
 //
 // A float32 operand is three planes of bfloat16, x = x1 + x2 + x3 with 8 bits each, and
 // the product the six terms x_i y_j with i + j <= 4 -- what is dropped is below 2^-24
-// of |x||y| -- the smallest terms first: the tensor core's sums are truncated to 32
-// bits, and a small term costs little while the sum is small.
+// of |x||y|.  The tensor core's sums are truncated to 32 bits at every step, so they run
+// over kHeadChunk blocks of K only, the smallest terms first (they cost little while the
+// sum is small), and the epilogue adds the chunks up in registers, rounded to nearest.
+// With whole sums in the tensor core, dh of 26 x 12 x 7,798 was off by 2.5e-6.
 //
 // Every wait ends after wait_ns: the CTA then marks itself dead, sets the status word,
 // lets its copies land and returns (its results are void).
@@ -286,7 +288,7 @@ __device__ __forceinline__ void store_f32(float* p, const float (&v)[32], int n)
   }
 }
 
-template <int EPI, int TN>
+template <int EPI, int TN, bool F32>
 __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads, 1)
     head_kernel(const __grid_constant__ HeadLaunch a) {
   constexpr int kBytesA = kHeadTileM * 128;
@@ -361,8 +363,9 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         // Each tile starts at another K block: tiles that run together would read the same
         // 128 bytes of every row, which are few of the memory's channels.
         const int turn = (t.m + t.n) % (k1 - k0);
-        for (int p = 6 - a.pairs; ok && p < 6; ++p)
-          for (int i = k0; i < k1; ++i) {
+        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0)
+          for (int p = F32 ? 0 : 5; ok && p < 6; ++p)
+          for (int i = c0; i < (F32 ? min(c0 + kHeadChunk, k1) : k1); ++i) {
             const int kb = i + turn < k1 ? i + turn : i + turn - (k1 - k0);
             ok = wait(empty + 8 * s, ph ^ 1);
             if (!ok) break;
@@ -413,36 +416,38 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         const HeadJob& q = a.job[t.job];
         int k0, k1;
         walk.blocks(t, &k0, &k1);
-        ok = wait(sums_empty + 8 * as, aph ^ 1);
-        if (!ok) break;
-        fence_after();
         // float32 sums of bfloat16, M 256 (both CTAs), N TN
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(q.a_mn) << 15) |
                                (uint32_t(q.b_mn) << 16) | (uint32_t(TN / 8) << 17) |
                                (uint32_t(kHeadPair * kHeadTileM / 16) << 24);
         const uint32_t step_a = q.a_mn ? 2048 / 16 : 32 / 16, step_b = q.b_mn ? 2048 / 16 : 32 / 16;
-        bool add = false;
-        const int steps = a.pairs * (k1 - k0);
-        for (int i = 0; i < steps; ++i) {
-          ok = wait(full + 8 * s, ph);
+        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0) {
+          ok = wait(sums_empty + 8 * as, aph ^ 1);
           if (!ok) break;
           fence_after();
-          const uint64_t da = descriptor(ring + s * kStage, q.a_mn);
-          const uint64_t db = descriptor(ring + s * kStage + kBytesA, q.b_mn);
+          bool add = false;
+          const int steps = F32 ? 6 * (min(c0 + kHeadChunk, k1) - c0) : k1 - k0;
+          for (int i = 0; i < steps; ++i) {
+            ok = wait(full + 8 * s, ph);
+            if (!ok) break;
+            fence_after();
+            const uint64_t da = descriptor(ring + s * kStage, q.a_mn);
+            const uint64_t db = descriptor(ring + s * kStage + kBytesA, q.b_mn);
 #pragma unroll
-          for (int k = 0; k < kHeadTileK / 16; ++k) {
-            mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
-            add = true;
+            for (int k = 0; k < kHeadTileK / 16; ++k) {
+              mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
+              add = true;
+            }
+            commit_both(empty + 8 * s);
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1;
+            }
           }
-          commit_both(empty + 8 * s);
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1;
-          }
+          if (ok) commit_both(sums_full + 8 * as);
+          as ^= 1;
+          if (as == 0) aph ^= 1;
         }
-        if (ok) commit_both(sums_full + 8 * as);
-        as ^= 1;
-        if (as == 0) aph ^= 1;
       }
     }
   } else {
@@ -451,23 +456,54 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
     int as = 0, aph = 0;
     const int quarter = warp % 4, half = (warp - 2) / 4;
     const HeadRows& r = a.r;
+    // this thread's row of the tile's half: chunks of sums added up (float32)
+    float sums[F32 ? TN / 2 : 1];
     while (walk.next(&t)) {
       const HeadJob& q = a.job[t.job];
-      bool ok = wait(sums_full + 8 * as, aph);
-      ok = __all_sync(~0u, ok);
+      int k0, k1;
+      walk.blocks(t, &k0, &k1);
+      bool ok = true;
+      uint32_t src = 0;
+      for (int c0 = k0; c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0) {
+        ok = __all_sync(~0u, wait(sums_full + 8 * as, aph));
+        if (!ok) break;
+        fence_after();
+        src = tmem + as * TN + (uint32_t(quarter * 32) << 16) + half * (TN / 2);
+        if constexpr (F32) {
+#pragma unroll
+          for (int c = 0; c < TN / 2; c += 32) {
+            float v[32];
+            tmem_load(src + c, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sums[c + i] = c0 == k0 ? v[i] : sums[c + i] + v[i];
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive_at(sums_empty + 8 * as, 0);
+          as ^= 1;
+          if (as == 0) aph ^= 1;
+        }
+      }
       if (!ok) break;
-      fence_after();
-      const uint32_t src = tmem + as * TN + (uint32_t(quarter * 32) << 16) + half * (TN / 2);
+      // 32 of the sums, by column
+      auto take = [&](int c, float (&v)[32]) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = sums[c + i];
+        } else {
+          tmem_load(src + c, v);
+        }
+      };
       const int row = (t.m * kHeadPair + int(rank)) * kHeadTileM + quarter * 32 + lane;
       const int col0 = t.n * TN + half * (TN / 2);
       if (EPI == kHeadLse) {
         const bool there = row < r.rows;
         const int y = there ? r.labels[row] : -1;
         float m = -INFINITY, sum = 0.f;
-#pragma unroll 1
+#pragma unroll(F32 ? 4 : 1)
         for (int c = 0; c < TN / 2; c += 32) {
           float v[32];
-          tmem_load(src + c, v);
+          take(c, v);
           const int n = r.classes - (col0 + c);
           online(v, n, m, sum);
           if (unsigned(y - (col0 + c)) < 32u && y < r.classes) {
@@ -486,10 +522,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         const float lse = there ? r.lse[row] : 0.f;
         const float up = known ? r.dloss[row] : 0.f;
         __nv_bfloat16* g = static_cast<__nv_bfloat16*>(r.g) + (long long)row * r.ld_g + col0;
-#pragma unroll 1
+#pragma unroll(F32 ? 4 : 1)
         for (int c = 0; c < TN / 2; c += 32) {
           float v[32];
-          tmem_load(src + c, v);
+          take(c, v);
           const int v0 = r.v0 + col0 + c;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -500,7 +536,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           const int n = int(r.ld_g) - (col0 + c);
           if (there && n > 0) {
             store_bf16(g + c, v, n);
-            if (a.pairs > 1) {
+            if constexpr (F32) {
 #pragma unroll
               for (int z = 1; z < 3; ++z) {
 #pragma unroll
@@ -513,10 +549,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       } else {
         const bool there = row < q.M;
         float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row) * q.N + col0 : nullptr;
-#pragma unroll 1
+#pragma unroll(F32 ? 4 : 1)
         for (int c = 0; c < TN / 2; c += 32) {
           float v[32];
-          tmem_load(src + c, v);
+          take(c, v);
           const int n = q.N - (col0 + c);
           if (!there || n <= 0) continue;
           if (q.acc_in) {
@@ -533,11 +569,13 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           }
         }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive_at(sums_empty + 8 * as, 0);
-      as ^= 1;
-      if (as == 0) aph ^= 1;
+      if constexpr (!F32) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_at(sums_empty + 8 * as, 0);
+        as ^= 1;
+        if (as == 0) aph ^= 1;
+      }
     }
   }
   __syncwarp();
@@ -552,27 +590,38 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
 
 // ---- the kernels around it ------------------------------------------------------
 
-// Planes of bfloat16 with 16-byte aligned rows: the terms of a float32, or a copy.
+// Planes of bfloat16 with 16-byte aligned rows: the terms of a float32, or a copy.  A
+// warp a row, eight values a lane; the rows of up to two matrices one after the other.
+// It also clears the status word.
 template <class T>
-__global__ void __launch_bounds__(256)
-    head_pack_kernel(const T* src, long long rows, int cols, long long ld, const int* labels,
-                     int classes, __nv_bfloat16* dst, int ldp) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * ldp) return;
-  const long long r = i / ldp;
-  int c = int(i - r * ldp);
-  if (labels && unsigned(labels[r]) >= unsigned(classes)) c = cols;  // zeros
-  if (sizeof(T) == 2) {
-    const unsigned short v = c < cols ? reinterpret_cast<const unsigned short*>(src)[r * ld + c] : 0;
-    reinterpret_cast<unsigned short*>(dst)[i] = v;
-    return;
-  }
-  float v = c < cols ? reinterpret_cast<const float*>(src)[r * ld + c] : 0.f;
+__global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack a, const HeadPack b, unsigned* status) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+  const int lane = threadIdx.x % 32;
+  long long r = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+  const bool second = r >= a.rows;
+  if (second) r -= a.rows;
+  const HeadPack& m = second ? b : a;
+  if (r >= m.rows) return;
+  // a row without a label becomes zeros
+  const int cols = m.labels && unsigned(m.labels[r]) >= unsigned(m.classes) ? 0 : int(m.cols);
+  const T* from = static_cast<const T*>(m.src) + r * m.ld;
+  __nv_bfloat16* to = static_cast<__nv_bfloat16*>(m.dst) + r * m.ldp;
+  const long long plane = m.rows * m.ldp;
+#pragma unroll 2
+  for (int c = lane * 8; c < int(m.ldp); c += 256) {
+    float v[8];
 #pragma unroll
-  for (int z = 0; z < 3; ++z) {
-    const __nv_bfloat16 t = __float2bfloat16_rn(v);
-    dst[z * rows * ldp + i] = t;
-    v = z == 0 && !isfinite(v) ? 0.f : v - __bfloat162float(t);
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? float(from[c + i]) : 0.f;
+#pragma unroll
+    for (int z = 0; z < (sizeof(T) == 4 ? 3 : 1); ++z) {
+      __nv_bfloat16 t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t[i] = __float2bfloat16_rn(v[i]);
+        v[i] = z == 0 && !isfinite(v[i]) ? 0.f : v[i] - __bfloat162float(t[i]);
+      }
+      *reinterpret_cast<uint4*>(to + z * plane + c) = *reinterpret_cast<const uint4*>(t);
+    }
   }
 }
 
@@ -627,11 +676,27 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Y threads a value, each every Y-th part.
+template <int Y>
 __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.M * a.N) return;
-  float v = a.acc_in ? a.acc[i] : 0.f;
-  for (int s = 0; s < a.splits; ++s) v += a.part[s * a.M * a.N + i];
+  __shared__ float sums[256];
+  constexpr int X = 256 / Y;
+  const int x = threadIdx.x % X, y = threadIdx.x / X;
+  const long long i = (long long)blockIdx.x * X + x, all = a.M * a.N;
+  float v = 0.f;
+  if (i < all) {
+    if (y == 0 && a.acc_in) v = a.acc[i];
+#pragma unroll 8
+    for (int s = y; s < a.splits; s += Y) v += a.part[s * all + i];
+  }
+  if (Y > 1) {
+    sums[threadIdx.x] = v;
+    __syncthreads();
+    if (y > 0) return;
+#pragma unroll
+    for (int q = 1; q < Y; ++q) v += sums[q * X + x];
+  }
+  if (i >= all) return;
   if (!a.final) {
     a.acc[i] = v;
     return;
@@ -926,11 +991,333 @@ cudaError_t narrow_type(const Narrow& a, bool grad, int blocks, cudaStream_t s) 
   return narrow_cols<T, 64>(a, grad, blocks, s);
 }
 
-template <int EPI, int TN>
-cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
+// ---- few rows -------------------------------------------------------------------
+//
+// A handful of rows against many classes: reading the weights bounds the work, so the
+// CUDA cores take them as they stream by, in float32 (the tensor cores would want 256
+// rows, and three planes of float32 weights written first).  The rows lie in shared
+// memory.  A warp takes C classes at once -- each 16 bytes of a row of h it reads serve C
+// classes -- and its C x NR <= 32 sums meet in 31 shuffles, one sum a lane.
+//
+// loss   lane (c, n) keeps the running maximum and sum of its classes' logits
+// grad   g goes to the workspace, dw's C rows are formed at once from g and h; a second
+//        kernel reads the weights again for dh = g w, a thread a few columns
+
+constexpr int kFewThreads = 256;
+
+struct Few {
+  const void *h, *w;
+  int rows, cols, classes;
+  long long ld_h, ld_w;
+  const int* labels;
+  const float *lse, *dloss;
+  float2* part;            // loss: blocks x rows
+  float* target;
+  float* g;                // grad: classes x NR
+  void* dw;                // or null
+  long long ld_dw;
+  float* dh_part;          // grad: chunks x rows x cols
+  unsigned* status;
+};
+
+// PER adjacent values of a row, as pairs of floats; PER = 1: two values `apart` columns
+// from each other, the second one if there are `left` > apart columns.
+template <class T, int PER>
+__device__ __forceinline__ void load_pairs(const T* p, int apart, int left, F2 (&v)[(PER + 1) / 2]) {
+  if constexpr (PER == 1) {
+    v[0] = pair(float(p[0]), left > apart ? float(p[apart]) : 0.f);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 q = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = pair(q.x, q.y);
+    v[1] = pair(q.z, q.w);
+  } else {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = pair(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+  }
+}
+template <int PER>
+__device__ __forceinline__ void load_shared(const float* p, F2 (&v)[(PER + 1) / 2]) {
+  if constexpr (PER == 1) {
+    v[0] = pair(p[0], p[32]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+      const F4 q = *reinterpret_cast<const F4*>(p + 4 * i);
+      v[2 * i] = q.lo;
+      v[2 * i + 1] = q.hi;
+    }
+  }
+}
+template <class T, int PER>
+__device__ __forceinline__ void store_pairs(T* p, int left, const F2 (&v)[(PER + 1) / 2]) {
+  if constexpr (PER == 1) {
+    const float2 x = split(v[0]);
+    p[0] = T(x.x);
+    if (left > 32) p[32] = T(x.y);
+  } else if constexpr (sizeof(T) == 4) {
+    const float2 x = split(v[0]), y = split(v[1]);
+    *reinterpret_cast<float4*>(p) = make_float4(x.x, x.y, y.x, y.y);
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = split(v[i]);
+      u[i] = pack2(x.x, x.y);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+template <class T, int NR, int PER, bool GRAD>
+__global__ void __launch_bounds__(kFewThreads, 2) head_few_kernel(const Few a) {
+  constexpr int C = NR > 4 ? 32 / NR : NR == 4 && PER == 8 ? 4 : 8;  // classes a warp
+  constexpr int S = C * NR;                 // sums: 8, 16 or 32
+  constexpr int P = (PER + 1) / 2;
+  extern __shared__ float4 few_shared[];
+  float* hs = reinterpret_cast<float*>(few_shared);  // NR x pitch
+  __shared__ float2 sums[kFewThreads / 32][NR];
+  constexpr int STEP = PER == 1 ? 64 : 32 * PER;  // columns a warp takes at once
+  const int pitch = few_pitch(a.cols);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;  // there is no wait to run out
+  for (int n = 0; n < NR; ++n) {
+    // rows that do not exist, and in the gradient rows without a label, are zeros
+    const bool there = n < a.rows && (!GRAD || unsigned(a.labels[n]) < unsigned(a.classes));
+    for (int d = threadIdx.x; d < pitch; d += kFewThreads)
+      hs[n * pitch + d] = there && d < a.cols ? float(static_cast<const T*>(a.h)[n * a.ld_h + d]) : 0.f;
+  }
+  __syncthreads();
+  const T* W = static_cast<const T*>(a.w);
+  // after the shuffles lane i has sum i / (32 / S)
+  const int mine = lane / (32 / S), mc = mine / NR, mn = mine % NR;
+  const bool there = mn < a.rows;
+  const int y = there ? a.labels[mn] : -1;
+  const bool known = unsigned(y) < unsigned(a.classes);
+  const float lse = GRAD && there ? a.lse[mn] : 0.f, up = GRAD && known ? a.dloss[mn] : 0.f;
+  float m = -INFINITY, sum = 0.f;
+  const int stride = int(gridDim.x) * (kFewThreads / 32) * C;
+  for (int v0 = (int(blockIdx.x) * (kFewThreads / 32) + warp) * C; v0 < a.classes; v0 += stride) {
+    F2 acc[C][NR];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) acc[c][n] = pair(0.f, 0.f);
+#pragma unroll 2
+    for (int d = lane * PER; d < a.cols; d += STEP) {
+      F2 w[C][P];
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        load_pairs<T, PER>(W + min(v0 + c, a.classes - 1) * a.ld_w + d, 32, a.cols - d, w[c]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        F2 h[P];
+        load_shared<PER>(hs + n * pitch + d, h);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < P; ++i) acc[c][n] = fma2(w[c][i], h[i], acc[c][n]);
+      }
+    }
+    float s[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const float2 x = split(acc[i / NR][i % NR]);
+      s[i] = x.x + x.y;
+    }
+    int o = 16;
+#pragma unroll
+    for (int k = S / 2; k > 0; k /= 2) {
+      const bool high = lane & o;
+#pragma unroll
+      for (int i = 0; i < k; ++i) {
+        const float give = high ? s[i] : s[i + k], keep = high ? s[i + k] : s[i];
+        s[i] = keep + __shfl_xor_sync(~0u, give, o);
+      }
+      o /= 2;
+    }
+    float l = s[0];
+    for (; o > 0; o /= 2) l += __shfl_xor_sync(~0u, l, o);
+    const int v = v0 + mc;
+    if (!GRAD) {
+      if (v < a.classes) {
+        const float top = fmaxf(m, l), base = fabsf(top) == INFINITY ? 0.f : top;
+        const float old = fabsf(m) == INFINITY ? 0.f : m;
+        sum = (sum == 0.f ? 0.f : sum * exp2_approx((old - base) * kLog2e)) +
+              exp2_approx((l - base) * kLog2e);
+        m = top;
+        if (v == y && lane % (32 / S) == 0) a.target[mn] = l;
+      }
+    } else {
+      float g = 0.f;
+      if (known && v < a.classes) {
+        const float p = exp2_approx((l - lse) * kLog2e);
+        g = up * (v == y ? p - 1.f : p);
+      }
+      if (lane % (32 / S) == 0 && v < a.classes) a.g[(long long)v * NR + mn] = g;
+      if (a.dw) {
+        float gs[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) gs[i] = __shfl_sync(~0u, g, i * (32 / S));
+        T* to = static_cast<T*>(a.dw) + v0 * a.ld_dw;
+        for (int d = lane * PER; d < a.cols; d += STEP) {
+          F2 x[C][P];
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < P; ++i) x[c][i] = pair(0.f, 0.f);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            F2 h[P];
+            load_shared<PER>(hs + n * pitch + d, h);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const F2 gg = pair(gs[c * NR + n], gs[c * NR + n]);
+#pragma unroll
+              for (int i = 0; i < P; ++i) x[c][i] = fma2(gg, h[i], x[c][i]);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            if (v0 + c < a.classes) store_pairs<T, PER>(to + c * a.ld_dw + d, a.cols - d, x[c]);
+        }
+      }
+    }
+  }
+  if (!GRAD) {
+    // lanes of one row, then the warps
+    auto join = [&](float m2, float s2) {
+      const float top = fmaxf(m, m2), base = fabsf(top) == INFINITY ? 0.f : top;
+      auto term = [&](float mm, float ss) {
+        return ss == 0.f ? 0.f : ss * exp2_approx(((fabsf(mm) == INFINITY ? 0.f : mm) - base) * kLog2e);
+      };
+      sum = term(m, sum) + term(m2, s2);
+      m = top;
+    };
+#pragma unroll
+    for (int o = NR * (32 / S); o < 32; o *= 2) {
+      const float m2 = __shfl_xor_sync(~0u, m, o), s2 = __shfl_xor_sync(~0u, sum, o);
+      join(m2, s2);
+    }
+    if (lane % (32 / S) == 0 && mc == 0) sums[warp][mn] = make_float2(m, sum);
+    __syncthreads();
+    if (threadIdx.x < NR && int(threadIdx.x) < a.rows) {
+      m = sums[0][threadIdx.x].x;
+      sum = sums[0][threadIdx.x].y;
+      for (int q = 1; q < kFewThreads / 32; ++q) join(sums[q][threadIdx.x].x, sums[q][threadIdx.x].y);
+      a.part[(long long)blockIdx.x * a.rows + threadIdx.x] = make_float2(m, sum);
+    }
+  }
+}
+
+// dh_part[chunk] = g w over the chunk's classes: `tx` threads for PER columns each,
+// 256 / tx classes at once.
+template <class T, int NR, int PER>
+__global__ void __launch_bounds__(kFewThreads) head_few_dh_kernel(const Few a, int tx, int chunk) {
+  constexpr int P = (PER + 1) / 2;
+  __shared__ F2 meet[kFewThreads];
+  const int ty = kFewThreads / tx, x = threadIdx.x % tx, yy = threadIdx.x / tx;
+  // PER columns from d on, or d and d + tx
+  const int d = PER == 1 ? int(blockIdx.x) * 2 * tx + x : (int(blockIdx.x) * tx + x) * PER;
+  const int v0 = int(blockIdx.y) * chunk, v1 = min(v0 + chunk, a.classes);
+  F2 acc[NR][P];
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int i = 0; i < P; ++i) acc[n][i] = pair(0.f, 0.f);
+  if (d < a.cols) {
+    const T* w = static_cast<const T*>(a.w) + d;
+#pragma unroll 4
+    for (int v = v0 + yy; v < v1; v += ty) {
+      F2 q[P];
+      load_pairs<T, PER>(w + v * a.ld_w, tx, a.cols - d, q);
+      float g[NR];
+      if constexpr (NR >= 4) {
+#pragma unroll
+        for (int n = 0; n < NR; n += 4) {
+          const float4 t = __ldg(reinterpret_cast<const float4*>(a.g + (long long)v * NR + n));
+          g[n] = t.x, g[n + 1] = t.y, g[n + 2] = t.z, g[n + 3] = t.w;
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) g[n] = __ldg(a.g + (long long)v * NR + n);
+      }
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const F2 gg = pair(g[n], g[n]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) acc[n][i] = fma2(gg, q[i], acc[n][i]);
+      }
+    }
+  }
+  for (int n = 0; n < NR; ++n) {
+    if (n >= a.rows) break;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      F2 v = acc[0][i];
+#pragma unroll
+      for (int k = 1; k < NR; ++k)
+        if (k == n) v = acc[k][i];
+      if (ty > 1) {
+        __syncthreads();
+        meet[threadIdx.x] = v;
+        __syncthreads();
+      }
+      if (yy == 0 && d < a.cols) {
+        float2 s = split(v);
+        for (int k = 1; k < ty; ++k) {
+          const float2 o = split(meet[k * tx + x]);
+          s.x += o.x;
+          s.y += o.y;
+        }
+        float* to = a.dh_part + ((long long)blockIdx.y * a.rows + n) * a.cols + d + 2 * i;
+        to[0] = s.x;
+        if (PER > 1)
+          to[1] = s.y;
+        else if (d + tx < a.cols)
+          to[tx] = s.y;
+      }
+    }
+  }
+}
+
+template <class T, int NR, int PER>
+cudaError_t few_of(const Few& a, bool grad, int blocks, int chunks, cudaStream_t s) {
+  const size_t smem = size_t(NR) * few_pitch(a.cols) * sizeof(float);
+  const auto k = grad ? head_few_kernel<T, NR, PER, true> : head_few_kernel<T, NR, PER, false>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  k<<<blocks, kFewThreads, smem, s>>>(a);
+  if (grad && a.dh_part) {
+    int tx = 32;
+    constexpr int PER2 = PER == 1 ? 2 : PER;  // columns a thread
+    while (tx < kFewThreads && tx * PER2 < a.cols) tx *= 2;
+    const int chunk = (a.classes + chunks - 1) / chunks;
+    head_few_dh_kernel<T, NR, PER>
+        <<<dim3((a.cols + tx * PER2 - 1) / (tx * PER2), chunks), kFewThreads, 0, s>>>(a, tx, chunk);
+  }
+  return cudaGetLastError();
+}
+
+template <class T, int PER>
+cudaError_t few_rows(const Few& a, bool grad, int blocks, int chunks, cudaStream_t s) {
+  if (a.rows <= 1) return few_of<T, 1, PER>(a, grad, blocks, chunks, s);
+  if (a.rows <= 2) return few_of<T, 2, PER>(a, grad, blocks, chunks, s);
+  if (a.rows <= 4) return few_of<T, 4, PER>(a, grad, blocks, chunks, s);
+  if constexpr (sizeof(T) == 4) {
+    if (a.rows <= 8) return few_of<T, 8, PER>(a, grad, blocks, chunks, s);
+    return few_of<T, 16, PER>(a, grad, blocks, chunks, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+template <int EPI, int TN, bool F32>
+cudaError_t go_type(const HeadLaunch& a, cudaStream_t s) {
   constexpr int kStage = kHeadTileM * 128 + TN / kHeadPair * 128;
   constexpr size_t smem = size_t((192 * 1024) / kStage) * kStage + 1024;
-  const cudaError_t e = cudaFuncSetAttribute(head_kernel<EPI, TN>,
+  const cudaError_t e = cudaFuncSetAttribute(head_kernel<EPI, TN, F32>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   long long tiles = 0;
@@ -938,8 +1325,13 @@ cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
     tiles += (long long)a.job[j].tiles_m * a.job[j].tiles_n * a.job[j].splits;
   if (tiles <= 0) return cudaSuccess;
   const int pairs = int(std::min<long long>(tiles, device_sms() / kHeadPair));
-  head_kernel<EPI, TN><<<pairs * kHeadPair, kHeadThreads, smem, s>>>(a);
+  head_kernel<EPI, TN, F32><<<pairs * kHeadPair, kHeadThreads, smem, s>>>(a);
   return cudaGetLastError();
+}
+
+template <int EPI, int TN>
+cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
+  return a.f32 ? go_type<EPI, TN, true>(a, s) : go_type<EPI, TN, false>(a, s);
 }
 
 }  // namespace
@@ -981,19 +1373,46 @@ cudaError_t launch_head_narrow(const HeadArgs& h, bool grad, float* part, int bl
   return cudaGetLastError();
 }
 
-cudaError_t launch_head_pack(int dtype, const void* src, int64_t rows, int64_t cols, int64_t ld,
-                             const int* labels, int64_t classes, void* dst, int64_t ldp,
+cudaError_t launch_head_few(const HeadArgs& h, bool grad, const HeadFew& f, cudaStream_t s) {
+  Few a{};
+  a.h = h.h;
+  a.w = h.w;
+  a.rows = int(h.rows);
+  a.cols = int(h.cols);
+  a.classes = int(h.classes);
+  a.ld_h = h.ld_h;
+  a.ld_w = h.ld_w;
+  a.labels = h.labels;
+  a.lse = h.lse;
+  a.dloss = h.dloss;
+  a.part = f.part;
+  a.target = f.target;
+  a.g = f.g;
+  a.dw = h.dw;
+  a.ld_dw = h.ld_dw;
+  a.dh_part = h.dh ? f.dh_part : nullptr;
+  a.status = static_cast<unsigned*>(h.workspace);
+  // 16 bytes at a time where the rows of w (and dw) start on them
+  const long long size = h.dtype == kF32 ? 4 : 2, per = 16 / size;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(h.w) | uintptr_t(h.ld_w * size) |
+                       uintptr_t(h.cols * size) |
+                       (grad && h.dw ? reinterpret_cast<uintptr_t>(h.dw) | uintptr_t(h.ld_dw * size) : 0);
+  const bool wide = at % 16 == 0 && h.cols % per == 0;
+  if (h.dtype == kF32)
+    return wide ? few_rows<float, 4>(a, grad, f.blocks, f.chunks, s)
+                : few_rows<float, 1>(a, grad, f.blocks, f.chunks, s);
+  return wide ? few_rows<__nv_bfloat16, 8>(a, grad, f.blocks, f.chunks, s)
+              : few_rows<__nv_bfloat16, 1>(a, grad, f.blocks, f.chunks, s);
+}
+
+cudaError_t launch_head_pack(int dtype, const HeadPack& a, const HeadPack& b, unsigned* status,
                              cudaStream_t s) {
-  const long long blocks = (rows * ldp + 255) / 256;
+  const long long blocks = (a.rows + b.rows + 7) / 8;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
   if (dtype == kF32)
-    head_pack_kernel<float><<<unsigned(blocks), 256, 0, s>>>(
-        static_cast<const float*>(src), rows, int(cols), ld, labels, int(classes),
-        static_cast<__nv_bfloat16*>(dst), int(ldp));
+    head_pack_kernel<float><<<unsigned(blocks), 256, 0, s>>>(a, b, status);
   else
-    head_pack_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(src), rows, int(cols), ld, labels, int(classes),
-        static_cast<__nv_bfloat16*>(dst), int(ldp));
+    head_pack_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, s>>>(a, b, status);
   return cudaGetLastError();
 }
 
@@ -1010,9 +1429,13 @@ cudaError_t launch_head_finish(const float2* part, const float* target, const in
 }
 
 cudaError_t launch_head_reduce(const HeadReduce& a, cudaStream_t s) {
-  const long long blocks = (a.M * a.N + 255) / 256;
+  const int x = a.splits >= 16 ? 32 : 256;
+  const long long blocks = (a.M * a.N + x - 1) / x;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  head_reduce_kernel<<<unsigned(blocks), 256, 0, s>>>(a);
+  if (x == 32)
+    head_reduce_kernel<8><<<unsigned(blocks), 256, 0, s>>>(a);
+  else
+    head_reduce_kernel<1><<<unsigned(blocks), 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 

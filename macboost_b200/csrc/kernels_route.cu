@@ -34,6 +34,14 @@ constexpr int kTile = 544;              // floats of a warp's tile: 32 x 17, 16 
 
 __device__ __forceinline__ float not_nan(float v) { return v != v ? -INFINITY : v; }
 
+// exp(x) of a probability beside the largest one, x <= 0: the argument's rounding, |x|
+// 2^-24 of e^x, is at most 2^-24 / e of 1.
+__device__ __forceinline__ float exp_term(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
 // A warp's rows (nr x E, row stride ld) between global memory and its tile, whose
 // rows are E | 1 floats apart so that a column is free of bank conflicts.  i / E by
 // a 16-bit reciprocal: exact for i < 512 and E <= 64.
@@ -111,7 +119,7 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
       top = found ? best : 0.f;
       if (a.norm == kRouteAll) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) total += expf(not_nan(v[i]) - top);
+        for (int i = 0; i < V; ++i) total += exp_term(not_nan(v[i]) - top);
 #pragma unroll
         for (int o = L / 2; o > 0; o /= 2) total += __shfl_xor_sync(~0u, total, o);
       }
@@ -149,14 +157,6 @@ __device__ __forceinline__ unsigned ordered(float v) {
 __device__ __forceinline__ float from_ordered(unsigned u) {
   return __uint_as_float(u ^ (unsigned(int(~u) >> 31) | 0x80000000u));
 }
-// exp(x) for a sum of terms up to 1: the argument's rounding, |x| 2^-24 of a term e^x,
-// is at most 2^-24 / e of the sum.
-__device__ __forceinline__ float exp_term(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-  return y;
-}
-
 // A warp a row of up to 32 V logits.
 template <int V>
 __global__ void __launch_bounds__(kWarps * 32) route_wide_kernel(const RouteArgs a) {
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const Ro
     if (a.norm == kRouteAll && id0 >= 0) {
       const float l0 = mine[id0];
 #pragma unroll
-      for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = -mean * (w0 * expf(not_nan(mine[e]) - l0));
+      for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = -mean * (w0 * exp_term(not_nan(mine[e]) - l0));
     } else {
 #pragma unroll
       for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = 0.f;
@@ -319,15 +319,15 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteArgs
       float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
       if (all) {
         q = *reinterpret_cast<const float4*>(l + e);
-        q.x = scale * expf(not_nan(q.x) - l0);
-        q.y = scale * expf(not_nan(q.y) - l0);
-        q.z = scale * expf(not_nan(q.z) - l0);
-        q.w = scale * expf(not_nan(q.w) - l0);
+        q.x = scale * exp_term(not_nan(q.x) - l0);
+        q.y = scale * exp_term(not_nan(q.y) - l0);
+        q.z = scale * exp_term(not_nan(q.z) - l0);
+        q.w = scale * exp_term(not_nan(q.w) - l0);
       }
       *reinterpret_cast<float4*>(d + e) = q;
     }
   } else {
-    for (int e = lane; e < E; e += 32) d[e] = all ? scale * expf(not_nan(l[e]) - l0) : 0.f;
+    for (int e = lane; e < E; e += 32) d[e] = all ? scale * exp_term(not_nan(l[e]) - l0) : 0.f;
   }
   __syncwarp();  // the warp's own stores before the choices' values replace some of them
   if (id >= 0) d[id] = w * (dw - mean);

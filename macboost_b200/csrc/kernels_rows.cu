@@ -245,6 +245,12 @@ __device__ __forceinline__ void zero_empty(const int* order, long long warp, lon
                                            U* out, long long ld, long long units, int lane) {
   const int slots = clear_slots(units);
   const long long first = warp * slots;
+  if (units <= 8) {  // a lane a slot
+    for (int t = lane; t < slots; t += 32)
+      if (first + t < capacity && order[first + t] < 0)
+        for (long long u = 0; u < units; ++u) out[(first + t) * ld + u] = zero<U>();
+    return;
+  }
   for (int t = 0; t < slots; t += 32) {
     const long long s = first + t + lane;
     unsigned empty = __ballot_sync(~0u, t + lane < slots && s < capacity && order[s] < 0);

@@ -124,6 +124,37 @@ def test_head(gpu, torch, rows, cols, classes, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, alone))
 
 
+# a handful of rows (a kernel of its own up to 8 or 16 of them), one more than that, and
+# narrow heads (at most 64 columns and 32 classes)
+FEW = [(1, 1024, 3001), (2, 65, 700), (2, 64, 33), (3, 257, 1000), (4, 512, 999), (5, 72, 20_000),
+       (7, 1000, 2049), (8, 2048, 130), (8, 9, 4000), (9, 72, 1500), (11, 100, 350), (16, 1030, 640),
+       (16, 64, 257), (17, 128, 600), (1, 65, 1), (4, 3000, 50), (1, 20_000, 40)]
+NARROW = [(1, 1, 1), (31, 64, 32), (33, 63, 31), (1000, 10, 10), (129, 16, 4), (300, 17, 5),
+          (97, 5, 17), (4000, 32, 12), (200_001, 3, 9), (65, 40, 13), (64, 48, 16)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,cols,classes", FEW + NARROW)
+def test_small_heads(gpu, torch, rows, cols, classes, dtype):
+    for pad in (0, 8, 3):
+        h, w, y, dloss = _inputs(torch, rows, cols, classes, dtype, pad, rows + cols, 0.2)
+        off = (y < 0) | (y >= classes)
+        h[off] = float("nan")
+        dloss[off] = float("nan")
+        loss, lse, dh, dw = _run(gpu, torch, h, w, y, dloss, cols, strided=True)
+        ref = _reference(torch, h, w, y, dloss, cols)
+        assert torch.all(loss[off] == 0) and torch.all(dh[off][:, :cols] == 0)
+        keep = ~off
+        _check(torch, (loss[keep], lse[keep], dh[keep], dw),
+               {k: (v[keep], b[keep]) if k != "dw" else (v, b) for k, (v, b) in ref.items()},
+               cols, f"pad {pad}")
+        assert torch.all(dh[:, cols:] == 7.0) and torch.all(dw[:, cols:] == 7.0)
+        alone = _run(gpu, torch, h, w, y, dloss, cols, want="dh", strided=True)
+        assert torch.equal(alone[2], dh) and torch.all(alone[3] == 7.0)
+        alone = _run(gpu, torch, h, w, y, dloss, cols, want="dw", strided=True)
+        assert torch.equal(alone[3], dw) and torch.all(alone[2] == 7.0)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("want", ["dh", "dw"])
 def test_one_gradient(gpu, torch, dtype, want):

@@ -52,8 +52,8 @@ def test_sort_refuses(core, change, match):
 def test_sort_sizes(core):
     assert core.sort_rows_capacity(10, 2, 4, 4) == 32
     assert core.sort_rows_workspace(0, 1, 4) == 0
-    assert core.sort_rows_workspace(4096, 1, 4) == 0
-    assert core.sort_rows_workspace(4097, 1, 4) > 0
+    assert core.sort_rows_workspace(500, 1, 4) == 0
+    assert core.sort_rows_workspace(10_000_000, 1, 4) > 0
     with pytest.raises(core.MacBoostError):
         core.sort_rows_workspace(10, 5, 4)
 
