@@ -60,11 +60,11 @@ bool in_place(int dtype, const void* p, int64_t ld) {
 }
 
 // Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
-// CTAs gets of `all` tile-blocks in total, so that they end together, and none shorter
-// than 8 blocks (float32: 2, of six products), so that the sums of parts stay few.
+// CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
+// blocks (float32: 2, of six products), so that the sums of parts stay few.
 int splits_for(int64_t kblocks, int64_t all, int dtype) {
-  const int64_t least = dtype == kF32 ? 2 : 8;
-  const int64_t most = std::max(least, all / 74);
+  const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
+  const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
   return int(std::max<int64_t>(1, std::min(parts(kblocks, most), kblocks / least)));
 }
 
@@ -97,7 +97,9 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad
     const int64_t dh_tiles = want_dh ? parts(rows, tm) * tn : 0;
     const int64_t dw_tiles = want_dw ? parts(p.piece, tm) * tn : 0;
     const int64_t dh_blocks = parts(p.piece, kHeadTileK), dw_blocks = parts(rows, kHeadTileK);
-    const int64_t all = dh_tiles * dh_blocks + dw_tiles * dw_blocks;
+    const int64_t steps = dtype == kF32 ? 6 : 1;
+    const int64_t all = dh_tiles * (dh_blocks * steps + kHeadEpilogue) +
+                        dw_tiles * (dw_blocks * steps + kHeadEpilogue);
     p.dh_splits = splits_for(dh_blocks, all, dtype);
     p.dw_splits = splits_for(dw_blocks, all, dtype);
     if (want_dh && p.pieces > 1) p.acc = take(rows * cols * 4);
@@ -439,6 +441,9 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   int64_t launches = o.launches;
   const bool f32 = a.dtype == kF32;
   const int64_t tm = kHeadPair * kHeadTileM;
+  auto four = [&](const void* q, int64_t ld) {
+    return int(aligned(q, size_t(4 * dtype_bytes(a.dtype))) && ld % 4 == 0);
+  };
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, n = std::min(p.piece, a.classes - v0);
     HeadLaunch l{};
@@ -477,6 +482,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
       dh.out = a.dh;
       dh.ld_out = a.ld_dh;
       dh.out_f32 = f32;
+      dh.wide = four(a.dh, a.ld_dh);
       float* acc = p.pieces > 1 ? reinterpret_cast<float*>(base + p.acc) : nullptr;
       const int in = i > 0, last = i + 1 == p.pieces;
       if (dh.splits > 1) {
@@ -502,6 +508,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
       dw.out = static_cast<char*>(a.dw) + v0 * a.ld_dw * dtype_bytes(a.dtype);
       dw.ld_out = a.ld_dw;
       dw.out_f32 = f32;
+      dw.wide = four(dw.out, a.ld_dw);
       dw.final = 1;
       if (dw.splits > 1) {
         dw.acc = reinterpret_cast<float*>(base + p.dw_part);

@@ -47,7 +47,7 @@ constexpr int kHeadTileM = 128;      // accumulator rows a CTA (TMEM lanes)
 constexpr int kHeadTileN = 256;      // accumulator columns
 constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit values
 constexpr int kHeadPair = 2;         // CTAs that share a tile
-constexpr int kHeadChunk = 4;        // float32: K blocks of one sum of the tensor core
+constexpr int kHeadEpilogue = 12;    // a tile's epilogue, in steps of one K block
 
 // One product C = A B^T over K, as tiles.  Operands are 16-bit values in `planes`
 // planes (the terms of a float32, or the value itself) behind tensor maps of
@@ -69,6 +69,7 @@ struct HeadJob {
   void* out;
   long long ld_out;
   int out_f32;
+  int wide;                          // rows of out start on four values
 };
 
 struct HeadRows {                    // what the logits' epilogues know of each row

@@ -4,16 +4,18 @@
 // head_kernel: a persistent kernel, a pair of CTAs a 256 x 256 tile (tcgen05.mma,
 // cta_group::2: each CTA holds 128 rows of A and half of B in shared memory and 128 x
 // 256 float32 sums in its tensor memory).  Warp 0 fetches 128-byte swizzled tiles with
-// TMA into a ring, warp 1 of the first CTA issues the products, warps 2 to 9 take the
+// TMA into a ring, warp 1 of the first CTA issues the products, warps 4 to 11 take the
 // sums out of tensor memory, 32 rows and half the columns each, while the next tile
 // fills the second half of it.
 //
 // A float32 operand is three planes of bfloat16, x = x1 + x2 + x3 with 8 bits each, and
 // the product the six terms x_i y_j with i + j <= 4 -- what is dropped is below 2^-24
 // of |x||y|.  The tensor core's sums are truncated to 32 bits at every step, so they run
-// over kHeadChunk blocks of K only, the smallest terms first (they cost little while the
-// sum is small), and the epilogue adds the chunks up in registers, rounded to nearest.
-// With whole sums in the tensor core, dh of 26 x 12 x 7,798 was off by 2.5e-6.
+// over one block of 64 of K only, the smallest terms first (they cost little while the sum
+// is small), and the epilogue adds the blocks up in registers, rounded to nearest.  With
+// whole sums in the tensor core, dh of 26 x 12 x 7,798 was off by 2.5e-6.  A stage of the
+// ring holds all three planes of both operands, so a block of K is fetched once for its
+// six products.
 //
 // Every wait ends after wait_ns: the CTA then marks itself dead, sets the status word,
 // lets its copies land and returns (its results are void).
@@ -31,7 +33,7 @@ namespace mb {
 namespace {
 
 constexpr int kEpilogueWarps = 8;
-constexpr int kHeadThreads = 64 + kEpilogueWarps * 32;
+constexpr int kHeadThreads = 128 + kEpilogueWarps * 32;  // three warpgroups
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- PTX ------------------------------------------------------------------------
@@ -151,6 +153,18 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -179,6 +193,10 @@ struct Walk {
   const HeadLaunch& a;
   int pairs, me, step = 0;
   int count[2], extra, light, bonus;
+  // a tile's time in steps of one K block
+  __device__ int weight(const HeadJob& q) const {
+    return (q.kblocks + q.splits - 1) / q.splits * (a.f32 ? 6 : 1) + kHeadEpilogue;
+  }
   __device__ Walk(const HeadLaunch& l) : a(l) {
     pairs = int(gridDim.x) / kHeadPair;
     me = int(blockIdx.x) / kHeadPair;
@@ -187,9 +205,8 @@ struct Walk {
     light = count[0] % pairs;  // pairs from here on have one tile of job 0 fewer
     extra = 0;
     if (a.jobs > 1 && light > 0) {
-      const int c0 = (a.job[0].kblocks + a.job[0].splits - 1) / a.job[0].splits;
-      const int c1 = (a.job[1].kblocks + a.job[1].splits - 1) / a.job[1].splits;
-      extra = c1 > 0 ? (c0 + c1 / 2) / c1 : 0;
+      const int c0 = weight(a.job[0]), c1 = weight(a.job[1]);
+      extra = (c0 + c1 / 2) / c1;
       const int most = count[1] / (pairs - light);
       if (extra > most) extra = most;
     }
@@ -263,27 +280,49 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// 32 values of one row to bfloat16, n of them (16-byte stores when the row allows it).
-__device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const float (&v)[32], int n) {
-  if (n >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+// A warp's 32 rows x 32 columns, a row a lane, to four rows at a time with eight lanes a
+// row: f(row, column, four values) then reads and writes global memory in whole sectors.
+// A row of the 4 KB buffer is eight 16-byte units, at positions permuted by the row, so
+// that both directions are free of bank conflicts.
+constexpr int kTurnBytes = 32 * 32 * 4;
+template <class F>
+__device__ __forceinline__ void turn(uint32_t buf, const float (&v)[32], int lane, F f) {
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      *reinterpret_cast<uint4*>(p + i) = make_uint4(pack2(v[i], v[i + 1]), pack2(v[i + 2], v[i + 3]),
-                                                    pack2(v[i + 4], v[i + 5]), pack2(v[i + 6], v[i + 7]));
+  for (int u = 0; u < 8; ++u)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)),
+                 "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
+                 : "memory");
+  __syncwarp();
+#pragma unroll 2
+  for (int i = 0; i < 8; ++i) {
+    const int row = i * 4 + lane / 8, u = lane % 8;
+    float4 x;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(buf + row * 128 + ((u ^ (row & 7)) << 4)));
+    f(row, 4 * u, x);
+  }
+}
+
+// Four adjacent values to memory; `n` of them exist, `wide`: p is aligned for all four.
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x, int n, bool wide) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
   } else {
+    const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 4; ++i)
       if (i < n) p[i] = __float2bfloat16_rn(v[i]);
   }
 }
-__device__ __forceinline__ void store_f32(float* p, const float (&v)[32], int n) {
-  if (n >= 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 4)
-      *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+__device__ __forceinline__ void store4(float* p, float4 x, int n, bool wide) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<float4*>(p) = x;
   } else {
+    const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 4; ++i)
       if (i < n) p[i] = v[i];
   }
 }
@@ -291,9 +330,10 @@ __device__ __forceinline__ void store_f32(float* p, const float (&v)[32], int n)
 template <int EPI, int TN, bool F32>
 __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads, 1)
     head_kernel(const __grid_constant__ HeadLaunch a) {
-  constexpr int kBytesA = kHeadTileM * 128;
+  constexpr int kPlanes = F32 ? 3 : 1;
+  constexpr int kBytesA = kHeadTileM * 128;           // of a plane
   constexpr int kBytesB = TN / kHeadPair * 128;
-  constexpr int kStage = kBytesA + kBytesB;
+  constexpr int kStage = kPlanes * (kBytesA + kBytesB);
   constexpr int kStages = (192 * 1024) / kStage;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bars[2 * kStages + 4];
@@ -331,9 +371,14 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
   // products of planes, small ones first; a single plane is the last of them
-  const int kPlaneA[6] = {2, 1, 0, 1, 0, 0};
-  const int kPlaneB[6] = {0, 1, 2, 0, 1, 0};
+  constexpr int kPlaneA[6] = {2, 1, 0, 1, 0, 0};
+  constexpr int kPlaneB[6] = {0, 1, 2, 0, 1, 0};
 
+  // float32: the epilogue keeps 128 sums a thread.  384 threads are launched with 168
+  // registers each (64,512); the first warpgroup keeps 56 a thread and the other two get
+  // 224: 128 x 56 + 256 x 224 = 64,512.
+  if (warp < 4) {
+  if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0) {
     if (lane == 0) {
       Walk walk(a);
@@ -358,47 +403,41 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
                         : n0 < q.N ? q.b_box * 128 : 0;
         };
         const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
-        const uint32_t bytes = uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
+        const uint32_t bytes = kPlanes * uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
                                         bytes_b(n0 + TN / kHeadPair));
         // Each tile starts at another K block: tiles that run together would read the same
         // 128 bytes of every row, which are few of the memory's channels.
         const int turn = (t.m + t.n) % (k1 - k0);
-        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0)
-          for (int p = F32 ? 0 : 5; ok && p < 6; ++p)
-          for (int i = c0; i < (F32 ? min(c0 + kHeadChunk, k1) : k1); ++i) {
-            const int kb = i + turn < k1 ? i + turn : i + turn - (k1 - k0);
-            ok = wait(empty + 8 * s, ph ^ 1);
-            if (!ok) break;
-            if (rank == 0) bar_expect(full + 8 * s, bytes);
-            const uint32_t sa = ring + s * kStage, sb = sa + kBytesA, bar = full + 8 * s;
-            if (++s == kStages) {
-              s = 0;
-              ph ^= 1;
-            }
-            if (a.stall) continue;
-            const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
-            int pa = 0, pb = 0;
-#pragma unroll
-            for (int z = 0; z < 6; ++z)
-              if (z == p) {
-                pa = kPlaneA[z];
-                pb = kPlaneB[z];
-              }
+        for (int i = k0; i < k1; ++i) {
+          const int kb = i + turn < k1 ? i + turn : i + turn - (k1 - k0);
+          ok = wait(empty + 8 * s, ph ^ 1);
+          if (!ok) break;
+          if (rank == 0) bar_expect(full + 8 * s, bytes);
+          const uint32_t bar = full + 8 * s;
+          uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
+          if (++s == kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (a.stall) continue;
+          const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
+          for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
             if (q.a_mn) {
 #pragma unroll
-              for (int i = 0; i < kHeadTileM / 64; ++i)
-                if (am + 64 * i < q.M) tma_load(sa + i * 8192, &q.a, q.a_row0 + am + 64 * i, ka, pa, bar);
+              for (int j = 0; j < kHeadTileM / 64; ++j)
+                if (am + 64 * j < q.M) tma_load(sa + j * 8192, &q.a, q.a_row0 + am + 64 * j, ka, z, bar);
             } else if (am < q.M) {
-              tma_load(sa, &q.a, ka, q.a_row0 + am, pa, bar);
+              tma_load(sa, &q.a, ka, q.a_row0 + am, z, bar);
             }
             if (q.b_mn) {
 #pragma unroll
-              for (int i = 0; i < TN / kHeadPair / 64; ++i)
-                if (bn + 64 * i < q.N) tma_load(sb + i * 8192, &q.b, q.b_row0 + bn + 64 * i, kk, pb, bar);
+              for (int j = 0; j < TN / kHeadPair / 64; ++j)
+                if (bn + 64 * j < q.N) tma_load(sb + j * 8192, &q.b, q.b_row0 + bn + 64 * j, kk, z, bar);
             } else if (bn < q.N) {
-              tma_load(sb, &q.b, kk, q.b_row0 + bn, pb, bar);
+              tma_load(sb, &q.b, kk, q.b_row0 + bn, z, bar);
             }
           }
+        }
       }
       if (!ok) {  // copies in flight land before the shared memory is given up
         const uint64_t t0 = now_ns();
@@ -421,22 +460,25 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
                                (uint32_t(q.b_mn) << 16) | (uint32_t(TN / 8) << 17) |
                                (uint32_t(kHeadPair * kHeadTileM / 16) << 24);
         const uint32_t step_a = q.a_mn ? 2048 / 16 : 32 / 16, step_b = q.b_mn ? 2048 / 16 : 32 / 16;
-        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0) {
+        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? 1 : k1 - k0) {
           ok = wait(sums_empty + 8 * as, aph ^ 1);
           if (!ok) break;
           fence_after();
           bool add = false;
-          const int steps = F32 ? 6 * (min(c0 + kHeadChunk, k1) - c0) : k1 - k0;
-          for (int i = 0; i < steps; ++i) {
+          for (int i = 0; i < (F32 ? 1 : k1 - k0); ++i) {
             ok = wait(full + 8 * s, ph);
             if (!ok) break;
             fence_after();
-            const uint64_t da = descriptor(ring + s * kStage, q.a_mn);
-            const uint64_t db = descriptor(ring + s * kStage + kBytesA, q.b_mn);
+            const uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
 #pragma unroll
-            for (int k = 0; k < kHeadTileK / 16; ++k) {
-              mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
-              add = true;
+            for (int p = F32 ? 0 : 5; p < 6; ++p) {
+              const uint64_t da = descriptor(sa + (F32 ? kPlaneA[p] : 0) * kBytesA, q.a_mn);
+              const uint64_t db = descriptor(sb + (F32 ? kPlaneB[p] : 0) * kBytesB, q.b_mn);
+#pragma unroll
+              for (int k = 0; k < kHeadTileK / 16; ++k) {
+                mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
+                add = true;
+              }
             }
             commit_both(empty + 8 * s);
             if (++s == kStages) {
@@ -450,12 +492,15 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         }
       }
     }
+  }
   } else {
+    if constexpr (F32) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     Walk walk(a);
     Tile t;
     int as = 0, aph = 0;
-    const int quarter = warp % 4, half = (warp - 2) / 4;
+    const int quarter = warp % 4, half = warp / 4 - 1;
     const HeadRows& r = a.r;
+    const uint32_t stage = ring + kStages * kStage + (warp - 4) * kTurnBytes;
     // this thread's row of the tile's half: chunks of sums added up (float32)
     float sums[F32 ? TN / 2 : 1];
     while (walk.next(&t)) {
@@ -464,18 +509,18 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       walk.blocks(t, &k0, &k1);
       bool ok = true;
       uint32_t src = 0;
-      for (int c0 = k0; c0 < k1; c0 += F32 ? kHeadChunk : k1 - k0) {
+      for (int c0 = k0; c0 < k1; c0 += F32 ? 1 : k1 - k0) {
         ok = __all_sync(~0u, wait(sums_full + 8 * as, aph));
         if (!ok) break;
         fence_after();
         src = tmem + as * TN + (uint32_t(quarter * 32) << 16) + half * (TN / 2);
         if constexpr (F32) {
 #pragma unroll
-          for (int c = 0; c < TN / 2; c += 32) {
-            float v[32];
-            tmem_load(src + c, v);
+          for (int c = 0; c < TN / 2; c += 16) {
+            float v[16];
+            tmem_load16(src + c, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sums[c + i] = c0 == k0 ? v[i] : sums[c + i] + v[i];
+            for (int i = 0; i < 16; ++i) sums[c + i] = c0 == k0 ? v[i] : sums[c + i] + v[i];
           }
           fence_before();
           __syncwarp();
@@ -494,14 +539,23 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           tmem_load(src + c, v);
         }
       };
+      // f for each 32 columns: sums in registers want their place known to the compiler
+      auto each_part = [&](auto f) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int c = 0; c < TN / 2; c += 32) f(c);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < TN / 2; c += 32) f(c);
+        }
+      };
       const int row = (t.m * kHeadPair + int(rank)) * kHeadTileM + quarter * 32 + lane;
       const int col0 = t.n * TN + half * (TN / 2);
       if (EPI == kHeadLse) {
         const bool there = row < r.rows;
         const int y = there ? r.labels[row] : -1;
         float m = -INFINITY, sum = 0.f;
-#pragma unroll(F32 ? 4 : 1)
-        for (int c = 0; c < TN / 2; c += 32) {
+        each_part([&](int c) {
           float v[32];
           take(c, v);
           const int n = r.classes - (col0 + c);
@@ -513,7 +567,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
               if (col0 + c + i == y) x = v[i];
             r.target[row] = x;
           }
-        }
+        });
         if (there) r.part[(long long)(t.n * 2 + half) * r.rows + row] = make_float2(m, sum);
       } else if (EPI == kHeadG) {
         const bool there = row < r.rows;
@@ -521,9 +575,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         const bool known = unsigned(y) < unsigned(r.classes);
         const float lse = there ? r.lse[row] : 0.f;
         const float up = known ? r.dloss[row] : 0.f;
-        __nv_bfloat16* g = static_cast<__nv_bfloat16*>(r.g) + (long long)row * r.ld_g + col0;
-#pragma unroll(F32 ? 4 : 1)
-        for (int c = 0; c < TN / 2; c += 32) {
+        // lanes past the last row hold zeros, which are not stored
+        __nv_bfloat16* g = static_cast<__nv_bfloat16*>(r.g) + (long long)(row - lane) * r.ld_g + col0;
+        const int rows = r.rows - (row - lane);
+        each_part([&](int c) {
           float v[32];
           take(c, v);
           const int v0 = r.v0 + col0 + c;
@@ -533,41 +588,52 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             if (v0 + i == y) p -= 1.f;
             v[i] = known && v0 + i < r.classes ? up * p : 0.f;
           }
-          const int n = int(r.ld_g) - (col0 + c);
-          if (there && n > 0) {
-            store_bf16(g + c, v, n);
+          const int n = int(r.ld_g) - (col0 + c);  // a multiple of 32
+          turn(stage, v, lane, [&](int rr, int cc, float4 x) {
+            if (rr >= rows || n <= 0) return;
+            __nv_bfloat16* p = g + rr * r.ld_g + c + cc;
+            store4(p, x, 4, true);
             if constexpr (F32) {
+              auto rest = [](float f) { return f - __bfloat162float(__float2bfloat16_rn(f)); };
 #pragma unroll
               for (int z = 1; z < 3; ++z) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
-                store_bf16(g + c + z * r.plane_g, v, n);
+                x = make_float4(rest(x.x), rest(x.y), rest(x.z), rest(x.w));
+                store4(p + z * r.plane_g, x, 4, true);
               }
             }
-          }
-        }
+          });
+        });
       } else {
-        const bool there = row < q.M;
-        float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row) * q.N + col0 : nullptr;
-#pragma unroll(F32 ? 4 : 1)
-        for (int c = 0; c < TN / 2; c += 32) {
+        const int row0 = row - lane, rows = q.M - row0;
+        float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row0) * q.N + col0 : nullptr;
+        const bool wide_acc = q.N % 4 == 0;  // its base is aligned
+        each_part([&](int c) {
           float v[32];
           take(c, v);
-          const int n = q.N - (col0 + c);
-          if (!there || n <= 0) continue;
-          if (q.acc_in) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < n) v[i] += acc[c + i];
-          }
-          if (!q.final) {
-            store_f32(acc + c, v, n);
-          } else if (q.out_f32) {
-            store_f32(static_cast<float*>(q.out) + (long long)row * q.ld_out + col0 + c, v, n);
-          } else {
-            store_bf16(static_cast<__nv_bfloat16*>(q.out) + (long long)row * q.ld_out + col0 + c, v, n);
-          }
-        }
+          turn(stage, v, lane, [&](int rr, int cc, float4 x) {
+            const int n = q.N - (col0 + c + cc);
+            if (rr >= rows || n <= 0) return;
+            float* sum = acc + (long long)rr * q.N + c + cc;
+            if (q.acc_in) {
+              if (wide_acc) {
+                const float4 o = *reinterpret_cast<const float4*>(sum);
+                x = make_float4(x.x + o.x, x.y + o.y, x.z + o.z, x.w + o.w);
+              } else {
+                x.x += sum[0];
+                if (n > 1) x.y += sum[1];
+                if (n > 2) x.z += sum[2];
+                if (n > 3) x.w += sum[3];
+              }
+            }
+            const long long at = (long long)(row0 + rr) * q.ld_out + col0 + c + cc;
+            if (!q.final)
+              store4(sum, x, n, wide_acc);
+            else if (q.out_f32)
+              store4(static_cast<float*>(q.out) + at, x, n, q.wide);
+            else
+              store4(static_cast<__nv_bfloat16*>(q.out) + at, x, n, q.wide);
+          });
+        });
       }
       if constexpr (!F32) {
         fence_before();
@@ -1315,8 +1381,9 @@ cudaError_t few_rows(const Few& a, bool grad, int blocks, int chunks, cudaStream
 
 template <int EPI, int TN, bool F32>
 cudaError_t go_type(const HeadLaunch& a, cudaStream_t s) {
-  constexpr int kStage = kHeadTileM * 128 + TN / kHeadPair * 128;
-  constexpr size_t smem = size_t((192 * 1024) / kStage) * kStage + 1024;
+  constexpr int kStage = (F32 ? 3 : 1) * (kHeadTileM * 128 + TN / kHeadPair * 128);
+  constexpr size_t smem = size_t((192 * 1024) / kStage) * kStage + 1024 +
+                          (EPI == kHeadLse ? 0 : kEpilogueWarps * kTurnBytes);
   const cudaError_t e = cudaFuncSetAttribute(head_kernel<EPI, TN, F32>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
