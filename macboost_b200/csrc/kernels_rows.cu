@@ -431,8 +431,9 @@ constexpr long long kRunEntries = 65536;
 // groups their entries by model once -- as the sort does, the model of a slot found by
 // bisection of the offsets -- and keeps the list (16 entries a thread) for `per` columns:
 // each column's values come in with adjacent loads, and leave in runs of adjacent slots.
-// A thread a slot would read a 32-byte sector of x for each 4-byte value.  Blocks from
-// `tiles` on clear the empty slots.
+// A thread a slot would read a 32-byte sector of x for each 4-byte value (10M x 28 among
+// 8: 1,392 us, here 457, 77% of copy speed; tiles of 2,048 took 555 and of 8,192, with
+// twice the threads, 510).  Blocks from `tiles` on clear the empty slots.
 template <class T>
 __global__ void __launch_bounds__(kSortThreads, 3)
     gather_runs_kernel(const GatherArgs a, int tile_rows, long long tiles, long long per) {
