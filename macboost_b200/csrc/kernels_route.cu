@@ -54,14 +54,15 @@ __device__ __forceinline__ void each_value(int nr, int E, int lane, F f) {
   }
 }
 
-// Rows of L x V logits at most; E: their number when a lane has a row (L = 1), else 0.
-template <int L, int V, int E1>
+// Rows of L x V logits at most; E1: their number when a lane has a row (L = 1), else 0; K:
+// choices of a lane's row that stay in registers, else 0.
+template <int L, int V, int E1, int K>
 __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
     route_kernel(const RouteArgs a) {
   constexpr int R = 32 / L;             // rows a warp
   __shared__ float tile[kWarps][E1 ? 32 * (E1 | 1) : kTile];
   // the choices, written out together: k <= E1, else k <= min(16 L, 32)
-  constexpr int kChoices = E1 ? 32 * E1 : R * 32;
+  constexpr int kChoices = K ? 1 : E1 ? 32 * E1 : R * 32;
   __shared__ int s_id[kWarps][kChoices];
   __shared__ float s_e[kWarps][kChoices];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
   const long long row0 = (long long)(blockIdx.x * (long long)kWarps + warp) * R;
   if (row0 >= a.rows) return;           // whole warps only: no block barrier below
   const int nr = int(a.rows - row0 < R ? a.rows - row0 : R);
-  const int E = E1 ? E1 : a.experts, k = a.k;
+  const int E = E1 ? E1 : a.experts, k = K ? K : a.k;
   float* t = tile[warp];
   const int sp = E | 1;
   if (E1 && nr == 32 && a.ld == E1) {
@@ -94,7 +95,10 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
     v[i] = e < E && r < nr ? t[r * sp + e] : -INFINITY;
   }
   float top = 0.f, total = 0.f;
-  for (int j = 0; j < k; ++j) {
+  int my_id[K ? K : 1];
+  float my_e[K ? K : 1];
+#pragma unroll
+  for (int j = 0; j < (K ? K : k); ++j) {
     // NaN is never greater, so it is never chosen
     float best = -INFINITY;
     int at = 0;
@@ -126,7 +130,10 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
     }
     const float e = expf(best - top);   // 0 for -inf
     if (a.norm == kRouteChosen) total += e;
-    if (sub == 0) {
+    if constexpr (K > 0) {
+      my_id[j] = found ? id : -1;
+      my_e[j] = e;
+    } else if (sub == 0) {
       s_id[warp][r * k + j] = found ? id : -1;
       s_e[warp][r * k + j] = e;
     }
@@ -136,9 +143,23 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
         if (i * L + sub == id) v[i] = -INFINITY;
     }
   }
+  const float over = total > 0.f || total != total ? total : 1.f;
+  if constexpr (K > 0) {
+    // one store of K values a lane
+    if (r < nr) {
+      const long long at = (row0 + r) * K;
+      if constexpr (K == 2) {
+        *reinterpret_cast<int2*>(a.ids + at) = make_int2(my_id[0], my_id[1]);
+        *reinterpret_cast<float2*>(a.weights + at) = make_float2(my_e[0] / over, my_e[1] / over);
+      } else {
+        a.ids[at] = my_id[0];
+        a.weights[at] = my_e[0] / over;
+      }
+    }
+    return;
+  }
   // the group's lanes divide their row's choices by the same total
   __syncwarp();
-  const float over = total > 0.f || total != total ? total : 1.f;
   for (int j = sub; j < k; j += L) s_e[warp][r * k + j] = s_e[warp][r * k + j] / over;
   __syncwarp();
   int* ids = a.ids + row0 * k;
@@ -236,12 +257,12 @@ __device__ __forceinline__ void choice(const RouteArgs& a, long long row, int j,
 }
 
 // Rows of up to 64 logits: 32 rows a warp when E <= 16 (E1 = E), 16 or 8 above, one
-// lane a row, through the warp's tile.
-template <int E1>
+// lane a row, through the warp's tile; K as above.
+template <int E1, int K>
 __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const RouteArgs a) {
   __shared__ float tile[kWarps][E1 ? 32 * (E1 | 1) : kTile];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int E = E1 ? E1 : a.experts, k = a.k, sp = E | 1;
+  const int E = E1 ? E1 : a.experts, k = K ? K : a.k, sp = E | 1;
   const int R = E1 ? 32 : E <= 32 ? 16 : 8;
   const long long row0 = (long long)(blockIdx.x * (long long)kWarps + warp) * R;
   if (row0 >= a.rows) return;
@@ -255,15 +276,34 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const Ro
     float* mine = t + lane * sp;
     float mean = 0.f, w0 = 0.f;
     int id0 = -1;
-    for (int j = 0; j < k; ++j) {
-      int id;
-      float w, dw;
-      choice(a, row, j, &id, &w, &dw);
+    int ids[K ? K : 1];
+    float w[K ? K : 1], dw[K ? K : 1];
+    if constexpr (K == 2) {
+      const int2 i2 = *reinterpret_cast<const int2*>(a.ids + row * 2);
+      const float2 w2 = *reinterpret_cast<const float2*>(a.weights + row * 2);
+      const float2 d2 = *reinterpret_cast<const float2*>(a.dweights + row * 2);
+      ids[0] = i2.x, ids[1] = i2.y;
+      w[0] = w2.x, w[1] = w2.y;
+      dw[0] = d2.x, dw[1] = d2.y;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (unsigned(ids[j]) >= unsigned(E)) {
+          ids[j] = -1;
+          w[j] = dw[j] = 0.f;
+        }
+    } else if constexpr (K == 1) {
+      choice(a, row, 0, &ids[0], &w[0], &dw[0]);
+    }
+#pragma unroll
+    for (int j = 0; j < (K ? K : k); ++j) {
+      constexpr int one = 0;
+      const int at = K ? j : one;
+      if (!K) choice(a, row, j, &ids[at], &w[at], &dw[at]);
       if (j == 0) {
-        id0 = id;
-        w0 = w;
+        id0 = ids[at];
+        w0 = w[at];
       }
-      mean += w * dw;
+      mean += w[at] * dw[at];
     }
     if (a.norm == kRouteAll && id0 >= 0) {
       const float l0 = mine[id0];
@@ -273,11 +313,11 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_narrow_kernel(const Ro
 #pragma unroll
       for (int e = 0; e < (E1 ? E1 : E); ++e) mine[e] = 0.f;
     }
-    for (int j = 0; j < k; ++j) {
-      int id;
-      float w, dw;
-      choice(a, row, j, &id, &w, &dw);
-      if (id >= 0) mine[id] = w * (dw - mean);
+#pragma unroll
+    for (int j = 0; j < (K ? K : k); ++j) {
+      const int at = K ? j : 0;
+      if (!K) choice(a, row, j, &ids[at], &w[at], &dw[at]);
+      if (ids[at] >= 0) mine[ids[at]] = w[at] * (dw[at] - mean);
     }
   }
   __syncwarp();
@@ -335,17 +375,30 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteArgs
 
 unsigned blocks_for(long long rows, int per) { return unsigned((rows + per - 1) / per); }
 
-template <int L, int V, int E1>
-cudaError_t go(const RouteArgs& a, bool grad, cudaStream_t s) {
+template <int L, int V, int E1, int K>
+cudaError_t go_k(const RouteArgs& a, bool grad, cudaStream_t s) {
   // at least 32 rows a block and below 2^31 rows: the grid fits
-  const unsigned blocks = blocks_for(a.rows, kWarps * (32 / L));
   if (grad) {
     const int R = E1 ? 32 : a.experts <= 32 ? 16 : 8;
-    route_grad_narrow_kernel<E1><<<blocks_for(a.rows, kWarps * R), kWarps * 32, 0, s>>>(a);
+    route_grad_narrow_kernel<E1, K><<<blocks_for(a.rows, kWarps * R), kWarps * 32, 0, s>>>(a);
   } else {
-    route_kernel<L, V, E1><<<blocks, kWarps * 32, 0, s>>>(a);
+    route_kernel<L, V, E1, K><<<blocks_for(a.rows, kWarps * (32 / L)), kWarps * 32, 0, s>>>(a);
   }
   return cudaGetLastError();
+}
+
+template <int L, int V, int E1>
+cudaError_t go(const RouteArgs& a, bool grad, cudaStream_t s) {
+  if constexpr (E1 > 0) {
+    if (a.k == 1) return go_k<L, V, E1, 1>(a, grad, s);
+    // two choices by one 8-byte access, where the arrays start on 8 bytes
+    if constexpr (E1 > 1) {
+      const auto at = reinterpret_cast<uintptr_t>(a.ids) | reinterpret_cast<uintptr_t>(a.weights) |
+                      reinterpret_cast<uintptr_t>(a.dweights);
+      if (a.k == 2 && at % 8 == 0) return go_k<L, V, E1, 2>(a, grad, s);
+    }
+  }
+  return go_k<L, V, E1, 0>(a, grad, s);
 }
 
 template <int V>
