@@ -355,16 +355,18 @@ __global__ void __launch_bounds__(kThreads)
 // several tiles a multiprocessor are in flight; then a lane a slot takes 16 bytes and
 // writes its values to their columns, 64 consecutive slots each.  Rows of the tile are an
 // odd number of units apart, which makes the 16-byte reads of 8 slots free of bank
-// conflicts.  Rows with k choices are read k times; blocks that walked the segments side
-// by side, to find the second reading in the L2 cache, took 250 us where this takes 131
-// (500,000 x 100 rows to two of 64), since a block's tiles then follow one another.
+// conflicts.  Rows with k choices are read k times.  Walking the segments side by side, to
+// find the second reading in the L2 cache, cost more than it saved (500,000 x 100 rows to
+// two of 64: 131 us here; 250 with a block walking a window of all segments, 166 with
+// blocks in the order of their tiles' place in the segments): the writes then go to 64
+// places at once.
 constexpr int kUnitSlots = 64, kMaxQuads = 32;
 template <class T>
 __global__ void __launch_bounds__(kThreads)
     gather_units_kernel(const T* x, long long entries, int units, long long ld, int k,
                         const int* order, long long capacity, T* out, long long ld_out, int quads) {
   constexpr int PER = 16 / int(sizeof(T));
-  __shared__ uint4 tile[kUnitSlots * (kMaxQuads + 1)];
+  extern __shared__ uint4 tile[];  // kUnitSlots rows of `pitch`
   const long long s0 = (long long)blockIdx.x * kUnitSlots;
   const int q0 = int(blockIdx.y) * quads;
   const int nq = min(quads, units - q0), pitch = nq | 1;
@@ -633,9 +635,12 @@ __device__ __forceinline__ void load_choices(const CombineArgs& a, const Lay& l,
     }
 }
 
-// K choices a row, or any number (K = 0).  FLIGHT groups of rows a warp at once.
+// K choices a row, or any number (K = 0).  FLIGHT groups of rows a warp at once.  Narrow
+// rows wait for memory: 1M x 10 of two models took 89 us, with the gradient, at 4 blocks a
+// multiprocessor and 82 at 8 and 6 (the gradient); four groups a warp, 96.
 template <class T, int BYTES, int K>
-__global__ void __launch_bounds__(kThreads) combine_kernel(const CombineArgs a, const Lay l) {
+__global__ void __launch_bounds__(kThreads, K == 1 || K == 2 ? 8 : 1)
+    combine_kernel(const CombineArgs a, const Lay l) {
   using U = typename Unit<BYTES>::T;
   using W = Values<T, BYTES>;
   constexpr int FLIGHT = K == 1 ? 4 : K == 2 ? 2 : 1;
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const CombineArgs a, 
 }
 
 template <class T, int BYTES, int K>
-__global__ void __launch_bounds__(kThreads, K == 8 ? 2 : 4)
+__global__ void __launch_bounds__(kThreads, K == 8 ? 2 : 6)
     combine_grad_kernel(const CombineArgs a, const Lay l, unsigned row_blocks) {
   using U = typename Unit<BYTES>::T;
   using W = Values<T, BYTES>;
@@ -854,7 +859,8 @@ cudaError_t gather_tiles(const GatherArgs& a, cudaStream_t s) {
     const long long parts = (units + quads - 1) / quads;
     quads = (units + parts - 1) / parts;
     if (parts > 65535) return cudaErrorInvalidValue;
-    gather_units_kernel<T><<<dim3(unsigned(tiles), unsigned(parts)), kThreads, 0, s>>>(
+    const size_t smem = size_t(kUnitSlots) * size_t(quads | 1) * 16;  // at most 33 KB
+    gather_units_kernel<T><<<dim3(unsigned(tiles), unsigned(parts)), kThreads, smem, s>>>(
         x, entries, int(units), a.ld, a.k, a.order, a.capacity, out, a.ld_out, int(quads));
     return cudaGetLastError();
   }

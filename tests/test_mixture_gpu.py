@@ -236,6 +236,32 @@ def test_gather(gpu, torch, rows, cols, k, experts, align, pad, source, target, 
     assert torch.all((out[:, cols:] if target else out[:, cap:]) == 7.0)
 
 
+@pytest.mark.parametrize("rows,cols,k,experts,align,kind", [
+    (200_001, 96, 2, 64, 4, "even"), (180_000, 100, 3, 7, 1, "uneven"), (17_000, 1_000, 2, 255, 4, "uneven"),
+    (17_000, 1_000, 2, 256, 1, "uneven"), (170_000, 100, 2, 40, 4, "one"), (170_000, 100, 8, 200, 4, "bad")])
+def test_gather_of_more_than_the_cache(gpu, torch, rows, cols, k, experts, align, kind):
+    """Large row-major inputs with several choices, laid out feature-major: tiles run in
+    the order of their place in the segments."""
+    core = gpu
+    r = np.random.default_rng(rows + experts)
+    u = r.random((rows, k))
+    ids = (u ** (3 if kind == "uneven" else 1) * experts).astype(np.int64)
+    if kind == "one":
+        ids[:] = 3
+        ids[::1000, 0] = 39
+    if kind == "bad":
+        ids[r.random(ids.shape) < 0.4] = -1
+    offsets, counts, order, slots = sort_on_gpu(core, torch, ids, experts, align)
+    cap = order.numel()
+    x = torch.randn((rows, cols), device="cuda")
+    out = torch.full((cols, cap), 7.0, device="cuda")
+    core.gather_rows_device(0, core.F32, x.data_ptr(), rows, cols, cols, 1, k, experts,
+                            offsets.data_ptr(), order.data_ptr(), slots.data_ptr(), cap,
+                            out.data_ptr(), cap, 0, stream=_stream(torch))
+    want = torch.where((order >= 0)[:, None], x[torch.clamp(order.long(), min=0) // k], 0.0)
+    assert torch.equal(out, want.t())
+
+
 # ---- combine -------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", TYPES)
