@@ -65,7 +65,8 @@ bool in_place(int dtype, const void* p, int64_t ld) {
 int splits_for(int64_t kblocks, int64_t all, int dtype) {
   const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
   const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
-  return int(std::max<int64_t>(1, std::min(parts(kblocks, most), kblocks / least)));
+  // (kblocks, at most 2^24, times parts stays below 2^31)
+  return int(std::max<int64_t>(1, std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100)));
 }
 
 Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool pack_h,
@@ -322,7 +323,9 @@ int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, 
   j.splits = 1;
   j.kblocks = int(parts(a.cols, kHeadTileK));
   j.group = int(std::max<int64_t>(1, kGroupBytes / (kHeadPair * kHeadTileM * a.cols * 2 * p.planes)));
+  j.group = std::min(j.group, j.tiles_m);
   j.b_row0 = int(v0);
+  j.divide();
   return 0;
 }
 
@@ -516,7 +519,11 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
         red[reds++] = HeadReduce{dw.acc, dw.splits, n, a.cols, nullptr, 0, 1, dw.out, a.ld_dw, f32};
       }
     }
-    for (HeadJob* j : {&dh, &dw}) j->group = 16;
+    for (HeadJob* j : {&dh, &dw})
+      if (j->tiles_m > 0) {
+        j->group = std::min(16, j->tiles_m);
+        j->divide();
+      }
     // the heavier tiles first
     const bool dw_first = !a.dh || (a.dw && dw.kblocks / dw.splits > dh.kblocks / dh.splits);
     if (a.dh && a.dw) {

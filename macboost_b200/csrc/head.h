@@ -49,6 +49,25 @@ constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit value
 constexpr int kHeadPair = 2;         // CTAs that share a tile
 constexpr int kHeadEpilogue = 12;    // a tile's epilogue, in steps of one K block
 
+// Division of numbers below 2^31 by a constant: with p = 31 + ceil(log2 d) and m = ceil(2^p
+// / d), n / d is n m >> p.  A tile's place takes four divisions, and a role that has to
+// divide in full between tiles leaves the tensor cores waiting for about a microsecond.
+struct HeadDiv {
+  unsigned d, m, s;
+  void set(int64_t by) {
+    d = unsigned(by);
+    unsigned log = 0;
+    while ((uint64_t(1) << log) < d) ++log;
+    s = log > 0 ? log - 1 : 0;
+    m = d > 1 ? unsigned(((uint64_t(1) << (31 + log)) + d - 1) / d) : 0;
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : int(__umulhi(unsigned(n), m) >> s);
+  }
+#endif
+};
+
 // One product C = A B^T over K, as tiles.  Operands are 16-bit values in `planes`
 // planes (the terms of a float32, or the value itself) behind tensor maps of
 // (inner, outer, plane).  a_mn / b_mn: the inner dimension is the tile's own (M or N),
@@ -59,6 +78,7 @@ struct HeadJob {
   int tiles_m, tiles_n, splits;      // splits: parts of K, each with its own output
   int kblocks;                       // ceil(K / kHeadTileK)
   int group;                         // tile rows walked together (L2 reuse)
+  HeadDiv by_split, by_group, by_rows, by_last, by_splits;  // see divide()
   int a_row0, b_row0;                // first outer coordinate of A and B (K-major) ...
   int a_k0, b_k0;                    // ... and first K coordinate of each
   int a_box, b_box;                  // rows of a K-major operand's box
@@ -70,6 +90,15 @@ struct HeadJob {
   long long ld_out;
   int out_f32;
   int wide;                          // rows of out start on four values
+
+  void divide() {                    // once tiles, group and splits are known
+    by_split.set(int64_t(tiles_m) * tiles_n);
+    by_group.set(int64_t(group) * tiles_n);
+    by_rows.set(group);
+    const int last = tiles_m % group;
+    by_last.set(last ? last : group);
+    by_splits.set(splits);
+  }
 };
 
 struct HeadRows {                    // what the logits' epilogues know of each row

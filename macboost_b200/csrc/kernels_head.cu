@@ -137,8 +137,9 @@ __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
 
-// 32 lanes x 32 columns of tensor memory: column c of lane i to v[c] of thread i.
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+// 32 lanes x 32 columns of tensor memory: column c of lane i to v[c] of thread i, which
+// are not there before tmem_wait.
+__device__ __forceinline__ void tmem_issue(uint32_t addr, float (&v)[32]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -150,9 +151,18 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
         "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-
+__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+        "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+        "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+        "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -230,49 +240,62 @@ struct Walk {
     ++step;
     const HeadJob& q = a.job[job];
     t->job = job;
-    const int tiles = q.tiles_m * q.tiles_n;
-    t->split = i / tiles;
-    i -= t->split * tiles;
+    t->split = 0;
+    if (q.splits > 1) {
+      t->split = q.by_split(i);
+      i -= t->split * q.tiles_m * q.tiles_n;
+    }
     // groups of tile rows, all columns of a group before the next group
-    const int per = q.group * q.tiles_n;
-    const int g = i / per;
+    const int g = q.by_group(i);
+    i -= g * q.group * q.tiles_n;
     const int rows = min(q.group, q.tiles_m - g * q.group);
-    i -= g * per;
-    t->m = g * q.group + i % rows;
-    t->n = i / rows;
+    t->n = rows == q.group ? q.by_rows(i) : q.by_last(i);
+    t->m = g * q.group + i - t->n * rows;
     return true;
   }
+  // K blocks of a tile: kblocks * split / splits ...
   __device__ void blocks(const Tile& t, int* k0, int* k1) const {
     const HeadJob& q = a.job[t.job];
-    *k0 = int((long long)q.kblocks * t.split / q.splits);
-    *k1 = int((long long)q.kblocks * (t.split + 1) / q.splits);
+    *k0 = 0;
+    *k1 = q.kblocks;
+    if (q.splits > 1) {
+      *k0 = q.by_splits(q.kblocks * t.split);
+      *k1 = q.by_splits(q.kblocks * (t.split + 1));
+    }
   }
 };
 
 // ---- epilogues ------------------------------------------------------------------
 
-// Running maximum and sum of exp(x - max), of 32 more columns of which `n` exist.
+// Running maximum and sum of exp(x - max), of 32 more columns of which `n` exist.  Four
+// chains each: two warps a scheduler do not hide a chain of 32.
 __device__ __forceinline__ void online(const float (&v)[32], int n, float& m, float& s) {
-  float top = m;
+  float t[4] = {m, -INFINITY, -INFINITY, -INFINITY};
   if (n >= 32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
+    for (int i = 0; i < 32; ++i) t[i % 4] = fmaxf(t[i % 4], v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      if (i < n) top = fmaxf(top, v[i]);
+      if (i < n) t[i % 4] = fmaxf(t[i % 4], v[i]);
   }
+  const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
   // an infinite maximum would make inf - inf of itself: such a row's sum is formed
   // around 0 and comes out inf, or stays 0 for -inf (NaN is kept either way)
   const float base = fabsf(top) == INFINITY ? 0.f : top;
   const float old = fabsf(m) == INFINITY ? 0.f : m;
-  float sum = s == 0.f ? 0.f : s * exp2_approx((old - base) * kLog2e);
+  float sum[4] = {s == 0.f ? 0.f : s * exp2_approx((old - base) * kLog2e), 0.f, 0.f, 0.f};
   const float b2 = base * kLog2e;
+  if (n >= 32) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < n) sum += exp2_approx(fmaf(v[i], kLog2e, -b2));
+    for (int i = 0; i < 32; ++i) sum[i % 4] += exp2_approx(fmaf(v[i], kLog2e, -b2));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) sum[i % 4] += exp2_approx(fmaf(v[i], kLog2e, -b2));
+  }
   m = top;
-  s = sum;
+  s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -407,7 +430,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
                                         bytes_b(n0 + TN / kHeadPair));
         // Each tile starts at another K block: tiles that run together would read the same
         // 128 bytes of every row, which are few of the memory's channels.
-        const int turn = (t.m + t.n) % (k1 - k0);
+        const int turn = k1 - k0 > 1 ? (t.m + t.n) % (k1 - k0) : 0;
         for (int i = k0; i < k1; ++i) {
           const int kb = i + turn < k1 ? i + turn : i + turn - (k1 - k0);
           ok = wait(empty + 8 * s, ph ^ 1);
@@ -507,6 +530,14 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       const HeadJob& q = a.job[t.job];
       int k0, k1;
       walk.blocks(t, &k0, &k1);
+      const int row = (t.m * kHeadPair + int(rank)) * kHeadTileM + quarter * 32 + lane;
+      const int col0 = t.n * TN + half * (TN / 2);
+      // what the epilogue knows of the row is fetched while the products run
+      const bool there = EPI != kHeadOut && row < r.rows;
+      const int y = there ? r.labels[row] : -1;
+      const bool known = unsigned(y) < unsigned(r.classes);
+      const float lse = EPI == kHeadG && there ? r.lse[row] : 0.f;
+      const float up = EPI == kHeadG && known ? r.dloss[row] : 0.f;
       bool ok = true;
       uint32_t src = 0;
       for (int c0 = k0; c0 < k1; c0 += F32 ? 1 : k1 - k0) {
@@ -530,34 +561,45 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         }
       }
       if (!ok) break;
-      // 32 of the sums, by column
-      auto take = [&](int c, float (&v)[32]) {
-        if constexpr (F32) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = sums[c + i];
-        } else {
-          tmem_load(src + c, v);
-        }
+      // the tile's tensor memory may be written again
+      auto release = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_at(sums_empty + 8 * as, 0);
+        as ^= 1;
+        if (as == 0) aph ^= 1;
       };
-      // f for each 32 columns: sums in registers want their place known to the compiler
+      // f(column, values) for each 32 columns: the sums in registers (their place has to be
+      // known to the compiler), or from tensor memory, the next ones on their way
       auto each_part = [&](auto f) {
         if constexpr (F32) {
 #pragma unroll
-          for (int c = 0; c < TN / 2; c += 32) f(c);
+          for (int c = 0; c < TN / 2; c += 32) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = sums[c + i];
+            f(c, v);
+          }
         } else {
+          float v[32], w[32];
+          tmem_issue(src, v);
 #pragma unroll 1
-          for (int c = 0; c < TN / 2; c += 32) f(c);
+          for (int c = 0; c < TN / 2; c += 64) {
+            tmem_wait(v);
+            tmem_issue(src + c + 32, w);
+            f(c, v);
+            tmem_wait(w);
+            if (c + 64 < TN / 2)
+              tmem_issue(src + c + 64, v);
+            else
+              release();  // all of it has been read
+            f(c + 32, w);
+          }
         }
       };
-      const int row = (t.m * kHeadPair + int(rank)) * kHeadTileM + quarter * 32 + lane;
-      const int col0 = t.n * TN + half * (TN / 2);
       if (EPI == kHeadLse) {
-        const bool there = row < r.rows;
-        const int y = there ? r.labels[row] : -1;
         float m = -INFINITY, sum = 0.f;
-        each_part([&](int c) {
-          float v[32];
-          take(c, v);
+        each_part([&](int c, float (&v)[32]) {
           const int n = r.classes - (col0 + c);
           online(v, n, m, sum);
           if (unsigned(y - (col0 + c)) < 32u && y < r.classes) {
@@ -570,17 +612,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         });
         if (there) r.part[(long long)(t.n * 2 + half) * r.rows + row] = make_float2(m, sum);
       } else if (EPI == kHeadG) {
-        const bool there = row < r.rows;
-        const int y = there ? r.labels[row] : -1;
-        const bool known = unsigned(y) < unsigned(r.classes);
-        const float lse = there ? r.lse[row] : 0.f;
-        const float up = known ? r.dloss[row] : 0.f;
         // lanes past the last row hold zeros, which are not stored
         __nv_bfloat16* g = static_cast<__nv_bfloat16*>(r.g) + (long long)(row - lane) * r.ld_g + col0;
         const int rows = r.rows - (row - lane);
-        each_part([&](int c) {
-          float v[32];
-          take(c, v);
+        each_part([&](int c, float (&v)[32]) {
           const int v0 = r.v0 + col0 + c;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -607,9 +642,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         const int row0 = row - lane, rows = q.M - row0;
         float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row0) * q.N + col0 : nullptr;
         const bool wide_acc = q.N % 4 == 0;  // its base is aligned
-        each_part([&](int c) {
-          float v[32];
-          take(c, v);
+        each_part([&](int c, float (&v)[32]) {
           turn(stage, v, lane, [&](int rr, int cc, float4 x) {
             const int n = q.N - (col0 + c + cc);
             if (rr >= rows || n <= 0) return;
@@ -634,13 +667,6 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
               store4(static_cast<__nv_bfloat16*>(q.out) + at, x, n, q.wide);
           });
         });
-      }
-      if constexpr (!F32) {
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive_at(sums_empty + 8 * as, 0);
-        as ^= 1;
-        if (as == 0) aph ^= 1;
       }
     }
   }
