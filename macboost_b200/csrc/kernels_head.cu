@@ -328,6 +328,29 @@ __device__ __forceinline__ void turn(uint32_t buf, const float (&v)[32], int lan
   }
 }
 
+// The same in bfloat16: eight rows at a time with four lanes a row, 16 bytes each.
+template <class F>
+__device__ __forceinline__ void turn_bf16(uint32_t buf, const float (&v)[32], int lane, F f) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 64 +
+                                                                  ((u ^ ((lane >> 1) & 3)) << 4)),
+                 "r"(pack2(v[8 * u], v[8 * u + 1])), "r"(pack2(v[8 * u + 2], v[8 * u + 3])),
+                 "r"(pack2(v[8 * u + 4], v[8 * u + 5])), "r"(pack2(v[8 * u + 6], v[8 * u + 7]))
+                 : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + lane / 4, u = lane % 4;
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(buf + row * 64 + ((u ^ ((row >> 1) & 3)) << 4)));
+    f(row, 8 * u, x);
+  }
+}
+
 // Four adjacent values to memory; `n` of them exist, `wide`: p is aligned for all four.
 __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x, int n, bool wide) {
   if (wide && n >= 4) {
@@ -617,26 +640,45 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         const int rows = r.rows - (row - lane);
         each_part([&](int c, float (&v)[32]) {
           const int v0 = r.v0 + col0 + c;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float p = exp2_approx((v[i] - lse) * kLog2e);
-            if (v0 + i == y) p -= 1.f;
-            v[i] = known && v0 + i < r.classes ? up * p : 0.f;
-          }
           const int n = int(r.ld_g) - (col0 + c);  // a multiple of 32
-          turn(stage, v, lane, [&](int rr, int cc, float4 x) {
-            if (rr >= rows || n <= 0) return;
-            __nv_bfloat16* p = g + rr * r.ld_g + c + cc;
-            store4(p, x, 4, true);
-            if constexpr (F32) {
+          if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float p = exp2_approx((v[i] - lse) * kLog2e);
+              if (v0 + i == y) p -= 1.f;
+              v[i] = known && v0 + i < r.classes ? up * p : 0.f;
+            }
+            turn(stage, v, lane, [&](int rr, int cc, float4 x) {
+              if (rr >= rows || n <= 0) return;
+              __nv_bfloat16* p = g + rr * r.ld_g + c + cc;
+              store4(p, x, 4, true);
               auto rest = [](float f) { return f - __bfloat162float(__float2bfloat16_rn(f)); };
 #pragma unroll
               for (int z = 1; z < 3; ++z) {
                 x = make_float4(rest(x.x), rest(x.y), rest(x.z), rest(x.w));
                 store4(p + z * r.plane_g, x, 4, true);
               }
+            });
+          } else {
+            // one product and sum, one exponential, one product a value; what only few
+            // columns or rows need is done apart
+            const float lse2 = lse * kLog2e;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = up * exp2_approx(fmaf(v[i], kLog2e, -lse2));
+            if (unsigned(y - v0) < 32u) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (v0 + i == y) v[i] -= up;
             }
-          });
+            if (!known || v0 + 32 > r.classes) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!known || v0 + i >= r.classes) v[i] = 0.f;
+            }
+            turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 x) {
+              if (rr < rows && n > 0) *reinterpret_cast<uint4*>(g + rr * r.ld_g + c + cc) = x;
+            });
+          }
         });
       } else {
         const int row0 = row - lane, rows = q.M - row0;
