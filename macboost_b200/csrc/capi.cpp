@@ -44,10 +44,16 @@ std::vector<int> default_devices() {
   return d;
 }
 
-// The end of an entry point: its message, if it failed.
-int32_t finish(int rc, const std::string& msg, char** err) {
-  if (rc == 0) return 0;
-  set_error(err, msg);
+// An entry point's call: 0, or its message and -1.  Nothing is thrown out of it.
+template <class F>
+int32_t guarded(char** err, F call) {
+  try {
+    std::string msg;
+    if (call(msg) == 0) return 0;
+    set_error(err, msg);
+  } catch (...) {
+    if (err) *err = strdup("out of host memory");
+  }
   return -1;
 }
 
@@ -614,8 +620,9 @@ int32_t macboost_route_device(int32_t device, const float* logits, int64_t rows,
   a.norm = norm;
   a.ids = ids;
   a.weights = weights;
-  std::string e;
-  return finish(mb::route_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::route_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_route_grad_device(int32_t device, const float* logits, int64_t rows,
@@ -635,8 +642,9 @@ int32_t macboost_route_grad_device(int32_t device, const float* logits, int64_t 
   a.dweights = dweights;
   a.dlogits = dlogits;
   a.ld_d = ld_d;
-  std::string e;
-  return finish(mb::route_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::route_grad_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int64_t macboost_sort_rows_workspace(int64_t rows, int64_t k, int64_t experts) {
@@ -648,11 +656,11 @@ int32_t macboost_sort_rows_device(int32_t device, const int32_t* ids, int64_t ro
                                   int32_t* counts, int32_t* order, int32_t* slots,
                                   void* workspace, int64_t workspace_bytes, void* stream,
                                   char** err) {
-  std::string e;
-  return finish(mb::sort_rows_device(device, ids, rows, k, experts, align, offsets, counts, order,
+  return guarded(err, [&](std::string& e) {
+    return mb::sort_rows_device(device, ids, rows, k, experts, align, offsets, counts, order,
                                      slots, workspace, workspace_bytes,
-                                     static_cast<cudaStream_t>(stream), e),
-                e, err);
+                                     static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_gather_rows_device(int32_t device, int32_t dtype, const void* x, int64_t rows,
@@ -677,8 +685,9 @@ int32_t macboost_gather_rows_device(int32_t device, int32_t dtype, const void* x
   a.ld_out = ld_out;
   a.layout_out = layout_out;
   a.dtype = dtype;
-  std::string e;
-  return finish(mb::gather_rows_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::gather_rows_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_combine_rows_device(int32_t device, int32_t dtype, const void* y,
@@ -698,8 +707,9 @@ int32_t macboost_combine_rows_device(int32_t device, int32_t dtype, const void* 
   a.k = narrow(k);
   a.out = out;
   a.ld_out = ld_out;
-  std::string e;
-  return finish(mb::combine_rows_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::combine_rows_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const void* y,
@@ -725,9 +735,9 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
   a.dy = dy;
   a.ld_dy = ld_dy;
   a.dweights = dweights;
-  std::string e;
-  return finish(mb::combine_rows_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e,
-                err);
+  return guarded(err, [&](std::string& e) {
+    return mb::combine_rows_grad_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int64_t macboost_head_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t classes,
@@ -754,8 +764,9 @@ int32_t macboost_head_loss_device(int32_t device, int32_t dtype, const void* h, 
   a.lse_out = lse;
   a.workspace = workspace;
   a.workspace_bytes = workspace_bytes;
-  std::string e;
-  return finish(mb::head_loss_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::head_loss_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void* h, int64_t rows,
@@ -782,13 +793,15 @@ int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void* h, 
   a.ld_dw = ld_dw;
   a.workspace = workspace;
   a.workspace_bytes = workspace_bytes;
-  std::string e;
-  return finish(mb::head_grad_device(device, a, static_cast<cudaStream_t>(stream), e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::head_grad_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
 }
 
 int32_t macboost_head_check_device(int32_t device, const void* workspace, char** err) {
-  std::string e;
-  return finish(mb::head_check_device(device, workspace, e), e, err);
+  return guarded(err, [&](std::string& e) {
+    return mb::head_check_device(device, workspace, e);
+  });
 }
 
 }  // extern "C"

@@ -318,6 +318,8 @@ int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, 
   if (encode(&j.a, o.h, a.cols, a.rows, o.ld_h, p.planes, j.a_box, err) ||
       encode(&j.b, o.w, a.cols, a.classes, o.ld_w, p.planes, j.b_box, err))
     return -1;
+  if (parts(a.rows, kHeadPair * kHeadTileM) * parts(n, kHeadTileN) > kMaxIndex)
+    return fail(err, "rows * classes are too many for one call");
   j.tiles_m = int(parts(a.rows, kHeadPair * kHeadTileM));
   j.tiles_n = int(parts(n, kHeadTileN));
   j.splits = 1;

@@ -1455,6 +1455,15 @@ cudaError_t go_type(const HeadLaunch& a, cudaStream_t s) {
   const cudaError_t e = cudaFuncSetAttribute(head_kernel<EPI, TN, F32>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
+  if (F32) {
+    // the warpgroups' registers are shared out of what the block is launched with
+    static const bool enough = [] {
+      cudaFuncAttributes f{};
+      return cudaFuncGetAttributes(&f, head_kernel<EPI, TN, F32>) == cudaSuccess &&
+             f.numRegs * kHeadThreads >= 128 * 56 + 256 * 224;
+    }();
+    if (!enough) return cudaErrorInvalidConfiguration;
+  }
   long long tiles = 0;
   for (int j = 0; j < a.jobs; ++j)
     tiles += (long long)a.job[j].tiles_m * a.job[j].tiles_n * a.job[j].splits;
