@@ -1086,17 +1086,25 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) head_narrow_kernel(const Na
   }
 }
 
-// dw from the blocks' sums, a warp a value.
+// dw from the blocks' sums, a block a value: every thread has its few loads in flight.
+constexpr int kNarrowReduce = 128;
 template <class T>
-__global__ void __launch_bounds__(256)
-    head_narrow_reduce_kernel(const float* part, int blocks, int classes, int cols, T* dw, long long ld) {
-  const int i = int(blockIdx.x) * 8 + int(threadIdx.x) / 32, lane = threadIdx.x % 32;
-  if (i >= classes * cols) return;
+__global__ void __launch_bounds__(kNarrowReduce)
+    head_narrow_reduce_kernel(const float* part, int blocks, int cols, int values, T* dw, long long ld) {
+  __shared__ float sums[kNarrowReduce / 32];
+  const int i = int(blockIdx.x);
   float v = 0.f;
-  for (int b = lane; b < blocks; b += 32) v += part[(long long)b * classes * cols + i];
+#pragma unroll 5
+  for (int b = threadIdx.x; b < blocks; b += kNarrowReduce) v += part[(long long)b * values + i];
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(~0u, v, o);
-  if (lane == 0) dw[i / cols * ld + i % cols] = T(v);
+  if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < kNarrowReduce / 32; ++w) v += sums[w];
+    dw[i / cols * ld + i % cols] = T(v);
+  }
 }
 
 template <class T, int DP, int VP>
@@ -1507,13 +1515,13 @@ cudaError_t launch_head_narrow(const HeadArgs& h, bool grad, float* part, int bl
   cudaError_t e = h.dtype == kF32 ? narrow_type<float>(a, grad, blocks, s)
                                   : narrow_type<__nv_bfloat16>(a, grad, blocks, s);
   if (e != cudaSuccess || !grad || !h.dw) return e;
-  const unsigned n = unsigned((h.classes * h.cols + 7) / 8);
+  const int values = a.classes * a.cols;
   if (h.dtype == kF32)
-    head_narrow_reduce_kernel<float><<<n, 256, 0, s>>>(part, blocks, a.classes, a.cols,
-                                                       static_cast<float*>(h.dw), h.ld_dw);
+    head_narrow_reduce_kernel<float><<<values, kNarrowReduce, 0, s>>>(
+        part, blocks, a.cols, values, static_cast<float*>(h.dw), h.ld_dw);
   else
-    head_narrow_reduce_kernel<__nv_bfloat16><<<n, 256, 0, s>>>(
-        part, blocks, a.classes, a.cols, static_cast<__nv_bfloat16*>(h.dw), h.ld_dw);
+    head_narrow_reduce_kernel<__nv_bfloat16><<<values, kNarrowReduce, 0, s>>>(
+        part, blocks, a.cols, values, static_cast<__nv_bfloat16*>(h.dw), h.ld_dw);
   return cudaGetLastError();
 }
 

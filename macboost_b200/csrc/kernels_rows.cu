@@ -639,7 +639,7 @@ __device__ __forceinline__ void load_choices(const CombineArgs& a, const Lay& l,
 // rows wait for memory: 1M x 10 of two models took 89 us, with the gradient, at 4 blocks a
 // multiprocessor and 82 at 8 and 6 (the gradient); four groups a warp, 96.
 template <class T, int BYTES, int K>
-__global__ void __launch_bounds__(kThreads, K == 1 || K == 2 ? 8 : 1)
+__global__ void __launch_bounds__(kThreads, K == 1 || K == 2 ? 8 : 4)
     combine_kernel(const CombineArgs a, const Lay l) {
   using U = typename Unit<BYTES>::T;
   using W = Values<T, BYTES>;
