@@ -427,118 +427,121 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
   // float32: the epilogue keeps 128 sums a thread.  384 threads are launched with 168
   // registers each (64,512); the first warpgroup keeps 56 a thread and the other two get
   // 224: 128 x 56 + 256 x 224 = 64,512.
+  // float32: the epilogue keeps 128 sums a thread.  384 threads are launched with 168
+  // registers each (64,512); the first warpgroup keeps 56 a thread and the other two get
+  // 224: 128 x 56 + 256 x 224 = 64,512.
   if (warp < 4) {
-  if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 0) {
-    if (lane == 0) {
-      Walk walk(a);
-      Tile t;
-      int s = 0, ph = 0;
-      bool ok = true;
-      while (ok && walk.next(&t)) {
-        const HeadJob& q = a.job[t.job];
-        int k0, k1;
-        walk.blocks(t, &k0, &k1);
-        const int am = (t.m * kHeadPair + int(rank)) * kHeadTileM;
-        const int bn = t.n * TN + int(rank) * (TN / kHeadPair);
-        // Boxes that lie outside the matrix are not fetched (what the shared memory holds
-        // there only reaches sums that are not used): a box that TMA has to fill with
-        // zeros is slower than one it reads.
-        auto bytes_a = [&](int m0) {
-          return q.a_mn ? min(kHeadTileM / 64, max(0, (q.M - m0 + 63) / 64)) * 8192
-                        : m0 < q.M ? q.a_box * 128 : 0;
-        };
-        auto bytes_b = [&](int n0) {
-          return q.b_mn ? min(TN / kHeadPair / 64, max(0, (q.N - n0 + 63) / 64)) * 8192
-                        : n0 < q.N ? q.b_box * 128 : 0;
-        };
-        const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
-        const uint32_t bytes = kPlanes * uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
-                                        bytes_b(n0 + TN / kHeadPair));
-        for (int kb = k0; kb < k1; ++kb) {
-          ok = wait(empty + 8 * s, ph ^ 1);
-          if (!ok) break;
-          if (rank == 0) bar_expect(full + 8 * s, bytes);
-          const uint32_t bar = full + 8 * s;
-          uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
-          if (++s == kStages) {
-            s = 0;
-            ph ^= 1;
-          }
-          if (a.stall) continue;
-          const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
-          for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
-            if (q.a_mn) {
-#pragma unroll
-              for (int j = 0; j < kHeadTileM / 64; ++j)
-                if (am + 64 * j < q.M) tma_load(sa + j * 8192, &q.a, q.a_row0 + am + 64 * j, ka, z, bar);
-            } else if (am < q.M) {
-              tma_load(sa, &q.a, ka, q.a_row0 + am, z, bar);
-            }
-            if (q.b_mn) {
-#pragma unroll
-              for (int j = 0; j < TN / kHeadPair / 64; ++j)
-                if (bn + 64 * j < q.N) tma_load(sb + j * 8192, &q.b, q.b_row0 + bn + 64 * j, kk, z, bar);
-            } else if (bn < q.N) {
-              tma_load(sb, &q.b, kk, q.b_row0 + bn, z, bar);
-            }
-          }
-        }
-      }
-      if (!ok) {  // copies in flight land before the shared memory is given up
-        const uint64_t t0 = now_ns();
-        while (now_ns() - t0 < 2000000) {
-        }
-      }
-    }
-  } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
-      Walk walk(a);
-      Tile t;
-      int s = 0, ph = 0, as = 0, aph = 0;
-      bool ok = true;
-      while (ok && walk.next(&t)) {
-        const HeadJob& q = a.job[t.job];
-        int k0, k1;
-        walk.blocks(t, &k0, &k1);
-        // float32 sums of bfloat16, M 256 (both CTAs), N TN
-        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(q.a_mn) << 15) |
-                               (uint32_t(q.b_mn) << 16) | (uint32_t(TN / 8) << 17) |
-                               (uint32_t(kHeadPair * kHeadTileM / 16) << 24);
-        const uint32_t step_a = q.a_mn ? 2048 / 16 : 32 / 16, step_b = q.b_mn ? 2048 / 16 : 32 / 16;
-        for (int c0 = k0; ok && c0 < k1; c0 += F32 ? 1 : k1 - k0) {
-          ok = wait(sums_empty + 8 * as, aph ^ 1);
-          if (!ok) break;
-          fence_after();
-          bool add = false;
-          for (int i = 0; i < (F32 ? 1 : k1 - k0); ++i) {
-            ok = wait(full + 8 * s, ph);
+    if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      if (lane == 0) {
+        Walk walk(a);
+        Tile t;
+        int s = 0, ph = 0;
+        bool ok = true;
+        while (ok && walk.next(&t)) {
+          const HeadJob& q = a.job[t.job];
+          int k0, k1;
+          walk.blocks(t, &k0, &k1);
+          const int am = (t.m * kHeadPair + int(rank)) * kHeadTileM;
+          const int bn = t.n * TN + int(rank) * (TN / kHeadPair);
+          // Boxes that lie outside the matrix are not fetched (what the shared memory holds
+          // there only reaches sums that are not used): a box that TMA has to fill with
+          // zeros is slower than one it reads.
+          auto bytes_a = [&](int m0) {
+            return q.a_mn ? min(kHeadTileM / 64, max(0, (q.M - m0 + 63) / 64)) * 8192
+                          : m0 < q.M ? q.a_box * 128 : 0;
+          };
+          auto bytes_b = [&](int n0) {
+            return q.b_mn ? min(TN / kHeadPair / 64, max(0, (q.N - n0 + 63) / 64)) * 8192
+                          : n0 < q.N ? q.b_box * 128 : 0;
+          };
+          const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
+          const uint32_t bytes = kPlanes * uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
+                                          bytes_b(n0 + TN / kHeadPair));
+          for (int kb = k0; kb < k1; ++kb) {
+            ok = wait(empty + 8 * s, ph ^ 1);
             if (!ok) break;
-            fence_after();
-            const uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
-#pragma unroll
-            for (int p = F32 ? 0 : 5; p < 6; ++p) {
-              const uint64_t da = descriptor(sa + (F32 ? kPlaneA[p] : 0) * kBytesA, q.a_mn);
-              const uint64_t db = descriptor(sb + (F32 ? kPlaneB[p] : 0) * kBytesB, q.b_mn);
-#pragma unroll
-              for (int k = 0; k < kHeadTileK / 16; ++k) {
-                mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
-                add = true;
-              }
-            }
-            commit_both(empty + 8 * s);
+            if (rank == 0) bar_expect(full + 8 * s, bytes);
+            const uint32_t bar = full + 8 * s;
+            uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
             if (++s == kStages) {
               s = 0;
               ph ^= 1;
             }
+            if (a.stall) continue;
+            const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
+            for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
+              if (q.a_mn) {
+#pragma unroll
+                for (int j = 0; j < kHeadTileM / 64; ++j)
+                  if (am + 64 * j < q.M) tma_load(sa + j * 8192, &q.a, q.a_row0 + am + 64 * j, ka, z, bar);
+              } else if (am < q.M) {
+                tma_load(sa, &q.a, ka, q.a_row0 + am, z, bar);
+              }
+              if (q.b_mn) {
+#pragma unroll
+                for (int j = 0; j < TN / kHeadPair / 64; ++j)
+                  if (bn + 64 * j < q.N) tma_load(sb + j * 8192, &q.b, q.b_row0 + bn + 64 * j, kk, z, bar);
+              } else if (bn < q.N) {
+                tma_load(sb, &q.b, kk, q.b_row0 + bn, z, bar);
+              }
+            }
           }
-          if (ok) commit_both(sums_full + 8 * as);
-          as ^= 1;
-          if (as == 0) aph ^= 1;
+        }
+        if (!ok) {  // copies in flight land before the shared memory is given up
+          const uint64_t t0 = now_ns();
+          while (now_ns() - t0 < 2000000) {
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (rank == 0 && lane == 0) {
+        Walk walk(a);
+        Tile t;
+        int s = 0, ph = 0, as = 0, aph = 0;
+        bool ok = true;
+        while (ok && walk.next(&t)) {
+          const HeadJob& q = a.job[t.job];
+          int k0, k1;
+          walk.blocks(t, &k0, &k1);
+          // float32 sums of bfloat16, M 256 (both CTAs), N TN
+          const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(q.a_mn) << 15) |
+                                 (uint32_t(q.b_mn) << 16) | (uint32_t(TN / 8) << 17) |
+                                 (uint32_t(kHeadPair * kHeadTileM / 16) << 24);
+          const uint32_t step_a = q.a_mn ? 2048 / 16 : 32 / 16, step_b = q.b_mn ? 2048 / 16 : 32 / 16;
+          for (int c0 = k0; ok && c0 < k1; c0 += F32 ? 1 : k1 - k0) {
+            ok = wait(sums_empty + 8 * as, aph ^ 1);
+            if (!ok) break;
+            fence_after();
+            bool add = false;
+            for (int i = 0; i < (F32 ? 1 : k1 - k0); ++i) {
+              ok = wait(full + 8 * s, ph);
+              if (!ok) break;
+              fence_after();
+              const uint32_t sa = ring + s * kStage, sb = sa + kPlanes * kBytesA;
+#pragma unroll
+              for (int p = F32 ? 0 : 5; p < 6; ++p) {
+                const uint64_t da = descriptor(sa + (F32 ? kPlaneA[p] : 0) * kBytesA, q.a_mn);
+                const uint64_t db = descriptor(sb + (F32 ? kPlaneB[p] : 0) * kBytesB, q.b_mn);
+#pragma unroll
+                for (int k = 0; k < kHeadTileK / 16; ++k) {
+                  mma(tmem + as * TN, da + k * step_a, db + k * step_b, idesc, add);
+                  add = true;
+                }
+              }
+              commit_both(empty + 8 * s);
+              if (++s == kStages) {
+                s = 0;
+                ph ^= 1;
+              }
+            }
+            if (ok) commit_both(sums_full + 8 * as);
+            as ^= 1;
+            if (as == 0) aph ^= 1;
+          }
         }
       }
     }
-  }
   } else {
     if constexpr (F32) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     Walk walk(a);
