@@ -43,7 +43,7 @@ constexpr int kSortThreads = kSortWarps * 32;
 // on, with registers for five blocks a multiprocessor (the launches wait for memory and
 // for the chain of steps, not for bandwidth); below that 4 give twice the blocks and half
 // the chain.
-constexpr int kSteps = 8, kFewSteps = 4;
+constexpr int kSteps = 8, kFewSteps = 4, kOneSteps = 16;  // kOneSteps: the most of one launch
 constexpr long long kFewEntries = 300000;
 constexpr int kRunSteps = 16;  // of gather_runs_kernel
 
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(const SortArgs a, int ti
 
 // ONE: the whole sort of up to one tile.
 template <bool ONE, int STEPS>
-__global__ void __launch_bounds__(kSortThreads, 5) sort_place_kernel(const SortArgs a, int tiles) {
+__global__ void __launch_bounds__(kSortThreads, ONE ? 1 : 5) sort_place_kernel(const SortArgs a, int tiles) {
   extern __shared__ int cnt[];  // kSortWarps x experts
   __shared__ int part[kSortWarps];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, E = a.experts;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void zero_empty(const int* order, long long warp, lon
                                            U* out, long long ld, long long units, int lane) {
   const int slots = clear_slots(units);
   const long long first = warp * slots;
-  if (units <= 8) {  // a lane a slot
+  if (units <= 32) {  // a lane a slot
     for (int t = lane; t < slots; t += 32)
       if (first + t < capacity && order[first + t] < 0)
         for (long long u = 0; u < units; ++u) out[(first + t) * ld + u] = zero<U>();
@@ -952,10 +952,11 @@ cudaError_t combine_any(const CombineArgs& a, bool grad, cudaStream_t s) {
 
 int sort_steps(long long entries) {
   // up to one tile: one launch, with the fewer steps when they do
-  return entries <= kSortThreads * kFewSteps  ? kFewSteps
-         : entries <= kSortThreads * kSteps   ? kSteps
-         : entries <= kFewEntries             ? kFewSteps
-                                              : kSteps;
+  return entries <= kSortThreads * kFewSteps   ? kFewSteps
+         : entries <= kSortThreads * kSteps    ? kSteps
+         : entries <= kSortThreads * kOneSteps ? kOneSteps
+         : entries <= kFewEntries              ? kFewSteps
+                                               : kSteps;
 }
 int sort_tiles(long long entries) {
   const long long tile = kSortThreads * sort_steps(entries);
@@ -986,8 +987,15 @@ long long sort_workspace_ints(long long entries, int experts) {
 
 cudaError_t launch_sort(const SortArgs& a, int* launches, cudaStream_t s) {
   const int tiles = sort_tiles(a.entries);
-  return sort_steps(a.entries) == kSteps ? sort<kSteps>(a, tiles, launches, s)
-                                         : sort<kFewSteps>(a, tiles, launches, s);
+  switch (sort_steps(a.entries)) {
+    case kFewSteps: return sort<kFewSteps>(a, tiles, launches, s);
+    case kSteps: return sort<kSteps>(a, tiles, launches, s);
+    default: break;
+  }
+  // up to kOneSteps steps a warp, always one tile
+  sort_place_kernel<true, kOneSteps><<<1, kSortThreads, size_t(kSortWarps) * a.experts * sizeof(int), s>>>(a, 1);
+  *launches = 1;
+  return cudaGetLastError();
 }
 
 cudaError_t launch_gather(const GatherArgs& a, cudaStream_t s) {
