@@ -22,7 +22,8 @@
 // tiles into shared memory (as many stages as three are as fast), in a loop by the power cap.
 //
 // Every wait ends after wait_ns: the CTA then marks itself dead, sets the status word,
-// lets its copies land and returns (its results are void).
+// waits (as long again at most) for its copies and products in flight and returns (its
+// results are void).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -105,6 +106,12 @@ struct Wait {
     }
     return false;
   }
+  // Until the barrier's phase is over or `limit` after t0, whatever happened before: for
+  // what is in flight when a CTA gives up.
+  __device__ __forceinline__ void settle(uint32_t bar, uint32_t parity, uint64_t t0) const {
+    while (!bar_try(bar, parity) && now_ns() - t0 <= limit) {
+    }
+  }
 };
 
 // The first CTA's barrier at the same offset: the pair's bit of a cluster address cleared.
@@ -132,6 +139,11 @@ __device__ __forceinline__ void commit_both(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
       "[%0], %1;" ::"r"(bar),
       "h"(uint16_t(3))
+      : "memory");
+}
+__device__ __forceinline__ void commit_here(uint32_t bar) {  // at this CTA's barrier alone
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void fence_after() {
@@ -389,12 +401,13 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
   constexpr int kStage = kPlanes * (kBytesA + kBytesB);
   constexpr int kStages = (192 * 1024) / kStage;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bars[2 * kStages + 4];
+  __shared__ uint64_t bars[2 * kStages + 5];
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t dead_flag;
   const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t full = smem_u32(bars), empty = full + 8 * kStages;
   const uint32_t sums_full = empty + 8 * kStages, sums_empty = sums_full + 16;
+  const uint32_t settled = sums_empty + 16;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
   const Wait wait{&dead_flag, a.status, a.wait_ns};
@@ -408,6 +421,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       bar_init(sums_full + 8 * i, 1);
       bar_init(sums_empty + 8 * i, kHeadPair * kEpilogueWarps);
     }
+    bar_init(settled, 1);
     dead_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -491,11 +505,17 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             }
           }
         }
-        if (!ok) {  // copies in flight land before the shared memory is given up
-          const uint64_t t0 = now_ns();
+        // The copies in flight land before the shared memory is given up: every stage's last
+        // copies, of both CTAs, complete the first CTA's barrier, and the second leaves with
+        // the first.  Without an expired wait that is a matter of a microsecond.  A step
+        // that the second CTA alone had begun when the first gave up has no barrier of its
+        // own; it gets 2 ms.
+        const uint64_t t0 = now_ns();
+        if (rank == 0)
+          for (int i = 0; i < kStages; ++i) wait.settle(full + 8 * i, i < s ? ph : ph ^ 1, t0);
+        if (!ok)
           while (now_ns() - t0 < 2000000) {
           }
-        }
       }
     } else if (warp == 1) {
       if (rank == 0 && lane == 0) {
@@ -542,6 +562,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             as ^= 1;
             if (as == 0) aph ^= 1;
           }
+        }
+        if (!ok) {  // the products in flight read the shared memory of both CTAs
+          commit_here(settled);
+          wait.settle(settled, 0, now_ns());
         }
       }
     }

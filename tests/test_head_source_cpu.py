@@ -21,3 +21,26 @@ def test_loads_from_tensor_memory_are_tied_to_their_wait():
     assert body["tmem_wait"].count('"+r"(r[') == 32
     alone = [a for a in _asm(SOURCE) if "tcgen05.ld" in a and "tcgen05.wait::ld" not in a]
     assert alone == _asm(body["tmem_issue"])
+
+
+def test_a_cta_that_gives_up_waits_for_what_is_in_flight():
+    """Copies into shared memory, and products that read it, end before a CTA leaves: the
+    producer waits on every stage's barrier, the issuer of products on one of its own."""
+    role = SOURCE[SOURCE.index("if (warp == 0) {"):SOURCE.index("if constexpr (F32) asm volatile(\"setmaxnreg.inc")]
+    copies, products = role.split("} else if (warp == 1) {")
+    call = re.search(r"wait\.settle\(full \+ 8 \* i, (.*?), t0\);", copies)
+    assert call and call.group(1) == "i < s ? ph : ph ^ 1"
+    assert re.search(r"if \(!ok\) \{[^}]*commit_here\(settled\);\s*wait\.settle\(settled, 0, ", products)
+
+
+def test_parity_of_each_stages_last_copies():
+    """The rule above against the barrier's definition: after `steps` steps over k stages,
+    stage i is in phase (number of its steps); waiting for parity p returns when the phase
+    before the present one has parity p, so it has to be that of the stage's last step --
+    or, without a step, that of the phase before the first."""
+    for k in range(1, 7):
+        for steps in range(40):
+            s, ph = steps % k, steps // k % 2
+            for i in range(k):
+                last = (steps - i + k - 1) // k - 1     # the stage's last step, -1: none
+                assert (ph if i < s else ph ^ 1) == last % 2
