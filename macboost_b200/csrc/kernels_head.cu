@@ -1081,6 +1081,13 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) head_narrow_kernel(const Na
               s.lo = fma2(gg, t.lo, s.lo);
               s.hi = fma2(gg, t.hi, s.hi);
             }
+            // columns D .. stay zero: there g times w's zeros is NaN for a g that is not
+            // finite, and the next row's logits read them
+            if (4 * q + 4 > D) {
+              const float2 lo = split(s.lo), hi = split(s.hi);
+              s.lo = pair(lo.x, 4 * q + 1 < D ? lo.y : 0.f);
+              s.hi = pair(4 * q + 2 < D ? hi.x : 0.f, 0.f);
+            }
             *reinterpret_cast<F4*>(tile + lane * PITCH + 4 * q) = s;
           }
         __syncwarp();
