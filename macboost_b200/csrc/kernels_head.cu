@@ -1471,7 +1471,9 @@ template <class T, int NR, int PER>
 cudaError_t few_of(const Few& a, bool grad, int blocks, int chunks, cudaStream_t s) {
   const size_t smem = size_t(NR) * few_pitch(a.cols) * sizeof(float);
   const auto k = grad ? head_few_kernel<T, NR, PER, true> : head_few_kernel<T, NR, PER, false>;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  // the limit of the largest call, not this one's: it is the kernel's, and another thread may
+  // launch between this thread's two calls
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kFewSmem));
   if (e != cudaSuccess) return e;
   k<<<blocks, kFewThreads, smem, s>>>(a);
   if (grad && a.dh_part) {

@@ -840,8 +840,11 @@ cudaError_t gather_tiles(const GatherArgs& a, cudaStream_t s) {
       const long long per = (a.cols + parts - 1) / parts;
       const dim3 grid(unsigned(tiles + clear), unsigned((a.cols + per - 1) / per));
       const size_t smem = (2 * kSortThreads * kRunSteps + size_t(kSortWarps + 1) * a.experts) * sizeof(int);
+      // the limit of the largest call, not this one's: it is the kernel's, and another
+      // thread may launch between this thread's two calls
+      constexpr int most = (2 * kSortThreads * kRunSteps + (kSortWarps + 1) * kMaxExperts) * int(sizeof(int));
       const cudaError_t e = cudaFuncSetAttribute(gather_runs_kernel<T>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e != cudaSuccess) return e;
       gather_runs_kernel<T><<<grid, kSortThreads, smem, s>>>(a, tile_rows, tiles, per);
       return cudaGetLastError();
