@@ -510,8 +510,9 @@ int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void *h, 
                                   int64_t ld_dw, void *workspace, int64_t workspace_bytes,
                                   void *stream, char **err);
 
-/* Synchronise `device` and report whether the last head call with this workspace
- * gave up waiting (its outputs are then void). */
+/* Synchronise `device` and report whether the last loss call with this workspace, or a
+ * gradient call since, gave up waiting (the outputs from there on are then void: the
+ * gradient works from the loss call's lse).  The next loss call starts anew. */
 int32_t macboost_head_check_device(int32_t device, const void *workspace, char **err);
 
 #ifdef __cplusplus

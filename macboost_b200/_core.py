@@ -791,5 +791,6 @@ def head_grad_device(device: int, dtype: int, h_ptr: int, rows: int, cols: int, 
 
 
 def head_check_device(device: int, workspace_ptr: int) -> None:
-    """Synchronise and raise if the last head call with this workspace gave up waiting."""
+    """Synchronise and raise if the last loss call with this workspace, or a gradient call
+    since, gave up waiting."""
     _enqueue(_lib.macboost_head_check_device, device, workspace_ptr)

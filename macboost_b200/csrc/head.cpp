@@ -256,7 +256,7 @@ struct Operands {
   int64_t ld_h, ld_w, launches;
 };
 
-// Status word cleared; operands packed where the plan says so, in one launch.
+// Operands packed where the plan says so, in one launch; the loss clears the status word.
 int operands(const HeadArgs& a, const Plan& p, bool grad, Operands* o, cudaStream_t s, std::string& err) {
   char* base = static_cast<char*>(a.workspace);
   o->h = a.h;
@@ -290,7 +290,8 @@ int operands(const HeadArgs& a, const Plan& p, bool grad, Operands* o, cudaStrea
     HEAD_CUDA(cudaMemsetAsync(base, 0, 4, s), "clearing the head's status word");
     return 0;
   }
-  HEAD_CUDA(launch_head_pack(a.dtype, h, w, reinterpret_cast<unsigned*>(base), s), "head pack launch");
+  unsigned* status = grad ? nullptr : reinterpret_cast<unsigned*>(base);
+  HEAD_CUDA(launch_head_pack(a.dtype, h, w, status, s), "head pack launch");
   o->launches = 1;
   return 0;
 }
@@ -551,7 +552,7 @@ int head_check_device(int device, const void* workspace, std::string& err) {
   HEAD_CUDA(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
   unsigned word = 0;
   HEAD_CUDA(cudaMemcpy(&word, workspace, 4, cudaMemcpyDeviceToHost), "reading the head's status word");
-  if (word)
+  if (word == kHeadExpired)
     return fail(err, "device " + std::to_string(device) +
                          ": head kernel gave up waiting for a shared-memory transfer");
   return 0;

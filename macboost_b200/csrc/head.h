@@ -38,11 +38,15 @@ int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, b
                        bool strided);
 int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string& err);
 int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string& err);
-// Wait for `device` and report a wait of these kernels that ran out.
+// Wait for `device` and report a wait of these kernels that ran out.  The word at the start
+// of the workspace is cleared by the loss call, and marked by a wait of either call; the
+// gradient call leaves it, since it works from an lse that a wait may have cost.
 int head_check_device(int device, const void* workspace, std::string& err);
 
 // ---- between head.cpp and kernels_head.cu ---------------------------------------
 
+// The mark: a value that a workspace without a loss call hardly holds.
+constexpr unsigned kHeadExpired = 0x9E37C0DEu;
 constexpr int kHeadTileM = 128;      // accumulator rows a CTA (TMEM lanes)
 constexpr int kHeadTileN = 256;      // accumulator columns
 constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit values

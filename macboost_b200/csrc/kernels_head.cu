@@ -101,7 +101,7 @@ struct Wait {
       if (bar_try(bar, parity)) return true;
       if (now_ns() - t0 > limit) {
         *dead = 1;
-        atomicOr(status, 1u);
+        atomicExch(status, kHeadExpired);
       }
     }
     return false;
@@ -756,10 +756,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
 
 // Planes of bfloat16 with 16-byte aligned rows: the terms of a float32, or a copy.  A
 // warp a row, eight values a lane; the rows of up to two matrices one after the other.
-// It also clears the status word.
+// It also clears the status word, unless null.
 template <class T>
 __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack a, const HeadPack b, unsigned* status) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+  if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
   const int lane = threadIdx.x % 32;
   long long r = (long long)blockIdx.x * 8 + threadIdx.x / 32;
   const bool second = r >= a.rows;
@@ -946,7 +946,8 @@ __global__ void __launch_bounds__(kNarrowWarps * 32) head_narrow_kernel(const Na
     w[i] = v < V && d < D ? load_f(W + v * a.ld_w + d) : 0.f;
   }
   for (int i = lane; i < 32 * PITCH; i += 32) tile[i] = 0.f;  // columns D .. stay zero
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;     // there is no wait to run out
+  // there is no wait to run out
+  if (!GRAD && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
   __syncthreads();
   const unsigned inv = ((1u << 20) + unsigned(D) - 1u) / unsigned(D);  // exact for i < 2,048
   F4 acc[GRAD ? NC : 1];
@@ -1266,7 +1267,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) head_few_kernel(const Few a) {
   constexpr int STEP = PER == 1 ? 64 : 32 * PER;  // columns a warp takes at once
   const int pitch = few_pitch(a.cols);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;  // there is no wait to run out
+  // there is no wait to run out
+  if (!GRAD && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
   for (int n = 0; n < NR; ++n) {
     // rows that do not exist, and in the gradient rows without a label, are zeros
     const bool there = n < a.rows && (!GRAD || unsigned(a.labels[n]) < unsigned(a.classes));
