@@ -61,12 +61,15 @@ bool in_place(int dtype, const void* p, int64_t ld) {
 
 // Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
 // CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
-// blocks (float32: 2, of six products), so that the sums of parts stay few.
+// blocks (float32: 2, of six products), so that the sums of parts stay few.  bfloat16 sums
+// stay in the tensor core, which truncates them at each step of 16: a sum whose terms have one
+// sign lost 1e-7 of itself a step (dw of 300,000 rows, 0.18%).  So its parts are 512 blocks
+// (2,048 steps, 2^-12) at most, and the parts are added up in float32.
 int splits_for(int64_t kblocks, int64_t all, int dtype) {
   const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
   const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
-  // (kblocks, at most 2^24, times parts stays below 2^31)
-  return int(std::max<int64_t>(1, std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100)));
+  const int64_t load = std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100);
+  return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
 }
 
 Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool pack_h,

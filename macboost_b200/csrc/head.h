@@ -81,8 +81,9 @@ struct HeadJob {
   int a_mn, b_mn;
   int tiles_m, tiles_n, splits;      // splits: parts of K, each with its own output
   int kblocks;                       // ceil(K / kHeadTileK)
+  int part, longer;                  // a part's K blocks; the first `longer` have one more
   int group;                         // tile rows walked together (L2 reuse)
-  HeadDiv by_split, by_group, by_rows, by_last, by_splits;  // see divide()
+  HeadDiv by_split, by_group, by_rows, by_last;  // see divide()
   int a_row0, b_row0;                // first outer coordinate of A and B (K-major) ...
   int a_k0, b_k0;                    // ... and first K coordinate of each
   int a_box, b_box;                  // rows of a K-major operand's box
@@ -95,13 +96,14 @@ struct HeadJob {
   int out_f32;
   int wide;                          // rows of out start on four values
 
-  void divide() {                    // once tiles, group and splits are known
+  void divide() {                    // once tiles, group, splits and kblocks are known
     by_split.set(int64_t(tiles_m) * tiles_n);
     by_group.set(int64_t(group) * tiles_n);
     by_rows.set(group);
     const int last = tiles_m % group;
     by_last.set(last ? last : group);
-    by_splits.set(splits);
+    part = kblocks / splits;
+    longer = kblocks % splits;
   }
 };
 

@@ -272,15 +272,11 @@ struct Walk {
     t->m = g * q.group + i - t->n * rows;
     return true;
   }
-  // K blocks of a tile: kblocks * split / splits ...
+  // K blocks of a tile
   __device__ void blocks(const Tile& t, int* k0, int* k1) const {
     const HeadJob& q = a.job[t.job];
-    *k0 = 0;
-    *k1 = q.kblocks;
-    if (q.splits > 1) {
-      *k0 = q.by_splits(q.kblocks * t.split);
-      *k1 = q.by_splits(q.kblocks * (t.split + 1));
-    }
+    *k0 = t.split * q.part + min(t.split, q.longer);
+    *k1 = *k0 + q.part + (t.split < q.longer ? 1 : 0);
   }
 };
 
