@@ -312,6 +312,16 @@ void settings(HeadLaunch& l, const HeadArgs& a) {
   l.stall = t && t[0] == '1';
 }
 
+// The inputs themselves, for float32 logits that the planes cannot form.
+void inputs(HeadRows& r, const HeadArgs& a) {
+  if (a.dtype != kF32) return;
+  r.h = static_cast<const float*>(a.h);
+  r.w = static_cast<const float*>(a.w);
+  r.ld_h = a.ld_h;
+  r.ld_w = a.ld_w;
+  r.cols = int(a.cols);
+}
+
 // The logits of classes v0 ... v0 + n - 1: A = h, B = w, both along cols.
 int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, int64_t v0, int64_t n,
                std::string& err) {
@@ -415,6 +425,7 @@ int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   l.r.target = reinterpret_cast<float*>(base + p.target);
   l.r.rows = int(a.rows);
   l.r.classes = int(a.classes);
+  inputs(l.r, a);
   HEAD_CUDA(launch_head(kHeadLse, kHeadTileN, l, s), "head launch");
   HEAD_CUDA(launch_head_finish(l.r.part, l.r.target, a.labels, a.rows, a.classes,
                                2 * l.job[0].tiles_n, a.loss, a.lse_out, s),
@@ -468,6 +479,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
     l.r.rows = int(a.rows);
     l.r.classes = int(a.classes);
     l.r.v0 = int(v0);
+    inputs(l.r, a);
     HEAD_CUDA(launch_head(kHeadG, kHeadTileN, l, s), "head launch");
 
     HeadLaunch q{};

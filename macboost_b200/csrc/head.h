@@ -116,6 +116,9 @@ struct HeadRows {                    // what the logits' epilogues know of each 
   void* g;                           // gradient: planes x rows x ld_g of bfloat16
   long long ld_g, plane_g;
   int rows, classes, v0;             // v0: first class of this piece
+  const float *h, *w;                // float32: the inputs themselves (see redo() there)
+  long long ld_h, ld_w;
+  int cols;
 };
 
 struct HeadLaunch {

@@ -313,6 +313,52 @@ __device__ __forceinline__ void online(const float (&v)[32], int n, float& m, fl
   s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// float32 logits that are not finite, formed again from the inputs.  The planes of an
+// infinity are (inf, 0, 0), so the products of planes hold 0 x inf and sums of both signs: NaN,
+// where a class that is switched off has -inf.  They are never finite, so what to form again
+// shows in the result: a sum over the columns for each such logit of this lane's row, one
+// class after the other, w read by all lanes at once.  A row of h that holds NaN is left as it
+// is.  A function of its own, called once a tile, so that it takes no registers from the
+// sums: inline for each 32 columns the loss was 20% slower.
+template <int N>
+__device__ __noinline__ void redo_logits(float* v, int n, bool mine, const HeadRows& r, int row,
+                                         int first) {
+  const float* h = r.h + (mine ? row * r.ld_h : 0);
+  int row_nan = -1;                      // not yet known
+  for (int i = 0; i < N; ++i) {
+    const float old = v[i];
+    const bool here = mine && i < n && !(fabsf(old) < INFINITY);
+    if (here && row_nan < 0) {
+      row_nan = 0;
+      for (int k = 0; k < r.cols && !row_nan; ++k) row_nan = isnan(h[k]);
+    }
+    if (!here || row_nan) continue;
+    const float* w = r.w + (first + i) * r.ld_w;
+    float x = 0.f;
+    for (int k0 = 0; k0 < r.cols && !isnan(x); k0 += 32) {
+      const int k1 = min(k0 + 32, r.cols);
+#pragma unroll 8
+      for (int k = k0; k < k1; ++k) x = fmaf(h[k], w[k], x);
+    }
+    v[i] = x;
+  }
+}
+// N of them, of which `n` exist: those of this lane's row, if it is `mine`.
+template <int N>
+__device__ __forceinline__ void redo(float (&v)[N], int n, bool mine, const HeadRows& r, int row, int first) {
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i % 4] = fmaf(v[i], 0.f, t[i % 4]);
+  const float all = (t[0] + t[1]) + (t[2] + t[3]);
+  if (!__any_sync(~0u, mine && all != all)) return;
+  float u[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) u[i] = v[i];
+  redo_logits<N>(u, n, mine, r, row, first);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = u[i];
+}
+
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&p);
@@ -646,6 +692,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           }
         }
       };
+      if constexpr (F32 && EPI != kHeadOut) {
+        const int v0 = (EPI == kHeadG ? r.v0 : 0) + col0;
+        redo(sums, r.classes - v0, EPI == kHeadG ? known : there, r, row, v0);
+      }
       if (EPI == kHeadLse) {
         float m = -INFINITY, sum = 0.f;
         each_part([&](int c, float (&v)[32]) {
@@ -753,6 +803,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
 // Planes of bfloat16 with 16-byte aligned rows: the terms of a float32, or a copy.  A
 // warp a row, eight values a lane; the rows of up to two matrices one after the other.
 // It also clears the status word, unless null.
+constexpr float kLargest = 3.3895313892515355e38f;  // of bfloat16
 template <class T>
 __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack a, const HeadPack b, unsigned* status) {
   if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
@@ -777,7 +828,9 @@ __global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack a, const 
       __nv_bfloat16 t[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        t[i] = __float2bfloat16_rn(v[i]);
+        // finite values that would round to infinity: bfloat16's largest, and a rest
+        const float u = sizeof(T) == 4 && isfinite(v[i]) ? fminf(fmaxf(v[i], -kLargest), kLargest) : v[i];
+        t[i] = __float2bfloat16_rn(u);
         v[i] = z == 0 && !isfinite(v[i]) ? 0.f : v[i] - __bfloat162float(t[i]);
       }
       *reinterpret_cast<uint4*>(to + z * plane + c) = *reinterpret_cast<const uint4*>(t);
