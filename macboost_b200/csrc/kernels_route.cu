@@ -45,6 +45,12 @@ __device__ __forceinline__ float exp_term(float x) {
   return y;
 }
 
+// A choice's weight: 0 where there is none, also beside an infinite logit, whose row's sum is
+// NaN.
+__device__ __forceinline__ float weight(int id, float e, float total) {
+  return id < 0 ? 0.f : e / (total > 0.f || total != total ? total : 1.f);
+}
+
 // A warp's rows (nr x E, row stride ld) between global memory and its tile, whose
 // rows are E | 1 floats apart so that a column is free of bank conflicts.  i / E by
 // a 16-bit reciprocal: exact for i < 512 and E <= 64.
@@ -146,24 +152,25 @@ __global__ void __launch_bounds__(kWarps * 32, E1 && E1 <= 12 ? 12 : 8)
         if (i * L + sub == id) v[i] = -INFINITY;
     }
   }
-  const float over = total > 0.f || total != total ? total : 1.f;
   if constexpr (K > 0) {
     // one store of K values a lane
     if (r < nr) {
       const long long at = (row0 + r) * K;
       if constexpr (K == 2) {
         *reinterpret_cast<int2*>(a.ids + at) = make_int2(my_id[0], my_id[1]);
-        *reinterpret_cast<float2*>(a.weights + at) = make_float2(my_e[0] / over, my_e[1] / over);
+        *reinterpret_cast<float2*>(a.weights + at) =
+            make_float2(weight(my_id[0], my_e[0], total), weight(my_id[1], my_e[1], total));
       } else {
         a.ids[at] = my_id[0];
-        a.weights[at] = my_e[0] / over;
+        a.weights[at] = weight(my_id[0], my_e[0], total);
       }
     }
     return;
   }
   // the group's lanes divide their row's choices by the same total
   __syncwarp();
-  for (int j = sub; j < k; j += L) s_e[warp][r * k + j] = s_e[warp][r * k + j] / over;
+  for (int j = sub; j < k; j += L)
+    s_e[warp][r * k + j] = weight(s_id[warp][r * k + j], s_e[warp][r * k + j], total);
   __syncwarp();
   int* ids = a.ids + row0 * k;
   float* weights = a.weights + row0 * k;
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_wide_kernel(const RouteArgs
   for (int o = 16; o > 0; o /= 2) total += __shfl_xor_sync(~0u, total, o);
   if (lane < k) {
     a.ids[row * k + lane] = id;
-    a.weights[row * k + lane] = e / (total > 0.f || total != total ? total : 1.f);
+    a.weights[row * k + lane] = weight(id, e, total);
   }
 }
 
