@@ -170,7 +170,7 @@ static int check_matrix(const char* name, const void* p, int64_t rows, int64_t c
                         int layout, int dtype, std::string& err) {
   if (ld < (layout == 0 ? rows : cols))
     return fail(err, std::string(name) + (layout == 0 ? " needs ld >= its rows" : " needs ld >= cols"));
-  if (layout == 1 && ld * dtype_bytes(dtype) > kMaxIndex)
+  if (layout == 1 && ld > kMaxIndex / dtype_bytes(dtype))
     return fail(err, std::string(name) + " needs rows of less than 2^31 bytes");
   if (rows > 0 && !p) return fail(err, "null argument");
   if (!aligned(p, size_t(dtype_bytes(dtype))))
