@@ -57,6 +57,16 @@ int32_t guarded(char** err, F call) {
   return -1;
 }
 
+// The same for a size: -1 for what is refused.
+template <class F>
+int64_t guarded_size(F call) {
+  try {
+    return call();
+  } catch (...) {
+    return -1;
+  }
+}
+
 // k and experts as the launches take them; out of int's range they are refused all the same.
 int narrow(int64_t v) { return v < 0 || v > 2147483647 ? -1 : int(v); }
 
@@ -648,7 +658,7 @@ int32_t macboost_route_grad_device(int32_t device, const float* logits, int64_t 
 }
 
 int64_t macboost_sort_rows_workspace(int64_t rows, int64_t k, int64_t experts) {
-  return mb::sort_rows_workspace(rows, k, experts);
+  return guarded_size([&] { return mb::sort_rows_workspace(rows, k, experts); });
 }
 
 int32_t macboost_sort_rows_device(int32_t device, const int32_t* ids, int64_t rows, int64_t k,
@@ -742,7 +752,9 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
 
 int64_t macboost_head_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t classes,
                                 int32_t grad, int32_t strided) {
-  return mb::head_workspace(dtype, rows, cols, classes, grad != 0, strided != 0);
+  return guarded_size([&] {
+    return mb::head_workspace(dtype, rows, cols, classes, grad != 0, strided != 0);
+  });
 }
 
 int32_t macboost_head_loss_device(int32_t device, int32_t dtype, const void* h, int64_t rows,
