@@ -403,7 +403,7 @@ enum { MACBOOST_ROUTE_CHOSEN = 0, MACBOOST_ROUTE_ALL = 1 };
  * logits are never chosen, and a row that runs out of others gets -1 with
  * weight 0.  weights (rows x k float32): softmax over the chosen
  * (MACBOOST_ROUTE_CHOSEN) or the full softmax at the chosen
- * (MACBOOST_ROUTE_ALL). */
+ * (MACBOOST_ROUTE_ALL); NaN at the choices of a row with an infinite logit. */
 int32_t macboost_route_device(int32_t device, const float *logits, int64_t rows, int64_t experts,
                               int64_t ld, int64_t k, int32_t norm, int32_t *ids, float *weights,
                               void *stream, char **err);
@@ -476,7 +476,10 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
  * outputs (class margins, embeddings), without the rows x classes logits in
  * memory.  h is rows x cols (stride ld_h), w classes x cols (stride ld_w), of
  * `dtype` MACBOOST_F32 or MACBOOST_BF16; products and sums are float32 (float32
- * inputs keep 24 bits in every product).  A constant column in h is a bias.
+ * inputs keep 24 bits in every product; sums of bfloat16 products on the tensor cores
+ * are truncated every 16 terms, over all cols for a logit and over at most 32,768 terms
+ * for a gradient, whose parts are then added up).  A constant column in h is a bias;
+ * -inf, or the type's lowest value, in it switches a class off.
  * Conventions as for the rows routed among models; `workspace` is device memory,
  * 256-byte aligned, used until the call's work is done.  Rows that start on 16
  * bytes are read in place, others are copied into the workspace first. */

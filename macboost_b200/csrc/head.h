@@ -53,7 +53,8 @@ constexpr int kHeadTileK = 64;       // one 128-byte swizzle row of 16-bit value
 constexpr int kHeadPair = 2;         // CTAs that share a tile
 constexpr int kHeadEpilogue = 12;    // a tile's epilogue, in steps of one K block
 
-// Division of numbers below 2^31 by a constant: with p = 31 + ceil(log2 d) and m = ceil(2^p
+// Division of numbers below 2^31 by a constant, by multiplication (Granlund and Montgomery,
+// "Division by Invariant Integers using Multiplication", 1994): with p = 31 + ceil(log2 d) and m = ceil(2^p
 // / d), n / d is n m >> p.  A tile's place takes four divisions, and a role that has to
 // divide in full between tiles leaves the tensor cores waiting for about a microsecond.
 struct HeadDiv {
@@ -116,7 +117,7 @@ struct HeadRows {                    // what the logits' epilogues know of each 
   void* g;                           // gradient: planes x rows x ld_g of bfloat16
   long long ld_g, plane_g;
   int rows, classes, v0;             // v0: first class of this piece
-  const float *h, *w;                // float32: the inputs themselves (see redo() there)
+  const float *h, *w;                // float32: the inputs themselves (redo_logits)
   long long ld_h, ld_w;
   int cols;
 };

@@ -15,11 +15,16 @@
 // is small), and the epilogue adds the blocks up in registers, rounded to nearest.  With
 // whole sums in the tensor core, dh of 26 x 12 x 7,798 was off by 2.5e-6.  A stage of the
 // ring holds all three planes of both operands, so a block of K is fetched once for its
-// six products.
+// six products.  Logits that infinities took part in are formed again (redo_logits).
+// bfloat16 sums stay in the tensor core: logits over all columns, the gradients over parts of
+// 2,048 steps (splits_for in head.cpp).
 //
 // Measured without other load: the loss of 8,192 x 1,024 x 131,072 bfloat16 1,633 us (1.35
-// PFLOP/s), g of 16,384 classes 213 us, dh and dw of them 473 us; bound by the transfer of
-// tiles into shared memory (as many stages as three are as fast), in a loop by the power cap.
+// PFLOP/s), g of 16,384 classes 213 us, dh and dw of them 473 us; paced by the copies into
+// shared memory (alone they take 88% of the time, three stages are as fast as six; the tensor
+// pipe is active for 62, 60 and 55% of the cycles), in a loop by the power cap.  float32, 2,048
+// x 1,024 x 32,768: loss 595 us (0.50 ms of bfloat16 products at the measured peak), with
+// gradient 2.65 ms.
 //
 // Every wait ends after wait_ns: the CTA then marks itself dead, sets the status word,
 // waits (as long again at most) for its copies and products in flight and returns (its
@@ -133,7 +138,8 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
       "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
       : "memory");
 }
-// The products issued so far, when done, arrive at this barrier of both CTAs.
+// The products issued so far, when done, arrive at this barrier of both CTAs (the multicast
+// is of the arrival; no copy is).
 __device__ __forceinline__ void commit_both(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
@@ -483,9 +489,6 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
   constexpr int kPlaneA[6] = {2, 1, 0, 1, 0, 0};
   constexpr int kPlaneB[6] = {0, 1, 2, 0, 1, 0};
 
-  // float32: the epilogue keeps 128 sums a thread.  384 threads are launched with 168
-  // registers each (64,512); the first warpgroup keeps 56 a thread and the other two get
-  // 224: 128 x 56 + 256 x 224 = 64,512.
   // float32: the epilogue keeps 128 sums a thread.  384 threads are launched with 168
   // registers each (64,512); the first warpgroup keeps 56 a thread and the other two get
   // 224: 128 x 56 + 256 x 224 = 64,512.

@@ -16,8 +16,8 @@
 // shared memory, since a lane's own loads would touch one 32-byte sector for every few
 // values of a row.  Wider: a warp a row.  Each lane keeps the best two of its values
 // and two reductions name the winner, so a choice is about 20 instructions however wide
-// the row; only a lane that wins a third time looks through its values again.  Lane j
-// keeps choice j, and the exponentials, divisions and stores are one for all choices.
+// the row; a lane that has given both away looks through its values again, and its warp
+// with it.  Lane j keeps choice j, and the exponentials, divisions and stores are one for all choices.
 // All are bound by instructions: 1M x 10, two choices, 14 us and 11 its gradient; 65,537 x
 // 256, eight choices of the full softmax, 48 us (16 lanes a row and a shuffle tree a
 // choice: 70) and 27 its gradient (5 TB/s).

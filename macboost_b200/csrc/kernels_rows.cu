@@ -1,12 +1,13 @@
 // Rows sorted by model, gathered into each model's segment, and the models'
 // outputs combined again, with the gradient (mixture.h).
 //
-// sort     A stable counting sort.  A tile of 4,096 entries belongs to a block, 512
-//          consecutive ones to a warp; lanes with equal ids find each other with a
+// sort     A stable counting sort.  A tile of entries belongs to a block, an eighth of it,
+//          consecutive ones, to a warp; lanes with equal ids find each other with a
 //          match and rank themselves by lane, so an entry's place among its
 //          warp's equals is known without an atomic and the result is the same
-//          every time.  Up to one tile: one launch.  More: counts of each (expert,
-//          tile), their running sums per expert, then the places.
+//          every time.  Up to 4,096 entries are one tile and one launch.  More, in
+//          tiles of 1,024 or 2,048: counts of each (expert, tile), their running sums
+//          per expert, then the places.
 // gather   out[slot] = x[row of the entry in slot], zeros in a slot without entry.
 //          Row-major to row-major reads every row once and writes it to its k
 //          slots; the forms with a feature-major side go through a tile in shared
@@ -901,7 +902,8 @@ cudaError_t combine_k(const CombineArgs& a, bool grad, cudaStream_t s) {
     l.inv = (65536 + l.units - 1) / l.units;
     per = (long long)(kThreads / 32) * l.rows * FLIGHT;
   } else {
-    // one warp a row when there are rows for 16 warps a multiprocessor, else more
+    // as many warps a row as have two units a lane; the gradient, whose sums then meet in
+    // shared memory, takes more than one only until there are 16 warps a multiprocessor
     const long long enough = 16ll * device_sms();
     l.warps = 1;
     while (l.warps < 8 && 64 * l.warps <= l.units && (!grad || a.rows * l.warps < enough)) l.warps *= 2;

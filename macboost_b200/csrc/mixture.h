@@ -51,7 +51,7 @@ struct SortArgs {
   int *counts, *order, *slots;
   int* tile_counts;      // workspace: experts x tiles
 };
-// Launches that a sort of `entries` takes, and the ints of its workspace.
+// The ints of the workspace of a sort of `entries`; 0 for one that is a single launch.
 long long sort_workspace_ints(long long entries, int experts);
 cudaError_t launch_sort(const SortArgs& a, int* launches, cudaStream_t s);
 
