@@ -479,7 +479,8 @@ int32_t macboost_combine_rows_grad_device(int32_t device, int32_t dtype, const v
  * inputs keep 24 bits in every product; sums of bfloat16 products on the tensor cores
  * are truncated every 16 terms, over all cols for a logit and over at most 32,768 terms
  * for a gradient, whose parts are then added up).  A constant column in h is a bias;
- * -inf, or the type's lowest value, in it switches a class off.
+ * the type's lowest value, or -inf, in it switches a class off (for float32 on the
+ * tensor cores each logit of a -inf class takes a sum of its own, a lowest value none).
  * Conventions as for the rows routed among models; `workspace` is device memory,
  * 256-byte aligned, used until the call's work is done.  Rows that start on 16
  * bytes are read in place, others are copied into the workspace first. */
