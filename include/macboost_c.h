@@ -519,6 +519,100 @@ int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void *h, 
  * gradient works from the loss call's lse).  The next loss call starts anew. */
 int32_t macboost_head_check_device(int32_t device, const void *workspace, char **err);
 
+/* ---- a network over the models' outputs (additive) ----------------------- */
+
+/* What stands between the forests and the softmax head when more than a linear
+ * layer is trained on them: embeddings of the leaves that rows reach
+ * (MACBOOST_KIND_LEAF), of categories or of tokens; a gated feed-forward block; and
+ * the norm of all gradients with their clipping before an update.  Conventions as
+ * for the rows routed among models: device memory, enqueued on `stream`, nothing
+ * allocated, results that do not depend on timing, sums in float32 rounded once. */
+
+/* out[n] = scale * sum over j of table[starts[j] + ids[n, j]], for rows rows of k
+ * int32 ids.  table is entries x cols (entries below 2^30, stride ld), out rows x
+ * cols (stride ld_out), both of `dtype`.  starts (k int32; NULL: zeros) is the
+ * first row of each column of ids, so that one table holds all trees' nodes:
+ * starts[j] = j * nodes.  An id that is negative, or that leads to no row of the
+ * table, adds nothing; k = 1 is a plain lookup. */
+int32_t macboost_embed_device(int32_t device, int32_t dtype, const void *table, int64_t entries,
+                              int64_t cols, int64_t ld, const int32_t *ids, int64_t rows,
+                              int64_t k, const int32_t *starts, float scale, void *out,
+                              int64_t ld_out, void *stream, char **err);
+
+/* Bytes of workspace for macboost_embed_grad_device; -1 for arguments it refuses. */
+int64_t macboost_embed_workspace(int64_t entries, int64_t cols, int64_t rows, int64_t k);
+
+/* Gradient of macboost_embed_device for dout (rows x cols, stride ld_dout): dtable
+ * (entries x cols, stride ld) = scale * the sum of dout[n] over the ids that led to
+ * each row, zeros in rows that none led to.  The ids are sorted first; `workspace`
+ * is device memory, 256-byte aligned, used until the call's work is done. */
+int32_t macboost_embed_grad_device(int32_t device, int32_t dtype, const void *dout, int64_t rows,
+                                   int64_t cols, int64_t ld_dout, const int32_t *ids, int64_t k,
+                                   const int32_t *starts, float scale, void *dtable,
+                                   int64_t entries, int64_t ld, void *workspace,
+                                   int64_t workspace_bytes, void *stream, char **err);
+
+/* Activations of a gated block: x / (1 + exp(-x)); x times the normal distribution
+ * function of x; the same by its tanh approximation, 0.5 x (1 + tanh(sqrt(2 / pi)
+ * (x + 0.044715 x^3))). */
+enum { MACBOOST_ACT_SILU = 0, MACBOOST_ACT_GELU = 1, MACBOOST_ACT_GELU_TANH = 2 };
+
+/* Bytes of workspace for macboost_ffn_device, or for both calls when `grad` is
+ * non-zero; -1 for arguments they refuse.  `strided` non-zero: also when cols, width
+ * and outs are multiples of 8 but rows of a matrix do not start on 16 bytes. */
+int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t width,
+                               int64_t outs, int32_t grad, int32_t strided);
+
+/* A gated feed-forward block: hidden = act(x Wg^T) * (x Wu^T), y = hidden Wo^T.
+ * x is rows x cols, w_in 2 width x cols (the rows of Wg, then those of Wu), w_out
+ * outs x width, hidden rows x width, y rows x outs, of `dtype` MACBOOST_F32 or
+ * MACBOOST_BF16, each with a stride.  pre (rows x 2 width: x w_in^T), unless NULL,
+ * is kept for the gradient.  Products and sums are float32 (float32 inputs keep 24
+ * bits in every product; bfloat16 sums on the tensor cores as in the head); the
+ * activation and the factor are formed in float32, and hidden is rounded to `dtype`
+ * before the second product.  A row whose x is not finite has values that are not
+ * finite, and NaN where the formula may have an infinity; other rows do not see it.
+ * `workspace` as for the head. */
+int32_t macboost_ffn_device(int32_t device, int32_t dtype, int32_t act, const void *x,
+                            int64_t rows, int64_t cols, int64_t ld_x, const void *w_in,
+                            int64_t width, int64_t ld_in, const void *w_out, int64_t outs,
+                            int64_t ld_out, void *hidden, int64_t ld_hidden, void *pre,
+                            int64_t ld_pre, void *y, int64_t ld_y, void *workspace,
+                            int64_t workspace_bytes, void *stream, char **err);
+
+/* Gradients of macboost_ffn_device for dy (rows x outs), from the hidden and pre that
+ * it wrote: dx (rows x cols), dw_in (2 width x cols) and dw_out (outs x width); each
+ * may be NULL.  The gradients of both halves of pre are rounded to bfloat16 for
+ * bfloat16 inputs, and held in three bfloat16 terms (24 bits) for float32. */
+int32_t macboost_ffn_grad_device(int32_t device, int32_t dtype, int32_t act, const void *x,
+                                 int64_t rows, int64_t cols, int64_t ld_x, const void *w_in,
+                                 int64_t width, int64_t ld_in, const void *w_out, int64_t outs,
+                                 int64_t ld_out, const void *hidden, int64_t ld_hidden,
+                                 const void *pre, int64_t ld_pre, const void *dy, int64_t ld_dy,
+                                 void *dx, int64_t ld_dx, void *dw_in, int64_t ld_din,
+                                 void *dw_out, int64_t ld_dout, void *workspace,
+                                 int64_t workspace_bytes, void *stream, char **err);
+
+/* Synchronise `device` and report whether the last macboost_ffn_device with this
+ * workspace, or a gradient call since, gave up waiting. */
+int32_t macboost_ffn_check_device(int32_t device, const void *workspace, char **err);
+
+/* Bytes of workspace for macboost_clip_device; -1 for lists it refuses. */
+int64_t macboost_clip_workspace(int64_t count, const int32_t *dtypes, const int64_t *sizes);
+
+/* norm (one float32 on the device) = the square root of the sum of squares of all
+ * values of `count` gradients; then, unless outs is NULL, outs[i] = grads[i] * (norm
+ * > max_norm ? max_norm / norm : 1), rounded once (NaN everywhere for a norm that is
+ * NaN).  dtypes, grads, sizes (values, each gradient without gaps) and outs are host
+ * arrays, free again when the call returns; grads[i] and outs[i] are device memory,
+ * either the same (then a factor of 1 writes nothing) or apart.  Squares are added up
+ * so that nothing overflows or vanishes that float32 holds as a norm.  `workspace` is
+ * device memory, 8-byte aligned, used until the call's work is done. */
+int32_t macboost_clip_device(int32_t device, int64_t count, const int32_t *dtypes,
+                             const void *const *grads, const int64_t *sizes, void *const *outs,
+                             double max_norm, float *norm, void *workspace,
+                             int64_t workspace_bytes, void *stream, char **err);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ KIND_PREDICT, KIND_RAW, KIND_PROBA, KIND_LEAF, KIND_CLI = 0, 1, 2, 3, 4
 LAYOUT_FEATURE_MAJOR, LAYOUT_ROW_MAJOR = 0, 1
 F32, BF16, F16 = 0, 1, 2
 ROUTE_CHOSEN, ROUTE_ALL = 0, 1
+ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2
 FORMATS = {"csv": 0, "tsv": 0, "libsvm": 1, "auto": 2}
 
 _PKG = Path(__file__).resolve().parent
@@ -130,6 +131,22 @@ def _configure(lib):
         "macboost_head_grad_device": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, P, P, P, P,
                                             I64, P, I64, P, I64, P, _c_char_pp]),
         "macboost_head_check_device": (I32, [I32, P, _c_char_pp]),
+        "macboost_embed_device": (I32, [I32, I32, P, I64, I64, I64, P, I64, I64, P,
+                                        ctypes.c_float, P, I64, P, _c_char_pp]),
+        "macboost_embed_workspace": (I64, [I64, I64, I64, I64]),
+        "macboost_embed_grad_device": (I32, [I32, I32, P, I64, I64, I64, P, I64, P,
+                                             ctypes.c_float, P, I64, I64, P, I64, P,
+                                             _c_char_pp]),
+        "macboost_ffn_workspace": (I64, [I32, I64, I64, I64, I64, I32, I32]),
+        "macboost_ffn_device": (I32, [I32, I32, I32, P, I64, I64, I64, P, I64, I64, P, I64, I64,
+                                      P, I64, P, I64, P, I64, P, I64, P, _c_char_pp]),
+        "macboost_ffn_grad_device": (I32, [I32, I32, I32, P, I64, I64, I64, P, I64, I64, P, I64,
+                                           I64, P, I64, P, I64, P, I64, P, I64, P, I64, P, I64,
+                                           P, I64, P, _c_char_pp]),
+        "macboost_ffn_check_device": (I32, [I32, P, _c_char_pp]),
+        "macboost_clip_workspace": (I64, [I64, P, P]),
+        "macboost_clip_device": (I32, [I32, I64, P, P, P, P, ctypes.c_double, P, P, I64, P,
+                                       _c_char_pp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -794,3 +811,111 @@ def head_check_device(device: int, workspace_ptr: int) -> None:
     """Synchronise and raise if the last loss call with this workspace, or a gradient call
     since, gave up waiting."""
     _enqueue(_lib.macboost_head_check_device, device, workspace_ptr)
+
+
+# ---- a network over the models' outputs (device pointers, enqueued on `stream`) ----
+
+def embed_device(device: int, dtype: int, table_ptr: int, entries: int, cols: int, ld: int,
+                 ids_ptr: int, rows: int, k: int, starts_ptr: int | None, scale: float,
+                 out_ptr: int, ld_out: int, stream: int = 0) -> None:
+    """out[n] = scale * sum over j of table[starts[j] + ids[n, j]] (starts 0/None: zeros);
+    negative ids, and those that lead to no row of the table, add nothing."""
+    _enqueue(_lib.macboost_embed_device, device, dtype, table_ptr, entries, cols, ld, ids_ptr, rows,
+             k, starts_ptr or None, scale, out_ptr, ld_out, stream or None)
+
+
+def embed_workspace(entries: int, cols: int, rows: int, k: int) -> int:
+    """Bytes of device workspace for embed_grad_device."""
+    n = _lib.macboost_embed_workspace(entries, cols, rows, k)
+    if n < 0:
+        raise MacBoostError(f"no embedding of entries={entries}, cols={cols}, rows={rows}, k={k}")
+    return n
+
+
+def embed_grad_device(device: int, dtype: int, dout_ptr: int, rows: int, cols: int, ld_dout: int,
+                      ids_ptr: int, k: int, starts_ptr: int | None, scale: float, dtable_ptr: int,
+                      entries: int, ld: int, workspace_ptr: int, workspace_bytes: int,
+                      stream: int = 0) -> None:
+    """Gradient of embed_device: dtable (entries x cols) from dout (rows x cols)."""
+    _enqueue(_lib.macboost_embed_grad_device, device, dtype, dout_ptr, rows, cols, ld_dout, ids_ptr,
+             k, starts_ptr or None, scale, dtable_ptr, entries, ld, workspace_ptr, workspace_bytes,
+             stream or None)
+
+
+def ffn_workspace(dtype: int, rows: int, cols: int, width: int, outs: int, grad: bool = False,
+                  strided: bool = False) -> int:
+    """Bytes of device workspace for ffn_device (grad: and ffn_grad_device); strided: rows
+    of a matrix may start off a 16-byte boundary."""
+    n = _lib.macboost_ffn_workspace(dtype, rows, cols, width, outs, int(grad), int(strided))
+    if n < 0:
+        raise MacBoostError(f"no block of dtype={dtype}, rows={rows}, cols={cols}, width={width}, "
+                            f"outs={outs}")
+    return n
+
+
+def ffn_device(device: int, dtype: int, act: int, x_ptr: int, rows: int, cols: int, ld_x: int,
+               w_in_ptr: int, width: int, ld_in: int, w_out_ptr: int, outs: int, ld_out: int,
+               hidden_ptr: int, ld_hidden: int, pre_ptr: int | None, ld_pre: int, y_ptr: int,
+               ld_y: int, workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """hidden = act(x Wg^T) * (x Wu^T) and y = hidden Wo^T, with w_in = (Wg, Wu) (2 width x
+    cols), w_out = Wo (outs x width); pre (x w_in^T, 0/None: not kept) is for the gradient."""
+    _enqueue(_lib.macboost_ffn_device, device, dtype, act, x_ptr, rows, cols, ld_x, w_in_ptr, width,
+             ld_in, w_out_ptr, outs, ld_out, hidden_ptr, ld_hidden, pre_ptr or None, ld_pre, y_ptr,
+             ld_y, workspace_ptr, workspace_bytes, stream or None)
+
+
+def ffn_grad_device(device: int, dtype: int, act: int, x_ptr: int, rows: int, cols: int, ld_x: int,
+                    w_in_ptr: int, width: int, ld_in: int, w_out_ptr: int, outs: int, ld_out: int,
+                    hidden_ptr: int, ld_hidden: int, pre_ptr: int, ld_pre: int, dy_ptr: int,
+                    ld_dy: int, dx_ptr: int | None, ld_dx: int, dw_in_ptr: int | None, ld_din: int,
+                    dw_out_ptr: int | None, ld_dout: int, workspace_ptr: int,
+                    workspace_bytes: int, stream: int = 0) -> None:
+    """Gradients dx, dw_in and dw_out (each may be 0/None) of ffn_device for dy, from the
+    hidden and pre that it wrote."""
+    _enqueue(_lib.macboost_ffn_grad_device, device, dtype, act, x_ptr, rows, cols, ld_x, w_in_ptr,
+             width, ld_in, w_out_ptr, outs, ld_out, hidden_ptr, ld_hidden, pre_ptr, ld_pre, dy_ptr,
+             ld_dy, dx_ptr or None, ld_dx, dw_in_ptr or None, ld_din, dw_out_ptr or None, ld_dout,
+             workspace_ptr, workspace_bytes, stream or None)
+
+
+def ffn_check_device(device: int, workspace_ptr: int) -> None:
+    """Synchronise and raise if the last ffn_device with this workspace, or a gradient call
+    since, gave up waiting."""
+    _enqueue(_lib.macboost_ffn_check_device, device, workspace_ptr)
+
+
+class GradientList:
+    """Gradients for clip_device: their dtypes (F32, BF16 or F16), addresses and numbers of
+    values, and where the clipped ones go (outs None: only the norm is wanted; the
+    gradients' own addresses: in place).  Host memory only; kept from step to step by a
+    program whose gradients stay where they are."""
+
+    def __init__(self, dtypes, grads, sizes, outs=None):
+        self.count = len(grads)
+        self.dtypes = np.ascontiguousarray(dtypes, dtype=np.int32)
+        self.grads = np.ascontiguousarray(grads, dtype=np.uint64)
+        self.sizes = np.ascontiguousarray(sizes, dtype=np.int64)
+        self.outs = None if outs is None else np.ascontiguousarray(outs, dtype=np.uint64)
+        for a in (self.dtypes, self.grads, self.sizes, self.outs):
+            if a is not None and a.shape != (self.count,):
+                raise ValueError(f"{self.count} gradients, but {a.size} of dtypes, sizes or outs")
+
+
+def clip_workspace(gradients: GradientList) -> int:
+    """Bytes of device workspace for clip_device."""
+    n = _lib.macboost_clip_workspace(gradients.count, gradients.dtypes.ctypes.data,
+                                     gradients.sizes.ctypes.data)
+    if n < 0:
+        raise MacBoostError(f"cannot clip a list of {gradients.count} gradients: unknown dtypes, "
+                            "or sizes out of range")
+    return n
+
+
+def clip_device(device: int, gradients: GradientList, max_norm: float, norm_ptr: int,
+                workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
+    """norm (a float32 on the device) of all gradients taken together, and the gradients
+    times min(1, max_norm / norm)."""
+    g = gradients
+    _enqueue(_lib.macboost_clip_device, device, g.count, g.dtypes.ctypes.data, g.grads.ctypes.data,
+             g.sizes.ctypes.data, None if g.outs is None else g.outs.ctypes.data, max_norm, norm_ptr,
+             workspace_ptr or None, workspace_bytes, stream or None)

@@ -13,7 +13,10 @@
 
 #include "../../include/macboost_c.h"
 #include "binned.h"
+#include "clip.h"
+#include "embed.h"
 #include "engine.h"
+#include "ffn.h"
 #include "head.h"
 #include "mixture.h"
 #include "table.h"
@@ -813,6 +816,165 @@ int32_t macboost_head_grad_device(int32_t device, int32_t dtype, const void* h, 
 int32_t macboost_head_check_device(int32_t device, const void* workspace, char** err) {
   return guarded(err, [&](std::string& e) {
     return mb::head_check_device(device, workspace, e);
+  });
+}
+
+int32_t macboost_embed_device(int32_t device, int32_t dtype, const void* table, int64_t entries,
+                              int64_t cols, int64_t ld, const int32_t* ids, int64_t rows,
+                              int64_t k, const int32_t* starts, float scale, void* out,
+                              int64_t ld_out, void* stream, char** err) {
+  mb::EmbedArgs a{};
+  a.dtype = dtype;
+  a.table = table;
+  a.entries = entries;
+  a.cols = cols;
+  a.ld = ld;
+  a.ids = ids;
+  a.rows = rows;
+  a.k = k;
+  a.starts = starts;
+  a.scale = scale;
+  a.out = out;
+  a.ld_out = ld_out;
+  return guarded(err, [&](std::string& e) {
+    return mb::embed_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
+}
+
+int64_t macboost_embed_workspace(int64_t entries, int64_t cols, int64_t rows, int64_t k) {
+  return guarded_size([&] { return mb::embed_workspace(entries, cols, rows, k); });
+}
+
+int32_t macboost_embed_grad_device(int32_t device, int32_t dtype, const void* dout, int64_t rows,
+                                   int64_t cols, int64_t ld_dout, const int32_t* ids, int64_t k,
+                                   const int32_t* starts, float scale, void* dtable,
+                                   int64_t entries, int64_t ld, void* workspace,
+                                   int64_t workspace_bytes, void* stream, char** err) {
+  mb::EmbedArgs a{};
+  a.dtype = dtype;
+  a.dout = dout;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld_out = ld_dout;
+  a.ids = ids;
+  a.k = k;
+  a.starts = starts;
+  a.scale = scale;
+  a.dtable = dtable;
+  a.entries = entries;
+  a.ld = ld;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return guarded(err, [&](std::string& e) {
+    return mb::embed_grad_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
+}
+
+int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_t width,
+                               int64_t outs, int32_t grad, int32_t strided) {
+  return guarded_size([&] {
+    return mb::ffn_workspace(dtype, rows, cols, width, outs, grad != 0, strided != 0);
+  });
+}
+
+int32_t macboost_ffn_device(int32_t device, int32_t dtype, int32_t act, const void* x,
+                            int64_t rows, int64_t cols, int64_t ld_x, const void* w_in,
+                            int64_t width, int64_t ld_in, const void* w_out, int64_t outs,
+                            int64_t ld_out, void* hidden, int64_t ld_hidden, void* pre,
+                            int64_t ld_pre, void* y, int64_t ld_y, void* workspace,
+                            int64_t workspace_bytes, void* stream, char** err) {
+  mb::FfnArgs a;
+  a.dtype = dtype;
+  a.act = act;
+  a.x = x;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld_x = ld_x;
+  a.w_in = w_in;
+  a.width = width;
+  a.ld_in = ld_in;
+  a.w_out = w_out;
+  a.outs = outs;
+  a.ld_out = ld_out;
+  a.hidden = hidden;
+  a.ld_hidden = ld_hidden;
+  a.pre = pre;
+  a.ld_pre = ld_pre;
+  a.y = y;
+  a.ld_y = ld_y;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return guarded(err, [&](std::string& e) {
+    return mb::ffn_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
+}
+
+int32_t macboost_ffn_grad_device(int32_t device, int32_t dtype, int32_t act, const void* x,
+                                 int64_t rows, int64_t cols, int64_t ld_x, const void* w_in,
+                                 int64_t width, int64_t ld_in, const void* w_out, int64_t outs,
+                                 int64_t ld_out, const void* hidden, int64_t ld_hidden,
+                                 const void* pre, int64_t ld_pre, const void* dy, int64_t ld_dy,
+                                 void* dx, int64_t ld_dx, void* dw_in, int64_t ld_din,
+                                 void* dw_out, int64_t ld_dout, void* workspace,
+                                 int64_t workspace_bytes, void* stream, char** err) {
+  mb::FfnArgs a;
+  a.dtype = dtype;
+  a.act = act;
+  a.x = x;
+  a.rows = rows;
+  a.cols = cols;
+  a.ld_x = ld_x;
+  a.w_in = w_in;
+  a.width = width;
+  a.ld_in = ld_in;
+  a.w_out = w_out;
+  a.outs = outs;
+  a.ld_out = ld_out;
+  a.hidden = const_cast<void*>(hidden);
+  a.ld_hidden = ld_hidden;
+  a.pre = const_cast<void*>(pre);
+  a.ld_pre = ld_pre;
+  a.dy = dy;
+  a.ld_dy = ld_dy;
+  a.dx = dx;
+  a.ld_dx = ld_dx;
+  a.dw_in = dw_in;
+  a.ld_din = ld_din;
+  a.dw_out = dw_out;
+  a.ld_dout = ld_dout;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return guarded(err, [&](std::string& e) {
+    return mb::ffn_grad_device(device, a, static_cast<cudaStream_t>(stream), e);
+  });
+}
+
+int32_t macboost_ffn_check_device(int32_t device, const void* workspace, char** err) {
+  return guarded(err, [&](std::string& e) {
+    return mb::ffn_check_device(device, workspace, e);
+  });
+}
+
+int64_t macboost_clip_workspace(int64_t count, const int32_t* dtypes, const int64_t* sizes) {
+  return guarded_size([&] { return mb::clip_workspace(count, dtypes, sizes); });
+}
+
+int32_t macboost_clip_device(int32_t device, int64_t count, const int32_t* dtypes,
+                             const void* const* grads, const int64_t* sizes, void* const* outs,
+                             double max_norm, float* norm, void* workspace,
+                             int64_t workspace_bytes, void* stream, char** err) {
+  mb::ClipArgs a{};
+  a.count = count;
+  a.dtypes = dtypes;
+  a.grads = grads;
+  a.sizes = sizes;
+  a.outs = outs;
+  a.max_norm = max_norm;
+  a.norm = norm;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  return guarded(err, [&](std::string& e) {
+    return mb::clip_device(device, a, static_cast<cudaStream_t>(stream), e);
   });
 }
 

@@ -1,0 +1,64 @@
+// The norm of many gradients taken together, and their clipping.
+//
+//   norm = sqrt(sum over all tensors and values of g^2)
+//   factor = max_norm / norm where norm > max_norm, else 1 (NaN for a norm that is NaN)
+//   out = factor * g, rounded once
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+namespace mb {
+
+struct ClipArgs {
+  int64_t count;
+  const int32_t* dtypes;          // host arrays of `count`
+  const void* const* grads;
+  const int64_t* sizes;
+  void* const* outs;              // null: only the norm
+  double max_norm;
+  float* norm;                    // device
+  void* workspace;
+  int64_t workspace_bytes;
+};
+
+int64_t clip_workspace(int64_t count, const int32_t* dtypes, const int64_t* sizes);
+int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err);
+
+// ---- between clip.cpp and kernels_clip.cu -----------------------------------------
+
+// A tensor's values in chunks, a chunk a block's at a time.  Tables of tensors travel as a
+// launch's parameters (at most 32,764 bytes): nothing is copied to the device first, so a
+// captured graph holds its tables.
+constexpr int kClipChunk = 32 * 1024;      // bytes
+constexpr int kClipTensors = 1024;         // of a launch
+constexpr int kClipFew = 64;               // of a launch with a small table
+constexpr int kClipBlocks = 592;           // of a launch, at most: four a multiprocessor
+
+template <int N>
+struct ClipTable {
+  const void* src[N];
+  void* dst[N];                            // may equal src
+  long long size[N];
+  unsigned chunk0[N];                      // the tensor's first chunk
+  unsigned char dtype[N];
+  int tensors;
+  unsigned chunks;
+};
+
+struct ClipState {
+  double* part;                            // a block's sum of squares, of all launches
+  int parts, first;                        // of all launches; this launch's first
+  double max_norm;
+  float* norm;
+  int in_place;                            // every dst is its src: a factor of 1 writes nothing
+};
+template <int N>
+cudaError_t launch_clip_norm(const ClipTable<N>& t, const ClipState& c, int blocks, cudaStream_t s);
+template <int N>
+cudaError_t launch_clip_scale(const ClipTable<N>& t, const ClipState& c, int blocks, cudaStream_t s);
+cudaError_t launch_clip_finish(const ClipState& c, cudaStream_t s);
+
+}  // namespace mb

@@ -1,0 +1,429 @@
+// Host side of the gated block (ffn.h): argument checks, the plan of tiles and splits, and
+// launches.  Its products are tiles of the head's kernel (head.h).
+#include "ffn.h"
+
+#include <algorithm>
+#include <climits>
+
+#include "engine.h"
+#include "head.h"
+#include "mixture.h"
+
+namespace mb {
+
+namespace {
+
+// Tile rows walked together keep about this much of A in the L2 cache (126 MB).
+constexpr int64_t kGroupBytes = int64_t(32) << 20;
+constexpr int64_t kTileM = kHeadPair * kHeadTileM;
+
+int fail(std::string& err, const std::string& msg) {
+  err = msg;
+  return -1;
+}
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t parts(int64_t v, int64_t m) { return (v + m - 1) / m; }
+
+struct Guard {
+  int prev = -1, want;
+  explicit Guard(int d) : want(d) {
+    cudaGetDevice(&prev);
+    if (prev != d) cudaSetDevice(d);
+  }
+  ~Guard() {
+    if (prev >= 0 && prev != want) cudaSetDevice(prev);
+  }
+};
+
+#define FFN_CUDA(call, what)                                                      \
+  do {                                                                            \
+    const cudaError_t e_ = (call);                                                \
+    if (e_ != cudaSuccess) {                                                      \
+      cudaGetLastError();                                                         \
+      return fail(err, std::string(what) + ": " + cudaGetErrorString(e_));        \
+    }                                                                             \
+  } while (0)
+
+// ---- the plan -------------------------------------------------------------------
+
+bool is_few(int64_t rows, int64_t cols, int64_t width) {
+  int64_t n = 1;
+  while (n < rows) n *= 2;
+  return rows <= kFfnFewRows && n * ffn_pitch(std::max(cols, width)) * 4 <= kFfnFewSmem;
+}
+
+// A product's tiles.
+struct Shape {
+  int64_t m, n, k;
+  int tile_n, splits;
+  int box;                           // rows of a K-major B that a CTA fetches
+  int64_t weight(int dtype) const {  // steps of all its tiles
+    return parts(m, kTileM) * parts(n, tile_n) * (parts(k, kHeadTileK) * (dtype == kF32 ? 6 : 1) + kHeadEpilogue);
+  }
+};
+Shape shape(int64_t m, int64_t n, int64_t k) {
+  const int tile = n <= 128 ? 128 : 256;
+  return Shape{m, n, k, tile, 1, tile / kHeadPair};
+}
+
+struct Plan {
+  Shape y, dx, dw_in, dw_out;
+  // offsets into the workspace, 0 for none: packed operands, sums of parts of K
+  int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, bytes = 0;
+  int64_t part = 0, part_in = 0;     // y's, dw_out's or dx's; dw_in's
+  int64_t ld_d = 0;
+};
+
+struct Packed {
+  bool x, w_in, w_out, hidden, dy;
+};
+
+Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t outs, bool grad, const Packed& pk) {
+  Plan p{};
+  const int64_t planes = dtype == kF32 ? 3 : 1;
+  int64_t at = 256;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  auto packed = [&](int64_t r, int64_t c) { return take(planes * r * up(c, 8) * 2); };
+  if (pk.x) p.x = packed(rows, cols);
+  if (pk.w_in) p.w_in = packed(2 * width, cols);
+  if (pk.w_out) p.w_out = packed(outs, width);
+  if (pk.hidden) p.hidden = packed(rows, width);
+  auto sums = [&](const Shape& q) { return q.splits > 1 ? q.splits * q.m * q.n * 4 : 0; };
+  auto split = [&](Shape& q, int64_t all) { q.splits = head_splits(parts(q.k, kHeadTileK), all, dtype); };
+  if (!grad) {
+    p.y = shape(rows, outs, width);
+    split(p.y, p.y.weight(dtype));
+    p.part = take(sums(p.y));
+  } else {
+    if (pk.dy) p.dy = packed(rows, outs);
+    p.ld_d = up(2 * width, 8);
+    p.dpre = take(planes * rows * p.ld_d * 2);
+    p.dx = shape(rows, cols, 2 * width);
+    p.dw_in = shape(2 * width, cols, rows);
+    p.dw_out = shape(outs, width, rows);
+    const int64_t both = p.dx.weight(dtype) + p.dw_in.weight(dtype);
+    split(p.dx, both);
+    split(p.dw_in, both);
+    split(p.dw_out, p.dw_out.weight(dtype));
+    // dw_out is done before the others begin
+    p.part = take(std::max(sums(p.dw_out), sums(p.dx)));
+    p.part_in = take(sums(p.dw_in));
+  }
+  p.bytes = at;
+  return p;
+}
+
+// ---- checks ---------------------------------------------------------------------
+
+int check_shape(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t outs, std::string& err) {
+  if (dtype != kF32 && dtype != kBF16)
+    return fail(err, "the block takes dtype 0 (float32) or 1 (bfloat16), got " + std::to_string(dtype));
+  if (rows < 0 || rows > (int64_t(1) << 30)) return fail(err, "rows must be in 0...2^30");
+  if (cols < 1 || cols > (int64_t(1) << 20)) return fail(err, "cols must be in 1...2^20");
+  if (width < 1 || width > (int64_t(1) << 20)) return fail(err, "width must be in 1...2^20");
+  if (outs < 1 || outs > (int64_t(1) << 20)) return fail(err, "outs must be in 1...2^20");
+  const int64_t tiles = parts(rows, kTileM) * parts(2 * std::max({cols, width, outs}), 128);
+  if (tiles > INT_MAX) return fail(err, "rows * width are too many for one call");
+  return 0;
+}
+
+int check_matrix(const char* name, const void* p, int64_t cols, int64_t ld, int dtype, std::string& err) {
+  if (!p) return fail(err, "null argument");
+  if (ld < cols) return fail(err, std::string(name) + " needs a stride of at least its columns");
+  if (ld > (int64_t(1) << 31)) return fail(err, std::string(name) + " needs a stride of at most 2^31");
+  if (!aligned(p, size_t(dtype_bytes(dtype))))
+    return fail(err, std::string(name) + " must be aligned to its values");
+  return 0;
+}
+
+int check(const FfnArgs& a, bool grad, std::string& err) {
+  if (check_shape(a.dtype, a.rows, a.cols, a.width, a.outs, err)) return -1;
+  if (a.act < kSilu || a.act > kGeluTanh)
+    return fail(err, "unknown activation " + std::to_string(a.act) + " (0 silu, 1 gelu, 2 gelu_tanh)");
+  if (a.rows > 0) {
+    if (check_matrix("x", a.x, a.cols, a.ld_x, a.dtype, err) ||
+        check_matrix("w_in", a.w_in, a.cols, a.ld_in, a.dtype, err) ||
+        check_matrix("w_out", a.w_out, a.width, a.ld_out, a.dtype, err) ||
+        check_matrix("hidden", a.hidden, a.width, a.ld_hidden, a.dtype, err))
+      return -1;
+    if ((grad || a.pre) && check_matrix("pre", a.pre, 2 * a.width, a.ld_pre, a.dtype, err)) return -1;
+    if (!grad && check_matrix("y", a.y, a.outs, a.ld_y, a.dtype, err)) return -1;
+    if (grad && check_matrix("dy", a.dy, a.outs, a.ld_dy, a.dtype, err)) return -1;
+    if (grad && a.dx && check_matrix("dx", a.dx, a.cols, a.ld_dx, a.dtype, err)) return -1;
+  }
+  if (grad && a.dw_in && check_matrix("dw_in", a.dw_in, a.cols, a.ld_din, a.dtype, err)) return -1;
+  if (grad && a.dw_out && check_matrix("dw_out", a.dw_out, a.width, a.ld_dout, a.dtype, err)) return -1;
+  if (!aligned(a.workspace, 256)) return fail(err, "workspace must be 256-byte aligned");
+  return 0;
+}
+
+int check_workspace(const FfnArgs& a, int64_t need, std::string& err) {
+  if (a.workspace && a.workspace_bytes >= need) return 0;
+  return fail(err, "workspace holds " + std::to_string(a.workspace ? a.workspace_bytes : 0) +
+                       " bytes, the block needs " + std::to_string(need));
+}
+
+// ---- operands and products --------------------------------------------------------
+
+// A matrix as the tiles read it: in place, or packed into the workspace.
+struct Operand {
+  const void* p = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0;
+};
+
+struct Call {
+  const FfnArgs& a;
+  const Plan& p;
+  cudaStream_t s;
+  std::string& err;
+  int64_t launches = 0;
+  char* base() const { return static_cast<char*>(a.workspace); }
+  int planes() const { return a.dtype == kF32 ? 3 : 1; }
+
+  Operand operand(const void* src, int64_t rows, int64_t cols, int64_t ld, int64_t at, HeadPack* todo) const {
+    Operand o{src, rows, cols, ld};
+    if (at) {
+      o.p = base() + at;
+      o.ld = up(cols, 8);
+      todo->src = src;
+      todo->rows = rows;
+      todo->cols = cols;
+      todo->ld = ld;
+      todo->dst = base() + at;
+      todo->ldp = o.ld;
+    }
+    return o;
+  }
+  // Up to two matrices, in one launch; `status`: it clears the status word as well.
+  int pack(const HeadPack& q, const HeadPack& r, bool status) {
+    unsigned* word = static_cast<unsigned*>(a.workspace);
+    if (!q.src && !r.src) {
+      if (status) FFN_CUDA(cudaMemsetAsync(word, 0, 4, s), "clearing the block's status word");
+      return 0;
+    }
+    FFN_CUDA(launch_head_pack(a.dtype, q, r, status ? word : nullptr, s), "pack launch");
+    ++launches;
+    return 0;
+  }
+  // C = A B^T along K; mn: the operand's rows are K, its columns C's rows (columns).
+  int job(HeadJob& j, const Operand& A, bool a_mn, const Operand& B, bool b_mn, const Shape& h) {
+    j.a_mn = a_mn;
+    j.b_mn = b_mn;
+    j.a_box = a_mn ? 64 : head_box_rows(A.rows, kHeadTileM);
+    j.b_box = b_mn ? 64 : head_box_rows(h.n, h.box);
+    if (head_encode(&j.a, A.p, A.cols, A.rows, A.ld, planes(), j.a_box, err) ||
+        head_encode(&j.b, B.p, B.cols, B.rows, B.ld, planes(), j.b_box, err))
+      return -1;
+    j.tiles_m = int(parts(h.m, kTileM));
+    j.tiles_n = int(parts(h.n, h.tile_n));
+    j.kblocks = int(parts(h.k, kHeadTileK));
+    j.splits = std::min(h.splits, j.kblocks);
+    j.M = int(h.m);
+    j.N = int(h.n);
+    // tile rows whose part of A stays in the L2 cache while the columns go by
+    const int64_t bytes = kTileM * int64_t(j.kblocks / j.splits) * kHeadTileK * 2 * planes();
+    j.group = int(std::max<int64_t>(1, std::min<int64_t>({kGroupBytes / std::max<int64_t>(bytes, 1), 16, j.tiles_m})));
+    j.divide();
+    return 0;
+  }
+  // Where a product goes, by way of sums of parts of K if it is split.
+  void target(HeadJob& j, const Shape& h, void* out, int64_t ld, int64_t part, HeadReduce* red, int* reds) const {
+    j.out = out;
+    j.ld_out = ld;
+    j.out_f32 = a.dtype == kF32;
+    j.wide = aligned(out, size_t(4 * dtype_bytes(a.dtype))) && ld % 4 == 0;
+    j.final = 1;
+    if (j.splits > 1) {
+      j.acc = reinterpret_cast<float*>(base() + part);
+      j.final = 0;
+      red[(*reds)++] = HeadReduce{j.acc, j.splits, h.m, h.n, nullptr, 0, 1, out, ld, j.out_f32};
+    }
+  }
+  int products(HeadLaunch& l, int tile_n, const HeadReduce* red, int reds) {
+    FFN_CUDA(launch_head(kHeadOut, tile_n, l, s), "block launch");
+    for (int r = 0; r < reds; ++r) FFN_CUDA(launch_head_reduce(red[r], s), "block reduce launch");
+    launches += 1 + reds;
+    return 0;
+  }
+};
+
+// What both gated epilogues know.
+void gate(HeadGate& g, const FfnArgs& a) {
+  g.act = a.act;
+  g.width = int(a.width);
+  g.rows = int(a.rows);
+  g.hidden = a.hidden;
+  g.ld_hidden = a.ld_hidden;
+  g.pre = a.pre;
+  g.ld_pre = a.ld_pre;
+  const int64_t per = 16 / dtype_bytes(a.dtype);
+  g.wide = aligned(a.hidden, 16) && a.ld_hidden % per == 0 &&
+           (!a.pre || (aligned(a.pre, 16) && a.ld_pre % per == 0 && a.width % per == 0));
+}
+
+Packed packed(const FfnArgs& a, bool grad) {
+  auto no = [&](const void* p, int64_t ld) { return !head_in_place(a.dtype, p, ld); };
+  return Packed{no(a.x, a.ld_x), no(a.w_in, a.ld_in), no(a.w_out, a.ld_out), no(a.hidden, a.ld_hidden),
+                grad && no(a.dy, a.ld_dy)};
+}
+
+}  // namespace
+
+int64_t ffn_workspace(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t outs, bool grad,
+                      bool strided) {
+  std::string err;
+  if (check_shape(dtype, rows, cols, width, outs, err)) return -1;
+  auto pack = [&](int64_t c) { return dtype == kF32 || strided || c % 8 != 0; };
+  const Packed pk{pack(cols), pack(cols), pack(width), pack(width), pack(outs)};
+  const int64_t forward =
+      is_few(rows, cols, width) ? 256 : make_plan(dtype, rows, cols, width, outs, false, pk).bytes;
+  return grad ? std::max(forward, make_plan(dtype, std::max<int64_t>(rows, 1), cols, width, outs, true, pk).bytes)
+              : forward;
+}
+
+int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
+  if (check(a, false, err)) return -1;
+  if (a.rows == 0) return 0;
+  if (is_few(a.rows, a.cols, a.width)) {
+    if (check_workspace(a, 256, err)) return -1;
+    if (use_device(device, err)) return -1;
+    Guard gd(device);
+    FFN_CUDA(launch_ffn_few(a, s), "block launch");
+    g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
+    return 0;
+  }
+  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.width, a.outs, false, packed(a, false));
+  if (check_workspace(a, p.bytes, err)) return -1;
+  if (use_device(device, err)) return -1;
+  Guard gd(device);
+  Call c{a, p, s, err};
+  HeadPack px, pin, pout, ph;
+  const Operand x = c.operand(a.x, a.rows, a.cols, a.ld_x, p.x, &px);
+  const Operand w_in = c.operand(a.w_in, 2 * a.width, a.cols, a.ld_in, p.w_in, &pin);
+  const Operand w_out = c.operand(a.w_out, a.outs, a.width, a.ld_out, p.w_out, &pout);
+  const Operand h = c.operand(a.hidden, a.rows, a.width, a.ld_hidden, p.hidden, &ph);
+  if (c.pack(px, pin, true)) return -1;
+
+  // gates and factors: a tile's 256 columns are 128 of each
+  HeadLaunch l{};
+  head_settings(l, a.dtype, a.workspace);
+  l.jobs = 1;
+  const Shape in{a.rows, a.width, a.cols, kHeadTileN / 2, 1, kHeadTileN / 2};
+  if (c.job(l.job[0], x, false, w_in, false, in)) return -1;
+  gate(l.g, a);
+  FFN_CUDA(launch_head(kHeadGate, kHeadTileN, l, s), "block launch");
+  ++c.launches;
+
+  if ((ph.src || pout.src) && c.pack(ph, pout, false)) return -1;
+  HeadLaunch q{};
+  head_settings(q, a.dtype, a.workspace);
+  q.jobs = 1;
+  HeadReduce red[1]{};
+  int reds = 0;
+  if (c.job(q.job[0], h, false, w_out, false, p.y)) return -1;
+  c.target(q.job[0], p.y, a.y, a.ld_y, p.part, red, &reds);
+  if (c.products(q, p.y.tile_n, red, reds)) return -1;
+  g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
+  return 0;
+}
+
+int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
+  if (check(a, true, err)) return -1;
+  if (!a.dx && !a.dw_in && !a.dw_out) return 0;
+  if (a.rows == 0) {
+    if (!a.dw_in && !a.dw_out) return 0;
+    if (use_device(device, err)) return -1;
+    Guard gd(device);
+    const size_t size = size_t(dtype_bytes(a.dtype));
+    if (a.dw_in)
+      FFN_CUDA(cudaMemset2DAsync(a.dw_in, size_t(a.ld_din) * size, 0, size_t(a.cols) * size, size_t(2 * a.width), s),
+               "clearing dw_in");
+    if (a.dw_out)
+      FFN_CUDA(cudaMemset2DAsync(a.dw_out, size_t(a.ld_dout) * size, 0, size_t(a.width) * size, size_t(a.outs), s),
+               "clearing dw_out");
+    return 0;
+  }
+  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.width, a.outs, true, packed(a, true));
+  if (check_workspace(a, p.bytes, err)) return -1;
+  if (use_device(device, err)) return -1;
+  Guard gd(device);
+  Call c{a, p, s, err};
+  HeadPack px, pin, pout, ph, pdy;
+  const Operand x = c.operand(a.x, a.rows, a.cols, a.ld_x, p.x, &px);
+  const Operand w_in = c.operand(a.w_in, 2 * a.width, a.cols, a.ld_in, p.w_in, &pin);
+  const Operand w_out = c.operand(a.w_out, a.outs, a.width, a.ld_out, p.w_out, &pout);
+  const Operand h = c.operand(a.hidden, a.rows, a.width, a.ld_hidden, p.hidden, &ph);
+  const Operand dy = c.operand(a.dy, a.rows, a.outs, a.ld_dy, p.dy, &pdy);
+  const Operand d{c.base() + p.dpre, a.rows, 2 * a.width, p.ld_d};
+  if (c.pack(pdy, pout, false)) return -1;
+  if (a.dw_out) {  // dw_out = dy^T h
+    if (c.pack(ph, HeadPack(), false)) return -1;
+    HeadLaunch q{};
+    head_settings(q, a.dtype, a.workspace);
+    q.jobs = 1;
+    HeadReduce red[1]{};
+    int reds = 0;
+    if (c.job(q.job[0], dy, true, h, true, p.dw_out)) return -1;
+    c.target(q.job[0], p.dw_out, a.dw_out, a.ld_dout, p.part, red, &reds);
+    if (c.products(q, p.dw_out.tile_n, red, reds)) return -1;
+  }
+  if (a.dx || a.dw_in) {
+    // dh = dy w_out, whose epilogue makes the gradients of gates and factors of it
+    HeadLaunch l{};
+    head_settings(l, a.dtype, a.workspace);
+    l.jobs = 1;
+    const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
+    if (c.job(l.job[0], dy, false, w_out, true, dh)) return -1;
+    gate(l.g, a);
+    l.g.dpre = const_cast<void*>(d.p);
+    l.g.ld_d = p.ld_d;
+    l.g.plane_d = a.rows * p.ld_d;
+    l.g.wide_d = a.width % 8 == 0;
+    FFN_CUDA(launch_head(kHeadGateGrad, kHeadTileN, l, s), "block launch");
+    ++c.launches;
+
+    if (c.pack(px, pin, false)) return -1;
+    HeadLaunch q{};
+    head_settings(q, a.dtype, a.workspace);
+    HeadReduce red[2]{};
+    int reds = 0;
+    HeadJob dx{}, dw{};
+    if (a.dx) {  // dx = dpre w_in
+      if (c.job(dx, d, false, w_in, true, p.dx)) return -1;
+      c.target(dx, p.dx, a.dx, a.ld_dx, p.part, red, &reds);
+    }
+    if (a.dw_in) {  // dw_in = dpre^T x
+      if (c.job(dw, d, true, x, true, p.dw_in)) return -1;
+      c.target(dw, p.dw_in, a.dw_in, a.ld_din, p.part_in, red, &reds);
+    }
+    // the heavier tiles first
+    const bool dw_first = !a.dx || (a.dw_in && dw.kblocks / dw.splits > dx.kblocks / dx.splits);
+    q.jobs = a.dx && a.dw_in ? 2 : 1;
+    q.job[0] = dw_first ? dw : dx;
+    if (q.jobs == 2) q.job[1] = dw_first ? dx : dw;
+    if (c.products(q, p.dx.tile_n, red, reds)) return -1;
+  }
+  g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
+  return 0;
+}
+
+int ffn_check_device(int device, const void* workspace, std::string& err) {
+  if (!workspace) return fail(err, "null argument");
+  if (use_device(device, err)) return -1;
+  Guard gd(device);
+  FFN_CUDA(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+  unsigned word = 0;
+  FFN_CUDA(cudaMemcpy(&word, workspace, 4, cudaMemcpyDeviceToHost), "reading the block's status word");
+  if (word == kHeadExpired)
+    return fail(err, "device " + std::to_string(device) +
+                         ": feed-forward kernel gave up waiting for a shared-memory transfer");
+  return 0;
+}
+
+}  // namespace mb

@@ -1,0 +1,60 @@
+// A gated feed-forward block and its gradient.
+//
+//   a = x Wg^T,  b = x Wu^T      (w_in: width rows of Wg, then width rows of Wu)
+//   h = act(a) b,  y = h Wo^T
+//   dh = dy Wo,  da = dh b act'(a),  db = dh act(a)
+//   dx = da Wg + db Wu,  dWg = da^T x,  dWu = db^T x,  dWo = dy^T h
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+namespace mb {
+
+constexpr int kSilu = 0, kGelu = 1, kGeluTanh = 2;   // MACBOOST_ACT_*
+
+struct FfnArgs {
+  int dtype = 0, act = 0;
+  const void* x = nullptr;       // rows x cols
+  int64_t rows = 0, cols = 0, ld_x = 0;
+  const void* w_in = nullptr;    // 2 width x cols
+  int64_t width = 0, ld_in = 0;
+  const void* w_out = nullptr;   // outs x width
+  int64_t outs = 0, ld_out = 0;
+  void* hidden = nullptr;        // rows x width: forward output, gradient input
+  int64_t ld_hidden = 0;
+  void* pre = nullptr;           // rows x 2 width, the same; forward: may be null
+  int64_t ld_pre = 0;
+  void* y = nullptr;             // forward: rows x outs
+  int64_t ld_y = 0;
+  const void* dy = nullptr;      // gradient: rows x outs
+  int64_t ld_dy = 0;
+  void* dx = nullptr;            // each may be null
+  int64_t ld_dx = 0;
+  void* dw_in = nullptr;
+  int64_t ld_din = 0;
+  void* dw_out = nullptr;
+  int64_t ld_dout = 0;
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+
+int64_t ffn_workspace(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t outs, bool grad,
+                      bool strided);
+int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err);
+int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err);
+// Wait for `device` and report a wait of these kernels that ran out (as the head's).
+int ffn_check_device(int device, const void* workspace, std::string& err);
+
+// ---- between ffn.cpp and kernels_ffn.cu -------------------------------------------
+
+// Up to four rows whose x and h fit in shared memory go to the CUDA cores: reading the
+// weights bounds them.
+constexpr int64_t kFfnFewRows = 4;
+constexpr int64_t kFfnFewSmem = 128 * 1024;
+inline int64_t ffn_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }  // floats between rows there
+cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);
+
+}  // namespace mb

@@ -54,24 +54,6 @@ struct Plan {
   int64_t bytes = 0;
 };
 
-// TMA reads rows in place when they start on 16 bytes.
-bool in_place(int dtype, const void* p, int64_t ld) {
-  return dtype == kBF16 && aligned(p, 16) && ld % 8 == 0;
-}
-
-// Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
-// CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
-// blocks (float32: 2, of six products), so that the sums of parts stay few.  bfloat16 sums
-// stay in the tensor core, which truncates them at each step of 16: a sum whose terms have one
-// sign lost 1e-7 of itself a step (dw of 300,000 rows, 0.18%).  So its parts are 512 blocks
-// (2,048 steps, 2^-12) at most, and the parts are added up in float32.
-int splits_for(int64_t kblocks, int64_t all, int dtype) {
-  const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
-  const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
-  const int64_t load = std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100);
-  return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
-}
-
 Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool pack_h,
                bool pack_w, bool want_dh, bool want_dw) {
   Plan p{};
@@ -104,8 +86,8 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad
     const int64_t steps = dtype == kF32 ? 6 : 1;
     const int64_t all = dh_tiles * (dh_blocks * steps + kHeadEpilogue) +
                         dw_tiles * (dw_blocks * steps + kHeadEpilogue);
-    p.dh_splits = splits_for(dh_blocks, all, dtype);
-    p.dw_splits = splits_for(dw_blocks, all, dtype);
+    p.dh_splits = head_splits(dh_blocks, all, dtype);
+    p.dw_splits = head_splits(dw_blocks, all, dtype);
     if (want_dh && p.pieces > 1) p.acc = take(rows * cols * 4);
     if (want_dh && p.dh_splits > 1) p.dh_part = take(p.dh_splits * rows * cols * 4);
     if (want_dw && p.dw_splits > 1) p.dw_part = take(p.dw_splits * p.piece * cols * 4);
@@ -177,27 +159,6 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-
-// A matrix of planes x outer x inner 16-bit values, stride ld, fetched in boxes of 64
-// inner x `box` outer values into 128-byte swizzled rows; zeros outside.
-int encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,
-           int box, std::string& err) {
-  EncodeFn fn = encode_fn();
-  if (!fn) return fail(err, "cuTensorMapEncodeTiled is not available from this driver");
-  const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(planes)};
-  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * cuuint64_t(outer) * 2};
-  const cuuint32_t boxes[3] = {64, cuuint32_t(box), 1}, ones[3] = {1, 1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides,
-                        boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(err, "cuTensorMapEncodeTiled failed with " + std::to_string(int(r)));
-  return 0;
-}
-
-// Rows of a K-major box: all of a tile's, or the matrix's when it has fewer (in groups
-// of 8, a swizzle atom).
-int box_rows(int64_t rows, int tile) { return int(std::min<int64_t>(tile, up(rows, 8))); }
 
 // ---- checks ---------------------------------------------------------------------
 
@@ -299,19 +260,6 @@ int operands(const HeadArgs& a, const Plan& p, bool grad, Operands* o, cudaStrea
   return 0;
 }
 
-void settings(HeadLaunch& l, const HeadArgs& a) {
-  l.f32 = a.dtype == kF32;
-  l.status = static_cast<unsigned*>(a.workspace);
-  l.wait_ns = kDefaultWaitNs;
-  if (const char* s = std::getenv("MACBOOST_WAIT_LIMIT_US")) {
-    char* end = nullptr;
-    const long long us = std::strtoll(s, &end, 10);
-    if (end != s && us > 0 && us <= 60000000ll) l.wait_ns = static_cast<unsigned long long>(us) * 1000ull;
-  }
-  const char* t = std::getenv("MACBOOST_TEST_STALL_TILES");
-  l.stall = t && t[0] == '1';
-}
-
 // The inputs themselves, for float32 logits that the planes cannot form.
 void inputs(HeadRows& r, const HeadArgs& a) {
   if (a.dtype != kF32) return;
@@ -327,10 +275,10 @@ int logits_job(HeadJob& j, const HeadArgs& a, const Plan& p, const Operands& o, 
                std::string& err) {
   j.M = int(a.rows);
   j.N = int(n);
-  j.a_box = box_rows(a.rows, kHeadTileM);
-  j.b_box = box_rows(n, kHeadTileN / kHeadPair);
-  if (encode(&j.a, o.h, a.cols, a.rows, o.ld_h, p.planes, j.a_box, err) ||
-      encode(&j.b, o.w, a.cols, a.classes, o.ld_w, p.planes, j.b_box, err))
+  j.a_box = head_box_rows(a.rows, kHeadTileM);
+  j.b_box = head_box_rows(n, kHeadTileN / kHeadPair);
+  if (head_encode(&j.a, o.h, a.cols, a.rows, o.ld_h, p.planes, j.a_box, err) ||
+      head_encode(&j.b, o.w, a.cols, a.classes, o.ld_w, p.planes, j.b_box, err))
     return -1;
   if (parts(a.rows, kHeadPair * kHeadTileM) * parts(n, kHeadTileN) > kMaxIndex)
     return fail(err, "rows * classes are too many for one call");
@@ -384,6 +332,58 @@ int few(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string& e
 
 }  // namespace
 
+// TMA reads rows in place when they start on 16 bytes.
+bool head_in_place(int dtype, const void* p, int64_t ld) {
+  return dtype == kBF16 && aligned(p, 16) && ld % 8 == 0;
+}
+
+// Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
+// CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
+// blocks (float32: 2, of six products), so that the sums of parts stay few.  bfloat16 sums
+// stay in the tensor core, which truncates them at each step of 16: a sum whose terms have one
+// sign lost 1e-7 of itself a step (dw of 300,000 rows, 0.18%).  So its parts are 512 blocks
+// (2,048 steps, 2^-12) at most, and the parts are added up in float32.
+int head_splits(int64_t kblocks, int64_t all, int dtype) {
+  const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
+  const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
+  const int64_t load = std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100);
+  return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
+}
+
+// A matrix of planes x outer x inner 16-bit values, stride ld, fetched in boxes of 64
+// inner x `box` outer values into 128-byte swizzled rows; zeros outside.
+int head_encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,
+                int box, std::string& err) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return fail(err, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(planes)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(ld) * cuuint64_t(outer) * 2};
+  const cuuint32_t boxes[3] = {64, cuuint32_t(box), 1}, ones[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides,
+                        boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(err, "cuTensorMapEncodeTiled failed with " + std::to_string(int(r)));
+  return 0;
+}
+
+// Rows of a K-major box: all of a tile's, or the matrix's when it has fewer (in groups
+// of 8, a swizzle atom).
+int head_box_rows(int64_t rows, int tile) { return int(std::min<int64_t>(tile, up(rows, 8))); }
+
+void head_settings(HeadLaunch& l, int dtype, void* workspace) {
+  l.f32 = dtype == kF32;
+  l.status = static_cast<unsigned*>(workspace);
+  l.wait_ns = kDefaultWaitNs;
+  if (const char* s = std::getenv("MACBOOST_WAIT_LIMIT_US")) {
+    char* end = nullptr;
+    const long long us = std::strtoll(s, &end, 10);
+    if (end != s && us > 0 && us <= 60000000ll) l.wait_ns = static_cast<unsigned long long>(us) * 1000ull;
+  }
+  const char* t = std::getenv("MACBOOST_TEST_STALL_TILES");
+  l.stall = t && t[0] == '1';
+}
+
 int64_t head_workspace(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool strided) {
   std::string err;
   if (check_shape(dtype, rows, cols, classes, err)) return -1;
@@ -408,8 +408,8 @@ int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   if (a.rows == 0) return 0;
   if (is_narrow(a.cols, a.classes)) return narrow(device, a, false, s, err);
   if (is_few(a.dtype, a.rows, a.cols)) return few(device, a, false, s, err);
-  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, false, !in_place(a.dtype, a.h, a.ld_h),
-                           !in_place(a.dtype, a.w, a.ld_w), true, true);
+  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, false, !head_in_place(a.dtype, a.h, a.ld_h),
+                           !head_in_place(a.dtype, a.w, a.ld_w), true, true);
   if (check_workspace(a, p.bytes, err)) return -1;
   if (use_device(device, err)) return -1;
   Guard gd(device);
@@ -417,7 +417,7 @@ int head_loss_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   Operands o{};
   if (operands(a, p, false, &o, s, err)) return -1;
   HeadLaunch l{};
-  settings(l, a);
+  head_settings(l, a.dtype, a.workspace);
   l.jobs = 1;
   if (logits_job(l.job[0], a, p, o, 0, a.classes, err)) return -1;
   l.r.labels = a.labels;
@@ -450,8 +450,8 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   }
   if (is_narrow(a.cols, a.classes)) return narrow(device, a, true, s, err);
   if (is_few(a.dtype, a.rows, a.cols)) return few(device, a, true, s, err);
-  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, true, !in_place(a.dtype, a.h, a.ld_h),
-                           !in_place(a.dtype, a.w, a.ld_w), a.dh != nullptr, a.dw != nullptr);
+  const Plan p = make_plan(a.dtype, a.rows, a.cols, a.classes, true, !head_in_place(a.dtype, a.h, a.ld_h),
+                           !head_in_place(a.dtype, a.w, a.ld_w), a.dh != nullptr, a.dw != nullptr);
   if (check_workspace(a, p.bytes, err)) return -1;
   if (use_device(device, err)) return -1;
   Guard gd(device);
@@ -467,7 +467,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, n = std::min(p.piece, a.classes - v0);
     HeadLaunch l{};
-    settings(l, a);
+    head_settings(l, a.dtype, a.workspace);
     l.jobs = 1;
     if (logits_job(l.job[0], a, p, o, v0, n, err)) return -1;
     l.r.labels = a.labels;
@@ -483,14 +483,14 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
     HEAD_CUDA(launch_head(kHeadG, kHeadTileN, l, s), "head launch");
 
     HeadLaunch q{};
-    settings(q, a);
+    head_settings(q, a.dtype, a.workspace);
     HeadReduce red[2]{};
     int reds = 0;
     HeadJob dh{}, dw{};
     if (a.dh) {  // dh = g w: A = g along its classes, B = w's columns
-      dh.a_box = box_rows(a.rows, kHeadTileM);
-      if (encode(&dh.a, base + p.g, n, a.rows, p.ld_g, p.planes, dh.a_box, err) ||
-          encode(&dh.b, o.w, a.cols, a.classes, o.ld_w, p.planes, 64, err))
+      dh.a_box = head_box_rows(a.rows, kHeadTileM);
+      if (head_encode(&dh.a, base + p.g, n, a.rows, p.ld_g, p.planes, dh.a_box, err) ||
+          head_encode(&dh.b, o.w, a.cols, a.classes, o.ld_w, p.planes, 64, err))
         return -1;
       dh.b_mn = 1;
       dh.tiles_m = int(parts(a.rows, tm));
@@ -516,8 +516,8 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
       }
     }
     if (a.dw) {  // dw = g^T h: A = g's columns, B = h's columns, along the rows
-      if (encode(&dw.a, base + p.g, n, a.rows, p.ld_g, p.planes, 64, err) ||
-          encode(&dw.b, o.h, a.cols, a.rows, o.ld_h, p.planes, 64, err))
+      if (head_encode(&dw.a, base + p.g, n, a.rows, p.ld_g, p.planes, 64, err) ||
+          head_encode(&dw.b, o.h, a.cols, a.rows, o.ld_h, p.planes, 64, err))
         return -1;
       dw.a_mn = dw.b_mn = 1;
       dw.tiles_m = int(parts(n, tm));

@@ -122,11 +122,23 @@ struct HeadRows {                    // what the logits' epilogues know of each 
   int cols;
 };
 
+struct HeadGate {                    // what the epilogues of a gated block know (ffn.h)
+  int act, width, rows;
+  void* hidden;                      // forward: rows x width
+  long long ld_hidden;
+  void* pre;                         // rows x 2 width, forward: or null
+  long long ld_pre;
+  void* dpre;                        // gradient: planes x rows x ld_d of bfloat16
+  long long ld_d, plane_d;
+  int wide, wide_d;                  // rows of hidden and of both halves of pre start on 16 bytes, of dpre
+};
+
 struct HeadLaunch {
   HeadJob job[2];
   int jobs;
   int f32;                           // three planes an operand, six products
   HeadRows r;
+  HeadGate g;
   unsigned* status;
   unsigned long long wait_ns;
   int stall;                         // test hook: no copy is issued, so waits run out
@@ -159,7 +171,7 @@ struct HeadFew {
 };
 cudaError_t launch_head_few(const HeadArgs& h, bool grad, const HeadFew& f, cudaStream_t s);
 
-enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2 };
+enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2, kHeadGate = 3, kHeadGateGrad = 4 };
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s);
 // Source rows (float32 or bfloat16) to planes of bfloat16 (3 or 1), stride ldp; rows
 // whose label (unless null) is none of the classes become zeros.
@@ -188,5 +200,19 @@ struct HeadReduce {
   int out_f32;
 };
 cudaError_t launch_head_reduce(const HeadReduce& a, cudaStream_t s);
+
+// Host side of products as tiles, for the blocks that use them (head.cpp).
+// TMA reads rows in place when they start on 16 bytes.
+bool head_in_place(int dtype, const void* p, int64_t ld);
+// Parts of K of a product whose tiles walk `kblocks`, of a launch of `all` steps.
+int head_splits(int64_t kblocks, int64_t all, int dtype);
+// A matrix of planes x outer x inner 16-bit values, stride ld, fetched in boxes of 64
+// inner x `box` outer values into 128-byte swizzled rows; zeros outside.
+int head_encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,
+                int box, std::string& err);
+// Rows of a K-major box: all of a tile's, or the matrix's when it has fewer.
+int head_box_rows(int64_t rows, int tile);
+// The status word, the limit of waits and the test hook.
+void head_settings(HeadLaunch& l, int dtype, void* workspace);
 
 }  // namespace mb

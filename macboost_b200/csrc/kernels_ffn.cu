@@ -1,0 +1,223 @@
+// The gated block of few rows (ffn.h); more rows are tiles of the tensor cores
+// (kernels_head.cu).
+//
+// Two launches, h between them.  The rows lie in shared memory in float32; a warp streams
+// two rows of weights (two gates and their two factors) at a time through registers, 16
+// bytes a lane, eight loads on their way, and its sums meet in shuffles.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "activation.cuh"
+#include "ffn.h"
+#include "mixture.h"
+
+namespace mb {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+struct Few {
+  const void* in;      // rows x cols
+  long long ld_in;
+  const void* w;       // weights, stride ld_w
+  long long ld_w;
+  int rows, cols, outs, pitch, act;
+  void* out;           // rows x outs
+  long long ld_out;
+  void* pre;           // gated: rows x 2 outs, or null
+  long long ld_pre;
+  unsigned* status;    // cleared by the first launch: there is no wait to run out
+};
+
+template <class T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+
+// PER adjacent weights as floats.
+template <class T, int PER>
+struct Load;
+template <class T>
+struct Load<T, 1> {
+  T v;
+  __device__ __forceinline__ void get(const T* p) { v = *p; }
+  __device__ __forceinline__ void values(float (&x)[1]) const { x[0] = float(v); }
+};
+template <>
+struct Load<float, 4> {
+  float4 v;
+  __device__ __forceinline__ void get(const float* p) { v = __ldcs(reinterpret_cast<const float4*>(p)); }
+  __device__ __forceinline__ void values(float (&x)[4]) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+};
+template <>
+struct Load<__nv_bfloat16, 8> {
+  uint4 v;
+  __device__ __forceinline__ void get(const __nv_bfloat16* p) { v = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  }
+};
+
+template <class T, int NR, int PER, bool GATE>
+__global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
+  constexpr int C = 2;                        // outputs a warp
+  constexpr int R = GATE ? 2 * C : C;         // rows of weights
+  constexpr int STEPS = 8 / R;                // of each, on their way at once
+  extern __shared__ float4 few_shared[];
+  float* rows = reinterpret_cast<float*>(few_shared);  // NR x pitch
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (GATE && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+  for (int n = 0; n < NR; ++n)
+    for (int d = threadIdx.x; d < a.pitch; d += kThreads)
+      rows[n * a.pitch + d] =
+          n < a.rows && d < a.cols ? float(static_cast<const T*>(a.in)[n * a.ld_in + d]) : 0.f;
+  __syncthreads();
+  const int stride = int(gridDim.x) * kWarps * C;
+  for (int o0 = (int(blockIdx.x) * kWarps + warp) * C; o0 < a.outs; o0 += stride) {
+    const T* w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      w[r] = static_cast<const T*>(a.w) +
+             (min(o0 + r % C, a.outs - 1) + (r >= C ? (long long)a.outs : 0)) * a.ld_w;
+    float acc[R][NR];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) acc[r][n] = 0.f;
+    for (int d0 = lane * PER; d0 < a.cols; d0 += STEPS * 32 * PER) {
+      Load<T, PER> q[STEPS][R];
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (d0 + t * 32 * PER < a.cols) q[t][r].get(w[r] + d0 + t * 32 * PER);
+#pragma unroll
+      for (int t = 0; t < STEPS; ++t) {
+        const int d = d0 + t * 32 * PER;
+        if (d >= a.cols) break;
+        float x[NR][PER];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          if constexpr (PER == 1) {
+            x[n][0] = rows[n * a.pitch + d];
+          } else {
+#pragma unroll
+            for (int i = 0; i < PER / 4; ++i) {
+              const float4 f = *reinterpret_cast<const float4*>(rows + n * a.pitch + d + 4 * i);
+              x[n][4 * i] = f.x, x[n][4 * i + 1] = f.y, x[n][4 * i + 2] = f.z, x[n][4 * i + 3] = f.w;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float v[PER];
+          q[t][r].values(v);
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[r][n] = fmaf(v[i], x[n][i], acc[r][n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) acc[r][n] += __shfl_xor_sync(~0u, acc[r][n], o);
+    // lane c * NR + n writes output c of row n
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+        if (lane == c * NR + n && n < a.rows && o0 + c < a.outs) {
+          float y = acc[c][n];
+          if constexpr (GATE) {
+            const float up = acc[C + c][n];
+            if (a.pre) {
+              T* p = static_cast<T*>(a.pre) + n * a.ld_pre + o0 + c;
+              p[0] = from_float<T>(y);
+              p[a.outs] = from_float<T>(up);
+            }
+            const float v[1] = {y}, u[1] = {up};
+            float h[1];
+            activate<sizeof(T) == 2>(a.act, v, u, h);
+            y = h[0];
+          }
+          static_cast<T*>(a.out)[n * a.ld_out + o0 + c] = from_float<T>(y);
+        }
+  }
+}
+
+template <class T, int NR, int PER, bool GATE>
+cudaError_t few_of(const Few& a, cudaStream_t s) {
+  // the limit of the largest call: it is the kernel's, and other threads launch it too
+  const auto k = ffn_few_kernel<T, NR, PER, GATE>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kFfnFewSmem));
+  if (e != cudaSuccess) return e;
+  const size_t smem = size_t(NR) * size_t(a.pitch) * sizeof(float);
+  const int per = int(std::max<size_t>(1, std::min<size_t>(4, (200 * 1024) / (smem + 1024))));
+  const int blocks = std::min((a.outs + 2 * kWarps - 1) / (2 * kWarps), per * device_sms());
+  k<<<blocks, kThreads, smem, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T, int PER, bool GATE>
+cudaError_t few_rows(const Few& a, cudaStream_t s) {
+  if (a.rows <= 1) return few_of<T, 1, PER, GATE>(a, s);
+  if (a.rows <= 2) return few_of<T, 2, PER, GATE>(a, s);
+  return few_of<T, 4, PER, GATE>(a, s);
+}
+
+template <class T, bool GATE>
+cudaError_t few_type(const Few& a, cudaStream_t s) {
+  constexpr int PER = 16 / int(sizeof(T));
+  const bool wide = (reinterpret_cast<uintptr_t>(a.w) | uintptr_t(a.ld_w) * sizeof(T) |
+                     uintptr_t(a.cols) * sizeof(T)) % 16 == 0;
+  return wide ? few_rows<T, PER, GATE>(a, s) : few_rows<T, 1, GATE>(a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
+  Few a{};
+  a.in = f.x;
+  a.ld_in = f.ld_x;
+  a.w = f.w_in;
+  a.ld_w = f.ld_in;
+  a.rows = int(f.rows);
+  a.cols = int(f.cols);
+  a.outs = int(f.width);
+  a.pitch = int(ffn_pitch(f.cols));
+  a.act = f.act;
+  a.out = f.hidden;
+  a.ld_out = f.ld_hidden;
+  a.pre = f.pre;
+  a.ld_pre = f.ld_pre;
+  a.status = static_cast<unsigned*>(f.workspace);
+  cudaError_t e = f.dtype == kF32 ? few_type<float, true>(a, s) : few_type<__nv_bfloat16, true>(a, s);
+  if (e != cudaSuccess) return e;
+  a.in = f.hidden;
+  a.ld_in = f.ld_hidden;
+  a.w = f.w_out;
+  a.ld_w = f.ld_out;
+  a.cols = int(f.width);
+  a.outs = int(f.outs);
+  a.pitch = int(ffn_pitch(f.width));
+  a.out = f.y;
+  a.ld_out = f.ld_y;
+  a.pre = nullptr;
+  return f.dtype == kF32 ? few_type<float, false>(a, s) : few_type<__nv_bfloat16, false>(a, s);
+}
+
+}  // namespace mb

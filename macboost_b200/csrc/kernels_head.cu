@@ -35,6 +35,7 @@
 #include <climits>
 #include <cmath>
 
+#include "activation.cuh"
 #include "head.h"
 #include "mixture.h"
 
@@ -44,7 +45,6 @@ namespace {
 
 constexpr int kEpilogueWarps = 8;
 constexpr int kHeadThreads = 128 + kEpilogueWarps * 32;  // three warpgroups
-constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- PTX ------------------------------------------------------------------------
 
@@ -198,12 +198,6 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(addr)
       : "memory");
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of 64 K values,
@@ -440,6 +434,54 @@ __device__ __forceinline__ void store4(float* p, float4 x, int n, bool wide) {
   }
 }
 
+// Eight adjacent bfloat16.
+__device__ __forceinline__ void store8(__nv_bfloat16* p, uint4 x, int n, bool wide) {
+  if (wide && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = x;
+  } else {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = __ushort_as_bfloat16(static_cast<unsigned short>(u[i / 2] >> (16 * (i % 2))));
+  }
+}
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int n, bool wide) {
+  if (wide && n >= 8) return *reinterpret_cast<const uint4*>(p);
+  uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) u[i / 2] |= uint32_t(__bfloat16_as_ushort(p[i])) << (16 * (i % 2));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ float4 load4(const float* p, int n, bool wide) {
+  if (wide && n >= 4) return *reinterpret_cast<const float4*>(p);
+  return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+}
+
+// A warp's 32 x 32 columns as in turn_bf16, the values still float32: eight rows at a time with
+// four lanes a row, f(step, row, column, eight values).
+template <class F>
+__device__ __forceinline__ void turn8(uint32_t buf, const float (&v)[32], int lane, F f) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)),
+                 "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
+                 : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + lane / 4, u = lane % 4 * 2;
+    float x[8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(x[4 * q]), "=f"(x[4 * q + 1]), "=f"(x[4 * q + 2]), "=f"(x[4 * q + 3])
+                   : "r"(buf + row * 128 + (((u + q) ^ (row & 7)) << 4)));
+    f(i, row, 4 * u, x);
+  }
+}
+
 template <int EPI, int TN, bool F32>
 __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads, 1)
     head_kernel(const __grid_constant__ HeadLaunch a) {
@@ -505,7 +547,10 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           int k0, k1;
           walk.blocks(t, &k0, &k1);
           const int am = (t.m * kHeadPair + int(rank)) * kHeadTileM;
-          const int bn = t.n * TN + int(rank) * (TN / kHeadPair);
+          // a gated product: the first CTA's half of B are gate rows, the second's the rows
+          // `width` below, so the tile's columns are 128 gates and their 128 factors
+          const int bn = EPI == kHeadGate ? t.n * (TN / 2) + int(rank) * a.g.width
+                                          : t.n * TN + int(rank) * (TN / kHeadPair);
           // Boxes that lie outside the matrix are not fetched (what the shared memory holds
           // there only reaches sums that are not used): a box that TMA has to fill with
           // zeros is slower than one it reads.
@@ -515,7 +560,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           };
           auto bytes_b = [&](int n0) {
             return q.b_mn ? min(TN / kHeadPair / 64, max(0, (q.N - n0 + 63) / 64)) * 8192
-                          : n0 < q.N ? q.b_box * 128 : 0;
+                          : EPI == kHeadGate || n0 < q.N ? q.b_box * 128 : 0;
           };
           const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
           const uint32_t bytes = kPlanes * uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
@@ -544,7 +589,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
 #pragma unroll
                 for (int j = 0; j < TN / kHeadPair / 64; ++j)
                   if (bn + 64 * j < q.N) tma_load(sb + j * 8192, &q.b, q.b_row0 + bn + 64 * j, kk, z, bar);
-              } else if (bn < q.N) {
+              } else if (EPI == kHeadGate || bn < q.N) {
                 tma_load(sb, &q.b, kk, q.b_row0 + bn, z, bar);
               }
             }
@@ -629,9 +674,9 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       int k0, k1;
       walk.blocks(t, &k0, &k1);
       const int row = (t.m * kHeadPair + int(rank)) * kHeadTileM + quarter * 32 + lane;
-      const int col0 = t.n * TN + half * (TN / 2);
+      const int col0 = EPI == kHeadGate ? t.n * (TN / 2) + half * (TN / 4) : t.n * TN + half * (TN / 2);
       // what the epilogue knows of the row is fetched while the products run
-      const bool there = EPI != kHeadOut && row < r.rows;
+      const bool there = (EPI == kHeadLse || EPI == kHeadG) && row < r.rows;
       const int y = there ? r.labels[row] : -1;
       const bool known = unsigned(y) < unsigned(r.classes);
       const float lse = EPI == kHeadG && there ? r.lse[row] : 0.f;
@@ -642,12 +687,13 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         ok = __all_sync(~0u, wait(sums_full + 8 * as, aph));
         if (!ok) break;
         fence_after();
-        src = tmem + as * TN + (uint32_t(quarter * 32) << 16) + half * (TN / 2);
+        src = tmem + as * TN + (uint32_t(quarter * 32) << 16) + half * (EPI == kHeadGate ? TN / 4 : TN / 2);
         if constexpr (F32) {
 #pragma unroll
           for (int c = 0; c < TN / 2; c += 16) {
             float v[16];
-            tmem_load16(src + c, v);
+            // a gated product: 64 gates, and their factors 128 columns on
+            tmem_load16(src + c + (EPI == kHeadGate && c >= TN / 4 ? TN / 4 : 0), v);
 #pragma unroll
             for (int i = 0; i < 16; ++i) sums[c + i] = c0 == k0 ? v[i] : sums[c + i] + v[i];
           }
@@ -695,7 +741,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           }
         }
       };
-      if constexpr (F32 && EPI != kHeadOut) {
+      if constexpr (F32 && (EPI == kHeadLse || EPI == kHeadG)) {
         const int v0 = (EPI == kHeadG ? r.v0 : 0) + col0;
         redo(sums, r.classes - v0, EPI == kHeadG ? known : there, r, row, v0);
       }
@@ -756,6 +802,116 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             }
             turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 x) {
               if (rr < rows && n > 0) *reinterpret_cast<uint4*>(g + rr * r.ld_g + c + cc) = x;
+            });
+          }
+        });
+      } else if constexpr (EPI == kHeadGate) {
+        const HeadGate& g = a.g;
+        const int rows = g.rows - (row - lane);
+        // 32 columns from col0 + c on: gates v, their factors w
+        auto part = [&](int c, float (&v)[32], float (&w)[32]) {
+          const int n0 = g.width - (col0 + c);
+          const long long r0 = row - lane;
+          auto put = [&](void* to, long long ld, int at, const float (&x)[32]) {
+            if constexpr (F32) {
+              float* p = static_cast<float*>(to) + r0 * ld + at;
+              turn(stage, x, lane, [&](int rr, int cc, float4 y) {
+                if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, g.wide);
+              });
+            } else {
+              __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to) + r0 * ld + at;
+              turn_bf16(stage, x, lane, [&](int rr, int cc, uint4 y) {
+                if (rr < rows && cc < n0) store8(p + rr * ld + cc, y, n0 - cc, g.wide);
+              });
+            }
+          };
+          if (g.pre) {
+            put(g.pre, g.ld_pre, col0 + c, v);
+            put(g.pre, g.ld_pre, g.width + col0 + c, w);
+          }
+          float h[32];
+          activate<!F32>(g.act, v, w, h);
+          put(g.hidden, g.ld_hidden, col0 + c, h);
+        };
+        if constexpr (F32) {
+#pragma unroll
+          for (int c = 0; c < TN / 4; c += 32) {
+            float v[32], w[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = sums[c + i], w[i] = sums[TN / 4 + c + i];
+            part(c, v, w);
+          }
+        } else {
+          float v[32], w[32];
+#pragma unroll 1
+          for (int c = 0; c < TN / 4; c += 32) {
+            tmem_issue(src + c, v);
+            tmem_issue(src + TN / 2 + c, w);
+            tmem_wait(v);
+            tmem_wait(w);
+            if (c + 32 == TN / 4) release();
+            part(c, v, w);
+          }
+        }
+      } else if constexpr (EPI == kHeadGateGrad) {
+        const HeadGate& g = a.g;
+        const int rows = g.rows - (row - lane);
+        const long long r0 = row - lane;
+        __nv_bfloat16* d = static_cast<__nv_bfloat16*>(g.dpre) + r0 * g.ld_d + col0;
+        each_part([&](int c, float (&v)[32]) {
+          const int n0 = g.width - (col0 + c);
+          if constexpr (F32) {
+            const float* p = static_cast<const float*>(g.pre) + r0 * g.ld_pre + col0 + c;
+            turn(stage, v, lane, [&](int rr, int cc, float4 dh) {
+              const int n = n0 - cc;
+              if (rr >= rows || n <= 0) return;
+              const float4 x = load4(p + rr * g.ld_pre + cc, n, g.wide);
+              const float4 y = load4(p + rr * g.ld_pre + g.width + cc, n, g.wide);
+              const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+              const float ds[4] = {dh.x, dh.y, dh.z, dh.w};
+              float dx[4], dy[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) gate_grad<false>(g.act, xs[i], ys[i], ds[i], dx[i], dy[i]);
+              auto rest = [](float f) { return f - __bfloat162float(__float2bfloat16_rn(f)); };
+#pragma unroll
+              for (int z = 0; z < 3; ++z) {
+                __nv_bfloat16* q = d + z * g.plane_d + rr * g.ld_d + c + cc;
+                store4(q, make_float4(dx[0], dx[1], dx[2], dx[3]), n, g.wide_d);
+                store4(q + g.width, make_float4(dy[0], dy[1], dy[2], dy[3]), n, g.wide_d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dx[i] = rest(dx[i]), dy[i] = rest(dy[i]);
+              }
+            });
+          } else {
+            // what the forward call kept, all of it on its way before the sums are turned
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(g.pre) + r0 * g.ld_pre + col0 + c;
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = i * 8 + lane / 4, cc = lane % 4 * 8;
+              x[i] = y[i] = make_uint4(0, 0, 0, 0);
+              if (rr < rows && cc < n0) {
+                x[i] = load8(p + rr * g.ld_pre + cc, n0 - cc, g.wide);
+                y[i] = load8(p + rr * g.ld_pre + g.width + cc, n0 - cc, g.wide);
+              }
+            }
+            turn8(stage, v, lane, [&](int i, int rr, int cc, const float (&dh)[8]) {
+              if (rr >= rows || cc >= n0) return;
+              const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+              uint32_t dx[4], dy[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float a0, a1, b0, b1;
+                gate_grad<true>(g.act, __uint_as_float(xs[q] << 16), __uint_as_float(ys[q] << 16), dh[2 * q],
+                                a0, b0);
+                gate_grad<true>(g.act, __uint_as_float(xs[q] & 0xFFFF0000u),
+                                __uint_as_float(ys[q] & 0xFFFF0000u), dh[2 * q + 1], a1, b1);
+                dx[q] = pack2(a0, a1);
+                dy[q] = pack2(b0, b1);
+              }
+              __nv_bfloat16* q = d + rr * g.ld_d + c + cc;
+              store8(q, make_uint4(dx[0], dx[1], dx[2], dx[3]), n0 - cc, g.wide_d);
+              store8(q + g.width, make_uint4(dy[0], dy[1], dy[2], dy[3]), n0 - cc, g.wide_d);
             });
           }
         });
@@ -1589,6 +1745,8 @@ cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s) {
   if (epilogue == kHeadLse) return go<kHeadLse, 256>(a, s);
   if (epilogue == kHeadG) return go<kHeadG, 256>(a, s);
+  if (epilogue == kHeadGate) return go<kHeadGate, 256>(a, s);
+  if (epilogue == kHeadGateGrad) return go<kHeadGateGrad, 256>(a, s);
   return tile_n == 128 ? go<kHeadOut, 128>(a, s) : go<kHeadOut, 256>(a, s);
 }
 
