@@ -566,8 +566,9 @@ int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_
 /* A gated feed-forward block: hidden = act(x Wg^T) * (x Wu^T), y = hidden Wo^T.
  * x is rows x cols, w_in 2 width x cols (the rows of Wg, then those of Wu), w_out
  * outs x width, hidden rows x width, y rows x outs, of `dtype` MACBOOST_F32 or
- * MACBOOST_BF16, each with a stride.  pre (rows x 2 width: x w_in^T), unless NULL,
- * is kept for the gradient.  Products and sums are float32 (float32 inputs keep 24
+ * MACBOOST_BF16, each with a stride.  pre (rows x 2 width float32: x w_in^T), unless
+ * NULL, is kept for the gradient; not rounded, since half of the error of bfloat16
+ * gradients would come from that.  Products and sums are float32 (float32 inputs keep 24
  * bits in every product; bfloat16 sums on the tensor cores as in the head); the
  * activation and the factor are formed in float32, and hidden is rounded to `dtype`
  * before the second product.  A row whose x is not finite has values that are not
@@ -576,7 +577,7 @@ int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_
 int32_t macboost_ffn_device(int32_t device, int32_t dtype, int32_t act, const void *x,
                             int64_t rows, int64_t cols, int64_t ld_x, const void *w_in,
                             int64_t width, int64_t ld_in, const void *w_out, int64_t outs,
-                            int64_t ld_out, void *hidden, int64_t ld_hidden, void *pre,
+                            int64_t ld_out, void *hidden, int64_t ld_hidden, float *pre,
                             int64_t ld_pre, void *y, int64_t ld_y, void *workspace,
                             int64_t workspace_bytes, void *stream, char **err);
 
@@ -588,7 +589,7 @@ int32_t macboost_ffn_grad_device(int32_t device, int32_t dtype, int32_t act, con
                                  int64_t rows, int64_t cols, int64_t ld_x, const void *w_in,
                                  int64_t width, int64_t ld_in, const void *w_out, int64_t outs,
                                  int64_t ld_out, const void *hidden, int64_t ld_hidden,
-                                 const void *pre, int64_t ld_pre, const void *dy, int64_t ld_dy,
+                                 const float *pre, int64_t ld_pre, const void *dy, int64_t ld_dy,
                                  void *dx, int64_t ld_dx, void *dw_in, int64_t ld_din,
                                  void *dw_out, int64_t ld_dout, void *workspace,
                                  int64_t workspace_bytes, void *stream, char **err);

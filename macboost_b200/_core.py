@@ -858,7 +858,7 @@ def ffn_device(device: int, dtype: int, act: int, x_ptr: int, rows: int, cols: i
                hidden_ptr: int, ld_hidden: int, pre_ptr: int | None, ld_pre: int, y_ptr: int,
                ld_y: int, workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
     """hidden = act(x Wg^T) * (x Wu^T) and y = hidden Wo^T, with w_in = (Wg, Wu) (2 width x
-    cols), w_out = Wo (outs x width); pre (x w_in^T, 0/None: not kept) is for the gradient."""
+    cols), w_out = Wo (outs x width); pre (x w_in^T in float32, 0/None: not kept) is for the gradient."""
     _enqueue(_lib.macboost_ffn_device, device, dtype, act, x_ptr, rows, cols, ld_x, w_in_ptr, width,
              ld_in, w_out_ptr, outs, ld_out, hidden_ptr, ld_hidden, pre_ptr or None, ld_pre, y_ptr,
              ld_y, workspace_ptr, workspace_bytes, stream or None)

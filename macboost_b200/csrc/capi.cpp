@@ -880,7 +880,7 @@ int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_
 int32_t macboost_ffn_device(int32_t device, int32_t dtype, int32_t act, const void* x,
                             int64_t rows, int64_t cols, int64_t ld_x, const void* w_in,
                             int64_t width, int64_t ld_in, const void* w_out, int64_t outs,
-                            int64_t ld_out, void* hidden, int64_t ld_hidden, void* pre,
+                            int64_t ld_out, void* hidden, int64_t ld_hidden, float* pre,
                             int64_t ld_pre, void* y, int64_t ld_y, void* workspace,
                             int64_t workspace_bytes, void* stream, char** err) {
   mb::FfnArgs a;
@@ -913,7 +913,7 @@ int32_t macboost_ffn_grad_device(int32_t device, int32_t dtype, int32_t act, con
                                  int64_t rows, int64_t cols, int64_t ld_x, const void* w_in,
                                  int64_t width, int64_t ld_in, const void* w_out, int64_t outs,
                                  int64_t ld_out, const void* hidden, int64_t ld_hidden,
-                                 const void* pre, int64_t ld_pre, const void* dy, int64_t ld_dy,
+                                 const float* pre, int64_t ld_pre, const void* dy, int64_t ld_dy,
                                  void* dx, int64_t ld_dx, void* dw_in, int64_t ld_din,
                                  void* dw_out, int64_t ld_dout, void* workspace,
                                  int64_t workspace_bytes, void* stream, char** err) {
@@ -932,7 +932,7 @@ int32_t macboost_ffn_grad_device(int32_t device, int32_t dtype, int32_t act, con
   a.ld_out = ld_out;
   a.hidden = const_cast<void*>(hidden);
   a.ld_hidden = ld_hidden;
-  a.pre = const_cast<void*>(pre);
+  a.pre = const_cast<float*>(pre);
   a.ld_pre = ld_pre;
   a.dy = dy;
   a.ld_dy = ld_dy;

@@ -152,7 +152,7 @@ int check(const FfnArgs& a, bool grad, std::string& err) {
         check_matrix("w_out", a.w_out, a.width, a.ld_out, a.dtype, err) ||
         check_matrix("hidden", a.hidden, a.width, a.ld_hidden, a.dtype, err))
       return -1;
-    if ((grad || a.pre) && check_matrix("pre", a.pre, 2 * a.width, a.ld_pre, a.dtype, err)) return -1;
+    if ((grad || a.pre) && check_matrix("pre", a.pre, 2 * a.width, a.ld_pre, kF32, err)) return -1;
     if (!grad && check_matrix("y", a.y, a.outs, a.ld_y, a.dtype, err)) return -1;
     if (grad && check_matrix("dy", a.dy, a.outs, a.ld_dy, a.dtype, err)) return -1;
     if (grad && a.dx && check_matrix("dx", a.dx, a.cols, a.ld_dx, a.dtype, err)) return -1;
@@ -262,9 +262,8 @@ void gate(HeadGate& g, const FfnArgs& a) {
   g.ld_hidden = a.ld_hidden;
   g.pre = a.pre;
   g.ld_pre = a.ld_pre;
-  const int64_t per = 16 / dtype_bytes(a.dtype);
-  g.wide = aligned(a.hidden, 16) && a.ld_hidden % per == 0 &&
-           (!a.pre || (aligned(a.pre, 16) && a.ld_pre % per == 0 && a.width % per == 0));
+  g.wide = aligned(a.hidden, 16) && a.ld_hidden % (16 / dtype_bytes(a.dtype)) == 0;
+  g.wide_pre = aligned(a.pre, 16) && a.ld_pre % 4 == 0 && a.width % 4 == 0;
 }
 
 Packed packed(const FfnArgs& a, bool grad) {

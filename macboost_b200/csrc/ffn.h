@@ -25,7 +25,7 @@ struct FfnArgs {
   int64_t outs = 0, ld_out = 0;
   void* hidden = nullptr;        // rows x width: forward output, gradient input
   int64_t ld_hidden = 0;
-  void* pre = nullptr;           // rows x 2 width, the same; forward: may be null
+  float* pre = nullptr;          // rows x 2 width, the same; forward: may be null
   int64_t ld_pre = 0;
   void* y = nullptr;             // forward: rows x outs
   int64_t ld_y = 0;

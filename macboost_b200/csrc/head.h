@@ -126,11 +126,11 @@ struct HeadGate {                    // what the epilogues of a gated block know
   int act, width, rows;
   void* hidden;                      // forward: rows x width
   long long ld_hidden;
-  void* pre;                         // rows x 2 width, forward: or null
+  float* pre;                        // rows x 2 width, forward: or null
   long long ld_pre;
   void* dpre;                        // gradient: planes x rows x ld_d of bfloat16
   long long ld_d, plane_d;
-  int wide, wide_d;                  // rows of hidden and of both halves of pre start on 16 bytes, of dpre
+  int wide, wide_pre, wide_d;        // rows of hidden, both halves of pre and of dpre start on 16 bytes
 };
 
 struct HeadLaunch {

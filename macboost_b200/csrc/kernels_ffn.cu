@@ -27,7 +27,7 @@ struct Few {
   int rows, cols, outs, pitch, act;
   void* out;           // rows x outs
   long long ld_out;
-  void* pre;           // gated: rows x 2 outs, or null
+  float* pre;          // gated: rows x 2 outs, or null
   long long ld_pre;
   unsigned* status;    // cleared by the first launch: there is no wait to run out
 };
@@ -145,9 +145,9 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
           if constexpr (GATE) {
             const float up = acc[C + c][n];
             if (a.pre) {
-              T* p = static_cast<T*>(a.pre) + n * a.ld_pre + o0 + c;
-              p[0] = from_float<T>(y);
-              p[a.outs] = from_float<T>(up);
+              float* p = a.pre + n * a.ld_pre + o0 + c;
+              p[0] = y;
+              p[a.outs] = up;
             }
             const float v[1] = {y}, u[1] = {up};
             float h[1];

@@ -445,17 +445,15 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, uint4 x, int n, bool wi
       if (i < n) p[i] = __ushort_as_bfloat16(static_cast<unsigned short>(u[i / 2] >> (16 * (i % 2))));
   }
 }
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int n, bool wide) {
-  if (wide && n >= 8) return *reinterpret_cast<const uint4*>(p);
-  uint32_t u[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) u[i / 2] |= uint32_t(__bfloat16_as_ushort(p[i])) << (16 * (i % 2));
-  return make_uint4(u[0], u[1], u[2], u[3]);
-}
 __device__ __forceinline__ float4 load4(const float* p, int n, bool wide) {
   if (wide && n >= 4) return *reinterpret_cast<const float4*>(p);
   return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+}
+
+__device__ __forceinline__ void load8(const float* p, int n, bool wide, float (&x)[8]) {
+  const float4 lo = load4(p, n, wide), hi = load4(p + 4, n - 4, wide);
+  x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+  x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
 }
 
 // A warp's 32 x 32 columns as in turn_bf16, the values still float32: eight rows at a time with
@@ -681,6 +679,21 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       const bool known = unsigned(y) < unsigned(r.classes);
       const float lse = EPI == kHeadG && there ? r.lse[row] : 0.f;
       const float up = EPI == kHeadG && known ? r.dloss[row] : 0.f;
+      // a gated block's gradient: what the forward call kept, eight rows of 32 columns a step
+      // (sixteen steps a tile), two steps on their way
+      float px[2][8], py[2][8];
+      auto fetch = [&](int step, float (&x)[8], float (&y)[8]) {
+        const int rr = step % 4 * 8 + lane / 4, cc = step / 4 * 32 + lane % 4 * 8;
+        const int n = a.g.width - (col0 + cc);
+        if (step >= 16 || row - lane + rr >= a.g.rows || n <= 0) return;
+        const float* p = a.g.pre + (long long)(row - lane + rr) * a.g.ld_pre + col0 + cc;
+        load8(p, n, a.g.wide_pre, x);
+        load8(p + a.g.width, n, a.g.wide_pre, y);
+      };
+      if constexpr (EPI == kHeadGateGrad && !F32) {
+        fetch(0, px[0], py[0]);
+        fetch(1, px[1], py[1]);
+      }
       bool ok = true;
       uint32_t src = 0;
       for (int c0 = k0; c0 < k1; c0 += F32 ? 1 : k1 - k0) {
@@ -812,26 +825,26 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         auto part = [&](int c, float (&v)[32], float (&w)[32]) {
           const int n0 = g.width - (col0 + c);
           const long long r0 = row - lane;
-          auto put = [&](void* to, long long ld, int at, const float (&x)[32]) {
-            if constexpr (F32) {
-              float* p = static_cast<float*>(to) + r0 * ld + at;
-              turn(stage, x, lane, [&](int rr, int cc, float4 y) {
-                if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, g.wide);
-              });
-            } else {
-              __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to) + r0 * ld + at;
-              turn_bf16(stage, x, lane, [&](int rr, int cc, uint4 y) {
-                if (rr < rows && cc < n0) store8(p + rr * ld + cc, y, n0 - cc, g.wide);
-              });
-            }
+          auto put32 = [&](float* to, long long ld, int at, bool wide, const float (&x)[32]) {
+            float* p = to + r0 * ld + at;
+            turn(stage, x, lane, [&](int rr, int cc, float4 y) {
+              if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, wide);
+            });
           };
           if (g.pre) {
-            put(g.pre, g.ld_pre, col0 + c, v);
-            put(g.pre, g.ld_pre, g.width + col0 + c, w);
+            put32(g.pre, g.ld_pre, col0 + c, g.wide_pre, v);
+            put32(g.pre, g.ld_pre, g.width + col0 + c, g.wide_pre, w);
           }
           float h[32];
           activate<!F32>(g.act, v, w, h);
-          put(g.hidden, g.ld_hidden, col0 + c, h);
+          if constexpr (F32) {
+            put32(static_cast<float*>(g.hidden), g.ld_hidden, col0 + c, g.wide, h);
+          } else {
+            __nv_bfloat16* p = static_cast<__nv_bfloat16*>(g.hidden) + r0 * g.ld_hidden + col0 + c;
+            turn_bf16(stage, h, lane, [&](int rr, int cc, uint4 y) {
+              if (rr < rows && cc < n0) store8(p + rr * g.ld_hidden + cc, y, n0 - cc, g.wide);
+            });
+          }
         };
         if constexpr (F32) {
 #pragma unroll
@@ -861,12 +874,12 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         each_part([&](int c, float (&v)[32]) {
           const int n0 = g.width - (col0 + c);
           if constexpr (F32) {
-            const float* p = static_cast<const float*>(g.pre) + r0 * g.ld_pre + col0 + c;
+            const float* p = g.pre + r0 * g.ld_pre + col0 + c;
             turn(stage, v, lane, [&](int rr, int cc, float4 dh) {
               const int n = n0 - cc;
               if (rr >= rows || n <= 0) return;
-              const float4 x = load4(p + rr * g.ld_pre + cc, n, g.wide);
-              const float4 y = load4(p + rr * g.ld_pre + g.width + cc, n, g.wide);
+              const float4 x = load4(p + rr * g.ld_pre + cc, n, g.wide_pre);
+              const float4 y = load4(p + rr * g.ld_pre + g.width + cc, n, g.wide_pre);
               const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
               const float ds[4] = {dh.x, dh.y, dh.z, dh.w};
               float dx[4], dy[4];
@@ -883,32 +896,19 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
               }
             });
           } else {
-            // what the forward call kept, all of it on its way before the sums are turned
-            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(g.pre) + r0 * g.ld_pre + col0 + c;
-            uint4 x[4], y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int rr = i * 8 + lane / 4, cc = lane % 4 * 8;
-              x[i] = y[i] = make_uint4(0, 0, 0, 0);
-              if (rr < rows && cc < n0) {
-                x[i] = load8(p + rr * g.ld_pre + cc, n0 - cc, g.wide);
-                y[i] = load8(p + rr * g.ld_pre + g.width + cc, n0 - cc, g.wide);
-              }
-            }
             turn8(stage, v, lane, [&](int i, int rr, int cc, const float (&dh)[8]) {
-              if (rr >= rows || cc >= n0) return;
-              const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+              float (&x)[8] = px[i % 2], (&y)[8] = py[i % 2];
               uint32_t dx[4], dy[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float a0, a1, b0, b1;
-                gate_grad<true>(g.act, __uint_as_float(xs[q] << 16), __uint_as_float(ys[q] << 16), dh[2 * q],
-                                a0, b0);
-                gate_grad<true>(g.act, __uint_as_float(xs[q] & 0xFFFF0000u),
-                                __uint_as_float(ys[q] & 0xFFFF0000u), dh[2 * q + 1], a1, b1);
+                gate_grad<true>(g.act, x[2 * q], y[2 * q], dh[2 * q], a0, b0);
+                gate_grad<true>(g.act, x[2 * q + 1], y[2 * q + 1], dh[2 * q + 1], a1, b1);
                 dx[q] = pack2(a0, a1);
                 dy[q] = pack2(b0, b1);
               }
+              fetch(c / 8 + i + 2, x, y);
+              if (rr >= rows || cc >= n0) return;
               __nv_bfloat16* q = d + rr * g.ld_d + c + cc;
               store8(q, make_uint4(dx[0], dx[1], dx[2], dx[3]), n0 - cc, g.wide_d);
               store8(q + g.width, make_uint4(dy[0], dy[1], dy[2], dy[3]), n0 - cc, g.wide_d);

@@ -7,8 +7,8 @@ their slopes' slopes below 0.85; an activation's own error is within |a| (|a| + 
 sigmoid or distribution function a few u, and |a| u of the exponential's argument; the
 formula used for bfloat16 is off by 1.5e-7 / 2, less than u), its slope's within (16 + 16 |a|) u.
 hidden carries the errors of both halves of pre and one rounding; the gradients of gates and
-factors those of the pre that was kept (one rounding more) and a rounding of their own (2^-8;
-2^-22 for three bfloat16 terms).  Each result adds the errors of what it sums, (terms + 16) u of
+factors those of the pre that was kept (float32) and a rounding of their own (2^-8; 2^-22 for
+three bfloat16 terms).  Each result adds the errors of what it sums, (terms + 16) u of
 the magnitudes and its rounding; products of two errors add less than 2%."""
 
 import numpy as np
@@ -46,7 +46,7 @@ class Block:
         self.w_in = normal(2 * width, cols, 2 / cols ** 0.5)
         self.w_out = normal(outs, width, 1 / width ** 0.5)
         self.dy = normal(rows, outs, 1.0)
-        self.hidden, self.pre, self.y = empty(rows, width), empty(rows, 2 * width), empty(rows, outs)
+        self.hidden, self.pre, self.y = empty(rows, width), empty(rows, 2 * width).float(), empty(rows, outs)
         self.dx, self.dw_in, self.dw_out = empty(rows, cols), empty(2 * width, cols), empty(outs, width)
         self.need = core.ffn_workspace(self.code, rows, cols, width, outs, grad=True, strided=pad % 8 != 0)
         self.room = torch.full((self.need + 512,), 255, dtype=torch.uint8, device="cuda")
@@ -112,7 +112,7 @@ class Block:
         eh = b.abs() * (1.13 * ea + own) + f.abs() * eb + h.abs() * half
         y = h @ w_out.t()
         ey = eh @ w_out.abs().t() + (width + 16) * U * (h.abs() @ w_out.abs().t()) + y.abs() * half
-        kept = e_pre + pre.abs() * half
+        kept = e_pre + pre.abs() * 2.0 ** -24
         ka, kb = kept[:, :width], kept[:, width:]
         dh = dy @ w_out
         edh = (outs + 16) * U * (dy.abs() @ w_out.abs())
