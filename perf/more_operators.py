@@ -281,7 +281,7 @@ def _own_ffn(s, c, core, stream):
     n, d, f, o = c["rows"], c["cols"], c["width"], c["outs"]
     code, t, act = CODES[c["type"]], s["x"].dtype, ACTIVATIONS[c["act"]]
     hidden = _kept(s, "hidden", (n, f), t)
-    pre = _kept(s, "pre", (n, 2 * f), t).data_ptr() if c["grad"] else 0
+    pre = _kept(s, "pre", (n, 2 * f), torch.float32).data_ptr() if c["grad"] else 0
     y = _kept(s, "y", (n, o), t)
     if "workspace" not in s["kept"]:
         s["room"] = core.ffn_workspace(code, n, d, f, o, grad=c["grad"])
