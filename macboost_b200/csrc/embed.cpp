@@ -83,27 +83,35 @@ EmbedPlan embed_plan(int64_t entries, int64_t cols, int64_t rows, int64_t k) {
   p.n = rows * k;
   int bits = 1;
   while ((int64_t(1) << bits) <= entries) ++bits;  // keys 0 ... entries
-  p.digits = p.n <= kEmbedOne ? (bits + 7) / 8 : (bits + 9) / 10;
+  const bool one = p.n <= kEmbedOne;
+  const int most = one ? kEmbedOneBits : 10;
+  p.digits = (bits + most - 1) / most;
   p.bits = (bits + p.digits - 1) / p.digits;
   p.tiles = int((p.n + kEmbedTile - 1) / kEmbedTile);
+  // short chunks where long ones are too few to fill the GPU (in units of four values)
+  p.chunk = p.n / 64 * cols / 4 < 300000 ? 16 : 64;
+  p.chunks = (p.n + p.chunk - 1) / p.chunk;
+  p.by_row = entries < p.chunks;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
     at += (bytes + 255) / 256 * 256;
     return o;
   };
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < (one ? 1 : 2); ++i) {
     p.keys[i] = take(p.n * 4);
     p.order[i] = take(p.n * 4);
   }
-  p.counts = take(p.n <= kEmbedOne ? 0 : (int64_t(p.tiles) << p.bits) * 4);
-  p.totals = take(p.n <= kEmbedOne ? 0 : (int64_t(1) << p.bits) * 4);
-  p.first = take(entries * 4);
-  p.last = take(entries * 4);
-  int64_t n = p.n;
+  p.counts = take(one ? 0 : (int64_t(p.tiles) << p.bits) * 4);
+  p.totals = take(one ? 0 : (int64_t(1) << p.bits) * 4);
+  p.heads = take(p.chunks * cols * 4);
+  p.tails = take(p.chunks * cols * 4);
+  p.begins = take(p.by_row ? entries * 4 : 0);
+  p.ends = take(entries * 4);
+  int64_t n = p.chunks;
   for (int l = 0; l < kEmbedLevels; ++l) {
-    n /= kEmbedPart;
-    p.parts[l] = n;
+    n /= kEmbedGroup;
+    p.groups[l] = n;
     p.sums[l] = take(n * cols * 4);
   }
   p.bytes = at;

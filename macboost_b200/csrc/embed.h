@@ -37,17 +37,21 @@ int embed_grad_device(int device, const EmbedArgs& a, cudaStream_t s, std::strin
 
 // The gradient's sort: a stable radix sort of the entries by row of the table, `digits` of
 // `bits` bits each; what adds nothing gets the row `entries`, behind all others.
-constexpr int kEmbedTile = 2048;          // entries a block of the sort
-constexpr int kEmbedOne = 4096;           // entries of a sort that is one block's, in one launch
-constexpr int kEmbedPart = 64;            // sorted entries (or sums of them) added up at once
-constexpr int kEmbedLevels = 3;           // sums of 64, of 64 x 64 and of 64^3 entries
+constexpr int kEmbedOne = 16384;          // entries of a sort that is one block's, in one launch
+constexpr int kEmbedOneBits = 9;          // of its digits, at most; else 10
+constexpr int kEmbedTile = 2048;          // entries a block of a larger sort
+constexpr int kEmbedGroup = 64;           // chunks (or sums of them) added up at once
+constexpr int kEmbedLevels = 2;           // sums of 64 and of 64 x 64 chunks
 
 struct EmbedPlan {
   long long n;                            // entries of the sort, rows * k
   int digits, bits, tiles;
+  int chunk;                              // sorted entries that a group of lanes adds up
+  long long chunks;
+  bool by_row;                            // the join goes by rows of the table, not by chunks
   // offsets into the workspace
-  long long keys[2], order[2], counts, totals, first, last, sums[kEmbedLevels], bytes;
-  long long parts[kEmbedLevels];          // sums a level
+  long long keys[2], order[2], counts, totals, heads, tails, begins, ends, sums[kEmbedLevels], bytes;
+  long long groups[kEmbedLevels];         // sums a level
 };
 EmbedPlan embed_plan(int64_t entries, int64_t cols, int64_t rows, int64_t k);
 
