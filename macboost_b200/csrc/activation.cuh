@@ -23,12 +23,11 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// 1 / (1 + exp(-x)).  FAST: approximate exponential and reciprocal, a few 2^-22 of it for
-// the |x| below 16 that bfloat16 results show.
+// 1 / (1 + exp(-x)).  FAST: approximate exponential, a few 2^-22 of it for the |x| below 16 that
+// bfloat16 results show; the approximate reciprocal is off by one unit in the last place.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float x) {
-  if constexpr (FAST) return rcp_approx(1.f + exp2_approx(-kLog2e * x));
-  return 1.f / (1.f + expf(-x));
+  return rcp_approx(1.f + (FAST ? exp2_approx(-kLog2e * x) : expf(-x)));
 }
 
 // The normal distribution function and its density.  FAST: formula 7.1.26 of Abramowitz and
@@ -89,18 +88,18 @@ __device__ __forceinline__ float activation_slope(float x, float& slope) {
   return y;
 }
 
-// h = act(v) * w
+// v = act(v) * w
 template <bool FAST, int N>
-__device__ __forceinline__ void activate(int act, const float (&v)[N], const float (&w)[N], float (&h)[N]) {
+__device__ __forceinline__ void activate(int act, float (&v)[N], const float (&w)[N]) {
   if (act == kSilu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) h[i] = activation<kSilu, FAST>(v[i]) * w[i];
+    for (int i = 0; i < N; ++i) v[i] = activation<kSilu, FAST>(v[i]) * w[i];
   } else if (act == kGelu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) h[i] = activation<kGelu, FAST>(v[i]) * w[i];
+    for (int i = 0; i < N; ++i) v[i] = activation<kGelu, FAST>(v[i]) * w[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) h[i] = activation<kGeluTanh, FAST>(v[i]) * w[i];
+    for (int i = 0; i < N; ++i) v[i] = activation<kGeluTanh, FAST>(v[i]) * w[i];
   }
 }
 

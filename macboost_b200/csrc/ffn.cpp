@@ -71,9 +71,9 @@ Shape shape(int64_t m, int64_t n, int64_t k) {
 struct Plan {
   Shape y, dx, dw_in, dw_out;
   // offsets into the workspace, 0 for none: packed operands, sums of parts of K
-  int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, bytes = 0;
+  int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, dh = 0, bytes = 0;
   int64_t part = 0, part_in = 0;     // y's, dw_out's or dx's; dw_in's
-  int64_t ld_d = 0;
+  int64_t half = 0;                  // columns of each half of dpre: width, up to a whole K block
 };
 
 struct Packed {
@@ -102,15 +102,16 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
     p.part = take(sums(p.y));
   } else {
     if (pk.dy) p.dy = packed(rows, outs);
-    p.ld_d = up(2 * width, 8);
-    p.dpre = take(planes * rows * p.ld_d * 2);
-    p.dx = shape(rows, cols, 2 * width);
-    p.dw_in = shape(2 * width, cols, rows);
+    p.half = up(width, kHeadTileK);
+    p.dpre = take(planes * rows * 2 * p.half * 2);
+    if (dtype == kF32) p.dh = take(rows * up(width, 4) * 4);
+    p.dx = shape(rows, cols, 2 * p.half);
+    p.dw_in = shape(p.half + width, cols, rows);
     p.dw_out = shape(outs, width, rows);
     const int64_t both = p.dx.weight(dtype) + p.dw_in.weight(dtype);
     split(p.dx, both);
     split(p.dw_in, both);
-    split(p.dw_out, p.dw_out.weight(dtype));
+    split(p.dw_out, p.dw_out.weight(dtype) + (dtype == kF32 ? 0 : shape(rows, width, outs).weight(dtype)));
     // dw_out is done before the others begin
     p.part = take(std::max(sums(p.dw_out), sums(p.dx)));
     p.part_in = take(sums(p.dw_in));
@@ -238,15 +239,17 @@ struct Call {
     j.ld_out = ld;
     j.out_f32 = a.dtype == kF32;
     j.wide = aligned(out, size_t(4 * dtype_bytes(a.dtype))) && ld % 4 == 0;
+    if (!j.out_f32 && aligned(out, 16) && ld % 8 == 0) j.wide = 2;
     j.final = 1;
     if (j.splits > 1) {
       j.acc = reinterpret_cast<float*>(base() + part);
       j.final = 0;
-      red[(*reds)++] = HeadReduce{j.acc, j.splits, h.m, h.n, nullptr, 0, 1, out, ld, j.out_f32};
+      red[(*reds)++] = HeadReduce{j.acc, j.splits, h.m, h.n, nullptr, 0, 1, out, ld, j.out_f32,
+                                  j.m_from, j.m_to};
     }
   }
-  int products(HeadLaunch& l, int tile_n, const HeadReduce* red, int reds) {
-    FFN_CUDA(launch_head(kHeadOut, tile_n, l, s), "block launch");
+  int products(int epilogue, HeadLaunch& l, int tile_n, const HeadReduce* red, int reds) {
+    FFN_CUDA(launch_head(epilogue, tile_n, l, s), "block launch");
     for (int r = 0; r < reds; ++r) FFN_CUDA(launch_head_reduce(red[r], s), "block reduce launch");
     launches += 1 + reds;
     return 0;
@@ -327,7 +330,7 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   int reds = 0;
   if (c.job(q.job[0], h, false, w_out, false, p.y)) return -1;
   c.target(q.job[0], p.y, a.y, a.ld_y, p.part, red, &reds);
-  if (c.products(q, p.y.tile_n, red, reds)) return -1;
+  if (c.products(kHeadOut, q, p.y.tile_n, red, reds)) return -1;
   g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
   return 0;
 }
@@ -359,46 +362,83 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
   const Operand w_out = c.operand(a.w_out, a.outs, a.width, a.ld_out, p.w_out, &pout);
   const Operand h = c.operand(a.hidden, a.rows, a.width, a.ld_hidden, p.hidden, &ph);
   const Operand dy = c.operand(a.dy, a.rows, a.outs, a.ld_dy, p.dy, &pdy);
-  const Operand d{c.base() + p.dpre, a.rows, 2 * a.width, p.ld_d};
+  const Operand d{c.base() + p.dpre, a.rows, 2 * p.half, 2 * p.half};
+  const bool f32 = a.dtype == kF32, inner = a.dx || a.dw_in;
   if (c.pack(pdy, pout, false)) return -1;
-  if (a.dw_out) {  // dw_out = dy^T h
-    if (c.pack(ph, HeadPack(), false)) return -1;
+  // dh = dy w_out; its epilogue (float32: a launch) makes the gradients of gates and factors of it
+  const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
+  if (inner && f32) {
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
     q.jobs = 1;
+    if (c.job(q.job[0], dy, false, w_out, true, dh)) return -1;
+    FfnSplit t{};
+    t.act = a.act;
+    t.rows = a.rows;
+    t.width = int(a.width);
+    t.half = int(p.half);
+    t.ld_h = int(up(a.width, 8));
+    t.dh = reinterpret_cast<const float*>(c.base() + p.dh);
+    t.ld_dh = up(a.width, 4);
+    t.pre = a.pre;
+    t.ld_pre = a.ld_pre;
+    t.hidden = static_cast<const float*>(a.hidden);
+    t.ld_hidden = a.ld_hidden;
+    t.dpre = c.base() + p.dpre;
+    t.h = a.dw_out ? c.base() + p.hidden : nullptr;
+    c.target(q.job[0], dh, c.base() + p.dh, t.ld_dh, 0, nullptr, nullptr);
+    if (c.products(kHeadOut, q, kHeadTileN, nullptr, 0)) return -1;
+    FFN_CUDA(launch_ffn_split(t, s), "block split launch");
+    ++c.launches;
+  } else if (a.dw_out && c.pack(ph, HeadPack(), false)) {
+    return -1;
+  }
+  if (a.dw_out || (inner && !f32)) {
+    // dw_out = dy^T h: in bfloat16 in one launch with dh, whose epilogue takes longer than its products
+    HeadLaunch q{};
+    head_settings(q, a.dtype, a.workspace);
     HeadReduce red[1]{};
     int reds = 0;
-    if (c.job(q.job[0], dy, true, h, true, p.dw_out)) return -1;
-    c.target(q.job[0], p.dw_out, a.dw_out, a.ld_dout, p.part, red, &reds);
-    if (c.products(q, p.dw_out.tile_n, red, reds)) return -1;
+    if (a.dw_out) {
+      HeadJob& j = q.job[q.jobs++];
+      if (c.job(j, dy, true, h, true, p.dw_out)) return -1;
+      c.target(j, p.dw_out, a.dw_out, a.ld_dout, p.part, red, &reds);
+      j.plain = 1;
+    }
+    const bool with = inner && !f32;
+    if (with) {
+      if (c.job(q.job[q.jobs++], dy, false, w_out, true, dh)) return -1;
+      gate(q.g, a);
+      q.g.dpre = const_cast<void*>(d.p);
+      q.g.ld_d = 2 * p.half;
+      q.g.half = int(p.half);
+    }
+    // tiles of one launch are of one width
+    const int tile = with ? kHeadTileN : p.dw_out.tile_n;
+    if (a.dw_out && tile != p.dw_out.tile_n) {
+      q.job[0].tiles_n = int(parts(p.dw_out.n, tile));
+      q.job[0].divide();
+    }
+    if (c.products(with ? kHeadGateGrad : kHeadOut, q, tile, red, reds)) return -1;
   }
-  if (a.dx || a.dw_in) {
-    // dh = dy w_out, whose epilogue makes the gradients of gates and factors of it
-    HeadLaunch l{};
-    head_settings(l, a.dtype, a.workspace);
-    l.jobs = 1;
-    const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
-    if (c.job(l.job[0], dy, false, w_out, true, dh)) return -1;
-    gate(l.g, a);
-    l.g.dpre = const_cast<void*>(d.p);
-    l.g.ld_d = p.ld_d;
-    l.g.plane_d = a.rows * p.ld_d;
-    l.g.wide_d = a.width % 8 == 0;
-    FFN_CUDA(launch_head(kHeadGateGrad, kHeadTileN, l, s), "block launch");
-    ++c.launches;
-
+  if (inner) {
     if (c.pack(px, pin, false)) return -1;
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
     HeadReduce red[2]{};
     int reds = 0;
     HeadJob dx{}, dw{};
+    const int gap = int(p.half - a.width);
     if (a.dx) {  // dx = dpre w_in
       if (c.job(dx, d, false, w_in, true, p.dx)) return -1;
+      dx.b_from = int(p.half);
+      dx.b_skip = gap;
       c.target(dx, p.dx, a.dx, a.ld_dx, p.part, red, &reds);
     }
     if (a.dw_in) {  // dw_in = dpre^T x
       if (c.job(dw, d, true, x, true, p.dw_in)) return -1;
+      dw.m_from = int(a.width);
+      dw.m_to = int(p.half);
       c.target(dw, p.dw_in, a.dw_in, a.ld_din, p.part_in, red, &reds);
     }
     // the heavier tiles first
@@ -406,7 +446,7 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     q.jobs = a.dx && a.dw_in ? 2 : 1;
     q.job[0] = dw_first ? dw : dx;
     if (q.jobs == 2) q.job[1] = dw_first ? dx : dw;
-    if (c.products(q, p.dx.tile_n, red, reds)) return -1;
+    if (c.products(kHeadOut, q, p.dx.tile_n, red, reds)) return -1;
   }
   g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
   return 0;

@@ -56,5 +56,20 @@ constexpr int64_t kFfnFewRows = 4;
 constexpr int64_t kFfnFewSmem = 128 * 1024;
 inline int64_t ffn_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }  // floats between rows there
 cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);
+// float32: from dh (stride ld_dh) and pre to the planes of the gradients of both halves
+// (3 x rows x 2 half, zeros from width to half), and of hidden (3 x rows x ld_h) unless null.
+struct FfnSplit {
+  int act;
+  long long rows;
+  int width, half, ld_h;
+  const float* dh;
+  long long ld_dh;
+  const float* pre;
+  long long ld_pre;
+  const float* hidden;
+  long long ld_hidden;
+  void *dpre, *h;
+};
+cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s);
 
 }  // namespace mb

@@ -323,7 +323,7 @@ int few(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string& e
   }
   if (a.dh)
     HEAD_CUDA(launch_head_reduce(HeadReduce{p.f.dh_part, p.f.chunks, a.rows, a.cols, nullptr, 0, 1, a.dh,
-                                            a.ld_dh, a.dtype == kF32},
+                                            a.ld_dh, a.dtype == kF32, 0, 0},
                                  s),
               "head reduce launch");
   g_kernel_launches.fetch_add(a.dh ? 3 : 1, std::memory_order_relaxed);
@@ -350,8 +350,6 @@ int head_splits(int64_t kblocks, int64_t all, int dtype) {
   return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
 }
 
-// A matrix of planes x outer x inner 16-bit values, stride ld, fetched in boxes of 64
-// inner x `box` outer values into 128-byte swizzled rows; zeros outside.
 int head_encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,
                 int box, std::string& err) {
   EncodeFn fn = encode_fn();
@@ -508,7 +506,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
       const int in = i > 0, last = i + 1 == p.pieces;
       if (dh.splits > 1) {
         dh.acc = reinterpret_cast<float*>(base + p.dh_part);
-        red[reds++] = HeadReduce{dh.acc, dh.splits, a.rows, a.cols, acc, in, last, a.dh, a.ld_dh, f32};
+        red[reds++] = HeadReduce{dh.acc, dh.splits, a.rows, a.cols, acc, in, last, a.dh, a.ld_dh, f32, 0, 0};
       } else {
         dh.acc = acc;
         dh.acc_in = in;
@@ -534,7 +532,7 @@ int head_grad_device(int device, const HeadArgs& a, cudaStream_t s, std::string&
       if (dw.splits > 1) {
         dw.acc = reinterpret_cast<float*>(base + p.dw_part);
         dw.final = 0;
-        red[reds++] = HeadReduce{dw.acc, dw.splits, n, a.cols, nullptr, 0, 1, dw.out, a.ld_dw, f32};
+        red[reds++] = HeadReduce{dw.acc, dw.splits, n, a.cols, nullptr, 0, 1, dw.out, a.ld_dw, f32, 0, 0};
       }
     }
     for (HeadJob* j : {&dh, &dw})

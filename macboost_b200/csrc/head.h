@@ -88,14 +88,17 @@ struct HeadJob {
   int a_row0, b_row0;                // first outer coordinate of A and B (K-major) ...
   int a_k0, b_k0;                    // ... and first K coordinate of each
   int a_box, b_box;                  // rows of a K-major operand's box
+  int b_from, b_skip;                // B's K coordinate is b_skip lower from K = b_from on
   int M, N;                          // the product's rows and columns
+  int m_from, m_to;                  // rows that are not written out; those behind move up
+  int plain;                         // in a launch with another epilogue: the plain one
   // output of the plain epilogue
   float* acc;                        // float32 sums, stride N, M * N apart per split
   int acc_in, final;                 // add what acc holds; write out (else acc)
   void* out;
   long long ld_out;
   int out_f32;
-  int wide;                          // rows of out start on four values
+  int wide;                          // rows of out start on four values; 2: on 16 bytes of bfloat16
 
   void divide() {                    // once tiles, group, splits and kblocks are known
     by_split.set(int64_t(tiles_m) * tiles_n);
@@ -128,9 +131,10 @@ struct HeadGate {                    // what the epilogues of a gated block know
   long long ld_hidden;
   float* pre;                        // rows x 2 width, forward: or null
   long long ld_pre;
-  void* dpre;                        // gradient: planes x rows x ld_d of bfloat16
-  long long ld_d, plane_d;
-  int wide, wide_pre, wide_d;        // rows of hidden, both halves of pre and of dpre start on 16 bytes
+  void* dpre;                        // gradient: rows x 2 half of bfloat16, zeros from `width` to `half`
+  long long ld_d;
+  int half;                          // width, up to a whole K block
+  int wide, wide_pre;                // rows of hidden, and of both halves of pre, start on 16 bytes
 };
 
 struct HeadLaunch {
@@ -198,6 +202,7 @@ struct HeadReduce {
   void* out;
   int64_t ld_out;
   int out_f32;
+  int64_t m_from, m_to;              // as a job's
 };
 cudaError_t launch_head_reduce(const HeadReduce& a, cudaStream_t s);
 

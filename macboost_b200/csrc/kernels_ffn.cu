@@ -7,9 +7,12 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <climits>
+#include <cstring>
 
 #include "activation.cuh"
 #include "ffn.h"
+#include "head.h"
 #include "mixture.h"
 
 namespace mb {
@@ -149,10 +152,10 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
               p[0] = y;
               p[a.outs] = up;
             }
-            const float v[1] = {y}, u[1] = {up};
-            float h[1];
-            activate<sizeof(T) == 2>(a.act, v, u, h);
-            y = h[0];
+            float v[1] = {y};
+            const float u[1] = {up};
+            activate<sizeof(T) == 2>(a.act, v, u);
+            y = v[0];
           }
           static_cast<T*>(a.out)[n * a.ld_out + o0 + c] = from_float<T>(y);
         }
@@ -187,7 +190,97 @@ cudaError_t few_type(const Few& a, cudaStream_t s) {
   return wide ? few_rows<T, PER, GATE>(a, s) : few_rows<T, 1, GATE>(a, s);
 }
 
+// ---- float32: the gradients of gates and factors ----------------------------------
+//
+// The tensor cores' epilogue keeps 128 sums a thread in float32, and fetching pre and three
+// planes a half on top of that stopped it for 85 us a tile of 256 x 256; written out as float32
+// and formed here, 2,048 x 4,096 takes 30 bytes a value.
+
+// A plane of a value, which becomes the rest: as the head's planes, finite values that would
+// round to infinity are bfloat16's largest, and the rest of what is not finite is zero.
+__device__ __forceinline__ __nv_bfloat16 plane_of(int z, float& v) {
+  constexpr float kLargest = 3.3895313892515355e38f;
+  const __nv_bfloat16 t = __float2bfloat16_rn(isfinite(v) ? fminf(fmaxf(v, -kLargest), kLargest) : v);
+  v = z == 0 && !isfinite(v) ? 0.f : v - __bfloat162float(t);
+  return t;
+}
+// Four adjacent values as three planes of bfloat16, `plane` apart.
+__device__ __forceinline__ void put_planes(__nv_bfloat16* to, long long plane, const float (&x)[4]) {
+  float v[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int z = 0; z < 3; ++z) {
+    __nv_bfloat16 t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = plane_of(z, v[i]);
+    uint2 w;
+    memcpy(&w, t, 8);
+    *reinterpret_cast<uint2*>(to + z * plane) = w;
+  }
+}
+
+// 128 columns a warp, four a lane: adjacent ones where rows of dh, hidden and both halves of
+// pre start on 16 bytes (WIDE), else 32 apart, so that lanes read and write side by side.
+template <bool WIDE>
+__global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, int per) {
+  const long long w = ((long long)blockIdx.x * kThreads + threadIdx.x) / 32, n = w / per;
+  if (n >= a.rows) return;
+  const int lane = threadIdx.x % 32, c = int(w - n * per) * 128 + (WIDE ? lane * 4 : lane);
+  constexpr int STEP = WIDE ? 1 : 32;
+  auto get = [&](const float* p, float (&x)[4]) {
+    if (WIDE && c + 4 <= a.width) {
+      const float4 f = *reinterpret_cast<const float4*>(p + c);
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = c + k * STEP < a.width ? p[c + k * STEP] : 0.f;
+    }
+  };
+  // planes of the four, columns of the row from c on, where they are below `end`
+  auto put = [&](void* to, long long ld, int at, int end, const float (&x)[4]) {
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to) + n * ld + at + c;
+    if (WIDE) {
+      if (c < end) put_planes(p, a.rows * ld, x);
+    } else {
+      float v[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int z = 0; z < 3; ++z)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __nv_bfloat16 t = plane_of(z, v[k]);
+          if (c + k * STEP < end) p[z * a.rows * ld + k * STEP] = t;
+        }
+    }
+  };
+  float dh[4], x[4], y[4], h[4], dx[4], dy[4];
+  get(a.dh + n * a.ld_dh, dh);
+  get(a.pre + n * a.ld_pre, x);
+  get(a.pre + n * a.ld_pre + a.width, y);
+  if (a.h) get(a.hidden + n * a.ld_hidden, h);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    gate_grad<false>(a.act, x[k], y[k], dh[k], dx[k], dy[k]);
+    if (c + k * STEP >= a.width) dx[k] = dy[k] = 0.f;
+  }
+  put(a.dpre, 2 * a.half, 0, a.half, dx);
+  put(a.dpre, 2 * a.half, a.half, a.half, dy);
+  if (a.h) put(a.h, a.ld_h, 0, a.ld_h, h);
+}
+
 }  // namespace
+
+cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s) {
+  const int per = (a.half + 127) / 128;  // warps a row
+  const long long blocks = (a.rows * per + kWarps - 1) / kWarps;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const bool wide = (reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.pre) |
+                     reinterpret_cast<uintptr_t>(a.hidden) | uintptr_t(a.ld_dh) * 4 | uintptr_t(a.ld_pre) * 4 |
+                     uintptr_t(a.ld_hidden) * 4 | uintptr_t(a.width) * 4) % 16 == 0;
+  if (wide)
+    ffn_split_kernel<true><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  else
+    ffn_split_kernel<false><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  return cudaGetLastError();
+}
 
 cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
   Few a{};

@@ -200,6 +200,20 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
       : "memory");
 }
 
+// 16 values of each thread to 32 lanes x 16 columns, there after tmem_stored.
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_stored() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of 64 K values,
 // groups of 8 rows 1,024 bytes apart.  M/N-major: boxes of 64 (M or N) x 64 (K), 8,192
 // bytes apart; inside one, groups of 8 K rows 1,024 bytes apart.
@@ -389,6 +403,27 @@ __device__ __forceinline__ void turn(uint32_t buf, const float (&v)[32], int lan
   }
 }
 
+// The same, a row at a time with a lane a column, f(row, column, value): what does not start on
+// 16 bytes is read and written side by side all the same.
+template <class F>
+__device__ __forceinline__ void turn1(uint32_t buf, const float (&v)[32], int lane, F f) {
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)),
+                 "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
+                 : "memory");
+  __syncwarp();
+#pragma unroll 8
+  for (int row = 0; row < 32; ++row) {
+    float x;
+    asm volatile("ld.shared.f32 %0, [%1];"
+                 : "=f"(x)
+                 : "r"(buf + row * 128 + (((lane / 4) ^ (row & 7)) << 4) + lane % 4 * 4));
+    f(row, lane, x);
+  }
+}
+
 // The same in bfloat16: eight rows at a time with four lanes a row, 16 bytes each.
 template <class F>
 __device__ __forceinline__ void turn_bf16(uint32_t buf, const float (&v)[32], int lane, F f) {
@@ -574,7 +609,8 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
               ph ^= 1;
             }
             if (a.stall) continue;
-            const int ka = q.a_k0 + kb * kHeadTileK, kk = q.b_k0 + kb * kHeadTileK;
+            const int ka = q.a_k0 + kb * kHeadTileK;
+            const int kk = q.b_k0 + kb * kHeadTileK - (kb * kHeadTileK >= q.b_from ? q.b_skip : 0);
             for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
               if (q.a_mn) {
 #pragma unroll
@@ -667,6 +703,9 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
     const uint32_t stage = ring + kStages * kStage + (warp - 4) * kTurnBytes;
     // this thread's row of the tile's half: chunks of sums added up (float32)
     float sums[F32 ? TN / 2 : 1];
+    // float32 sums go back to tensor memory, and from there the way of bfloat16's: an epilogue
+    // unrolled over 128 registers runs at the speed of instruction fetches (25 us a tile)
+    constexpr bool kBack = F32 && (EPI == kHeadOut || EPI == kHeadGate);
     while (walk.next(&t)) {
       const HeadJob& q = a.job[t.job];
       int k0, k1;
@@ -690,9 +729,11 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
         load8(p, n, a.g.wide_pre, x);
         load8(p + a.g.width, n, a.g.wide_pre, y);
       };
-      if constexpr (EPI == kHeadGateGrad && !F32) {
-        fetch(0, px[0], py[0]);
-        fetch(1, px[1], py[1]);
+      if constexpr (EPI == kHeadGateGrad) {
+        if (!q.plain) {
+          fetch(0, px[0], py[0]);
+          fetch(1, px[1], py[1]);
+        }
       }
       bool ok = true;
       uint32_t src = 0;
@@ -709,6 +750,13 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             tmem_load16(src + c + (EPI == kHeadGate && c >= TN / 4 ? TN / 4 : 0), v);
 #pragma unroll
             for (int i = 0; i < 16; ++i) sums[c + i] = c0 == k0 ? v[i] : sums[c + i] + v[i];
+          }
+          if (kBack && c0 + 1 == k1) {
+#pragma unroll
+            for (int c = 0; c < TN / 2; c += 16)
+              tmem_store16(src + c + (EPI == kHeadGate && c >= TN / 4 ? TN / 4 : 0), sums + c);
+            tmem_stored();
+            break;
           }
           fence_before();
           __syncwarp();
@@ -729,7 +777,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       // f(column, values) for each 32 columns: the sums in registers (their place has to be
       // known to the compiler), or from tensor memory, the next ones on their way
       auto each_part = [&](auto f) {
-        if constexpr (F32) {
+        if constexpr (F32 && !kBack) {
 #pragma unroll
           for (int c = 0; c < TN / 2; c += 32) {
             float v[32];
@@ -753,6 +801,63 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             f(c + 32, w);
           }
         }
+      };
+      auto store_out = [&] {
+        const int row0 = row - lane, rows = q.M - row0;
+        float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row0) * q.N + col0 : nullptr;
+        const bool wide_acc = q.N % 4 == 0;  // its base is aligned
+        // where row r of the product goes, -1: nowhere
+        auto place = [&](int r) {
+          return r < q.m_from ? r : r < q.m_to ? -1 : r - (q.m_to - q.m_from);
+        };
+        each_part([&](int c, float (&v)[32]) {
+          if (q.final && !q.acc_in && q.wide != 1) {
+            // rows that start on 16 bytes of bfloat16, or off four values
+            if (q.wide) {
+              turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 x) {
+                const int n = q.N - (col0 + c + cc), to = place(row0 + rr);
+                if (rr >= rows || n <= 0 || to < 0) return;
+                store8(static_cast<__nv_bfloat16*>(q.out) + (long long)to * q.ld_out + col0 + c + cc, x, n, true);
+              });
+              return;
+            }
+            turn1(stage, v, lane, [&](int rr, int cc, float x) {
+              const int to = place(row0 + rr);
+              if (rr >= rows || col0 + c + cc >= q.N || to < 0) return;
+              const long long at = (long long)to * q.ld_out + col0 + c + cc;
+              if (q.out_f32)
+                static_cast<float*>(q.out)[at] = x;
+              else
+                static_cast<__nv_bfloat16*>(q.out)[at] = __float2bfloat16_rn(x);
+            });
+            return;
+          }
+          turn(stage, v, lane, [&](int rr, int cc, float4 x) {
+            const int n = q.N - (col0 + c + cc);
+            if (rr >= rows || n <= 0) return;
+            float* sum = acc + (long long)rr * q.N + c + cc;
+            if (q.acc_in) {
+              if (wide_acc) {
+                const float4 o = *reinterpret_cast<const float4*>(sum);
+                x = make_float4(x.x + o.x, x.y + o.y, x.z + o.z, x.w + o.w);
+              } else {
+                x.x += sum[0];
+                if (n > 1) x.y += sum[1];
+                if (n > 2) x.z += sum[2];
+                if (n > 3) x.w += sum[3];
+              }
+            }
+            const int to = place(row0 + rr);
+            if (q.final && to < 0) return;
+            const long long at = (long long)to * q.ld_out + col0 + c + cc;
+            if (!q.final)
+              store4(sum, x, n, wide_acc);
+            else if (q.out_f32)
+              store4(static_cast<float*>(q.out) + at, x, n, q.wide);
+            else
+              store4(static_cast<__nv_bfloat16*>(q.out) + at, x, n, q.wide);
+          });
+        });
       };
       if constexpr (F32 && (EPI == kHeadLse || EPI == kHeadG)) {
         const int v0 = (EPI == kHeadG ? r.v0 : 0) + col0;
@@ -827,123 +932,74 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           const long long r0 = row - lane;
           auto put32 = [&](float* to, long long ld, int at, bool wide, const float (&x)[32]) {
             float* p = to + r0 * ld + at;
-            turn(stage, x, lane, [&](int rr, int cc, float4 y) {
-              if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, wide);
-            });
+            if (wide)
+              turn(stage, x, lane, [&](int rr, int cc, float4 y) {
+                if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, true);
+              });
+            else
+              turn1(stage, x, lane, [&](int rr, int cc, float y) {
+                if (rr < rows && cc < n0) p[rr * ld + cc] = y;
+              });
           };
           if (g.pre) {
             put32(g.pre, g.ld_pre, col0 + c, g.wide_pre, v);
             put32(g.pre, g.ld_pre, g.width + col0 + c, g.wide_pre, w);
           }
-          float h[32];
-          activate<!F32>(g.act, v, w, h);
+          activate<!F32>(g.act, v, w);
           if constexpr (F32) {
-            put32(static_cast<float*>(g.hidden), g.ld_hidden, col0 + c, g.wide, h);
+            put32(static_cast<float*>(g.hidden), g.ld_hidden, col0 + c, g.wide, v);
           } else {
             __nv_bfloat16* p = static_cast<__nv_bfloat16*>(g.hidden) + r0 * g.ld_hidden + col0 + c;
-            turn_bf16(stage, h, lane, [&](int rr, int cc, uint4 y) {
+            turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 y) {
               if (rr < rows && cc < n0) store8(p + rr * g.ld_hidden + cc, y, n0 - cc, g.wide);
             });
           }
         };
-        if constexpr (F32) {
-#pragma unroll
-          for (int c = 0; c < TN / 4; c += 32) {
-            float v[32], w[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = sums[c + i], w[i] = sums[TN / 4 + c + i];
-            part(c, v, w);
-          }
-        } else {
-          float v[32], w[32];
+        float v[32], w[32];
 #pragma unroll 1
-          for (int c = 0; c < TN / 4; c += 32) {
-            tmem_issue(src + c, v);
-            tmem_issue(src + TN / 2 + c, w);
-            tmem_wait(v);
-            tmem_wait(w);
-            if (c + 32 == TN / 4) release();
-            part(c, v, w);
-          }
+        for (int c = 0; c < TN / 4; c += 32) {
+          tmem_issue(src + c, v);
+          tmem_issue(src + TN / 2 + c, w);
+          tmem_wait(v);
+          tmem_wait(w);
+          if (c + 32 == TN / 4) release();
+          part(c, v, w);
         }
       } else if constexpr (EPI == kHeadGateGrad) {
+        if (q.plain) {
+          store_out();
+          continue;
+        }
+        // up to `half` columns a half, zeros from `width` on: whole units of eight
         const HeadGate& g = a.g;
-        const int rows = g.rows - (row - lane);
-        const long long r0 = row - lane;
-        __nv_bfloat16* d = static_cast<__nv_bfloat16*>(g.dpre) + r0 * g.ld_d + col0;
+        const int rows = g.rows - (row - lane), n0 = g.width - col0, n1 = g.half - col0;
+        __nv_bfloat16* d = static_cast<__nv_bfloat16*>(g.dpre) + (long long)(row - lane) * g.ld_d + col0;
         each_part([&](int c, float (&v)[32]) {
-          const int n0 = g.width - (col0 + c);
-          if constexpr (F32) {
-            const float* p = g.pre + r0 * g.ld_pre + col0 + c;
-            turn(stage, v, lane, [&](int rr, int cc, float4 dh) {
-              const int n = n0 - cc;
-              if (rr >= rows || n <= 0) return;
-              const float4 x = load4(p + rr * g.ld_pre + cc, n, g.wide_pre);
-              const float4 y = load4(p + rr * g.ld_pre + g.width + cc, n, g.wide_pre);
-              const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-              const float ds[4] = {dh.x, dh.y, dh.z, dh.w};
-              float dx[4], dy[4];
+          turn8(stage, v, lane, [&](int i, int rr, int cc, const float (&dh)[8]) {
+            float (&x)[8] = px[i % 2], (&y)[8] = py[i % 2];
+            uint32_t dx[4], dy[4];
+            cc += c;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) gate_grad<false>(g.act, xs[i], ys[i], ds[i], dx[i], dy[i]);
-              auto rest = [](float f) { return f - __bfloat162float(__float2bfloat16_rn(f)); };
-#pragma unroll
-              for (int z = 0; z < 3; ++z) {
-                __nv_bfloat16* q = d + z * g.plane_d + rr * g.ld_d + c + cc;
-                store4(q, make_float4(dx[0], dx[1], dx[2], dx[3]), n, g.wide_d);
-                store4(q + g.width, make_float4(dy[0], dy[1], dy[2], dy[3]), n, g.wide_d);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dx[i] = rest(dx[i]), dy[i] = rest(dy[i]);
+            for (int k = 0; k < 4; ++k) {
+              float a0, a1, b0, b1;
+              gate_grad<true>(g.act, x[2 * k], y[2 * k], dh[2 * k], a0, b0);
+              gate_grad<true>(g.act, x[2 * k + 1], y[2 * k + 1], dh[2 * k + 1], a1, b1);
+              if (cc + 8 > n0) {
+                if (cc + 2 * k >= n0) a0 = b0 = 0.f;
+                if (cc + 2 * k + 1 >= n0) a1 = b1 = 0.f;
               }
-            });
-          } else {
-            turn8(stage, v, lane, [&](int i, int rr, int cc, const float (&dh)[8]) {
-              float (&x)[8] = px[i % 2], (&y)[8] = py[i % 2];
-              uint32_t dx[4], dy[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                float a0, a1, b0, b1;
-                gate_grad<true>(g.act, x[2 * q], y[2 * q], dh[2 * q], a0, b0);
-                gate_grad<true>(g.act, x[2 * q + 1], y[2 * q + 1], dh[2 * q + 1], a1, b1);
-                dx[q] = pack2(a0, a1);
-                dy[q] = pack2(b0, b1);
-              }
-              fetch(c / 8 + i + 2, x, y);
-              if (rr >= rows || cc >= n0) return;
-              __nv_bfloat16* q = d + rr * g.ld_d + c + cc;
-              store8(q, make_uint4(dx[0], dx[1], dx[2], dx[3]), n0 - cc, g.wide_d);
-              store8(q + g.width, make_uint4(dy[0], dy[1], dy[2], dy[3]), n0 - cc, g.wide_d);
-            });
-          }
-        });
-      } else {
-        const int row0 = row - lane, rows = q.M - row0;
-        float* acc = q.acc ? q.acc + ((long long)t.split * q.M + row0) * q.N + col0 : nullptr;
-        const bool wide_acc = q.N % 4 == 0;  // its base is aligned
-        each_part([&](int c, float (&v)[32]) {
-          turn(stage, v, lane, [&](int rr, int cc, float4 x) {
-            const int n = q.N - (col0 + c + cc);
-            if (rr >= rows || n <= 0) return;
-            float* sum = acc + (long long)rr * q.N + c + cc;
-            if (q.acc_in) {
-              if (wide_acc) {
-                const float4 o = *reinterpret_cast<const float4*>(sum);
-                x = make_float4(x.x + o.x, x.y + o.y, x.z + o.z, x.w + o.w);
-              } else {
-                x.x += sum[0];
-                if (n > 1) x.y += sum[1];
-                if (n > 2) x.z += sum[2];
-                if (n > 3) x.w += sum[3];
-              }
+              dx[k] = pack2(a0, a1);
+              dy[k] = pack2(b0, b1);
             }
-            const long long at = (long long)(row0 + rr) * q.ld_out + col0 + c + cc;
-            if (!q.final)
-              store4(sum, x, n, wide_acc);
-            else if (q.out_f32)
-              store4(static_cast<float*>(q.out) + at, x, n, q.wide);
-            else
-              store4(static_cast<__nv_bfloat16*>(q.out) + at, x, n, q.wide);
+            fetch(c / 8 + i + 2, x, y);
+            if (rr >= rows || cc >= n1) return;
+            __nv_bfloat16* to = d + rr * g.ld_d + cc;
+            *reinterpret_cast<uint4*>(to) = make_uint4(dx[0], dx[1], dx[2], dx[3]);
+            *reinterpret_cast<uint4*>(to + g.half) = make_uint4(dy[0], dy[1], dy[2], dy[3]);
           });
         });
+      } else {
+        store_out();
       }
     }
   }
@@ -1073,7 +1129,13 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(const HeadReduce a) {
     a.acc[i] = v;
     return;
   }
-  const long long r = i / a.N, o = r * a.ld_out + (i - r * a.N);
+  const long long r = i / a.N;
+  long long to = r;
+  if (to >= a.m_from) {
+    if (to < a.m_to) return;
+    to -= a.m_to - a.m_from;
+  }
+  const long long o = to * a.ld_out + (i - r * a.N);
   if (a.out_f32)
     static_cast<float*>(a.out)[o] = v;
   else
@@ -1714,8 +1776,8 @@ cudaError_t go_type(const HeadLaunch& a, cudaStream_t s) {
   constexpr int kStage = (F32 ? 3 : 1) * (kHeadTileM * 128 + TN / kHeadPair * 128);
   constexpr size_t smem = size_t((192 * 1024) / kStage) * kStage + 1024 +
                           (EPI == kHeadLse ? 0 : kEpilogueWarps * kTurnBytes);
-  const cudaError_t e = cudaFuncSetAttribute(head_kernel<EPI, TN, F32>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  const auto k = head_kernel<EPI, TN, F32>;
+  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   if (F32) {
     // the warpgroups' registers are shared out of what the block is launched with
@@ -1731,7 +1793,7 @@ cudaError_t go_type(const HeadLaunch& a, cudaStream_t s) {
     tiles += (long long)a.job[j].tiles_m * a.job[j].tiles_n * a.job[j].splits;
   if (tiles <= 0) return cudaSuccess;
   const int pairs = int(std::min<long long>(tiles, device_sms() / kHeadPair));
-  head_kernel<EPI, TN, F32><<<pairs * kHeadPair, kHeadThreads, smem, s>>>(a);
+  k<<<pairs * kHeadPair, kHeadThreads, smem, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -1746,7 +1808,8 @@ cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStrea
   if (epilogue == kHeadLse) return go<kHeadLse, 256>(a, s);
   if (epilogue == kHeadG) return go<kHeadG, 256>(a, s);
   if (epilogue == kHeadGate) return go<kHeadGate, 256>(a, s);
-  if (epilogue == kHeadGateGrad) return go<kHeadGateGrad, 256>(a, s);
+  if (epilogue == kHeadGateGrad)  // float32: a launch of its own (launch_ffn_split)
+    return a.f32 ? cudaErrorInvalidValue : go_type<kHeadGateGrad, 256, false>(a, s);
   return tile_n == 128 ? go<kHeadOut, 128>(a, s) : go<kHeadOut, 256>(a, s);
 }
 
