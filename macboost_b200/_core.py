@@ -899,12 +899,15 @@ class GradientList:
         for a in (self.dtypes, self.grads, self.sizes, self.outs):
             if a is not None and a.shape != (self.count,):
                 raise ValueError(f"{self.count} gradients, but {a.size} of dtypes, sizes or outs")
+        # the arrays' addresses: asking numpy for them takes longer than the call
+        self.addresses = [None if a is None else a.ctypes.data
+                          for a in (self.dtypes, self.grads, self.sizes, self.outs)]
 
 
 def clip_workspace(gradients: GradientList) -> int:
     """Bytes of device workspace for clip_device."""
-    n = _lib.macboost_clip_workspace(gradients.count, gradients.dtypes.ctypes.data,
-                                     gradients.sizes.ctypes.data)
+    dtypes, _, sizes, _ = gradients.addresses
+    n = _lib.macboost_clip_workspace(gradients.count, dtypes, sizes)
     if n < 0:
         raise MacBoostError(f"cannot clip a list of {gradients.count} gradients: unknown dtypes, "
                             "or sizes out of range")
@@ -915,7 +918,5 @@ def clip_device(device: int, gradients: GradientList, max_norm: float, norm_ptr:
                 workspace_ptr: int, workspace_bytes: int, stream: int = 0) -> None:
     """norm (a float32 on the device) of all gradients taken together, and the gradients
     times min(1, max_norm / norm)."""
-    g = gradients
-    _enqueue(_lib.macboost_clip_device, device, g.count, g.dtypes.ctypes.data, g.grads.ctypes.data,
-             g.sizes.ctypes.data, None if g.outs is None else g.outs.ctypes.data, max_norm, norm_ptr,
-             workspace_ptr or None, workspace_bytes, stream or None)
+    _enqueue(_lib.macboost_clip_device, device, gradients.count, *gradients.addresses, max_norm,
+             norm_ptr, workspace_ptr or None, workspace_bytes, stream or None)

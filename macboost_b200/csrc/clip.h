@@ -31,21 +31,34 @@ int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err)
 
 // A tensor's values in chunks, a chunk a block's at a time.  Tables of tensors travel as a
 // launch's parameters (at most 32,764 bytes): nothing is copied to the device first, so a
-// captured graph holds its tables.
+// captured graph holds its tables.  16 bytes a tensor: where it starts behind the lowest
+// address of its table, in units of two bytes, so a table's tensors lie within 8 GB.
 constexpr int kClipChunk = 32 * 1024;      // bytes
-constexpr int kClipTensors = 1024;         // of a launch
+constexpr int kClipTensors = 2032;         // of a launch
 constexpr int kClipFew = 64;               // of a launch with a small table
 constexpr int kClipBlocks = 592;           // of a launch, at most: four a multiprocessor
+constexpr int64_t kClipMost = int64_t(1) << 31;  // values of an entry; a larger tensor is several
+// One launch for gradients that a cluster of eight blocks holds in a few rounds: up to 1 MB.
+constexpr int kClipCluster = 8, kClipOne = 32;  // blocks; chunks
+
+struct ClipEntry {
+  uint32_t src, dst;                       // behind the table's bases, in units of two bytes
+  uint32_t size;                           // values
+  uint32_t chunk0;                         // first chunk * 4 + dtype
+};
+
+constexpr int kClipBuckets = 64;
 
 template <int N>
 struct ClipTable {
-  const void* src[N];
-  void* dst[N];                            // may equal src
-  long long size[N];
-  unsigned chunk0[N];                      // the tensor's first chunk
-  unsigned char dtype[N];
+  const char* src;
+  char* dst;                               // null: only the norm
   int tensors;
   unsigned chunks;
+  // where a search begins and ends: the tensors of chunks 0, 1 << shift, 2 << shift ..., and the last
+  int shift;
+  uint16_t bucket[kClipBuckets + 1];
+  ClipEntry entry[N];
 };
 
 struct ClipState {
@@ -53,12 +66,14 @@ struct ClipState {
   int parts, first;                        // of all launches; this launch's first
   double max_norm;
   float* norm;
-  int in_place;                            // every dst is its src: a factor of 1 writes nothing
+  int in_place;                            // every out is its gradient: a factor of 1 writes nothing
+  unsigned keep;                           // chunks from here on are expected in the L2 cache again
 };
 template <int N>
 cudaError_t launch_clip_norm(const ClipTable<N>& t, const ClipState& c, int blocks, cudaStream_t s);
 template <int N>
 cudaError_t launch_clip_scale(const ClipTable<N>& t, const ClipState& c, int blocks, cudaStream_t s);
+cudaError_t launch_clip_one(const ClipTable<kClipFew>& t, const ClipState& c, cudaStream_t s);
 cudaError_t launch_clip_finish(const ClipState& c, cudaStream_t s);
 
 }  // namespace mb

@@ -48,10 +48,10 @@ struct Guard {
 
 // ---- the plan -------------------------------------------------------------------
 
-bool is_few(int64_t rows, int64_t cols, int64_t width) {
+bool is_few(int dtype, int64_t rows, int64_t cols, int64_t width) {
   int64_t n = 1;
   while (n < rows) n *= 2;
-  return rows <= kFfnFewRows && n * ffn_pitch(std::max(cols, width)) * 4 <= kFfnFewSmem;
+  return rows <= (dtype == kF32 ? kFfnFewRowsF32 : kFfnFewRows) && n * ffn_pitch(std::max(cols, width)) * 4 <= kFfnFewSmem;
 }
 
 // A product's tiles.
@@ -95,7 +95,13 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
   if (pk.w_out) p.w_out = packed(outs, width);
   if (pk.hidden) p.hidden = packed(rows, width);
   auto sums = [&](const Shape& q) { return q.splits > 1 ? q.splits * q.m * q.n * 4 : 0; };
-  auto split = [&](Shape& q, int64_t all) { q.splits = head_splits(parts(q.k, kHeadTileK), all, dtype); };
+  auto split = [&](Shape& q, int64_t all) {
+    const int64_t blocks = parts(q.k, kHeadTileK), tiles = parts(q.m, kTileM) * parts(q.n, q.tile_n);
+    q.splits = head_splits(blocks, all, dtype);
+    // few tiles: one round of parts for the pairs of CTAs, not two
+    const int64_t least = dtype == kF32 ? 1 : parts(blocks, 512);
+    if (tiles < 74) q.splits = int(std::max<int64_t>(least, std::min<int64_t>(q.splits, 74 / tiles)));
+  };
   if (!grad) {
     p.y = shape(rows, outs, width);
     split(p.y, p.y.weight(dtype));
@@ -284,7 +290,7 @@ int64_t ffn_workspace(int dtype, int64_t rows, int64_t cols, int64_t width, int6
   auto pack = [&](int64_t c) { return dtype == kF32 || strided || c % 8 != 0; };
   const Packed pk{pack(cols), pack(cols), pack(width), pack(width), pack(outs)};
   const int64_t forward =
-      is_few(rows, cols, width) ? 256 : make_plan(dtype, rows, cols, width, outs, false, pk).bytes;
+      is_few(dtype, rows, cols, width) ? 256 : make_plan(dtype, rows, cols, width, outs, false, pk).bytes;
   return grad ? std::max(forward, make_plan(dtype, std::max<int64_t>(rows, 1), cols, width, outs, true, pk).bytes)
               : forward;
 }
@@ -292,7 +298,7 @@ int64_t ffn_workspace(int dtype, int64_t rows, int64_t cols, int64_t width, int6
 int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   if (check(a, false, err)) return -1;
   if (a.rows == 0) return 0;
-  if (is_few(a.rows, a.cols, a.width)) {
+  if (is_few(a.dtype, a.rows, a.cols, a.width)) {
     if (check_workspace(a, 256, err)) return -1;
     if (use_device(device, err)) return -1;
     Guard gd(device);

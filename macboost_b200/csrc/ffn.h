@@ -50,9 +50,9 @@ int ffn_check_device(int device, const void* workspace, std::string& err);
 
 // ---- between ffn.cpp and kernels_ffn.cu -------------------------------------------
 
-// Up to four rows whose x and h fit in shared memory go to the CUDA cores: reading the
-// weights bounds them.
-constexpr int64_t kFfnFewRows = 4;
+// Up to four rows (float32: 16) whose x and h fit in shared memory go to the CUDA cores:
+// reading the weights bounds them.
+constexpr int64_t kFfnFewRows = 4, kFfnFewRowsF32 = 16;
 constexpr int64_t kFfnFewSmem = 128 * 1024;
 inline int64_t ffn_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }  // floats between rows there
 cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);

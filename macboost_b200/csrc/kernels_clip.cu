@@ -5,7 +5,10 @@
 //         start where 32 would overflow or vanish), so that a norm is right wherever float32
 //         holds it.  A block's sum goes to the workspace.
 // scale   Every block adds the blocks' sums up in the same order, forms the factor and scales
-//         its chunks, the last ones read first: they are still in the L2 cache.
+//         its chunks, the last ones read first: they are still in the L2 cache (what comes
+//         before them is read, and what is written stored, so that it leaves first).
+// one     Both at once for little: a cluster of eight blocks, whose sums meet in its shared
+//         memory.
 //
 // Both read or write what they have to once; bytes bound them.
 #include <cuda_bf16.h>
@@ -77,9 +80,8 @@ __device__ __forceinline__ double squares(uint4 u) {
 // boundary, whole units and the rest.
 template <class T>
 struct Span {
-  const T* p;
   int head, units, tail;
-  __device__ Span(const T* from, long long left, bool whole) : p(from) {
+  __device__ Span(const T* from, long long left, bool whole) {
     const int n = int(left < kClipChunk / int(sizeof(T)) ? left : kClipChunk / int(sizeof(T)));
     head = whole ? int((16 - reinterpret_cast<uintptr_t>(from) % 16) % 16 / sizeof(T)) : n;
     head = head < n ? head : n;
@@ -88,30 +90,40 @@ struct Span {
   }
 };
 
+constexpr int kStep = 4;  // units of a thread on their way
+
 template <class T>
-__device__ __forceinline__ double chunk_squares(const T* src, long long left) {
+__device__ __forceinline__ double chunk_squares(const T* src, long long left, bool once) {
   const Span<T> c(src, left, true);
+  constexpr int N = 16 / int(sizeof(T));
   double sum = 0.0;
-  constexpr int STEP = 4;
-  const uint4* q = reinterpret_cast<const uint4*>(c.p + c.head);
-  for (int i = threadIdx.x; i < c.units; i += STEP * kThreads) {
-    uint4 u[STEP];
+  const uint4* q = reinterpret_cast<const uint4*>(src + c.head) + threadIdx.x;
+  int n = c.units - int(threadIdx.x);
+  for (; n > (kStep - 1) * kThreads; n -= kStep * kThreads, q += kStep * kThreads) {
+    uint4 u[kStep];
 #pragma unroll
-    for (int t = 0; t < STEP; ++t)
-      u[t] = i + t * kThreads < c.units ? q[i + t * kThreads] : make_uint4(0, 0, 0, 0);
+    for (int t = 0; t < kStep; ++t) u[t] = once ? __ldcs(q + t * kThreads) : q[t * kThreads];
 #pragma unroll
-    for (int t = 0; t < STEP; ++t) sum += squares<T>(u[t]);
+    for (int t = 0; t < kStep; ++t) sum += squares<T>(u[t]);
   }
-  for (int i = threadIdx.x; i < c.head; i += kThreads) {
-    const double x = to_float(c.p[i]);
-    sum = fma(x, x, sum);
-  }
-  const T* end = c.p + c.head + c.units * (16 / int(sizeof(T)));
-  for (int i = threadIdx.x; i < c.tail; i += kThreads) {
-    const double x = to_float(end[i]);
+  for (; n > 0; n -= kThreads, q += kThreads) sum += squares<T>(*q);
+  // what lies in front of and behind the units
+  for (int i = threadIdx.x; i < c.head + c.tail; i += kThreads) {
+    const double x = to_float(src[i < c.head ? i : i + c.units * N]);
     sum = fma(x, x, sum);
   }
   return sum;
+}
+
+template <class T>
+__device__ __forceinline__ uint4 scaled(uint4 u, float factor) {
+  constexpr int N = 16 / int(sizeof(T));
+  T v[N];
+  memcpy(v, &u, 16);
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = from_float<T>(to_float(v[k]) * factor);
+  memcpy(&u, v, 16);
+  return u;
 }
 
 template <class T>
@@ -119,37 +131,33 @@ __device__ __forceinline__ void chunk_scale(const T* src, T* dst, long long left
   // 16 bytes at a time where both sides reach a boundary together
   const bool whole = (reinterpret_cast<uintptr_t>(src) - reinterpret_cast<uintptr_t>(dst)) % 16 == 0;
   const Span<T> c(src, left, whole);
-  constexpr int STEP = 4, N = 16 / int(sizeof(T));
-  const uint4* q = reinterpret_cast<const uint4*>(c.p + c.head);
-  uint4* to = reinterpret_cast<uint4*>(dst + c.head);
-  for (int i = threadIdx.x; i < c.units; i += STEP * kThreads) {
-    uint4 u[STEP];
+  constexpr int N = 16 / int(sizeof(T));
+  const uint4* q = reinterpret_cast<const uint4*>(src + c.head) + threadIdx.x;
+  uint4* to = reinterpret_cast<uint4*>(dst + c.head) + threadIdx.x;
+  int n = c.units - int(threadIdx.x);
+  for (; n > (kStep - 1) * kThreads; n -= kStep * kThreads, q += kStep * kThreads, to += kStep * kThreads) {
+    uint4 u[kStep];
 #pragma unroll
-    for (int t = 0; t < STEP; ++t)
-      if (i + t * kThreads < c.units) u[t] = q[i + t * kThreads];
+    for (int t = 0; t < kStep; ++t) u[t] = q[t * kThreads];
 #pragma unroll
-    for (int t = 0; t < STEP; ++t) {
-      T v[N];
-      memcpy(v, &u[t], 16);
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = from_float<T>(to_float(v[k]) * factor);
-      memcpy(&u[t], v, 16);
-      if (i + t * kThreads < c.units) to[i + t * kThreads] = u[t];
-    }
+    for (int t = 0; t < kStep; ++t) __stcs(to + t * kThreads, scaled<T>(u[t], factor));
   }
-  for (int i = threadIdx.x; i < c.head; i += kThreads) dst[i] = from_float<T>(to_float(c.p[i]) * factor);
-  const int end = c.head + c.units * N;
-  for (int i = threadIdx.x; i < c.tail; i += kThreads)
-    dst[end + i] = from_float<T>(to_float(c.p[end + i]) * factor);
+  for (; n > 0; n -= kThreads, q += kThreads, to += kThreads) __stcs(to, scaled<T>(*q, factor));
+  for (int i = threadIdx.x; i < c.head + c.tail; i += kThreads) {
+    const int at = i < c.head ? i : i + c.units * N;
+    dst[at] = from_float<T>(to_float(src[at]) * factor);
+  }
 }
 
-// The tensor of a chunk: the last one that does not start behind it.
+// The tensor of a chunk: the last one that does not start behind it.  The chunk is the block's,
+// so the search reads one parameter after the other.
 template <int N>
 __device__ __forceinline__ int tensor_of(const ClipTable<N>& t, unsigned chunk) {
-  int lo = 0, hi = t.tensors - 1;
+  const unsigned b = chunk >> t.shift;
+  int lo = t.bucket[b], hi = t.bucket[b + 1];
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (t.chunk0[mid] <= chunk)
+    if (t.entry[mid].chunk0 / 4 <= chunk)
       lo = mid;
     else
       hi = mid - 1;
@@ -157,22 +165,31 @@ __device__ __forceinline__ int tensor_of(const ClipTable<N>& t, unsigned chunk) 
   return lo;
 }
 
+// f(values of the type, the chunk's first value of the gradient and of the output, values from there on)
+template <int N, class F>
+__device__ __forceinline__ void with_chunk(const ClipTable<N>& t, unsigned chunk, F f) {
+  const ClipEntry& e = t.entry[tensor_of(t, chunk)];
+  const long long at = (long long)(chunk - e.chunk0 / 4) * kClipChunk;  // bytes
+  const char* src = t.src + 2ll * e.src + at;
+  char* dst = t.dst + 2ll * e.dst + at;
+  const int dtype = e.chunk0 % 4;
+  if (dtype == kF32)
+    f(reinterpret_cast<const float*>(src), reinterpret_cast<float*>(dst), e.size - at / 4);
+  else if (dtype == kBF16)
+    f(reinterpret_cast<const __nv_bfloat16*>(src), reinterpret_cast<__nv_bfloat16*>(dst), e.size - at / 2);
+  else
+    f(reinterpret_cast<const __half*>(src), reinterpret_cast<__half*>(dst), e.size - at / 2);
+}
+
 template <int N>
 __global__ void __launch_bounds__(kThreads, 4)
     clip_norm_kernel(const __grid_constant__ ClipTable<N> t, const ClipState c) {
   __shared__ double shared[kThreads / 32];
   double sum = 0.0;
-  for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
-    const int i = tensor_of(t, chunk);
-    const long long at = (long long)(chunk - t.chunk0[i]) * kClipChunk;  // bytes
-    const char* src = static_cast<const char*>(t.src[i]) + at;
-    if (t.dtype[i] == kF32)
-      sum += chunk_squares(reinterpret_cast<const float*>(src), t.size[i] - at / 4);
-    else if (t.dtype[i] == kBF16)
-      sum += chunk_squares(reinterpret_cast<const __nv_bfloat16*>(src), t.size[i] - at / 2);
-    else
-      sum += chunk_squares(reinterpret_cast<const __half*>(src), t.size[i] - at / 2);
-  }
+  for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x)
+    with_chunk(t, chunk, [&](const auto* src, auto*, long long left) {
+      sum += chunk_squares(src, left, chunk < c.keep);
+    });
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) c.part[c.first + blockIdx.x] = sum;
 }
@@ -183,30 +200,60 @@ __device__ __forceinline__ double norm_of(const ClipState& c, double* shared) {
   return sqrt(block_sum(sum, shared));
 }
 
+__device__ __forceinline__ float factor_of(double norm, double max_norm) {
+  return norm > max_norm ? float(max_norm / norm) : norm == norm ? 1.f : float(norm);
+}
+
 template <int N>
 __global__ void __launch_bounds__(kThreads, 4)
     clip_scale_kernel(const __grid_constant__ ClipTable<N> t, const ClipState c) {
   __shared__ double shared[kThreads / 32];
   const double norm = norm_of(c, shared);
   if (c.first == 0 && blockIdx.x == 0 && threadIdx.x == 0) *c.norm = float(norm);
-  const float factor = norm > c.max_norm ? float(c.max_norm / norm) : norm == norm ? 1.f : float(norm);
+  const float factor = factor_of(norm, c.max_norm);
   if (c.in_place && factor == 1.f) return;
-  for (unsigned k = blockIdx.x; k < t.chunks; k += gridDim.x) {
-    const unsigned chunk = t.chunks - 1 - k;
-    const int i = tensor_of(t, chunk);
-    const long long at = (long long)(chunk - t.chunk0[i]) * kClipChunk;
-    const char* src = static_cast<const char*>(t.src[i]) + at;
-    char* dst = static_cast<char*>(t.dst[i]) + at;
-    if (t.dtype[i] == kF32)
-      chunk_scale(reinterpret_cast<const float*>(src), reinterpret_cast<float*>(dst), t.size[i] - at / 4,
-                  factor);
-    else if (t.dtype[i] == kBF16)
-      chunk_scale(reinterpret_cast<const __nv_bfloat16*>(src), reinterpret_cast<__nv_bfloat16*>(dst),
-                  t.size[i] - at / 2, factor);
-    else
-      chunk_scale(reinterpret_cast<const __half*>(src), reinterpret_cast<__half*>(dst), t.size[i] - at / 2,
-                  factor);
+  for (unsigned k = blockIdx.x; k < t.chunks; k += gridDim.x)
+    with_chunk(t, t.chunks - 1 - k, [&](const auto* src, auto* dst, long long left) {
+      chunk_scale(src, dst, left, factor);
+    });
+}
+
+// All of it in one launch: a cluster's blocks read each other's sums.
+__global__ void __cluster_dims__(kClipCluster, 1, 1) __launch_bounds__(kThreads)
+    clip_one_kernel(const __grid_constant__ ClipTable<kClipFew> t, const ClipState c) {
+  __shared__ double shared[kThreads / 32];
+  __shared__ double mine;
+  double sum = 0.0;
+  for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += kClipCluster)
+    with_chunk(t, chunk, [&](const auto* src, auto*, long long left) {
+      sum += chunk_squares(src, left, false);
+    });
+  sum = block_sum(sum, shared);
+  if (threadIdx.x == 0) mine = sum;
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(&mine));
+  sum = 0.0;
+#pragma unroll
+  for (int b = 0; b < kClipCluster; ++b) {
+    double v;
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f64 %0, [a];\n}\n"
+        : "=d"(v)
+        : "r"(at), "r"(b)
+        : "memory");
+    sum += v;
   }
+  // no block leaves while another may still read its sum
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const double norm = sqrt(sum);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = float(norm);
+  const float factor = factor_of(norm, c.max_norm);
+  if (t.dst && !(c.in_place && factor == 1.f))
+    for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += kClipCluster)
+      with_chunk(t, chunk, [&](const auto* src, auto* dst, long long left) {
+        chunk_scale(src, dst, left, factor);
+      });
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(kThreads) clip_finish_kernel(const ClipState c) {
@@ -233,6 +280,11 @@ template cudaError_t launch_clip_norm<kClipTensors>(const ClipTable<kClipTensors
 template cudaError_t launch_clip_scale<kClipFew>(const ClipTable<kClipFew>&, const ClipState&, int, cudaStream_t);
 template cudaError_t launch_clip_scale<kClipTensors>(const ClipTable<kClipTensors>&, const ClipState&, int,
                                                      cudaStream_t);
+
+cudaError_t launch_clip_one(const ClipTable<kClipFew>& t, const ClipState& c, cudaStream_t s) {
+  clip_one_kernel<<<kClipCluster, kThreads, 0, s>>>(t, c);
+  return cudaGetLastError();
+}
 
 cudaError_t launch_clip_finish(const ClipState& c, cudaStream_t s) {
   clip_finish_kernel<<<1, kThreads, 0, s>>>(c);

@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) acc[r][n] += __shfl_xor_sync(~0u, acc[r][n], o);
     // lane c * NR + n writes output c of row n
+    static_assert(C * NR <= 32, "a lane each");
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -179,7 +180,12 @@ template <class T, int PER, bool GATE>
 cudaError_t few_rows(const Few& a, cudaStream_t s) {
   if (a.rows <= 1) return few_of<T, 1, PER, GATE>(a, s);
   if (a.rows <= 2) return few_of<T, 2, PER, GATE>(a, s);
-  return few_of<T, 4, PER, GATE>(a, s);
+  if (a.rows <= 4) return few_of<T, 4, PER, GATE>(a, s);
+  if constexpr (sizeof(T) == 4) {
+    if (a.rows <= 8) return few_of<T, 8, PER, GATE>(a, s);
+    return few_of<T, 16, PER, GATE>(a, s);
+  }
+  return cudaErrorInvalidValue;
 }
 
 template <class T, bool GATE>
@@ -218,37 +224,28 @@ __device__ __forceinline__ void put_planes(__nv_bfloat16* to, long long plane, c
   }
 }
 
-// 128 columns a warp, four a lane: adjacent ones where rows of dh, hidden and both halves of
-// pre start on 16 bytes (WIDE), else 32 apart, so that lanes read and write side by side.
+// 128 columns a warp, four adjacent ones a lane.  WIDE: rows of dh, hidden and both halves of pre
+// start on 16 bytes; else they are read side by side and change lanes in shared memory.
 template <bool WIDE>
 __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, int per) {
-  const long long w = ((long long)blockIdx.x * kThreads + threadIdx.x) / 32, n = w / per;
+  __shared__ float turn[WIDE ? 1 : kWarps][WIDE ? 1 : 128];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long w = (long long)blockIdx.x * kWarps + warp, n = w / per;
   if (n >= a.rows) return;
-  const int lane = threadIdx.x % 32, c = int(w - n * per) * 128 + (WIDE ? lane * 4 : lane);
-  constexpr int STEP = WIDE ? 1 : 32;
+  const int c0 = int(w - n * per) * 128, c = c0 + lane * 4;
   auto get = [&](const float* p, float (&x)[4]) {
-    if (WIDE && c + 4 <= a.width) {
-      const float4 f = *reinterpret_cast<const float4*>(p + c);
+    if constexpr (WIDE) {
+      const float4 f = c < a.width ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
       x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = c + k * STEP < a.width ? p[c + k * STEP] : 0.f;
-    }
-  };
-  // planes of the four, columns of the row from c on, where they are below `end`
-  auto put = [&](void* to, long long ld, int at, int end, const float (&x)[4]) {
-    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(to) + n * ld + at + c;
-    if (WIDE) {
-      if (c < end) put_planes(p, a.rows * ld, x);
-    } else {
-      float v[4] = {x[0], x[1], x[2], x[3]};
+      for (int k = 0; k < 4; ++k) x[k] = c0 + 32 * k + lane < a.width ? p[c0 + 32 * k + lane] : 0.f;
+      __syncwarp();
 #pragma unroll
-      for (int z = 0; z < 3; ++z)
+      for (int k = 0; k < 4; ++k) turn[warp][32 * k + lane] = x[k];
+      __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __nv_bfloat16 t = plane_of(z, v[k]);
-          if (c + k * STEP < end) p[z * a.rows * ld + k * STEP] = t;
-        }
+      for (int k = 0; k < 4; ++k) x[k] = turn[warp][4 * lane + k];
     }
   };
   float dh[4], x[4], y[4], h[4], dx[4], dy[4];
@@ -259,11 +256,14 @@ __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, i
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     gate_grad<false>(a.act, x[k], y[k], dh[k], dx[k], dy[k]);
-    if (c + k * STEP >= a.width) dx[k] = dy[k] = 0.f;
+    if (c + k >= a.width) dx[k] = dy[k] = 0.f;
   }
-  put(a.dpre, 2 * a.half, 0, a.half, dx);
-  put(a.dpre, 2 * a.half, a.half, a.half, dy);
-  if (a.h) put(a.h, a.ld_h, 0, a.ld_h, h);
+  if (c < a.half) {
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(a.dpre) + n * 2 * a.half + c;
+    put_planes(d, a.rows * 2 * a.half, dx);
+    put_planes(d + a.half, a.rows * 2 * a.half, dy);
+  }
+  if (a.h && c < a.ld_h) put_planes(static_cast<__nv_bfloat16*>(a.h) + n * a.ld_h + c, a.rows * a.ld_h, h);
 }
 
 }  // namespace

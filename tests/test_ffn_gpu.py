@@ -143,7 +143,8 @@ class Block:
 SIZES = [(5, 8, 10, 1), (6, 16, 8, 8), (128, 64, 128, 256), (129, 65, 257, 7), (257, 100, 403, 10),
          (300, 72, 513, 65), (1000, 264, 96, 300), (33, 1030, 130, 130), (48, 512, 1024, 256),
          (700, 128, 256, 1), (2000, 24, 40, 16), (4100, 32, 64, 129), (17, 4096, 24, 40)]
-FEW = [(1, 1, 1, 1), (1, 1024, 3001, 300), (2, 65, 70, 33), (3, 257, 100, 10), (4, 512, 999, 128),
+FEW = [(5, 64, 2048, 72), (8, 40, 4000, 136), (11, 264, 72, 1000), (16, 2056, 640, 48), (25, 8, 8, 8), (47, 128, 1032, 512),
+       (64, 512, 2000, 264), (65, 512, 2000, 264), (12, 33, 70, 9), (16, 96, 130, 260), (1, 1, 1, 1), (1, 1024, 3001, 300), (2, 65, 70, 33), (3, 257, 100, 10), (4, 512, 999, 128),
        (1, 72, 16_384, 64), (2, 8, 20_000, 24), (4, 1000, 136, 1), (1, 40_000, 8, 8)]
 
 
