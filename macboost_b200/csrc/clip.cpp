@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <memory>
-#include <utility>
 #include <vector>
 
 #include "engine.h"
@@ -32,135 +31,143 @@ struct Guard {
   }
 };
 
+// Chunks of `size` values; a division for each of a few thousand tensors would take as long as
+// the launches.
 int64_t chunks_of(int dtype, int64_t size) {
-  const int64_t per = kClipChunk / dtype_bytes(dtype);
-  return (size + per - 1) / per;
+  static_assert(kClipChunk == 1 << 15, "values of a chunk as a power of two");
+  const int bits = dtype == kF32 ? 13 : 14;
+  return (size + (int64_t(1) << bits) - 1) >> bits;
 }
 
-int check_list(int64_t count, const int32_t* dtypes, const int64_t* sizes, std::string& err) {
+// The list's types and sizes; `room`: the workspace it needs.
+int check_list(int64_t count, const int32_t* dtypes, const int64_t* sizes, int64_t* room, std::string& err) {
   if (count < 0 || count > (int64_t(1) << 24)) return fail(err, "count must be in 0...2^24");
   if (count > 0 && (!dtypes || !sizes)) return fail(err, "null argument");
-  int64_t chunks = 0;
+  int64_t chunks = 0, entries = 0;
   for (int64_t i = 0; i < count; ++i) {
-    if (!dtype_bytes(dtypes[i]))
-      return fail(err, "unknown dtype " + std::to_string(dtypes[i]) + " (0 float32, 1 bfloat16, 2 float16)");
+    const int dtype = dtypes[i];
+    if (!dtype_bytes(dtype))
+      return fail(err, "unknown dtype " + std::to_string(dtype) + " (0 float32, 1 bfloat16, 2 float16)");
     if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40)) return fail(err, "sizes must be in 0...2^40");
-    chunks += chunks_of(dtypes[i], sizes[i]);
+    chunks += chunks_of(dtype, sizes[i]);
+    entries += (sizes[i] + kClipMost - 1) / kClipMost;  // a shift
     if (chunks > (int64_t(1) << 27)) return fail(err, "the gradients hold too many values for one call");
   }
+  // a block's sum of every launch: no more than chunks, nor than entries that all lie far apart ask for
+  *room = std::min(chunks, entries * kClipBlocks) * int64_t(sizeof(double));
   return 0;
 }
 
 // Chunks that the norm's launch leaves in the L2 cache for the scaling: 80 MB of its 126.
 constexpr unsigned kKeep = (80u << 20) / kClipChunk;
 
-// A launch's tensors, those without values left out and large ones in several entries.
+// The list's entries one after the other: tensors without values left out, large ones in
+// several.
+struct Entry {
+  uintptr_t src, dst;
+  int64_t size;
+  int dtype;
+};
+struct Cursor {
+  int64_t tensor = 0, done = 0;
+  bool next(const ClipArgs& a, Entry* e) {
+    while (tensor < a.count && a.sizes[tensor] == done) {
+      ++tensor;
+      done = 0;
+    }
+    if (tensor >= a.count) return false;
+    e->dtype = a.dtypes[tensor];
+    const uintptr_t at = uintptr_t(done) * uintptr_t(e->dtype == kF32 ? 4 : 2);
+    e->src = reinterpret_cast<uintptr_t>(a.grads[tensor]) + at;
+    e->dst = a.outs ? reinterpret_cast<uintptr_t>(a.outs[tensor]) + at : 0;
+    e->size = std::min(a.sizes[tensor] - done, kClipMost);
+    done += e->size;
+    return true;
+  }
+};
+
+// A launch's entries, from a place of the list on, and their lowest addresses.
 struct Group {
-  std::vector<ClipEntry> entries;
-  uintptr_t src = UINTPTR_MAX, src_end = 0, dst = UINTPTR_MAX, dst_end = 0;
+  Cursor from;
+  int entries = 0;
+  uintptr_t src = UINTPTR_MAX, dst = UINTPTR_MAX;
   unsigned chunks = 0;
   int blocks() const { return int(std::min<unsigned>(chunks, kClipBlocks)); }
 };
 
 constexpr uintptr_t kReach = uintptr_t(1) << 33;  // 2^32 units of two bytes
 
-// f(dtype, address of the gradient, of the output, values) for each entry.
-template <class F>
-void each_entry(const ClipArgs& a, F f) {
-  for (int64_t i = 0; i < a.count; ++i) {
-    const uintptr_t size = uintptr_t(dtype_bytes(a.dtypes[i]));
-    uintptr_t src = a.grads ? reinterpret_cast<uintptr_t>(a.grads[i]) : 0;
-    uintptr_t dst = a.outs ? reinterpret_cast<uintptr_t>(a.outs[i]) : 0;
-    for (int64_t left = a.sizes[i]; left > 0; left -= kClipMost) {
-      const int64_t n = std::min(left, kClipMost);
-      f(a.dtypes[i], src, dst, n);
-      src += uintptr_t(n) * size;
-      if (dst) dst += uintptr_t(n) * size;
-    }
-  }
-}
-
 std::vector<Group> groups_of(const ClipArgs& a) {
   std::vector<Group> all;
-  // first the groups' sizes and reach, the entries' addresses from their start
-  std::vector<std::pair<uintptr_t, uintptr_t>> at;
-  auto close = [&] {
-    Group& g = all.back();
-    for (size_t i = 0; i < g.entries.size(); ++i) {
-      g.entries[i].src = uint32_t((at[i].first - g.src) / 2);
-      g.entries[i].dst = uint32_t((at[i].second - g.dst) / 2);
-    }
-    at.clear();
-  };
-  each_entry(a, [&](int dtype, uintptr_t src, uintptr_t dst, int64_t n) {
-    bool fits = !all.empty() && all.back().entries.size() < size_t(kClipTensors);
-    if (fits) {
-      const Group& g = all.back();
-      fits = std::max(g.src_end, src) - std::min(g.src, src) < kReach &&
-             std::max(g.dst_end, dst) - std::min(g.dst, dst) < kReach;
-    }
-    if (!fits) {
-      if (!all.empty()) close();
+  uintptr_t src_end = 0, dst_end = 0;
+  Cursor at;
+  Entry e;
+  for (Cursor before = at; at.next(a, &e); before = at) {
+    if (all.empty() || all.back().entries == kClipTensors ||
+        std::max(src_end, e.src) - std::min(all.back().src, e.src) >= kReach ||
+        std::max(dst_end, e.dst) - std::min(all.back().dst, e.dst) >= kReach) {
       all.emplace_back();
-      const size_t most = size_t(std::min<int64_t>(a.count, kClipTensors));
-      all.back().entries.reserve(most);
-      at.reserve(most);
+      all.back().from = before;
+      src_end = dst_end = 0;
     }
     Group& g = all.back();
-    g.src = std::min(g.src, src);
-    g.src_end = std::max(g.src_end, src);
-    g.dst = std::min(g.dst, dst);
-    g.dst_end = std::max(g.dst_end, dst);
-    at.emplace_back(src, dst);
-    g.entries.push_back(ClipEntry{0, 0, uint32_t(n), g.chunks * 4 + unsigned(dtype)});
-    g.chunks += unsigned(chunks_of(dtype, n));
-  });
-  if (!all.empty()) close();
+    ++g.entries;
+    g.src = std::min(g.src, e.src);
+    g.dst = std::min(g.dst, e.dst);
+    src_end = std::max(src_end, e.src);
+    dst_end = std::max(dst_end, e.dst);
+    g.chunks += unsigned(chunks_of(e.dtype, e.size));
+  }
   return all;
 }
 
 template <int N>
-void fill(ClipTable<N>& t, const Group& g, bool outs) {
+void fill(ClipTable<N>& t, const ClipArgs& a, const Group& g) {
   t.src = reinterpret_cast<const char*>(g.src);
-  t.dst = outs ? reinterpret_cast<char*>(g.dst) : nullptr;
-  t.tensors = int(g.entries.size());
+  t.dst = a.outs ? reinterpret_cast<char*>(g.dst) : nullptr;
+  t.tensors = g.entries;
   t.chunks = g.chunks;
-  std::copy(g.entries.begin(), g.entries.end(), t.entry);
   t.shift = 0;
   while (((t.chunks - 1) >> t.shift) >= unsigned(kClipBuckets)) ++t.shift;
-  int i = 0;
-  for (int b = 0; b <= kClipBuckets; ++b) {
-    const uint64_t chunk = uint64_t(b) << t.shift;
-    while (i + 1 < t.tensors && g.entries[size_t(i) + 1].chunk0 / 4 <= chunk) ++i;
-    t.bucket[b] = static_cast<uint16_t>(i);
+  Cursor at = g.from;
+  Entry e;
+  unsigned chunk = 0;
+  int bucket = 0;
+  for (int i = 0; i < g.entries && at.next(a, &e); ++i) {
+    t.entry[i] = ClipEntry{uint32_t((e.src - g.src) / 2), uint32_t((e.dst - g.dst) / 2), uint32_t(e.size),
+                           chunk * 4 + unsigned(e.dtype)};
+    chunk += unsigned(chunks_of(e.dtype, e.size));
+    // the buckets whose first chunk is this entry's
+    for (; bucket <= kClipBuckets && (uint64_t(bucket) << t.shift) < chunk; ++bucket)
+      t.bucket[bucket] = static_cast<uint16_t>(i);
   }
+  for (; bucket <= kClipBuckets; ++bucket) t.bucket[bucket] = static_cast<uint16_t>(g.entries - 1);
 }
 
+// The launches of a group: its sums, then (another time) its outputs.
 template <int N>
-cudaError_t run(const Group& g, const ClipState& c, bool outs, int pass, cudaStream_t s) {
-  // its entries beyond the tensors' are not read
-  const std::unique_ptr<ClipTable<N>> t(new ClipTable<N>);
-  fill(*t, g, outs);
-  return pass ? launch_clip_scale<N>(*t, c, g.blocks(), s) : launch_clip_norm<N>(*t, c, g.blocks(), s);
-}
+struct Launch {
+  std::unique_ptr<ClipTable<N>> table;
+  cudaError_t operator()(const ClipArgs& a, const Group& g, const ClipState& c, int pass, cudaStream_t s) {
+    if (!table) {
+      table.reset(new ClipTable<N>);  // entries beyond the tensors' are not read
+      fill(*table, a, g);
+    }
+    return pass ? launch_clip_scale<N>(*table, c, g.blocks(), s) : launch_clip_norm<N>(*table, c, g.blocks(), s);
+  }
+};
 
 }  // namespace
 
 int64_t clip_workspace(int64_t count, const int32_t* dtypes, const int64_t* sizes) {
   std::string err;
-  if (check_list(count, dtypes, sizes, err)) return -1;
-  // a block of every launch: no more than chunks, nor than there are launches for tensors that
-  // lie anywhere
-  int64_t chunks = 0, tensors = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    chunks += chunks_of(dtypes[i], sizes[i]);
-    tensors += (sizes[i] + kClipMost - 1) / kClipMost;
-  }
-  return std::min(chunks, tensors * kClipBlocks) * int64_t(sizeof(double));
+  int64_t room = 0;
+  return check_list(count, dtypes, sizes, &room, err) ? -1 : room;
 }
 
 int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err) {
-  if (check_list(a.count, a.dtypes, a.sizes, err)) return -1;
+  int64_t need = 0;
+  if (check_list(a.count, a.dtypes, a.sizes, &need, err)) return -1;
   if (!(a.max_norm >= 0)) return fail(err, "max_norm must be >= 0");
   if (!a.norm || (a.count > 0 && !a.grads)) return fail(err, "null argument");
   if (!aligned(a.norm, 4)) return fail(err, "norm must be 4-byte aligned");
@@ -178,7 +185,6 @@ int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err)
   c.part = static_cast<double*>(a.workspace);
   for (const Group& g : groups) c.parts += g.blocks();
   if (!aligned(a.workspace, 8)) return fail(err, "workspace must be 8-byte aligned");
-  const int64_t need = clip_workspace(a.count, a.dtypes, a.sizes);
   if (need > 0 && (!a.workspace || a.workspace_bytes < need))
     return fail(err, "workspace holds " + std::to_string(a.workspace ? a.workspace_bytes : 0) +
                          " bytes, the norm needs " + std::to_string(need));
@@ -190,15 +196,17 @@ int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err)
   int launches = 0;
   cudaError_t e = cudaSuccess;
   const bool outs = a.outs != nullptr;
-  if (groups.size() == 1 && groups[0].entries.size() <= size_t(kClipFew) && groups[0].chunks <= unsigned(kClipOne)) {
+  if (groups.size() == 1 && groups[0].entries <= kClipFew && groups[0].chunks <= unsigned(kClipOne)) {
     ClipTable<kClipFew> t;
-    fill(t, groups[0], outs);
+    fill(t, a, groups[0]);
     e = launch_clip_one(t, c, s);
     launches = 1;
   } else if (groups.empty()) {
     e = launch_clip_finish(c, s);
     launches = 1;
   } else {
+    std::vector<Launch<kClipFew>> few(groups.size());
+    std::vector<Launch<kClipTensors>> many(groups.size());
     for (int pass = 0; pass < (outs ? 2 : 1) && e == cudaSuccess; ++pass) {
       c.first = 0;
       for (size_t i = 0; i < groups.size() && e == cudaSuccess; ++i) {
@@ -206,8 +214,7 @@ int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err)
         const size_t at = pass ? groups.size() - 1 - i : i;
         const Group& g = groups[at];
         c.keep = outs && at + 1 == groups.size() && g.chunks > kKeep ? g.chunks - kKeep : 0;
-        e = g.entries.size() <= size_t(kClipFew) ? run<kClipFew>(g, c, outs, pass, s)
-                                                 : run<kClipTensors>(g, c, outs, pass, s);
+        e = g.entries <= kClipFew ? few[at](a, g, c, pass, s) : many[at](a, g, c, pass, s);
         c.first += g.blocks();
         ++launches;
       }
