@@ -117,6 +117,28 @@ __device__ __forceinline__ void gate_grad(int act, float x, float y, float dh, f
   dy = dh * h;
 }
 
+// Four of them, for bfloat16.
+template <int ACT>
+__device__ __forceinline__ void gate_grads(const float (&x)[4], const float (&y)[4], const float (&dh)[4],
+                                           float (&dx)[4], float (&dy)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float slope;
+    const float h = activation_slope<ACT, true>(x[i], slope);
+    dx[i] = dh[i] * y[i] * slope;
+    dy[i] = dh[i] * h;
+  }
+}
+__device__ __forceinline__ void gate_grad4(int act, const float (&x)[4], const float (&y)[4], const float (&dh)[4],
+                                           float (&dx)[4], float (&dy)[4]) {
+  if (act == kSilu)
+    gate_grads<kSilu>(x, y, dh, dx, dy);
+  else if (act == kGelu)
+    gate_grads<kGelu>(x, y, dh, dx, dy);
+  else
+    gate_grads<kGeluTanh>(x, y, dh, dx, dy);
+}
+
 }  // namespace
 
 }  // namespace mb

@@ -414,7 +414,7 @@ __device__ __forceinline__ void turn1(uint32_t buf, const float (&v)[32], int la
                  "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
                  : "memory");
   __syncwarp();
-#pragma unroll 8
+#pragma unroll 4
   for (int row = 0; row < 32; ++row) {
     float x;
     asm volatile("ld.shared.f32 %0, [%1];"
@@ -485,35 +485,34 @@ __device__ __forceinline__ float4 load4(const float* p, int n, bool wide) {
   return make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
 }
 
-__device__ __forceinline__ void load8(const float* p, int n, bool wide, float (&x)[8]) {
-  const float4 lo = load4(p, n, wide), hi = load4(p + 4, n - 4, wide);
-  x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-  x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+// 16 columns of gates and 16 of their factors, a row a lane, to rows of 32 floats (the gates
+// first) in the warp's buffer.  A row is eight 16-byte units, at positions permuted so that
+// two neighbouring rows' gates, read by eight lanes, have banks of their own.
+__device__ __forceinline__ uint32_t pair_unit(uint32_t buf, int row, int unit) {
+  return buf + row * 128 + ((unit ^ ((row & 1) << 2 | (row >> 1 & 3))) << 4);
 }
-
-// A warp's 32 x 32 columns as in turn_bf16, the values still float32: eight rows at a time with
-// four lanes a row, f(step, row, column, eight values).
-template <class F>
-__device__ __forceinline__ void turn8(uint32_t buf, const float (&v)[32], int lane, F f) {
+__device__ __forceinline__ void put_pairs(uint32_t buf, const float (&v)[16], const float (&w)[16], int lane) {
   __syncwarp();
 #pragma unroll
-  for (int u = 0; u < 8; ++u)
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)),
-                 "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
+  for (int u = 0; u < 8; ++u) {
+    const float* x = u < 4 ? v + 4 * u : w + 4 * (u - 4);
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(pair_unit(buf, lane, u)), "f"(x[0]), "f"(x[1]),
+                 "f"(x[2]), "f"(x[3])
                  : "memory");
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = i * 8 + lane / 4, u = lane % 4 * 2;
-    float x[8];
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(x[4 * q]), "=f"(x[4 * q + 1]), "=f"(x[4 * q + 2]), "=f"(x[4 * q + 3])
-                   : "r"(buf + row * 128 + (((u + q) ^ (row & 7)) << 4)));
-    f(i, row, 4 * u, x);
   }
+  __syncwarp();
 }
+__device__ __forceinline__ void read4(uint32_t at, float (&x)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+               : "r"(at));
+}
+__device__ __forceinline__ float read1(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at));
+  return x;
+}
+__device__ __forceinline__ float4 four(const float (&x)[4]) { return make_float4(x[0], x[1], x[2], x[3]); }
 
 template <int EPI, int TN, bool F32>
 __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads, 1)
@@ -718,21 +717,23 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       const bool known = unsigned(y) < unsigned(r.classes);
       const float lse = EPI == kHeadG && there ? r.lse[row] : 0.f;
       const float up = EPI == kHeadG && known ? r.dloss[row] : 0.f;
-      // a gated block's gradient: what the forward call kept, eight rows of 32 columns a step
-      // (sixteen steps a tile), two steps on their way
-      float px[2][8], py[2][8];
-      auto fetch = [&](int step, float (&x)[8], float (&y)[8]) {
-        const int rr = step % 4 * 8 + lane / 4, cc = step / 4 * 32 + lane % 4 * 8;
+      // a gated block's gradient: what the forward call kept, four rows of 32 columns a step
+      // (32 steps a tile), four steps on their way
+      constexpr int kAhead = 4;
+      float px[kAhead][4], py[kAhead][4];
+      auto fetch = [&](int step, float (&x)[4], float (&y)[4]) {
+        const int rr = step % 8 * 4 + lane / 8, cc = step / 8 * 32 + lane % 8 * 4;
         const int n = a.g.width - (col0 + cc);
-        if (step >= 16 || row - lane + rr >= a.g.rows || n <= 0) return;
+        if (step >= TN / 8 || row - lane + rr >= a.g.rows || n <= 0) return;
         const float* p = a.g.pre + (long long)(row - lane + rr) * a.g.ld_pre + col0 + cc;
-        load8(p, n, a.g.wide_pre, x);
-        load8(p + a.g.width, n, a.g.wide_pre, y);
+        const float4 f = load4(p, n, a.g.wide_pre), h = load4(p + a.g.width, n, a.g.wide_pre);
+        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        y[0] = h.x, y[1] = h.y, y[2] = h.z, y[3] = h.w;
       };
       if constexpr (EPI == kHeadGateGrad) {
         if (!q.plain) {
-          fetch(0, px[0], py[0]);
-          fetch(1, px[1], py[1]);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) fetch(i, px[i], py[i]);
         }
       }
       bool ok = true;
@@ -783,6 +784,16 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             float v[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = sums[c + i];
+            f(c, v);
+          }
+        } else if constexpr (EPI != kHeadLse && EPI != kHeadG) {
+          // one copy of an epilogue that is long: its instructions come from far
+          float v[32];
+#pragma unroll 1
+          for (int c = 0; c < TN / 2; c += 32) {
+            tmem_issue(src + c, v);
+            tmem_wait(v);
+            if (c + 32 == TN / 2) release();  // all of it has been read
             f(c, v);
           }
         } else {
@@ -926,77 +937,94 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       } else if constexpr (EPI == kHeadGate) {
         const HeadGate& g = a.g;
         const int rows = g.rows - (row - lane);
-        // 32 columns from col0 + c on: gates v, their factors w
-        auto part = [&](int c, float (&v)[32], float (&w)[32]) {
-          const int n0 = g.width - (col0 + c);
-          const long long r0 = row - lane;
-          auto put32 = [&](float* to, long long ld, int at, bool wide, const float (&x)[32]) {
-            float* p = to + r0 * ld + at;
-            if (wide)
-              turn(stage, x, lane, [&](int rr, int cc, float4 y) {
-                if (rr < rows && cc < n0) store4(p + rr * ld + cc, y, n0 - cc, true);
-              });
-            else
-              turn1(stage, x, lane, [&](int rr, int cc, float y) {
-                if (rr < rows && cc < n0) p[rr * ld + cc] = y;
-              });
-          };
-          if (g.pre) {
-            put32(g.pre, g.ld_pre, col0 + c, g.wide_pre, v);
-            put32(g.pre, g.ld_pre, g.width + col0 + c, g.wide_pre, w);
-          }
-          activate<!F32>(g.act, v, w);
-          if constexpr (F32) {
-            put32(static_cast<float*>(g.hidden), g.ld_hidden, col0 + c, g.wide, v);
-          } else {
-            __nv_bfloat16* p = static_cast<__nv_bfloat16*>(g.hidden) + r0 * g.ld_hidden + col0 + c;
-            turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 y) {
-              if (rr < rows && cc < n0) store8(p + rr * g.ld_hidden + cc, y, n0 - cc, g.wide);
-            });
-          }
-        };
-        float v[32], w[32];
+        const long long r0 = row - lane;
+        const bool wide = g.wide && (g.wide_pre || !g.pre);
+        float* pre = g.pre ? g.pre + r0 * g.ld_pre + col0 : nullptr;
+        // 16 gates and their factors at a time
 #pragma unroll 1
-        for (int c = 0; c < TN / 4; c += 32) {
-          tmem_issue(src + c, v);
-          tmem_issue(src + TN / 2 + c, w);
-          tmem_wait(v);
-          tmem_wait(w);
-          if (c + 32 == TN / 4) release();
-          part(c, v, w);
+        for (int c = 0; c < TN / 4; c += 16) {
+          const int n0 = g.width - (col0 + c);
+          {
+            float v[16], w[16];
+            tmem_load16(src + c, v);
+            tmem_load16(src + TN / 2 + c, w);
+            if (c + 16 == TN / 4) release();
+            put_pairs(stage, v, w, lane);
+          }
+          if (wide) {
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {  // eight rows, four columns a lane
+              const int rr = i * 8 + lane / 4, cc = lane % 4 * 4, n = n0 - cc;
+              float x[4], y[4];
+              read4(pair_unit(stage, rr, lane % 4), x);
+              read4(pair_unit(stage, rr, 4 + lane % 4), y);
+              if (rr >= rows || n <= 0) continue;
+              if (pre) {
+                store4(pre + rr * g.ld_pre + c + cc, four(x), n, true);
+                store4(pre + rr * g.ld_pre + g.width + c + cc, four(y), n, true);
+              }
+              activate<!F32>(g.act, x, y);
+              const long long at = (r0 + rr) * g.ld_hidden + col0 + c + cc;
+              if (F32)
+                store4(static_cast<float*>(g.hidden) + at, four(x), n, true);
+              else
+                store4(static_cast<__nv_bfloat16*>(g.hidden) + at, four(x), n, true);
+            }
+          } else {
+#pragma unroll 2
+            for (int i = 0; i < 16; ++i) {  // two rows, a column a lane
+              const int rr = i * 2 + lane / 16, cc = lane % 16;
+              float x[1] = {read1(pair_unit(stage, rr, cc / 4) + cc % 4 * 4)};
+              const float y[1] = {read1(pair_unit(stage, rr, 4 + cc / 4) + cc % 4 * 4)};
+              if (rr >= rows || cc >= n0) continue;
+              if (pre) {
+                pre[rr * g.ld_pre + c + cc] = x[0];
+                pre[rr * g.ld_pre + g.width + c + cc] = y[0];
+              }
+              activate<!F32>(g.act, x, y);
+              const long long at = (r0 + rr) * g.ld_hidden + col0 + c + cc;
+              if (F32)
+                static_cast<float*>(g.hidden)[at] = x[0];
+              else
+                static_cast<__nv_bfloat16*>(g.hidden)[at] = __float2bfloat16_rn(x[0]);
+            }
+          }
         }
       } else if constexpr (EPI == kHeadGateGrad) {
         if (q.plain) {
           store_out();
           continue;
         }
-        // up to `half` columns a half, zeros from `width` on: whole units of eight
+        // up to `half` columns a half, zeros from `width` on: whole units of four
         const HeadGate& g = a.g;
         const int rows = g.rows - (row - lane), n0 = g.width - col0, n1 = g.half - col0;
         __nv_bfloat16* d = static_cast<__nv_bfloat16*>(g.dpre) + (long long)(row - lane) * g.ld_d + col0;
         each_part([&](int c, float (&v)[32]) {
-          turn8(stage, v, lane, [&](int i, int rr, int cc, const float (&dh)[8]) {
-            float (&x)[8] = px[i % 2], (&y)[8] = py[i % 2];
-            uint32_t dx[4], dy[4];
-            cc += c;
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float a0, a1, b0, b1;
-              gate_grad<true>(g.act, x[2 * k], y[2 * k], dh[2 * k], a0, b0);
-              gate_grad<true>(g.act, x[2 * k + 1], y[2 * k + 1], dh[2 * k + 1], a1, b1);
-              if (cc + 8 > n0) {
-                if (cc + 2 * k >= n0) a0 = b0 = 0.f;
-                if (cc + 2 * k + 1 >= n0) a1 = b1 = 0.f;
-              }
-              dx[k] = pack2(a0, a1);
-              dy[k] = pack2(b0, b1);
+          for (int u = 0; u < 8; ++u)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((u ^ (lane & 7)) << 4)),
+                         "f"(v[4 * u]), "f"(v[4 * u + 1]), "f"(v[4 * u + 2]), "f"(v[4 * u + 3])
+                         : "memory");
+          __syncwarp();
+#pragma unroll 1
+          for (int i0 = 0; i0 < 8; i0 += kAhead)
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {  // four rows, four columns a lane
+              const int rr = (i0 + k) * 4 + lane / 8, u = lane % 8, cc = c + 4 * u;
+              float dh[4], dx[4], dy[4];
+              read4(stage + rr * 128 + ((u ^ (rr & 7)) << 4), dh);
+              gate_grad4(g.act, px[k], py[k], dh, dx, dy);
+              fetch(c / 4 + i0 + k + kAhead, px[k], py[k]);
+              if (rr >= rows || cc >= n1) continue;
+              if (cc + 4 > n0)
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                  if (cc + z >= n0) dx[z] = dy[z] = 0.f;
+              __nv_bfloat16* to = d + rr * g.ld_d + cc;
+              store4(to, four(dx), 4, true);
+              store4(to + g.half, four(dy), 4, true);
             }
-            fetch(c / 8 + i + 2, x, y);
-            if (rr >= rows || cc >= n1) return;
-            __nv_bfloat16* to = d + rr * g.ld_d + cc;
-            *reinterpret_cast<uint4*>(to) = make_uint4(dx[0], dx[1], dx[2], dx[3]);
-            *reinterpret_cast<uint4*>(to + g.half) = make_uint4(dy[0], dy[1], dy[2], dy[3]);
-          });
         });
       } else {
         store_out();
