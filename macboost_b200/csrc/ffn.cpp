@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 
 #include "engine.h"
 #include "head.h"
@@ -59,13 +60,48 @@ struct Shape {
   int64_t m, n, k;
   int tile_n, splits;
   int box;                           // rows of a K-major B that a CTA fetches
-  int64_t weight(int dtype) const {  // steps of all its tiles
-    return parts(m, kTileM) * parts(n, tile_n) * (parts(k, kHeadTileK) * (dtype == kF32 ? 6 : 1) + kHeadEpilogue);
-  }
+  int64_t tiles() const { return parts(m, kTileM) * parts(n, tile_n); }
+  int64_t blocks() const { return parts(k, kHeadTileK); }
 };
 Shape shape(int64_t m, int64_t n, int64_t k) {
   const int tile = n <= 128 ? 128 : 256;
   return Shape{m, n, k, tile, 1, tile / kHeadPair};
+}
+
+// Parts of K of one or two products of a launch: those that end first by an estimate, in steps
+// of one K block (0.42 us for 256 columns).  A pair's time is the longest tile's, or its share
+// of all steps and half a tile more; the sums of parts are written and read once more, at
+// 6 TB/s.  Bounds of a part as head_splits has them: no shorter than 8 blocks (float32: 2),
+// bfloat16 no longer than 512.  `whole`: the second one's epilogue needs all of its sums.
+void choose_splits(int dtype, Shape* a, Shape* b, bool whole = false) {
+  constexpr int64_t kPairs = 74;
+  const int64_t steps = dtype == kF32 ? 6 : 1, shortest = dtype == kF32 ? 2 : 8;
+  auto least = [&](const Shape& q) { return dtype == kF32 ? int64_t(1) : parts(q.blocks(), 512); };
+  auto most = [&](const Shape& q) { return std::max(least(q), std::min<int64_t>(q.blocks() / shortest, 32)); };
+  auto tile = [&](const Shape& q, int64_t s) {
+    return (double(parts(q.blocks(), s) * steps) + kHeadEpilogue) * q.tile_n / 256;
+  };
+  auto sums = [&](const Shape& q, int64_t s) {
+    return s > 1 ? double(2 * s + 1) * double(q.m) * double(q.n) * 4 / 6e6 / 0.42 + 8 : 0.0;
+  };
+  double best = 0;
+  const int64_t first = b && !whole ? least(*b) : 1, last = b && !whole ? most(*b) : 1;
+  for (int64_t s = least(*a); s <= most(*a); ++s)
+    for (int64_t t = first; t <= last; ++t) {
+      const double ta = tile(*a, s), tb = b ? tile(*b, t) : 0;
+      const int64_t na = a->tiles() * s, nb = b ? b->tiles() * t : 0;
+      const double all = double(na) * ta + double(nb) * tb, longest = std::max(ta, tb);
+      const double shortest_tile = nb ? std::min(ta, tb) : ta;
+      double time = longest;
+      if (na + nb > kPairs)
+        time = nb ? std::max(longest, all / kPairs + shortest_tile / 2) : double(parts(na, kPairs)) * ta;
+      time += sums(*a, s) + (b ? sums(*b, t) : 0);
+      if (best == 0 || time < best) {
+        best = time;
+        a->splits = int(s);
+        if (b) b->splits = int(t);
+      }
+    }
 }
 
 struct Plan {
@@ -95,16 +131,9 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
   if (pk.w_out) p.w_out = packed(outs, width);
   if (pk.hidden) p.hidden = packed(rows, width);
   auto sums = [&](const Shape& q) { return q.splits > 1 ? q.splits * q.m * q.n * 4 : 0; };
-  auto split = [&](Shape& q, int64_t all) {
-    const int64_t blocks = parts(q.k, kHeadTileK), tiles = parts(q.m, kTileM) * parts(q.n, q.tile_n);
-    q.splits = head_splits(blocks, all, dtype);
-    // few tiles: one round of parts for the pairs of CTAs, not two
-    const int64_t least = dtype == kF32 ? 1 : parts(blocks, 512);
-    if (tiles < 74) q.splits = int(std::max<int64_t>(least, std::min<int64_t>(q.splits, 74 / tiles)));
-  };
   if (!grad) {
     p.y = shape(rows, outs, width);
-    split(p.y, p.y.weight(dtype));
+    choose_splits(dtype, &p.y, nullptr);
     p.part = take(sums(p.y));
   } else {
     if (pk.dy) p.dy = packed(rows, outs);
@@ -114,10 +143,9 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
     p.dx = shape(rows, cols, 2 * p.half);
     p.dw_in = shape(p.half + width, cols, rows);
     p.dw_out = shape(outs, width, rows);
-    const int64_t both = p.dx.weight(dtype) + p.dw_in.weight(dtype);
-    split(p.dx, both);
-    split(p.dw_in, both);
-    split(p.dw_out, p.dw_out.weight(dtype) + (dtype == kF32 ? 0 : shape(rows, width, outs).weight(dtype)));
+    choose_splits(dtype, &p.dx, &p.dw_in);
+    Shape dh = shape(rows, width, outs);
+    choose_splits(dtype, &p.dw_out, dtype == kF32 ? nullptr : &dh, true);
     // dw_out is done before the others begin
     p.part = take(std::max(sums(p.dw_out), sums(p.dx)));
     p.part_in = take(sums(p.dw_in));
@@ -207,14 +235,18 @@ struct Call {
     }
     return o;
   }
-  // Up to two matrices, in one launch; `status`: it clears the status word as well.
-  int pack(const HeadPack& q, const HeadPack& r, bool status) {
+  // Matrices that are to be packed, in one launch; `status`: it clears the status word as well.
+  int pack(std::initializer_list<const HeadPack*> list, bool status) {
     unsigned* word = static_cast<unsigned*>(a.workspace);
-    if (!q.src && !r.src) {
+    HeadPack todo[kHeadPacks];
+    int count = 0;
+    for (const HeadPack* q : list)
+      if (q->src) todo[count++] = *q;
+    if (count == 0) {
       if (status) FFN_CUDA(cudaMemsetAsync(word, 0, 4, s), "clearing the block's status word");
       return 0;
     }
-    FFN_CUDA(launch_head_pack(a.dtype, q, r, status ? word : nullptr, s), "pack launch");
+    FFN_CUDA(launch_head_pack(a.dtype, todo, count, status ? word : nullptr, s), "pack launch");
     ++launches;
     return 0;
   }
@@ -316,7 +348,8 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   const Operand w_in = c.operand(a.w_in, 2 * a.width, a.cols, a.ld_in, p.w_in, &pin);
   const Operand w_out = c.operand(a.w_out, a.outs, a.width, a.ld_out, p.w_out, &pout);
   const Operand h = c.operand(a.hidden, a.rows, a.width, a.ld_hidden, p.hidden, &ph);
-  if (c.pack(px, pin, true)) return -1;
+  // w_out beside the others, for the second product
+  if (c.pack({&px, &pin, &pout}, true)) return -1;
 
   // gates and factors: a tile's 256 columns are 128 of each
   HeadLaunch l{};
@@ -328,7 +361,7 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   FFN_CUDA(launch_head(kHeadGate, kHeadTileN, l, s), "block launch");
   ++c.launches;
 
-  if ((ph.src || pout.src) && c.pack(ph, pout, false)) return -1;
+  if (c.pack({&ph}, false)) return -1;
   HeadLaunch q{};
   head_settings(q, a.dtype, a.workspace);
   q.jobs = 1;
@@ -370,10 +403,15 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
   const Operand dy = c.operand(a.dy, a.rows, a.outs, a.ld_dy, p.dy, &pdy);
   const Operand d{c.base() + p.dpre, a.rows, 2 * p.half, 2 * p.half};
   const bool f32 = a.dtype == kF32, inner = a.dx || a.dw_in;
-  if (c.pack(pdy, pout, false)) return -1;
+  // h with the others, unless a launch of its own makes its planes
+  const HeadPack none;
+  const bool split = inner && f32;
+  if (c.pack({&pdy, inner ? &pout : &none, a.dw_out && !split ? &ph : &none, inner ? &px : &none,
+              a.dx ? &pin : &none}, false))
+    return -1;
   // dh = dy w_out; its epilogue (float32: a launch) makes the gradients of gates and factors of it
   const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
-  if (inner && f32) {
+  if (split) {
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
     q.jobs = 1;
@@ -396,8 +434,6 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     if (c.products(kHeadOut, q, kHeadTileN, nullptr, 0)) return -1;
     FFN_CUDA(launch_ffn_split(t, s), "block split launch");
     ++c.launches;
-  } else if (a.dw_out && c.pack(ph, HeadPack(), false)) {
-    return -1;
   }
   if (a.dw_out || (inner && !f32)) {
     // dw_out = dy^T h: in bfloat16 in one launch with dh, whose epilogue takes longer than its products
@@ -428,7 +464,6 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     if (c.products(with ? kHeadGateGrad : kHeadOut, q, tile, red, reds)) return -1;
   }
   if (inner) {
-    if (c.pack(px, pin, false)) return -1;
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
     HeadReduce red[2]{};

@@ -255,7 +255,8 @@ int operands(const HeadArgs& a, const Plan& p, bool grad, Operands* o, cudaStrea
     return 0;
   }
   unsigned* status = grad ? nullptr : reinterpret_cast<unsigned*>(base);
-  HEAD_CUDA(launch_head_pack(a.dtype, h, w, status, s), "head pack launch");
+  const HeadPack list[2] = {h, w};
+  HEAD_CUDA(launch_head_pack(a.dtype, list, 2, status, s), "head pack launch");
   o->launches = 1;
   return 0;
 }

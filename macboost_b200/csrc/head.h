@@ -187,8 +187,8 @@ struct HeadPack {
   void* dst = nullptr;
   long long ldp = 0;
 };
-cudaError_t launch_head_pack(int dtype, const HeadPack& a, const HeadPack& b, unsigned* status,
-                             cudaStream_t s);
+constexpr int kHeadPacks = 5;        // matrices of a launch, at most
+cudaError_t launch_head_pack(int dtype, const HeadPack* list, int count, unsigned* status, cudaStream_t s);
 cudaError_t launch_head_finish(const float2* part, const float* target, const int* labels,
                                int64_t rows, int64_t classes, int64_t parts, float* loss,
                                float* lse, cudaStream_t s);

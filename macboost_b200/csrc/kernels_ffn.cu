@@ -202,25 +202,25 @@ cudaError_t few_type(const Few& a, cudaStream_t s) {
 // planes a half on top of that stopped it for 85 us a tile of 256 x 256; written out as float32
 // and formed here, 2,048 x 4,096 takes 30 bytes a value.
 
-// A plane of a value, which becomes the rest: as the head's planes, finite values that would
-// round to infinity are bfloat16's largest, and the rest of what is not finite is zero.
-__device__ __forceinline__ __nv_bfloat16 plane_of(int z, float& v) {
-  constexpr float kLargest = 3.3895313892515355e38f;
-  const __nv_bfloat16 t = __float2bfloat16_rn(isfinite(v) ? fminf(fmaxf(v, -kLargest), kLargest) : v);
-  v = z == 0 && !isfinite(v) ? 0.f : v - __bfloat162float(t);
-  return t;
-}
-// Four adjacent values as three planes of bfloat16, `plane` apart.
+// Four adjacent values as three planes of bfloat16, `plane` apart.  As the head's planes:
+// finite values that would round to infinity are bfloat16's largest and a rest, and the rest
+// of what is not finite is zero.
 __device__ __forceinline__ void put_planes(__nv_bfloat16* to, long long plane, const float (&x)[4]) {
-  float v[4] = {x[0], x[1], x[2], x[3]};
+  constexpr float kLargest = 3.3895313892515355e38f;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = fabsf(x[i]) < INFINITY ? fminf(fmaxf(x[i], -kLargest), kLargest) : x[i];
 #pragma unroll
   for (int z = 0; z < 3; ++z) {
-    __nv_bfloat16 t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = plane_of(z, v[i]);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
     uint2 w;
-    memcpy(&w, t, 8);
+    memcpy(&w.x, &lo, 4);
+    memcpy(&w.y, &hi, 4);
     *reinterpret_cast<uint2*>(to + z * plane) = w;
+    const float t[4] = {__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                        __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = z == 0 ? (fabsf(x[i]) < INFINITY ? x[i] - t[i] : 0.f) : v[i] - t[i];
   }
 }
 

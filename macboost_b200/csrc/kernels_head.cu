@@ -1044,18 +1044,22 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
 // ---- the kernels around it ------------------------------------------------------
 
 // Planes of bfloat16 with 16-byte aligned rows: the terms of a float32, or a copy.  A
-// warp a row, eight values a lane; the rows of up to two matrices one after the other.
+// warp a row, eight values a lane; the rows of several matrices one after the other.
 // It also clears the status word, unless null.
 constexpr float kLargest = 3.3895313892515355e38f;  // of bfloat16
+struct HeadPackList {
+  HeadPack m[kHeadPacks];
+  int count;
+};
 template <class T>
-__global__ void __launch_bounds__(256) head_pack_kernel(const HeadPack a, const HeadPack b, unsigned* status) {
+__global__ void __launch_bounds__(256) head_pack_kernel(const __grid_constant__ HeadPackList list, unsigned* status) {
   if (status && blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
   const int lane = threadIdx.x % 32;
   long long r = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-  const bool second = r >= a.rows;
-  if (second) r -= a.rows;
-  const HeadPack& m = second ? b : a;
-  if (r >= m.rows) return;
+  int at = 0;
+  while (at < list.count && r >= list.m[at].rows) r -= list.m[at++].rows;
+  if (at == list.count) return;
+  const HeadPack& m = list.m[at];
   // a row without a label becomes zeros
   const int cols = m.labels && unsigned(m.labels[r]) >= unsigned(m.classes) ? 0 : int(m.cols);
   const T* from = static_cast<const T*>(m.src) + r * m.ld;
@@ -1904,14 +1908,19 @@ cudaError_t launch_head_few(const HeadArgs& h, bool grad, const HeadFew& f, cuda
               : few_rows<__nv_bfloat16, 1>(a, grad, f.blocks, f.chunks, s);
 }
 
-cudaError_t launch_head_pack(int dtype, const HeadPack& a, const HeadPack& b, unsigned* status,
-                             cudaStream_t s) {
-  const long long blocks = (a.rows + b.rows + 7) / 8;
+cudaError_t launch_head_pack(int dtype, const HeadPack* list, int count, unsigned* status, cudaStream_t s) {
+  HeadPackList all{};
+  long long rows = 0;
+  for (; all.count < count; ++all.count) {
+    all.m[all.count] = list[all.count];
+    rows += list[all.count].rows;
+  }
+  const long long blocks = (rows + 7) / 8;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
   if (dtype == kF32)
-    head_pack_kernel<float><<<unsigned(blocks), 256, 0, s>>>(a, b, status);
+    head_pack_kernel<float><<<unsigned(blocks), 256, 0, s>>>(all, status);
   else
-    head_pack_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, s>>>(a, b, status);
+    head_pack_kernel<__nv_bfloat16><<<unsigned(blocks), 256, 0, s>>>(all, status);
   return cudaGetLastError();
 }
 
