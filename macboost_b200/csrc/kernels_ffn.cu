@@ -80,10 +80,29 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
   float* rows = reinterpret_cast<float*>(few_shared);  // NR x pitch
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (GATE && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
-  for (int n = 0; n < NR; ++n)
-    for (int d = threadIdx.x; d < a.pitch; d += kThreads)
-      rows[n * a.pitch + d] =
-          n < a.rows && d < a.cols ? float(static_cast<const T*>(a.in)[n * a.ld_in + d]) : 0.f;
+  // the rows, PER values at a time, all of a thread's loads on their way: a value after the
+  // other took 6 us of 16,384
+  for (int n = 0; n < NR; ++n) {
+    const T* from = static_cast<const T*>(a.in) + n * a.ld_in;
+    const bool whole = PER > 1 && n < a.rows && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+    if (whole) {
+#pragma unroll 8
+      for (int d = threadIdx.x * PER; d < a.cols; d += kThreads * PER) {
+        Load<T, PER> q;
+        q.get(from + d);
+        float v[PER];
+        q.values(v);
+#pragma unroll
+        for (int i = 0; i < PER; i += 4)
+          *reinterpret_cast<float4*>(rows + n * a.pitch + d + i) =
+              make_float4(v[i], v[i + (PER > 1)], v[i + 2 * (PER > 2)], v[i + 3 * (PER > 2)]);
+      }
+    } else {
+#pragma unroll 8
+      for (int d = threadIdx.x; d < a.cols; d += kThreads)
+        rows[n * a.pitch + d] = n < a.rows ? float(from[d]) : 0.f;
+    }
+  }
   __syncthreads();
   const int stride = int(gridDim.x) * kWarps * C;
   for (int o0 = (int(blockIdx.x) * kWarps + warp) * C; o0 < a.outs; o0 += stride) {
