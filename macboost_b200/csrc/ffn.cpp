@@ -263,6 +263,7 @@ struct Call {
     j.tiles_n = int(parts(h.n, h.tile_n));
     j.kblocks = int(parts(h.k, kHeadTileK));
     j.splits = std::min(h.splits, j.kblocks);
+    if (h.tiles() * j.splits > INT_MAX) return fail(err, "rows * width are too many for one call");
     j.M = int(h.m);
     j.N = int(h.n);
     // tile rows whose part of A stays in the L2 cache while the columns go by

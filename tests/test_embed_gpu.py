@@ -40,12 +40,13 @@ def _grad(core, torch, dout, entries, cols, ids, starts, scale, pad=0):
     need = core.embed_workspace(entries, cols, rows, k)
     room = torch.full((need + 256,), 255, dtype=torch.uint8, device="cuda")
     room[need:] = 3
-    d = torch.full((entries, cols + pad), 7.0, dtype=dout.dtype, device="cuda")
+    whole = torch.full((entries + 1, cols + pad), 7.0, dtype=dout.dtype, device="cuda")
+    d = whole[:entries]
     core.embed_grad_device(0, CODES[str(dout.dtype)[6:]], dout.data_ptr(), rows, cols, dout.stride(0),
                            ids.data_ptr(), k, 0 if starts is None else starts.data_ptr(), scale,
                            d.data_ptr(), entries, d.stride(0), room.data_ptr(), need,
                            stream=torch.cuda.current_stream().cuda_stream)
-    assert torch.all(d[:, cols:] == 7.0) and torch.all(room[need:] == 3)
+    assert torch.all(d[:, cols:] == 7.0) and torch.all(whole[entries] == 7.0) and torch.all(room[need:] == 3)
     return d[:, :cols]
 
 

@@ -40,13 +40,14 @@ class Block:
             return (torch.randn((r, c + pad), device="cuda", generator=g) * s).to(t)
 
         def empty(r, c):
-            return torch.full((r, c + pad), 7.0, dtype=t, device="cuda")
+            return torch.full((r + 2, c + pad), 7.0, dtype=t, device="cuda")[:r]
 
         self.x = normal(rows, cols, scale)
         self.w_in = normal(2 * width, cols, 2 / cols ** 0.5)
         self.w_out = normal(outs, width, 1 / width ** 0.5)
         self.dy = normal(rows, outs, 1.0)
-        self.hidden, self.pre, self.y = empty(rows, width), empty(rows, 2 * width).float(), empty(rows, outs)
+        self.hidden, self.y = empty(rows, width), empty(rows, outs)
+        self.pre = torch.full((rows + 2, 2 * width + pad), 7.0, device="cuda")[:rows]
         self.dx, self.dw_in, self.dw_out = empty(rows, cols), empty(2 * width, cols), empty(outs, width)
         self.need = core.ffn_workspace(self.code, rows, cols, width, outs, grad=True, strided=pad % 8 != 0)
         self.room = torch.full((self.need + 512,), 255, dtype=torch.uint8, device="cuda")
@@ -83,11 +84,11 @@ class Block:
                 "dx": self.dx[:, :cols], "dw_in": self.dw_in[:, :cols], "dw_out": self.dw_out[:, :width]}
 
     def intact(self):
-        """Nothing was written behind the columns."""
+        """Nothing was written behind the columns, nor behind the last row."""
         rows, cols, width, outs = self.shape
         for t, c in ((self.hidden, width), (self.pre, 2 * width), (self.y, outs), (self.dx, cols),
                      (self.dw_in, cols), (self.dw_out, width)):
-            assert self.torch.all(t[:, c:] == 7.0)
+            assert self.torch.all(t[:, c:] == 7.0) and self.torch.all(t._base[t.shape[0]:] == 7.0)
         end = self.at + self.need - self.room.data_ptr()
         assert self.torch.all(self.room[end:] == 255)
 
@@ -143,9 +144,10 @@ class Block:
 SIZES = [(5, 8, 10, 1), (6, 16, 8, 8), (128, 64, 128, 256), (129, 65, 257, 7), (257, 100, 403, 10),
          (300, 72, 513, 65), (1000, 264, 96, 300), (33, 1030, 130, 130), (48, 512, 1024, 256),
          (700, 128, 256, 1), (2000, 24, 40, 16), (4100, 32, 64, 129), (17, 4096, 24, 40)]
-FEW = [(5, 64, 2048, 72), (8, 40, 4000, 136), (11, 264, 72, 1000), (16, 2056, 640, 48), (25, 8, 8, 8), (47, 128, 1032, 512),
-       (64, 512, 2000, 264), (65, 512, 2000, 264), (12, 33, 70, 9), (16, 96, 130, 260), (1, 1, 1, 1), (1, 1024, 3001, 300), (2, 65, 70, 33), (3, 257, 100, 10), (4, 512, 999, 128),
-       (1, 72, 16_384, 64), (2, 8, 20_000, 24), (4, 1000, 136, 1), (1, 40_000, 8, 8)]
+FEW = [(1, 1, 1, 1), (1, 1024, 3001, 300), (2, 65, 70, 33), (3, 257, 100, 10), (4, 512, 999, 128),
+       (1, 72, 16_384, 64), (2, 8, 20_000, 24), (4, 1000, 136, 1), (1, 40_000, 8, 8), (5, 64, 2048, 72),
+       (8, 40, 4000, 136), (8, 512, 1000, 64), (11, 264, 72, 1000), (12, 33, 70, 9), (16, 96, 130, 260),
+       (16, 2056, 640, 48), (25, 8, 8, 8), (47, 128, 1032, 512), (64, 512, 2000, 264), (65, 512, 2000, 264)]
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
