@@ -68,6 +68,14 @@ Shape shape(int64_t m, int64_t n, int64_t k) {
   return Shape{m, n, k, tile, 1, tile / kHeadPair};
 }
 
+// The first product: 128 gates and their factors a tile, or 64 where that ends sooner.  Narrow tiles
+// cost six tenths of a wide one each (bfloat16: more bytes for what they compute).
+Shape gate_shape(int dtype, int64_t rows, int64_t width, int64_t cols) {
+  auto rounds = [&](int64_t gates) { return double(parts(parts(rows, kTileM) * parts(width, gates), 74)); };
+  const int gates = rounds(64) * (dtype == kF32 ? 0.55 : 0.6) < rounds(128) ? 64 : 128;
+  return Shape{rows, width, cols, gates, 1, gates};
+}
+
 // Parts of K of one or two products of a launch: those that end first by an estimate, in steps
 // of one K block (0.42 us for 256 columns).  A pair's time is the longest tile's, or its share
 // of all steps and half a tile more; the sums of parts are written and read once more, at
@@ -352,14 +360,14 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   // w_out beside the others, for the second product
   if (c.pack({&px, &pin, &pout}, true)) return -1;
 
-  // gates and factors: a tile's 256 columns are 128 of each
+  // gates and factors: half of a tile's columns each
+  const Shape in = gate_shape(a.dtype, a.rows, a.width, a.cols);
   HeadLaunch l{};
   head_settings(l, a.dtype, a.workspace);
   l.jobs = 1;
-  const Shape in{a.rows, a.width, a.cols, kHeadTileN / 2, 1, kHeadTileN / 2};
   if (c.job(l.job[0], x, false, w_in, false, in)) return -1;
   gate(l.g, a);
-  FFN_CUDA(launch_head(kHeadGate, kHeadTileN, l, s), "block launch");
+  FFN_CUDA(launch_head(kHeadGate, 2 * in.tile_n, l, s), "block launch");
   ++c.launches;
 
   if (c.pack({&ph}, false)) return -1;

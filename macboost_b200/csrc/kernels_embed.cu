@@ -141,6 +141,37 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
+// One id a row, Q units a lane: little but the loads and stores, so that eight blocks fit a
+// multiprocessor.
+template <class T, int BYTES, int Q>
+__global__ void __launch_bounds__(kThreads, 8)
+    embed_lookup_kernel(const EmbedArgs a, int lanes, int units, int slabs) {
+  using V = Values<T, BYTES>;
+  using U = typename V::U;
+  const int lane = threadIdx.x % lanes;
+  const long long g = (long long)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
+  const long long n = g / slabs;
+  if (n >= a.rows) return;
+  const int u = int(g - n * slabs) * (Q * lanes) + lane;
+  const int e = looked_up(a.ids[n], a.starts ? a.starts[0] : 0, int(a.entries));
+  const U* row = static_cast<const U*>(a.table) + (long long)max(e, 0) * (a.ld / V::N) + u;
+  V v[Q];
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+    if (e >= 0 && u + q * lanes < units) v[q].u = __ldg(row + q * lanes);
+  U* out = static_cast<U*>(a.out) + n * (a.ld_out / V::N) + u;
+#pragma unroll
+  for (int q = 0; q < Q; ++q)
+    if (u + q * lanes < units) {
+      float acc[V::N];
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) acc[i] = 0.f;
+      if (e >= 0) v[q].add_to(acc);
+      v[q].set(acc, a.scale);
+      __stcs(out + q * lanes, v[q].u);
+    }
+}
+
 // Many ids a row.  Each lane of a group finds the rows of the table that one id of each of the
 // group's R rows looks up, and hands them round.  The rows of a block (neighbours) meet the
 // same columns of ids at the same time, so a column's few rows of the table are found in
@@ -759,6 +790,14 @@ cudaError_t forward(const EmbedArgs& a, cudaStream_t s) {
   // four units a lane where a row has that many for every lane and few rows are added up
   const bool wide = a.k < 4 && a.cols / N >= 128 && a.rows * (a.cols / N) >= 4ll * kThreads * device_sms();
   const Shape h = shape(a.cols, N, wide ? 4 : 1);
+  const unsigned blocks1 = h.blocks(a.rows);
+  if (a.k == 1 && blocks1) {
+    if (wide)
+      embed_lookup_kernel<T, BYTES, 4><<<blocks1, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
+    else
+      embed_lookup_kernel<T, BYTES, 1><<<blocks1, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
+    return cudaGetLastError();
+  }
   // several rows a group where that leaves enough of them for the GPU
   const long long tile = Values<T, BYTES>::ROWS * (kThreads / h.lanes), many = (a.rows + tile - 1) / tile * h.slabs;
   if (a.k >= 8 && h.lanes >= 8 && many >= 4 * device_sms() && many <= INT_MAX) {

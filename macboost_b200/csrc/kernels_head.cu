@@ -1839,7 +1839,7 @@ cudaError_t go(const HeadLaunch& a, cudaStream_t s) {
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s) {
   if (epilogue == kHeadLse) return go<kHeadLse, 256>(a, s);
   if (epilogue == kHeadG) return go<kHeadG, 256>(a, s);
-  if (epilogue == kHeadGate) return go<kHeadGate, 256>(a, s);
+  if (epilogue == kHeadGate) return tile_n == 128 ? go<kHeadGate, 128>(a, s) : go<kHeadGate, 256>(a, s);
   if (epilogue == kHeadGateGrad)  // float32: a launch of its own (launch_ffn_split)
     return a.f32 ? cudaErrorInvalidValue : go_type<kHeadGateGrad, 256, false>(a, s);
   return tile_n == 128 ? go<kHeadOut, 128>(a, s) : go<kHeadOut, 256>(a, s);
