@@ -718,8 +718,8 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
       const float lse = EPI == kHeadG && there ? r.lse[row] : 0.f;
       const float up = EPI == kHeadG && known ? r.dloss[row] : 0.f;
       // a gated block's gradient: what the forward call kept, four rows of 32 columns a step
-      // (32 steps a tile), four steps on their way
-      constexpr int kAhead = 4;
+      // (32 steps a tile), eight steps on their way
+      constexpr int kAhead = 8;
       float px[kAhead][4], py[kAhead][4];
       auto fetch = [&](int step, float (&x)[4], float (&y)[4]) {
         const int rr = step % 8 * 4 + lane / 8, cc = step / 8 * 32 + lane % 8 * 4;
