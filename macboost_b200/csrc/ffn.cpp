@@ -55,6 +55,13 @@ bool is_few(int dtype, int64_t rows, int64_t cols, int64_t width) {
   return rows <= (dtype == kF32 ? kFfnFewRowsF32 : kFfnFewRows) && n * ffn_pitch(std::max(cols, width)) * 4 <= kFfnFewSmem;
 }
 
+// The products of warps: all rows in place, 16 bytes at a time.
+bool is_warps(const FfnArgs& a) {
+  auto whole = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) | uintptr_t(ld) * 2) % 16 == 0; };
+  return a.dtype == kBF16 && a.rows >= 2 && a.rows <= kFfnWarpRows && a.cols % 8 == 0 && a.width % 8 == 0 &&
+         whole(a.x, a.ld_x) && whole(a.w_in, a.ld_in) && whole(a.w_out, a.ld_out) && whole(a.hidden, a.ld_hidden);
+}
+
 // A product's tiles.
 struct Shape {
   int64_t m, n, k;
@@ -339,11 +346,12 @@ int64_t ffn_workspace(int dtype, int64_t rows, int64_t cols, int64_t width, int6
 int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   if (check(a, false, err)) return -1;
   if (a.rows == 0) return 0;
-  if (is_few(a.dtype, a.rows, a.cols, a.width)) {
+  const bool warps = is_warps(a);
+  if (warps || is_few(a.dtype, a.rows, a.cols, a.width)) {
     if (check_workspace(a, 256, err)) return -1;
     if (use_device(device, err)) return -1;
     Guard gd(device);
-    FFN_CUDA(launch_ffn_few(a, s), "block launch");
+    FFN_CUDA(warps ? launch_ffn_rows(a, s) : launch_ffn_few(a, s), "block launch");
     g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
     return 0;
   }

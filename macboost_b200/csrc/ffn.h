@@ -56,6 +56,9 @@ constexpr int64_t kFfnFewRows = 4, kFfnFewRowsF32 = 16;
 constexpr int64_t kFfnFewSmem = 128 * 1024;
 inline int64_t ffn_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }  // floats between rows there
 cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);
+// Two to 16 rows of bfloat16 whose matrices' rows lie on 16 bytes, and are as long: products of warps.
+constexpr int64_t kFfnWarpRows = 16;
+cudaError_t launch_ffn_rows(const FfnArgs& a, cudaStream_t s);
 // float32: from dh (stride ld_dh) and pre to the planes of the gradients of both halves
 // (3 x rows x 2 half, zeros from width to half), and of hidden (3 x rows x ld_h) unless null.
 struct FfnSplit {

@@ -76,6 +76,8 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
   constexpr int C = 2;                        // outputs a warp
   constexpr int R = GATE ? 2 * C : C;         // rows of weights
   constexpr int STEPS = 8 / R;                // of each, on their way at once
+  // float32: shorter sums, which are then added up, round less; many rows have no registers for it
+  constexpr bool PARTS = sizeof(T) == 4 && NR <= 4;
   extern __shared__ float4 few_shared[];
   float* rows = reinterpret_cast<float*>(few_shared);  // NR x pitch
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -123,6 +125,11 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (d0 + t * 32 * PER < a.cols) q[t][r].get(w[r] + d0 + t * 32 * PER);
+      float part[R][NR];
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) part[r][n] = PARTS ? 0.f : acc[r][n];
 #pragma unroll
       for (int t = 0; t < STEPS; ++t) {
         const int d = d0 + t * 32 * PER;
@@ -147,9 +154,13 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
 #pragma unroll
           for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) acc[r][n] = fmaf(v[i], x[n][i], acc[r][n]);
+            for (int i = 0; i < PER; ++i) part[r][n] = fmaf(v[i], x[n][i], part[r][n]);
         }
       }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) acc[r][n] = PARTS ? acc[r][n] + part[r][n] : part[r][n];
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -213,6 +224,125 @@ cudaError_t few_type(const Few& a, cudaStream_t s) {
   const bool wide = (reinterpret_cast<uintptr_t>(a.w) | uintptr_t(a.ld_w) * sizeof(T) |
                      uintptr_t(a.cols) * sizeof(T)) % 16 == 0;
   return wide ? few_rows<T, PER, GATE>(a, s) : few_rows<T, 1, GATE>(a, s);
+}
+
+// ---- bfloat16: up to 16 rows by products of warps ---------------------------------------
+//
+// What ffn_few_kernel spends on a weight (unpacking, a product a row, rows from shared memory) takes
+// longer than fetching it from two rows on.  Here a warp's mma.m16n8k16 has 16 rows of weights as A
+// and eight rows of x as B.  The order of K within a product is free, so a lane takes 16 adjacent
+// bytes of a row of weights, and the same of a row of x, as its part of two products: no
+// shuffles, nothing through shared memory.  A block's warps share K, WARPS chunks of 128 at a
+// time, and join their sums in shared memory in one order.  x and h are read over and over from the
+// L1 cache, where weights leave no trace.  Gates are an A's first eight rows and their factors its
+// last eight, so a lane's sums are of both.
+
+struct Rows16 {
+  uint4 v;
+  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void stream(const __nv_bfloat16* p) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  }
+};
+
+__device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                      uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: eights of rows.
+template <int WARPS, int NT, bool GATE>
+__global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
+  constexpr int STEPS = 4;                          // of 32 of K, on their way at once
+  constexpr int OUTS = GATE ? 8 : 16;               // of an A
+  __shared__ float4 sums[2][WARPS][NT][32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  if (GATE && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
+  const __nv_bfloat16* x[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)                      // a row that is not there: another's sums, never written
+    x[n] = static_cast<const __nv_bfloat16*>(a.in) + min(8 * n + g, a.rows - 1) * a.ld_in + 8 * t;
+  const int units = (a.outs + OUTS - 1) / OUTS;
+  int turn = 0;
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+    const int o = unit * OUTS;
+    const long long lo = min(o + g, a.outs - 1), hi = GATE ? lo + a.outs : min(o + 8 + g, a.outs - 1);
+    const __nv_bfloat16* w0 = static_cast<const __nv_bfloat16*>(a.w) + lo * a.ld_w + 8 * t;
+    const __nv_bfloat16* w1 = static_cast<const __nv_bfloat16*>(a.w) + hi * a.ld_w + 8 * t;
+    float c[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[n][i] = 0.f;
+    for (int d0 = warp * 32 * STEPS; d0 < a.cols; d0 += WARPS * 32 * STEPS) {
+      Rows16 q0[STEPS], q1[STEPS];
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        q0[i].clear(), q1[i].clear();
+        if (d0 + 32 * i + 8 * t < a.cols) q0[i].stream(w0 + d0 + 32 * i), q1[i].stream(w1 + d0 + 32 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint4 b = make_uint4(0, 0, 0, 0);
+          if (d0 + 32 * i + 8 * t < a.cols) b = *reinterpret_cast<const uint4*>(x[n] + d0 + 32 * i);
+          mma16(c[n], q0[i].v.x, q1[i].v.x, q0[i].v.y, q1[i].v.y, b.x, b.y);
+          mma16(c[n], q0[i].v.z, q1[i].v.z, q0[i].v.w, q1[i].v.w, b.z, b.w);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sums[turn][warp][n][lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+    __syncthreads();  // the next unit's sums go beside these; what they overwrite was read before it
+    if (warp < NT) {
+      float v[4] = {};
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float4 f = sums[turn][w][warp][lane];
+        v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+      }
+      // v[0], v[1]: output g of rows 2 t and 2 t + 1; v[2], v[3]: their factors, or output g + 8
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 8 * warp + 2 * t + i;
+        if (row >= a.rows) continue;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + row * a.ld_out;
+        if constexpr (GATE) {
+          if (o + g < a.outs) {
+            if (a.pre) {
+              float* p = a.pre + row * a.ld_pre + o + g;
+              p[0] = v[i];
+              p[a.outs] = v[2 + i];
+            }
+            float y[1] = {v[i]};
+            const float u[1] = {v[2 + i]};
+            activate<true>(a.act, y, u);
+            out[o + g] = __float2bfloat16_rn(y[0]);
+          }
+        } else {
+          if (o + g < a.outs) out[o + g] = __float2bfloat16_rn(v[i]);
+          if (o + 8 + g < a.outs) out[o + 8 + g] = __float2bfloat16_rn(v[2 + i]);
+        }
+      }
+    }
+  }
+}
+
+template <int NT, bool GATE>
+cudaError_t rows_of(const Few& a, cudaStream_t s) {
+  const int units = (a.outs + (GATE ? 8 : 16) - 1) / (GATE ? 8 : 16), sms = device_sms();
+  // sixteen warps where there is no second block for a multiprocessor
+  if (units <= sms)
+    ffn_rows_kernel<16, NT, GATE><<<units, 512, 0, s>>>(a);
+  else
+    ffn_rows_kernel<8, NT, GATE><<<std::min(units, 4 * sms), 256, 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 // ---- float32: the gradients of gates and factors ----------------------------------
@@ -301,7 +431,10 @@ cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
+namespace {
+
+// Both products' arguments.
+Few few_in(const FfnArgs& f) {
   Few a{};
   a.in = f.x;
   a.ld_in = f.ld_x;
@@ -317,19 +450,39 @@ cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
   a.pre = f.pre;
   a.ld_pre = f.ld_pre;
   a.status = static_cast<unsigned*>(f.workspace);
-  cudaError_t e = f.dtype == kF32 ? few_type<float, true>(a, s) : few_type<__nv_bfloat16, true>(a, s);
-  if (e != cudaSuccess) return e;
+  return a;
+}
+
+Few few_out(const FfnArgs& f) {
+  Few a{};
   a.in = f.hidden;
   a.ld_in = f.ld_hidden;
   a.w = f.w_out;
   a.ld_w = f.ld_out;
+  a.rows = int(f.rows);
   a.cols = int(f.width);
   a.outs = int(f.outs);
   a.pitch = int(ffn_pitch(f.width));
   a.out = f.y;
   a.ld_out = f.ld_y;
-  a.pre = nullptr;
-  return f.dtype == kF32 ? few_type<float, false>(a, s) : few_type<__nv_bfloat16, false>(a, s);
+  return a;
+}
+
+}  // namespace
+
+cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
+  const Few in = few_in(f), out = few_out(f);
+  const bool f32 = f.dtype == kF32;
+  const cudaError_t e = f32 ? few_type<float, true>(in, s) : few_type<__nv_bfloat16, true>(in, s);
+  if (e != cudaSuccess) return e;
+  return f32 ? few_type<float, false>(out, s) : few_type<__nv_bfloat16, false>(out, s);
+}
+
+cudaError_t launch_ffn_rows(const FfnArgs& f, cudaStream_t s) {
+  const Few in = few_in(f), out = few_out(f);
+  const cudaError_t e = f.rows <= 8 ? rows_of<1, true>(in, s) : rows_of<2, true>(in, s);
+  if (e != cudaSuccess) return e;
+  return f.rows <= 8 ? rows_of<1, false>(out, s) : rows_of<2, false>(out, s);
 }
 
 }  // namespace mb

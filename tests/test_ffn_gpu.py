@@ -172,6 +172,30 @@ def test_ffn(gpu, torch, shape, dtype):
         assert torch.equal(b.results()[name], first[name]), name
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("sizes", [(8, 8, 1), (136, 1184, 17), (1000, 24, 2400), (520, 4800, 40), (24, 9608, 2369)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_warp_products(gpu, torch, sizes, rows):
+    """A few rows of bfloat16 on 16 bytes; K below, at and beyond a step of all warps, outputs that
+    end inside a block's, and more of them than blocks."""
+    for pad in (0, 8):
+        b = Block(gpu, torch, rows, *sizes, "bfloat16", ACTS[rows % 3], pad=pad, seed=rows)
+        b.forward()
+        b.check()
+        b.compare(("hidden", "pre", "y"))
+        b.intact()
+        y = b.results()["y"].clone()
+        b.forward(keep=False)
+        assert torch.equal(b.results()["y"], y)
+        if rows > 1:
+            b.x[rows // 2, 3] = float("nan")
+            b.w_in[0, 0] = float("inf")  # of a gate that every row's y takes part of
+            b.forward()
+            keep = b.results()["pre"][[i for i in range(rows) if i != rows // 2]]
+            assert torch.isfinite(keep[:, 1:]).all() and not torch.isfinite(keep[:, 0]).any()
+            assert torch.isnan(b.results()["y"][rows // 2]).all()
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 def test_activations(gpu, torch, act, dtype):
