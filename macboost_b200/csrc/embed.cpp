@@ -83,13 +83,22 @@ EmbedPlan embed_plan(int64_t entries, int64_t cols, int64_t rows, int64_t k) {
   p.n = rows * k;
   int bits = 1;
   while ((int64_t(1) << bits) <= entries) ++bits;  // keys 0 ... entries
-  const bool one = p.n <= kEmbedOne;
-  const int most = one ? kEmbedOneBits : 10;
+  // one block's sort takes as long as seven launches from some 5,000 entries on (8,192 of 32,000
+  // x 512: 53 against 43 us; 4,096: 27 against 41), but a large table is cleared meanwhile (16,384 of
+  // 131,072 x 1,024: 88 against 100)
+  p.one = p.n <= kEmbedOne / 4 || (p.n <= kEmbedOne && entries * cols >= int64_t(1) << 26);
+  const int most = p.one ? kEmbedOneBits : 10;
   p.digits = (bits + most - 1) / most;
   p.bits = (bits + p.digits - 1) / p.digits;
   p.tiles = int((p.n + kEmbedTile - 1) / kEmbedTile);
-  // short chunks where long ones are too few to fill the GPU (in units of four values)
-  p.chunk = p.n / 64 * cols / 4 < 300000 ? 16 : 64;
+  // The shorter the chunks the more groups of lanes, and the more borders.  Units are of four
+  // values.  Gradients on one B200, with chunks of 16, 64 and 128: 16,384 entries of 131,072 x
+  // 512 (32,768 units at 64) 71, 79 us; 40,000 of 1,000 x 256 (40,000; long stretches) 63, 54; 65,536 x 4 of
+  // 40,000 x 64 (65,536) 84, 78; 32,768 of 32,000 x 2,048 (262,144) 152, 115, 124; 131,072 of 32,000 x
+  // 1,024 (524,288) 207, 190, 161; 65,537 x 100 of 12,700 x 64 (1.6M) 441 at 64, 428 at 128, 438 at 256.
+  p.stretches = p.n / entries >= 16;
+  const int64_t units = p.n / 64 * cols / 4;
+  p.chunk = units < (p.stretches ? 40000 : 60000) ? 16 : units < 400000 ? 64 : 128;
   p.chunks = (p.n + p.chunk - 1) / p.chunk;
   p.by_row = entries < p.chunks;
   int64_t at = 0;
@@ -98,12 +107,12 @@ EmbedPlan embed_plan(int64_t entries, int64_t cols, int64_t rows, int64_t k) {
     at += (bytes + 255) / 256 * 256;
     return o;
   };
-  for (int i = 0; i < (one ? 1 : 2); ++i) {
+  for (int i = 0; i < (p.one ? 1 : 2); ++i) {
     p.keys[i] = take(p.n * 4);
     p.order[i] = take(p.n * 4);
   }
-  p.counts = take(one ? 0 : (int64_t(p.tiles) << p.bits) * 4);
-  p.totals = take(one ? 0 : (int64_t(1) << p.bits) * 4);
+  p.counts = take(p.one ? 0 : (int64_t(p.tiles) << p.bits) * 4);
+  p.totals = take(p.one ? 0 : (int64_t(1) << p.bits) * 4);
   p.heads = take(p.chunks * cols * 4);
   p.tails = take(p.chunks * cols * 4);
   p.begins = take(p.by_row ? entries * 4 : 0);

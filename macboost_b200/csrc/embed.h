@@ -46,6 +46,8 @@ constexpr int kEmbedLevels = 2;           // sums of 64 and of 64 x 64 chunks
 struct EmbedPlan {
   long long n;                            // entries of the sort, rows * k
   int digits, bits, tiles;
+  bool one;                               // that is one block's, in one launch
+  bool stretches;                         // of 16 entries and more, on average
   int chunk;                              // sorted entries that a group of lanes adds up
   long long chunks;
   bool by_row;                            // the join goes by rows of the table, not by chunks

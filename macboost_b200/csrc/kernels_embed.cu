@@ -5,7 +5,7 @@
 //           eight at a time.  Sums in 32 bits, in the order of j, rounded once.
 // gradient  The entries are sorted by row of the table (a stable radix sort: an entry's place
 //           among its equals does not depend on timing), so that a row's dout lie in one
-//           stretch of the sorted list.  Groups of lanes walk chunks of 16 or 64 sorted
+//           stretch of the sorted list.  Groups of lanes walk chunks of 16 to 128 sorted
 //           entries: a stretch inside a chunk is done, the sums of one that crosses a border
 //           are joined by a second launch, 64 chunks (and 64 x 64) at a time where it is
 //           long.  Every sum is in 32 bits and in one order, all groups have the same work,
@@ -538,19 +538,20 @@ struct Sums {
   float* sums[kEmbedLevels]; // sums[l][g]: of the heads g 64^(l+1) ..., all of one stretch
 };
 
-// A chunk's entries in order, Q units a lane.  LONG: stretches are long, so a chunk has few of
-// them: one after the other, with nothing to look at but the rows.  Else eight entries at a
-// time, whatever rows of the table they are of.
-template <class T, int BYTES, int Q, bool LONG>
+// A chunk's entries in order, a unit a lane.  LONG: stretches are long, so a chunk has few of
+// them: one after the other, with nothing to look at but the rows.  Else several entries at a
+// time, whatever rows of the table they are of.  From an average of 16 entries a row on: 8,192 x 100
+// of 12,700 x 64 (65 a row) 105 against 130 us; 32,768 of 32,000 x 2,048 (one a row) 177 against 154.
+template <class T, int BYTES, bool LONG>
 __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, const Shape h) {
   using V = Values<T, BYTES>;
   using U = typename V::U;
-  constexpr int N = V::N, STEP = Q > 1 || (!LONG && N > 4) ? 4 : 8;
+  constexpr int N = V::N, STEP = !LONG && N > 4 ? 4 : 8;
   const int lane = threadIdx.x % h.lanes;
   const long long g = (long long)blockIdx.x * (kThreads / h.lanes) + threadIdx.x / h.lanes;
   const long long c = g / h.slabs;
-  if (c >= a.chunks) return;
-  const int u = int(g - c * h.slabs) * (Q * h.lanes) + lane, entries = int(a.entries);
+  const int u = int(g - c * h.slabs) * h.lanes + lane, entries = int(a.entries);
+  if (c >= a.chunks || u >= h.units) return;
   const long long lo = c * a.chunk;
   const int n = int(min((long long)a.chunk, a.n - lo));
   const int *keys = a.keys + lo, *order = a.order + lo;
@@ -558,25 +559,18 @@ __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, c
   const unsigned ld = unsigned(a.ld_out / N);
   int now = keys[0];
   bool begun = lo == 0 || keys[-1] != now;  // in this chunk
-  float acc[Q][N];
+  float acc[N];
   auto clear = [&] {
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
-#pragma unroll
-      for (int x = 0; x < N; ++x) acc[q][x] = 0.f;
+    for (int x = 0; x < N; ++x) acc[x] = 0.f;
   };
   // the stretch `now` ends here (in this chunk), or goes on behind it
   auto flush = [&](bool ends) {
     if (now >= entries) return;
     if (begun && ends) {
-      U* to = static_cast<U*>(a.dtable) + now * (a.ld / N) + u;
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (u + q * h.lanes < h.units) {
-          V v;
-          v.set(acc[q], a.scale);
-          to[q * h.lanes] = v.u;
-        }
+      V v;
+      v.set(acc, a.scale);
+      static_cast<U*>(a.dtable)[now * (a.ld / N) + u] = v.u;
     } else {
       if (u == 0) {
         if (!begun && ends) a.ends[now] = int(c);
@@ -584,10 +578,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, c
       }
       float* to = (begun ? a.tails : a.heads) + c * a.cols + u * N;
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (u + q * h.lanes < h.units)
-#pragma unroll
-          for (int x = 0; x < N; ++x) to[q * h.lanes * N + x] = acc[q][x];
+      for (int x = 0; x < N; ++x) to[x] = acc[x];
     }
   };
   clear();
@@ -609,21 +600,14 @@ __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, c
 #pragma unroll 1
       for (; p < end; p += STEP) {
         int row[STEP];
-        V v[STEP][Q];
+        V v[STEP];
 #pragma unroll
         for (int i = 0; i < STEP; ++i) row[i] = __ldg(order + min(p + i, end - 1));
 #pragma unroll
-        for (int i = 0; i < STEP; ++i)
-#pragma unroll
-          for (int q = 0; q < Q; ++q)
-            if (u + q * h.lanes < h.units)
-              v[i][q].u = __ldg(d + (unsigned long long)unsigned(row[i]) * ld + q * h.lanes);
+        for (int i = 0; i < STEP; ++i) v[i].u = __ldg(d + (unsigned long long)unsigned(row[i]) * ld);
 #pragma unroll
         for (int i = 0; i < STEP; ++i)
-          if (p + i < end)
-#pragma unroll
-            for (int q = 0; q < Q; ++q)
-              if (u + q * h.lanes < h.units) v[i][q].add_to(acc[q]);
+          if (p + i < end) v[i].add_to(acc);
       }
       p = end;
       if (p < n) {
@@ -644,13 +628,10 @@ __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, c
     };
     look(0);
     for (int p = 0; p < n; p += STEP) {
-      V v[STEP][Q];
+      V v[STEP];
 #pragma unroll
       for (int i = 0; i < STEP; ++i)
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-          if (key[i] < entries && u + q * h.lanes < h.units)
-            v[i][q].u = __ldg(d + (unsigned long long)unsigned(row[i]) * ld + q * h.lanes);
+        if (key[i] < entries) v[i].u = __ldg(d + (unsigned long long)unsigned(row[i]) * ld);
       int k[STEP];
 #pragma unroll
       for (int i = 0; i < STEP; ++i) k[i] = key[i];
@@ -664,10 +645,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_walk_kernel(const Sums a, c
           now = k[i];
           begun = true;
         }
-        if (now < entries)
-#pragma unroll
-          for (int q = 0; q < Q; ++q)
-            if (u + q * h.lanes < h.units) v[i][q].add_to(acc[q]);
+        if (now < entries) v[i].add_to(acc);
       }
     }
   }
@@ -819,15 +797,15 @@ cudaError_t forward(const EmbedArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <class T, int BYTES, int Q>
-cudaError_t walk(const Sums& a, cudaStream_t s) {
-  const Shape h = shape(a.cols, BYTES / int(sizeof(T)), Q);
+template <class T, int BYTES>
+cudaError_t walk(const Sums& a, bool stretches, cudaStream_t s) {
+  const Shape h = shape(a.cols, BYTES / int(sizeof(T)), 1);
   const unsigned blocks = h.blocks(a.chunks);
   if (!blocks) return cudaErrorInvalidValue;
-  if (a.n / a.entries >= 16)
-    embed_walk_kernel<T, BYTES, Q, true><<<blocks, kThreads, 0, s>>>(a, h);
+  if (stretches)
+    embed_walk_kernel<T, BYTES, true><<<blocks, kThreads, 0, s>>>(a, h);
   else
-    embed_walk_kernel<T, BYTES, Q, false><<<blocks, kThreads, 0, s>>>(a, h);
+    embed_walk_kernel<T, BYTES, false><<<blocks, kThreads, 0, s>>>(a, h);
   return cudaGetLastError();
 }
 
@@ -876,14 +854,13 @@ cudaError_t gradient(const EmbedArgs& a, const EmbedPlan& p, int* launches, cuda
   t.tiles = p.tiles;
   t.counts = ints(p.counts);
   t.totals = ints(p.totals);
-  const bool one = p.n <= kEmbedOne;
   cudaError_t e = cudaSuccess;
   // rows that no id leads to; the one-launch sort clears them itself
-  if (!one)
+  if (!p.one)
     e = cudaMemset2DAsync(a.dtable, size_t(a.ld) * sizeof(T), 0, size_t(a.cols) * sizeof(T), size_t(a.entries), s);
   if (e != cudaSuccess) return e;
   int now = 0;
-  if (one) {
+  if (p.one) {
     t.keys = ints(p.keys[0]);
     t.order = ints(p.order[0]);
     e = p.n <= kEmbedOne / 4 ? sort_one<kEmbedOne / 4 / kOneThreads, U>(t, p, a, N, s)
@@ -891,7 +868,7 @@ cudaError_t gradient(const EmbedArgs& a, const EmbedPlan& p, int* launches, cuda
     if (e != cudaSuccess) return e;
     ++*launches;
   }
-  for (int d = 0; d < p.digits && !one; ++d) {
+  for (int d = 0; d < p.digits && !p.one; ++d) {
     now = d % 2;
     t.keys_in = d ? ints(p.keys[now ^ 1]) : nullptr;
     t.order_in = d ? ints(p.order[now ^ 1]) : nullptr;
@@ -924,12 +901,7 @@ cudaError_t gradient(const EmbedArgs& a, const EmbedPlan& p, int* launches, cuda
     if (e != cudaSuccess) return e;
   }
   for (int l = 0; l < kEmbedLevels; ++l) q.sums[l] = reinterpret_cast<float*>(base + p.sums[l]);
-  // several units a lane where rows are wide and chunks many
-  bool wide = false;
-  if constexpr (BYTES == 16) wide = a.cols / N >= 128 && p.chunk == 64;
-  if constexpr (BYTES == 16)
-    if (wide) e = walk<T, BYTES, 2>(q, s);
-  if (!wide) e = walk<T, BYTES, 1>(q, s);
+  e = walk<T, BYTES>(q, p.stretches, s);
   if (e != cudaSuccess) return e;
   ++*launches;
   if (p.chunks < 2) return cudaSuccess;
