@@ -58,7 +58,9 @@ bool is_few(int dtype, int64_t rows, int64_t cols, int64_t width) {
 // The products of warps: all rows in place, 16 bytes at a time.
 bool is_warps(const FfnArgs& a) {
   auto whole = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) | uintptr_t(ld) * 2) % 16 == 0; };
-  return a.dtype == kBF16 && a.rows >= 2 && a.rows <= kFfnWarpRows && a.cols % 8 == 0 && a.width % 8 == 0 &&
+  const double products = double(a.rows) * double(a.width) * double(2 * a.cols + a.outs);
+  if (a.rows < 2 || a.rows > kFfnWarpMost || (a.rows > kFfnWarpRows && products > kFfnWarpProducts)) return false;
+  return a.dtype == kBF16 && a.cols % 8 == 0 && a.width % 8 == 0 &&
          whole(a.x, a.ld_x) && whole(a.w_in, a.ld_in) && whole(a.w_out, a.ld_out) && whole(a.hidden, a.ld_hidden);
 }
 

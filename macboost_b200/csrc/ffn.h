@@ -51,13 +51,20 @@ int ffn_check_device(int device, const void* workspace, std::string& err);
 // ---- between ffn.cpp and kernels_ffn.cu -------------------------------------------
 
 // Up to four rows (float32: 16) whose x and h fit in shared memory go to the CUDA cores:
-// reading the weights bounds them.
+// reading the weights bounds them.  In us, against tiles of the tensor cores: float32 1, 4 rows of
+// 2,048 x 8,192 41, 55 against 249; 8 of 1,024 x 4,096 33 against 94; bfloat16 1, 2, 4 of 2,048 x 8,192 25,
+// 33, 43 against 39, of 1,024 x 4,096 10.5, 14.5, 18.6 against 27 (2 and 4 only where the
+// products of warps cannot).
 constexpr int64_t kFfnFewRows = 4, kFfnFewRowsF32 = 16;
 constexpr int64_t kFfnFewSmem = 128 * 1024;
 inline int64_t ffn_pitch(int64_t cols) { return (cols + 63) / 64 * 64; }  // floats between rows there
 cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);
-// Two to 16 rows of bfloat16 whose matrices' rows lie on 16 bytes, and are as long: products of warps.
-constexpr int64_t kFfnWarpRows = 16;
+// Products of warps: two to 16 rows of bfloat16 whose matrices' rows start on 16 bytes and are whole
+// 16 bytes long, and up to 48 where they take no more than this many products.  In us, against tiles:
+// 32 x 2,048 x 8,192 (1.6e9) 41 against 47 and 40 rows (2.0e9) 53 against 47; 32 x 1,024 x 16,384 (1.6e9) 50
+// against 47; 48 x 1,536 x 4,096 (0.9e9) 30 against 37; 24 x 4,096 x 16,384 (4.8e9) 132 against 103.
+constexpr int64_t kFfnWarpRows = 16, kFfnWarpMost = 48;
+constexpr double kFfnWarpProducts = 1.4e9;
 cudaError_t launch_ffn_rows(const FfnArgs& a, cudaStream_t s);
 // float32: from dh (stride ld_dh) and pre to the planes of the gradients of both halves
 // (3 x rows x 2 half, zeros from width to half), and of hidden (3 x rows x ld_h) unless null.

@@ -3,7 +3,10 @@
 //
 // Two launches, h between them.  The rows lie in shared memory in float32; a warp streams
 // two rows of weights (two gates and their two factors) at a time through registers, 16
-// bytes a lane, eight loads on their way, and its sums meet in shuffles.
+// bytes a lane, eight loads on their way, and its sums meet in shuffles.  Reading the weights
+// bounds it: one row of 4,096 x 16,384 x 4,096 bfloat16 (403 MB) 69 us, 5.8 TB/s; of 2,048 x 8,192
+// float32 41 us.  More rows of bfloat16 are products of warps, or where rows do not start on 16
+// bytes up to four of them here.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -226,7 +229,7 @@ cudaError_t few_type(const Few& a, cudaStream_t s) {
   return wide ? few_rows<T, PER, GATE>(a, s) : few_rows<T, 1, GATE>(a, s);
 }
 
-// ---- bfloat16: up to 16 rows by products of warps ---------------------------------------
+// ---- bfloat16: up to 48 rows by products of warps ---------------------------------------
 //
 // What ffn_few_kernel spends on a weight (unpacking, a product a row, rows from shared memory) takes
 // longer than fetching it from two rows on.  Here a warp's mma.m16n8k16 has 16 rows of weights as A
@@ -236,6 +239,12 @@ cudaError_t few_type(const Few& a, cudaStream_t s) {
 // time, and join their sums in shared memory in one order.  x and h are read over and over from the
 // L1 cache, where weights leave no trace.  Gates are an A's first eight rows and their factors its
 // last eight, so a lane's sums are of both.
+//
+// Measured, 2,048 x 8,192 x 2,048 (101 MB of weights): 25 us at 2 to 8 rows (4.1 TB/s, both
+// launches), 27 at 16, 35 at 24, 41 at 32; x and h from the L1 and L2 caches bound it from there
+// on (at 48 rows the first launch reads 187 MB from L2 and takes 40 us; tiles of the tensor
+// cores take 45 to 47 for any of these).  1,024 x 4,096: 10.4, 12.4, 16.5 and 20.6 us at 8, 16, 32 and
+// 48 rows against 27 to 33.  Two A's a warp: the same up to 16 rows, 45 and 64 us at 32 and 48.
 
 struct Rows16 {
   uint4 v;
@@ -261,7 +270,7 @@ template <int WARPS, int NT, bool GATE>
 __global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
   constexpr int STEPS = 4;                          // of 32 of K, on their way at once
   constexpr int OUTS = GATE ? 8 : 16;               // of an A
-  __shared__ float4 sums[2][WARPS][NT][32];
+  __shared__ float4 sums[WARPS][NT][32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   if (GATE && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 0;
   const __nv_bfloat16* x[NT];
@@ -269,8 +278,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
   for (int n = 0; n < NT; ++n)                      // a row that is not there: another's sums, never written
     x[n] = static_cast<const __nv_bfloat16*>(a.in) + min(8 * n + g, a.rows - 1) * a.ld_in + 8 * t;
   const int units = (a.outs + OUTS - 1) / OUTS;
-  int turn = 0;
-  for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+  for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int o = unit * OUTS;
     const long long lo = min(o + g, a.outs - 1), hi = GATE ? lo + a.outs : min(o + 8 + g, a.outs - 1);
     const __nv_bfloat16* w0 = static_cast<const __nv_bfloat16*>(a.w) + lo * a.ld_w + 8 * t;
@@ -288,23 +296,28 @@ __global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
         if (d0 + 32 * i + 8 * t < a.cols) q0[i].stream(w0 + d0 + 32 * i), q1[i].stream(w1 + d0 + 32 * i);
       }
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i)
+      for (int i = 0; i < STEPS; ++i) {
+        uint4 b[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if (d0 + 32 * i + 8 * t < a.cols) b = *reinterpret_cast<const uint4*>(x[n] + d0 + 32 * i);
-          mma16(c[n], q0[i].v.x, q1[i].v.x, q0[i].v.y, q1[i].v.y, b.x, b.y);
-          mma16(c[n], q0[i].v.z, q1[i].v.z, q0[i].v.w, q1[i].v.w, b.z, b.w);
+          b[n] = make_uint4(0, 0, 0, 0);
+          if (d0 + 32 * i + 8 * t < a.cols) b[n] = *reinterpret_cast<const uint4*>(x[n] + d0 + 32 * i);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16(c[n], q0[i].v.x, q1[i].v.x, q0[i].v.y, q1[i].v.y, b[n].x, b[n].y);
+          mma16(c[n], q0[i].v.z, q1[i].v.z, q0[i].v.w, q1[i].v.w, b[n].z, b[n].w);
+        }
+      }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sums[turn][warp][n][lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
-    __syncthreads();  // the next unit's sums go beside these; what they overwrite was read before it
+    for (int n = 0; n < NT; ++n) sums[warp][n][lane] = make_float4(c[n][0], c[n][1], c[n][2], c[n][3]);
+    __syncthreads();
     if (warp < NT) {
       float v[4] = {};
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float4 f = sums[turn][w][warp][lane];
+        const float4 f = sums[w][warp][lane];
         v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
       }
       // v[0], v[1]: output g of rows 2 t and 2 t + 1; v[2], v[3]: their factors, or output g + 8
@@ -331,6 +344,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
         }
       }
     }
+    if (unit + int(gridDim.x) < units) __syncthreads();  // before the next unit's sums
   }
 }
 
@@ -348,8 +362,8 @@ cudaError_t rows_of(const Few& a, cudaStream_t s) {
 // ---- float32: the gradients of gates and factors ----------------------------------
 //
 // The tensor cores' epilogue keeps 128 sums a thread in float32, and fetching pre and three
-// planes a half on top of that stopped it for 85 us a tile of 256 x 256; written out as float32
-// and formed here, 2,048 x 4,096 takes 30 bytes a value.
+// planes a half on top of that stopped it for 85 us a tile of 256 x 256.  Written out as float32
+// and formed here: 30 bytes a value, 2,048 x 4,096 in 42 us (6.0 TB/s).
 
 // Four adjacent values as three planes of bfloat16, `plane` apart.  As the head's planes:
 // finite values that would round to infinity are bfloat16's largest and a rest, and the rest
@@ -478,11 +492,19 @@ cudaError_t launch_ffn_few(const FfnArgs& f, cudaStream_t s) {
   return f32 ? few_type<float, false>(out, s) : few_type<__nv_bfloat16, false>(out, s);
 }
 
+template <bool GATE>
+static cudaError_t rows_type(const Few& a, cudaStream_t s) {
+  if (a.rows <= 8) return rows_of<1, GATE>(a, s);
+  if (a.rows <= 16) return rows_of<2, GATE>(a, s);
+  if (a.rows <= 24) return rows_of<3, GATE>(a, s);
+  if (a.rows <= 32) return rows_of<4, GATE>(a, s);
+  if (a.rows <= 48) return rows_of<6, GATE>(a, s);
+  return cudaErrorInvalidValue;
+}
+
 cudaError_t launch_ffn_rows(const FfnArgs& f, cudaStream_t s) {
-  const Few in = few_in(f), out = few_out(f);
-  const cudaError_t e = f.rows <= 8 ? rows_of<1, true>(in, s) : rows_of<2, true>(in, s);
-  if (e != cudaSuccess) return e;
-  return f.rows <= 8 ? rows_of<1, false>(out, s) : rows_of<2, false>(out, s);
+  const cudaError_t e = rows_type<true>(few_in(f), s);
+  return e != cudaSuccess ? e : rows_type<false>(few_out(f), s);
 }
 
 }  // namespace mb

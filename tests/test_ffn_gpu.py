@@ -172,7 +172,7 @@ def test_ffn(gpu, torch, shape, dtype):
         assert torch.equal(b.results()[name], first[name]), name
 
 
-@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 15, 16, 17, 24, 25, 32, 33, 47, 48, 49])
 @pytest.mark.parametrize("sizes", [(8, 8, 1), (136, 1184, 17), (1000, 24, 2400), (520, 4800, 40), (24, 9608, 2369)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_warp_products(gpu, torch, sizes, rows):
