@@ -94,51 +94,40 @@ __device__ __forceinline__ int looked_up(int id, int start, int entries) {
 
 // ---- forward --------------------------------------------------------------------
 
-// Q units a lane, `lanes` apart; slabs of Q * lanes units.
-template <class T, int BYTES, int Q>
+// A unit a lane.
+template <class T, int BYTES>
 __global__ void __launch_bounds__(kThreads)
     embed_kernel(const EmbedArgs a, int lanes, int units, int slabs) {
   using V = Values<T, BYTES>;
   using U = typename V::U;
-  constexpr int STEP = Q > 1 ? 2 : 8;
+  constexpr int STEP = 8;
   const int lane = threadIdx.x % lanes, entries = int(a.entries);
   const long long g = (long long)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
   const long long n = g / slabs;
-  if (n >= a.rows) return;
-  const int u0 = int(g - n * slabs) * (Q * lanes) + lane;
-  const U* table = static_cast<const U*>(a.table);
+  const int u = int(g - n * slabs) * lanes + lane;
+  if (n >= a.rows || u >= units) return;
+  const U* table = static_cast<const U*>(a.table) + u;
   const long long ld = a.ld / V::N;
   const int* ids = a.ids + n * a.k;
-  float acc[Q][V::N];
+  float acc[V::N];
 #pragma unroll
-  for (int q = 0; q < Q; ++q)
-#pragma unroll
-    for (int i = 0; i < V::N; ++i) acc[q][i] = 0.f;
+  for (int i = 0; i < V::N; ++i) acc[i] = 0.f;
   for (int j0 = 0; j0 < int(a.k); j0 += STEP) {
     int e[STEP];
 #pragma unroll
     for (int j = 0; j < STEP; ++j)
       e[j] = j0 + j < int(a.k) ? looked_up(ids[j0 + j], a.starts ? a.starts[j0 + j] : 0, entries) : -1;
-    V v[STEP][Q];
+    V v[STEP];
 #pragma unroll
     for (int j = 0; j < STEP; ++j)
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (e[j] >= 0 && u0 + q * lanes < units) v[j][q].u = __ldg(table + e[j] * ld + u0 + q * lanes);
+      if (e[j] >= 0) v[j].u = __ldg(table + e[j] * ld);
 #pragma unroll
     for (int j = 0; j < STEP; ++j)
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-        if (e[j] >= 0 && u0 + q * lanes < units) v[j][q].add_to(acc[q]);
+      if (e[j] >= 0) v[j].add_to(acc);
   }
-  U* out = static_cast<U*>(a.out) + n * (a.ld_out / V::N);
-#pragma unroll
-  for (int q = 0; q < Q; ++q)
-    if (u0 + q * lanes < units) {
-      V v;
-      v.set(acc[q], a.scale);
-      out[u0 + q * lanes] = v.u;
-    }
+  V v;
+  v.set(acc, a.scale);
+  static_cast<U*>(a.out)[n * (a.ld_out / V::N) + u] = v.u;
 }
 
 // One id a row, Q units a lane: little but the loads and stores, so that eight blocks fit a
@@ -765,20 +754,26 @@ int unit_bytes(uintptr_t all) { return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : a
 template <class T, int BYTES>
 cudaError_t forward(const EmbedArgs& a, cudaStream_t s) {
   constexpr int N = BYTES / int(sizeof(T));
-  // four units a lane where a row has that many for every lane and few rows are added up
-  const bool wide = a.k < 4 && a.cols / N >= 128 && a.rows * (a.cols / N) >= 4ll * kThreads * device_sms();
-  const Shape h = shape(a.cols, N, wide ? 4 : 1);
-  const unsigned blocks1 = h.blocks(a.rows);
-  if (a.k == 1 && blocks1) {
+  if (a.k == 1) {
+    // Four units a lane where the GPU stays full: in us, against one, 65,536 rows of 512 bfloat16 16.3 and
+    // 28.8, 262,144 of 64 float32 14.5 and 26.7, 16,384 of 2,048 bfloat16 16.5 and 28.9 (4.1 TB/s
+    // stored); 4,096 of 256 float32 4.2 and 4.2.
+    const bool wide = a.cols / N >= 8 && a.rows * (a.cols / N) >= 2ll * kThreads * device_sms();
+    const Shape h = shape(a.cols, N, wide ? 4 : 1);
+    const unsigned blocks = h.blocks(a.rows);
+    if (!blocks) return cudaErrorInvalidValue;
     if (wide)
-      embed_lookup_kernel<T, BYTES, 4><<<blocks1, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
+      embed_lookup_kernel<T, BYTES, 4><<<blocks, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
     else
-      embed_lookup_kernel<T, BYTES, 1><<<blocks1, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
+      embed_lookup_kernel<T, BYTES, 1><<<blocks, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
     return cudaGetLastError();
   }
-  // several rows a group where that leaves enough of them for the GPU
+  const Shape h = shape(a.cols, N, 1);
+  // Several rows a group where that leaves enough of them for the GPU: in us, against one, 65,536 x 4 of
+  // 40,000 x 64 float32 12.5 and 22.7, 8,192 x 32 of 12,700 x 512 bfloat16 24.7 and 40.2, 65,537 x 100 of
+  // 12,700 x 64 float32 134 and 170; 8,192 x 100 of these (128 blocks) 41 and 33.
   const long long tile = Values<T, BYTES>::ROWS * (kThreads / h.lanes), many = (a.rows + tile - 1) / tile * h.slabs;
-  if (a.k >= 8 && h.lanes >= 8 && many >= 4 * device_sms() && many <= INT_MAX) {
+  if (h.lanes >= 8 && many >= 4 * device_sms() && many <= INT_MAX) {
     const unsigned blocks = unsigned(many);
     if (h.lanes == 8)
       embed_many_kernel<T, BYTES, 8><<<blocks, kThreads, 0, s>>>(a, h.units, h.slabs);
@@ -790,10 +785,7 @@ cudaError_t forward(const EmbedArgs& a, cudaStream_t s) {
   }
   const unsigned blocks = h.blocks(a.rows);
   if (!blocks) return cudaErrorInvalidValue;
-  if (wide)
-    embed_kernel<T, BYTES, 4><<<blocks, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
-  else
-    embed_kernel<T, BYTES, 1><<<blocks, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
+  embed_kernel<T, BYTES><<<blocks, kThreads, 0, s>>>(a, h.lanes, h.units, h.slabs);
   return cudaGetLastError();
 }
 

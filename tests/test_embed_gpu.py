@@ -111,7 +111,8 @@ def test_embed(gpu, torch, rows, k, entries, cols, dtype):
 @pytest.mark.parametrize("rows,k,entries,cols", [
     (65_003, 1, 900, 256), (64_900, 1, 30_011, 260),      # chunks of 64 entries, long stretches and short ones
     (60_001, 1, 500, 2048), (26_001, 5, 20_011, 1000),    # of 128
-    (5_000, 1, 1 << 20, 64), (16_384, 1, 1 << 19, 129)])  # one block's sort while a large table is cleared
+    (5_000, 1, 1 << 20, 64), (16_384, 1, 1 << 19, 129),   # one block's sort while a large table is cleared
+    (50_001, 1, 300, 100), (9_999, 1, 777, 520), (12_345, 2, 999, 520), (20_003, 3, 500, 96)])  # several units, rows
 def test_plans(gpu, torch, rows, k, entries, cols, dtype):
     _check(gpu, torch, _ids(torch, rows, k, entries, rows), None, entries, cols, dtype, 1.0, 0, rows)
 
