@@ -10,7 +10,9 @@
 // one     Both at once for little: a cluster of eight blocks, whose sums meet in its shared
 //         memory.
 //
-// Both read or write what they have to once; bytes bound them.
+// Both read or write what they have to once; bytes bound them.  170M values of bfloat16 in 300
+// tensors (340 MB): the norm 58 us (5.9 TB/s), the scaling 112 (6.1 TB/s with a cold cache), 166
+// together; 9.5M values in 1,500 tensors 23 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

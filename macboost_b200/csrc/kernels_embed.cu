@@ -10,6 +10,10 @@
 //           are joined by a second launch, 64 chunks (and 64 x 64) at a time where it is
 //           long.  Every sum is in 32 bits and in one order, all groups have the same work,
 //           and a stretch of millions takes no longer than one of hundreds.
+//
+// Measured: 65,537 x 100 ids of 12,700 x 64 float32, forward 134 us (1.7 GB of gathers from the L2
+// cache, 12.5 TB/s), gradient 295 (sort 172, its walk another 1.7 GB in 130 or less, joins 30); lookup
+// of 16,384 x 2,048 bfloat16 16.5 us, its gradient 125, 87 of them for clearing 537 MB (6.2 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -26,6 +26,13 @@
 // x 1,024 x 32,768: loss 595 us (0.50 ms of bfloat16 products at the measured peak), with
 // gradient 2.65 ms.
 //
+// The gated block's products are tiles of the same kernel: kHeadGate's second CTA holds rows of the
+// factors in place of B's second half, so that an epilogue has gates and factors of the same
+// columns, kHeadGateGrad forms both gradients of a tile of dh.  Bound by the copies into shared
+// memory and by the epilogues' traffic: 8,192 x 1,024 x 4,096 bfloat16 gates 130 us (268 MB of pre and 67
+// of h written; tensor pipe 55%), y 69, dh and dw_out 207 (268 MB of pre read; 31%), dx and dw_in 297;
+// 2,048 x 1,024 x 4,096 float32 164, 88, 94 and 88, 329 (54 to 66%).
+//
 // Every wait ends after wait_ns: the CTA then marks itself dead, sets the status word,
 // waits (as long again at most) for its copies and products in flight and returns (its
 // results are void).
