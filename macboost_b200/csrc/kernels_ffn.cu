@@ -370,7 +370,22 @@ cudaError_t rows_of(const Few& a, cudaStream_t s) {
 // of what is not finite is zero.
 __device__ __forceinline__ void put_planes(__nv_bfloat16* to, long long plane, const float (&x)[4]) {
   constexpr float kLargest = 3.3895313892515355e38f;
-  float v[4];
+  float v[4] = {x[0], x[1], x[2], x[3]};
+  // (a NaN is not below anything)
+  const bool plain = fabsf(x[0]) < kLargest && fabsf(x[1]) < kLargest && fabsf(x[2]) < kLargest && fabsf(x[3]) < kLargest;
+  if (plain) {
+#pragma unroll
+    for (int z = 0; z < 3; ++z) {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+      uint2 w;
+      memcpy(&w.x, &lo, 4);
+      memcpy(&w.y, &hi, 4);
+      *reinterpret_cast<uint2*>(to + z * plane) = w;
+      v[0] -= __uint_as_float(w.x << 16), v[1] -= __uint_as_float(w.x & 0xFFFF0000u);
+      v[2] -= __uint_as_float(w.y << 16), v[3] -= __uint_as_float(w.y & 0xFFFF0000u);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = fabsf(x[i]) < INFINITY ? fminf(fmaxf(x[i], -kLargest), kLargest) : x[i];
 #pragma unroll
