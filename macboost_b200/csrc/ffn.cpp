@@ -64,6 +64,14 @@ bool is_warps(const FfnArgs& a) {
          whole(a.x, a.ld_x) && whole(a.w_in, a.ld_in) && whole(a.w_out, a.ld_out) && whole(a.hidden, a.ld_hidden);
 }
 
+bool is_narrow(int dtype, int64_t width, int64_t outs) {
+  return dtype == kF32 && outs <= kFfnNarrow && outs * width <= kFfnNarrowValues;
+}
+// Rows that a warp of the narrow gradient adds up.
+int64_t narrow_rows(int64_t rows, int64_t half) {
+  return std::max<int64_t>(8, parts(rows, std::max<int64_t>(1, kFfnNarrowWarps / parts(half, 128))));
+}
+
 // A product's tiles.
 struct Shape {
   int64_t m, n, k;
@@ -166,7 +174,8 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
     Shape dh = shape(rows, width, outs);
     choose_splits(dtype, &p.dw_out, dtype == kF32 ? nullptr : &dh, true);
     // dw_out is done before the others begin
-    p.part = take(std::max(sums(p.dw_out), sums(p.dx)));
+    const int64_t chunks = is_narrow(dtype, width, outs) ? parts(rows, narrow_rows(rows, p.half)) : 0;
+    p.part = take(std::max({sums(p.dw_out), sums(p.dx), chunks * outs * width * 4}));
     p.part_in = take(sums(p.dw_in));
   }
   p.bytes = at;
@@ -370,7 +379,9 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   const Operand w_out = c.operand(a.w_out, a.outs, a.width, a.ld_out, p.w_out, &pout);
   const Operand h = c.operand(a.hidden, a.rows, a.width, a.ld_hidden, p.hidden, &ph);
   // w_out beside the others, for the second product
-  if (c.pack({&px, &pin, &pout}, true)) return -1;
+  const HeadPack none;
+  const bool narrow = is_narrow(a.dtype, a.width, a.outs);
+  if (c.pack({&px, &pin, narrow ? &none : &pout}, true)) return -1;
 
   // gates and factors: half of a tile's columns each
   const Shape in = gate_shape(a.dtype, a.rows, a.width, a.cols);
@@ -382,6 +393,11 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   FFN_CUDA(launch_head(kHeadGate, 2 * in.tile_n, l, s), "block launch");
   ++c.launches;
 
+  if (narrow) {
+    FFN_CUDA(launch_ffn_narrow(a, s), "block launch");
+    g_kernel_launches.fetch_add(c.launches + 1, std::memory_order_relaxed);
+    return 0;
+  }
   if (c.pack({&ph}, false)) return -1;
   HeadLaunch q{};
   head_settings(q, a.dtype, a.workspace);
@@ -426,10 +442,37 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
   const bool f32 = a.dtype == kF32, inner = a.dx || a.dw_in;
   // h with the others, unless a launch of its own makes its planes
   const HeadPack none;
-  const bool split = inner && f32;
-  if (c.pack({&pdy, inner ? &pout : &none, a.dw_out && !split ? &ph : &none, inner ? &px : &none,
-              a.dx ? &pin : &none}, false))
+  const bool narrow = is_narrow(a.dtype, a.width, a.outs), split = inner && f32 && !narrow;
+  if (c.pack({narrow ? &none : &pdy, inner && !narrow ? &pout : &none, a.dw_out && !split && !narrow ? &ph : &none,
+              inner ? &px : &none, a.dx ? &pin : &none}, false))
     return -1;
+  if (narrow) {  // dh, dpre and dw_out at once
+    FfnNarrow t{};
+    t.act = a.act;
+    t.outs = int(a.outs);
+    t.rows = a.rows;
+    t.per = narrow_rows(a.rows, p.half);
+    t.width = int(a.width);
+    t.half = int(p.half);
+    t.dy = static_cast<const float*>(a.dy);
+    t.ld_dy = a.ld_dy;
+    t.w = static_cast<const float*>(a.w_out);
+    t.ld_w = a.ld_out;
+    t.pre = a.pre;
+    t.ld_pre = a.ld_pre;
+    t.hidden = static_cast<const float*>(a.hidden);
+    t.ld_hidden = a.ld_hidden;
+    t.dpre = inner ? c.base() + p.dpre : nullptr;
+    t.part = a.dw_out ? reinterpret_cast<float*>(c.base() + p.part) : nullptr;
+    FFN_CUDA(launch_ffn_narrow_grad(t, s), "block gradient launch");
+    ++c.launches;
+    if (a.dw_out) {
+      const int chunks = int(parts(a.rows, t.per));
+      FFN_CUDA(launch_head_reduce(HeadReduce{t.part, chunks, a.outs, a.width, nullptr, 0, 1, a.dw_out, a.ld_dout, 1, 0, 0}, s),
+               "block reduce launch");
+      ++c.launches;
+    }
+  }
   // dh = dy w_out; its epilogue (float32: a launch) makes the gradients of gates and factors of it
   const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
   if (split) {
@@ -456,7 +499,7 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     FFN_CUDA(launch_ffn_split(t, s), "block split launch");
     ++c.launches;
   }
-  if (a.dw_out || (inner && !f32)) {
+  if ((a.dw_out && !narrow) || (inner && !f32)) {
     // dw_out = dy^T h: in bfloat16 in one launch with dh, whose epilogue takes longer than its products
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);

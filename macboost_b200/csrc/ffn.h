@@ -82,4 +82,26 @@ struct FfnSplit {
 };
 cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s);
 
+// float32 with few outputs (a class margin each, say): y, dh and dw_out are too little for tiles that
+// want planes of h first, and go to the CUDA cores.
+constexpr int64_t kFfnNarrow = 16, kFfnNarrowValues = 16384;  // outs; outs * width
+constexpr int64_t kFfnNarrowWarps = 1184;                     // of the gradient, about: eight a multiprocessor
+cudaError_t launch_ffn_narrow(const FfnArgs& a, cudaStream_t s);
+struct FfnNarrow {
+  int act, outs;
+  long long rows, per;       // rows, and those of a warp
+  int width, half;
+  const float* dy;
+  long long ld_dy;
+  const float* w;            // outs x width
+  long long ld_w;
+  const float* pre;
+  long long ld_pre;
+  const float* hidden;
+  long long ld_hidden;
+  void* dpre;                // planes as FfnSplit's, or null
+  float* part;               // dw_out's sums of `per` rows, outs x width each, or null
+};
+cudaError_t launch_ffn_narrow_grad(const FfnNarrow& a, cudaStream_t s);
+
 }  // namespace mb

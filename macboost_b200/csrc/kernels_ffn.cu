@@ -444,7 +444,176 @@ __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, i
   if (a.h && c < a.ld_h) put_planes(static_cast<__nv_bfloat16*>(a.h) + n * a.ld_h + c, a.rows * a.ld_h, h);
 }
 
+// ---- float32, few outputs ------------------------------------------------------------
+//
+// y = h Wo^T: a warp has four rows, a lane every 32nd column of them, and all outputs' sums, which lanes
+// then halve among themselves.  The gradients in one pass over pre, h and dy: a warp has 128
+// columns, four adjacent ones a lane, of `per` rows; its part of Wo and its sums of dw_out stay in
+// registers, dy comes by shuffles.  10,007 x 403 x 10: FORWARD and GRADIENT us in place of
+// 36 (planes of h, tiles) and 117 (planes, dh, the split above, dw_out and its sums).
+
+template <int OUTS>
+__global__ void __launch_bounds__(kThreads)
+    ffn_narrow_kernel(const float* __restrict__ h, long long ld_h, const float* __restrict__ w, long long ld_w,
+                      float* y, long long ld_y, long long rows, int width, int outs) {
+  constexpr int R = 4;
+  const int lane = threadIdx.x % 32;
+  const long long n0 = ((long long)blockIdx.x * kWarps + threadIdx.x / 32) * R;
+  if (n0 >= rows) return;
+  const float* from[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) from[r] = h + min(n0 + r, rows - 1) * ld_h;
+  float v[R * OUTS];
+#pragma unroll
+  for (int i = 0; i < R * OUTS; ++i) v[i] = 0.f;
+#pragma unroll 2
+  for (int c = lane; c < width; c += 32) {
+    float x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = __ldg(from[r] + c);
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      const float f = __ldg(w + min(o, outs - 1) * ld_w + c);
+#pragma unroll
+      for (int r = 0; r < R; ++r) v[r * OUTS + o] = fmaf(x[r], f, v[r * OUTS + o]);
+    }
+  }
+  // at each step a lane keeps one half of its sums and hands the other over
+  int first = 0, n = R * OUTS;
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2) {
+    if (n % 2 == 0) {
+      n /= 2;
+      const bool high = lane & step;
+#pragma unroll
+      for (int i = 0; i < R * OUTS / 2; ++i)
+        if (i < n) v[i] = (high ? v[n + i] : v[i]) + __shfl_xor_sync(~0u, high ? v[i] : v[n + i], step);
+      first += high ? n : 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < R * OUTS; ++i)
+        if (i < n) v[i] += __shfl_xor_sync(~0u, v[i], step);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R * OUTS; ++i)
+    if (i < n) {
+      const int r = (first + i) / OUTS, o = (first + i) % OUTS;
+      if (n0 + r < rows && o < outs) y[(n0 + r) * ld_y + o] = v[i];
+    }
+}
+
+template <int OUTS, bool WIDE>
+__global__ void __launch_bounds__(kThreads) ffn_narrow_grad_kernel(const FfnNarrow a, int groups, long long chunks) {
+  const int lane = threadIdx.x % 32;
+  const long long item = (long long)blockIdx.x * kWarps + threadIdx.x / 32, chunk = item / groups;
+  if (chunk >= chunks) return;
+  const int c = int(item - chunk * groups) * 128 + lane * 4;
+  auto get = [&](const float* p, float (&x)[4]) {
+    if constexpr (WIDE) {
+      const float4 f = c < a.width ? __ldg(reinterpret_cast<const float4*>(p + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = c + k < a.width ? __ldg(p + c + k) : 0.f;
+    }
+  };
+  float w[OUTS][4], sum[OUTS][4];
+#pragma unroll
+  for (int o = 0; o < OUTS; ++o) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[o][k] = o < a.outs && c + k < a.width ? a.w[o * a.ld_w + c + k] : 0.f;
+      sum[o][k] = 0.f;
+    }
+  }
+  const long long lo = chunk * a.per, hi = min(lo + a.per, a.rows);
+  float x[4], y[4], h[4], g;  // of the next row
+  auto fetch = [&](long long n) {
+    g = lane < a.outs ? __ldg(a.dy + n * a.ld_dy + lane) : 0.f;
+    if (a.dpre) {
+      get(a.pre + n * a.ld_pre, x);
+      get(a.pre + n * a.ld_pre + a.width, y);
+    }
+    if (a.part) get(a.hidden + n * a.ld_hidden, h);
+  };
+  fetch(lo);
+#pragma unroll 1
+  for (long long n = lo; n < hi; ++n) {
+    float x0[4], y0[4], h0[4], dh[4] = {};
+    const float g0 = g;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x0[k] = x[k], y0[k] = y[k], h0[k] = h[k];
+    if (n + 1 < hi) fetch(n + 1);
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      const float d = __shfl_sync(~0u, g0, o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        dh[k] = fmaf(d, w[o][k], dh[k]);
+        if (a.part) sum[o][k] = fmaf(d, h0[k], sum[o][k]);
+      }
+    }
+    if (!a.dpre) continue;
+    float dx[4], dz[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      gate_grad<false>(a.act, x0[k], y0[k], dh[k], dx[k], dz[k]);
+      if (c + k >= a.width) dx[k] = dz[k] = 0.f;
+    }
+    if (c < a.half) {
+      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(a.dpre) + n * 2 * a.half + c;
+      put_planes(d, a.rows * 2 * a.half, dx);
+      put_planes(d + a.half, a.rows * 2 * a.half, dz);
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int o = 0; o < OUTS; ++o)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (o < a.outs && c + k < a.width) a.part[(chunk * a.outs + o) * a.width + c + k] = sum[o][k];
+}
+
+template <int OUTS>
+cudaError_t narrow_grad(const FfnNarrow& a, cudaStream_t s) {
+  const int groups = (a.half + 127) / 128;
+  const long long chunks = (a.rows + a.per - 1) / a.per, blocks = (chunks * groups + kWarps - 1) / kWarps;
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const bool wide = (reinterpret_cast<uintptr_t>(a.pre) | reinterpret_cast<uintptr_t>(a.hidden) | uintptr_t(a.ld_pre) * 4 |
+                     uintptr_t(a.ld_hidden) * 4 | uintptr_t(a.width) * 4) % 16 == 0;
+  if (wide)
+    ffn_narrow_grad_kernel<OUTS, true><<<unsigned(blocks), kThreads, 0, s>>>(a, groups, chunks);
+  else
+    ffn_narrow_grad_kernel<OUTS, false><<<unsigned(blocks), kThreads, 0, s>>>(a, groups, chunks);
+  return cudaGetLastError();
+}
+
+template <int OUTS>
+cudaError_t narrow(const FfnArgs& a, cudaStream_t s) {
+  const long long blocks = (a.rows + 4 * kWarps - 1) / (4 * kWarps);
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  ffn_narrow_kernel<OUTS><<<unsigned(blocks), kThreads, 0, s>>>(
+      static_cast<const float*>(a.hidden), a.ld_hidden, static_cast<const float*>(a.w_out), a.ld_out,
+      static_cast<float*>(a.y), a.ld_y, a.rows, int(a.width), int(a.outs));
+  return cudaGetLastError();
+}
+
 }  // namespace
+
+cudaError_t launch_ffn_narrow(const FfnArgs& a, cudaStream_t s) {
+  if (a.outs <= 4) return narrow<4>(a, s);
+  if (a.outs <= 8) return narrow<8>(a, s);
+  if (a.outs <= 12) return narrow<12>(a, s);
+  return a.outs <= kFfnNarrow ? narrow<16>(a, s) : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_ffn_narrow_grad(const FfnNarrow& a, cudaStream_t s) {
+  if (a.outs <= 4) return narrow_grad<4>(a, s);
+  if (a.outs <= 8) return narrow_grad<8>(a, s);
+  if (a.outs <= 12) return narrow_grad<12>(a, s);
+  return a.outs <= kFfnNarrow ? narrow_grad<16>(a, s) : cudaErrorInvalidValue;
+}
 
 cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s) {
   const int per = (a.half + 127) / 128;  // warps a row

@@ -196,6 +196,42 @@ def test_warp_products(gpu, torch, sizes, rows):
             assert torch.isnan(b.results()["y"][rows // 2]).all()
 
 
+@pytest.mark.parametrize("outs", [1, 4, 5, 8, 11, 12, 13, 16, 17])
+@pytest.mark.parametrize("sizes", [(17, 12, 24), (33, 9, 403), (1001, 16, 1000), (20_003, 5, 136)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_few_outputs(gpu, torch, sizes, outs):
+    """float32 with a few outputs, up to one more than the last that has kernels of its own."""
+    for pad in (0, 3, 4):
+        b = Block(gpu, torch, *sizes, outs, "float32", ACTS[outs % 3], pad=pad, seed=outs)
+        b.forward()
+        b.grad()
+        b.check()
+        b.compare()
+        b.intact()
+        first = {k: v.clone() for k, v in b.results().items()}
+        b.forward(keep=False)
+        assert torch.equal(b.results()["y"], first["y"])
+        for name in ("dx", "dw_in", "dw_out"):
+            getattr(b, name).fill_(7.0)
+            b.grad((name,))
+            assert torch.equal(b.results()[name], first[name]), name
+            b.intact()
+
+
+def test_few_outputs_rows_apart(gpu, torch):
+    b = Block(gpu, torch, 100, 24, 200, 7, "float32", "silu", seed=3)
+    b.forward()
+    b.grad(("dx",))
+    y, dx = b.results()["y"].clone(), b.results()["dx"].clone()
+    b.x[10, 3], b.dy[20, 2], b.dy[21, 6] = float("nan"), float("inf"), float("nan")
+    b.forward()
+    b.grad(("dx",))
+    keep = [i for i in range(100) if i not in (10, 20, 21)]
+    assert torch.equal(b.results()["y"][keep], y[keep]) and torch.equal(b.results()["dx"][keep], dx[keep])
+    assert torch.equal(b.results()["y"][20:22], y[20:22]) and torch.isnan(b.results()["y"][10]).all()
+    assert not torch.isfinite(b.results()["dx"][[10, 20, 21]]).any()
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 def test_activations(gpu, torch, act, dtype):
