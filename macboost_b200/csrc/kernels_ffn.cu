@@ -449,8 +449,11 @@ __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, i
 // y = h Wo^T: a warp has four rows, a lane every 32nd column of them, and all outputs' sums, which lanes
 // then halve among themselves.  The gradients in one pass over pre, h and dy: a warp has 128
 // columns, four adjacent ones a lane, of `per` rows; its part of Wo and its sums of dw_out stay in
-// registers, dy comes by shuffles.  10,007 x 403 x 10: FORWARD and GRADIENT us in place of
-// 36 (planes of h, tiles) and 117 (planes, dh, the split above, dw_out and its sums).
+// registers, dy comes by shuffles.  10,007 x 403 x 10, rows of odd length: 20 and 43 us (and 9 for dw_out's
+// sums of rows) in place of 36 (planes of h, tiles) and 94 (dh, the split above, dw_out and its
+// sums); loads and stores of a few bytes a lane bound the second (twice as many warps with Wo in
+// shared memory: 49).  Whole steps in us, against tiles: 10,007 x 100 x 403 x 10 138 and 197, 500 rows 55
+// and 85, 20,000 x 256 x 1,024 x 16 635 and 755, 5,000 x 1,024 x 4,096 x 4 1,533 and 1,674.
 
 template <int OUTS>
 __global__ void __launch_bounds__(kThreads)
