@@ -79,7 +79,7 @@ class LeafNetwork:
 
     def forward_backward(self, ids: torch.Tensor, labels: torch.Tensor, max_norm: float = 1.0) -> None:
         """loss, lse, norm and the clipped gradients (labels int32; one outside the classes leaves
-        its row out)."""
+        its row out).  Raises where a kernel gave up waiting."""
         w, d, rows = self.weights, self.grads, self.rows
         stream = torch.cuda.current_stream().cuda_stream
         space = (self.space.data_ptr(), self.room)
@@ -92,7 +92,7 @@ class LeafNetwork:
         block = (address(self.x), rows, COLS, COLS, address(w["w_in"]), WIDTH, COLS, address(w["w_out"]), COLS,
                  WIDTH, address(self.hidden), WIDTH, address(self.pre), 2 * WIDTH)
         _core.ffn_device(0, _core.F32, _core.ACT_SILU, *block, address(self.y), COLS, *space, stream=stream)
-        _core.ffn_check_device(0, space[0])
+        _core.ffn_check_device(0, space[0])  # the head's loss begins a status of its own
         head = (address(self.y), rows, COLS, COLS, address(w["head"]), CLASSES, COLS, address(labels))
         _core.head_loss_device(0, _core.F32, *head, address(self.loss), address(self.lse), *space, stream=stream)
         _core.head_grad_device(0, _core.F32, *head, address(self.lse), address(self.dloss), address(self.dy), COLS,
@@ -103,6 +103,8 @@ class LeafNetwork:
                                 address(self.starts), 1.0, address(d["table"]), self.entries, COLS, *space,
                                 stream=stream)
         _core.clip_device(0, self.list, max_norm, address(self.norm), *space, stream=stream)
+        # the head's calls and the block's gradient, whose status the calls since left alone
+        _core.ffn_check_device(0, space[0])
 
     def update(self, rate: float) -> None:
         for k, w in self.weights.items():

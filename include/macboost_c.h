@@ -545,7 +545,8 @@ int64_t macboost_embed_workspace(int64_t entries, int64_t cols, int64_t rows, in
 /* Gradient of macboost_embed_device for dout (rows x cols, stride ld_dout): dtable
  * (entries x cols, stride ld) = scale * the sum of dout[n] over the ids that led to
  * each row, zeros in rows that none led to.  The ids are sorted first; `workspace`
- * is device memory, 256-byte aligned, used until the call's work is done. */
+ * is device memory, 256-byte aligned, used until the call's work is done, but for its
+ * first 256 bytes: the head's or the block's status there stays. */
 int32_t macboost_embed_grad_device(int32_t device, int32_t dtype, const void *dout, int64_t rows,
                                    int64_t cols, int64_t ld_dout, const int32_t *ids, int64_t k,
                                    const int32_t *starts, float scale, void *dtable,
@@ -608,7 +609,8 @@ int64_t macboost_clip_workspace(int64_t count, const int32_t *dtypes, const int6
  * arrays, free again when the call returns; grads[i] and outs[i] are device memory,
  * either the same (then a factor of 1 writes nothing) or apart.  Squares are added up
  * so that nothing overflows or vanishes that float32 holds as a norm.  `workspace` is
- * device memory, 8-byte aligned, used until the call's work is done. */
+ * device memory, 8-byte aligned, used until the call's work is done, but for its first
+ * 256 bytes, as in macboost_embed_grad_device. */
 int32_t macboost_clip_device(int32_t device, int64_t count, const int32_t *dtypes,
                              const void *const *grads, const int64_t *sizes, void *const *outs,
                              double max_norm, float *norm, void *workspace,

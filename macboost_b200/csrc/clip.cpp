@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "engine.h"
+#include "head.h"
 #include "mixture.h"
 
 namespace mb {
@@ -54,7 +55,7 @@ int check_list(int64_t count, const int32_t* dtypes, const int64_t* sizes, int64
     if (chunks > (int64_t(1) << 27)) return fail(err, "the gradients hold too many values for one call");
   }
   // a block's sum of every launch: no more than chunks, nor than entries that all lie far apart ask for
-  *room = std::min(chunks, entries * kClipBlocks) * int64_t(sizeof(double));
+  *room = chunks > 0 ? kStatusBytes + std::min(chunks, entries * kClipBlocks) * int64_t(sizeof(double)) : 0;
   return 0;
 }
 
@@ -183,7 +184,7 @@ int clip_device(int device, const ClipArgs& a, cudaStream_t s, std::string& err)
   }
   const std::vector<Group> groups = groups_of(a);
   ClipState c{};
-  c.part = static_cast<double*>(a.workspace);
+  if (a.workspace) c.part = reinterpret_cast<double*>(static_cast<char*>(a.workspace) + kStatusBytes);
   for (const Group& g : groups) c.parts += g.blocks();
   if (!aligned(a.workspace, 8)) return fail(err, "workspace must be 8-byte aligned");
   if (need > 0 && (!a.workspace || a.workspace_bytes < need))

@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "engine.h"
+#include "head.h"
 #include "mixture.h"
 
 namespace mb {
@@ -101,7 +102,7 @@ EmbedPlan embed_plan(int64_t entries, int64_t cols, int64_t rows, int64_t k) {
   p.chunk = units < (p.stretches ? 40000 : 60000) ? 16 : units < 400000 ? 64 : 128;
   p.chunks = (p.n + p.chunk - 1) / p.chunk;
   p.by_row = entries < p.chunks;
-  int64_t at = 0;
+  int64_t at = kStatusBytes;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
     at += (bytes + 255) / 256 * 256;

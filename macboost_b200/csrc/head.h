@@ -206,6 +206,10 @@ struct HeadReduce {
 };
 cudaError_t launch_head_reduce(const HeadReduce& a, cudaStream_t s);
 
+// What a workspace begins with: the status word of the calls whose waits may run out.  Calls whose waits
+// cannot leave it alone too, so that the word outlives those that follow in the same workspace.
+constexpr int64_t kStatusBytes = 256;
+
 // Host side of products as tiles, for the blocks that use them (head.cpp).
 // TMA reads rows in place when they start on 16 bytes.
 bool head_in_place(int dtype, const void* p, int64_t ld);
