@@ -570,9 +570,10 @@ int64_t macboost_ffn_workspace(int32_t dtype, int64_t rows, int64_t cols, int64_
  * MACBOOST_BF16, each with a stride.  pre (rows x 2 width float32: x w_in^T), unless
  * NULL, is kept for the gradient; not rounded, since half of the error of bfloat16
  * gradients would come from that.  Products and sums are float32 (float32 inputs keep 24
- * bits in every product; bfloat16 sums on the tensor cores as in the head); the
- * activation and the factor are formed in float32, and hidden is rounded to `dtype`
- * before the second product.  A row whose x is not finite has values that are not
+ * bits in every product; bfloat16 sums on the tensor cores are truncated every 16
+ * terms, over at most 32,768 terms, and such sums are then added up); the activation and
+ * the factor are formed in float32, and hidden is rounded to `dtype` before the second
+ * product.  A row whose x is not finite has values that are not
  * finite, and NaN where the formula may have an infinity; other rows do not see it.
  * `workspace` as for the head. */
 int32_t macboost_ffn_device(int32_t device, int32_t dtype, int32_t act, const void *x,

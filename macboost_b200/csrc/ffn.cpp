@@ -60,9 +60,14 @@ bool is_warps(const FfnArgs& a) {
   auto whole = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) | uintptr_t(ld) * 2) % 16 == 0; };
   const double products = double(a.rows) * double(a.width) * double(2 * a.cols + a.outs);
   if (a.rows < 2 || a.rows > kFfnWarpMost || (a.rows > kFfnWarpRows && products > kFfnWarpProducts)) return false;
+  if (std::max(a.cols, a.width) > kFfnWarpLong) return false;
   return a.dtype == kBF16 && a.cols % 8 == 0 && a.width % 8 == 0 &&
          whole(a.x, a.ld_x) && whole(a.w_in, a.ld_in) && whole(a.w_out, a.ld_out) && whole(a.hidden, a.ld_hidden);
 }
+
+// bfloat16 sums of more terms than the tensor core may truncate in one place: epilogues that need
+// all of a sum cannot have it, so the product goes to memory, in parts of K, and a launch follows.
+bool is_long(int dtype, int64_t k) { return dtype == kBF16 && k > kFfnLong; }
 
 bool is_narrow(int dtype, int64_t width, int64_t outs) {
   return dtype == kF32 && outs <= kFfnNarrow && outs * width <= kFfnNarrowValues;
@@ -132,10 +137,11 @@ void choose_splits(int dtype, Shape* a, Shape* b, bool whole = false) {
 }
 
 struct Plan {
-  Shape y, dx, dw_in, dw_out;
+  Shape y{}, gates{}, dx{}, dw_in{}, dw_out{};  // gates: where cols are long
   // offsets into the workspace, 0 for none: packed operands, sums of parts of K
   int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, dh = 0, bytes = 0;
-  int64_t part = 0, part_in = 0;     // y's, dw_out's or dx's; dw_in's
+  int64_t part = 0, part_in = 0;     // y's, gates', dw_out's or dx's; dw_in's
+  int64_t pre = 0;                   // where cols are long and no pre is kept
   int64_t half = 0;                  // columns of each half of dpre: width, up to a whole K block
 };
 
@@ -161,7 +167,12 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
   if (!grad) {
     p.y = shape(rows, outs, width);
     choose_splits(dtype, &p.y, nullptr);
-    p.part = take(sums(p.y));
+    if (is_long(dtype, cols)) {
+      p.gates = shape(rows, 2 * width, cols);
+      choose_splits(dtype, &p.gates, nullptr);
+      p.pre = take(rows * 2 * width * 4);
+    }
+    p.part = take(std::max(sums(p.y), sums(p.gates)));
   } else {
     if (pk.dy) p.dy = packed(rows, outs);
     p.half = up(width, kHeadTileK);
@@ -302,10 +313,14 @@ struct Call {
   }
   // Where a product goes, by way of sums of parts of K if it is split.
   void target(HeadJob& j, const Shape& h, void* out, int64_t ld, int64_t part, HeadReduce* red, int* reds) const {
+    target(j, h, out, ld, a.dtype, part, red, reds);
+  }
+  void target(HeadJob& j, const Shape& h, void* out, int64_t ld, int dtype, int64_t part, HeadReduce* red,
+              int* reds) const {
     j.out = out;
     j.ld_out = ld;
-    j.out_f32 = a.dtype == kF32;
-    j.wide = aligned(out, size_t(4 * dtype_bytes(a.dtype))) && ld % 4 == 0;
+    j.out_f32 = dtype == kF32;
+    j.wide = aligned(out, size_t(4 * dtype_bytes(dtype))) && ld % 4 == 0;
     if (!j.out_f32 && aligned(out, 16) && ld % 8 == 0) j.wide = 2;
     j.final = 1;
     if (j.splits > 1) {
@@ -384,13 +399,23 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   if (c.pack({&px, &pin, narrow ? &none : &pout}, true)) return -1;
 
   // gates and factors: half of a tile's columns each
-  const Shape in = gate_shape(a.dtype, a.rows, a.width, a.cols);
+  const Shape in = is_long(a.dtype, a.cols) ? p.gates : gate_shape(a.dtype, a.rows, a.width, a.cols);
   HeadLaunch l{};
   head_settings(l, a.dtype, a.workspace);
   l.jobs = 1;
   if (c.job(l.job[0], x, false, w_in, false, in)) return -1;
-  gate(l.g, a);
-  FFN_CUDA(launch_head(kHeadGate, 2 * in.tile_n, l, s), "block launch");
+  if (is_long(a.dtype, a.cols)) {
+    float* pre = a.pre ? a.pre : reinterpret_cast<float*>(c.base() + p.pre);
+    const int64_t ld = a.pre ? a.ld_pre : 2 * a.width;
+    HeadReduce red[1]{};
+    int reds = 0;
+    c.target(l.job[0], in, pre, ld, kF32, p.part, red, &reds);
+    if (c.products(kHeadOut, l, in.tile_n, red, reds)) return -1;
+    FFN_CUDA(launch_ffn_gate(a, pre, ld, s), "block launch");
+  } else {
+    gate(l.g, a);
+    FFN_CUDA(launch_head(kHeadGate, 2 * in.tile_n, l, s), "block launch");
+  }
   ++c.launches;
 
   if (narrow) {

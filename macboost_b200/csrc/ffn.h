@@ -65,7 +65,13 @@ cudaError_t launch_ffn_few(const FfnArgs& a, cudaStream_t s);
 // against 47; 48 x 1,536 x 4,096 (0.9e9) 30 against 37; 24 x 4,096 x 16,384 (4.8e9) 132 against 103.
 constexpr int64_t kFfnWarpRows = 16, kFfnWarpMost = 48;
 constexpr double kFfnWarpProducts = 1.4e9;
+// Terms of a bfloat16 sum that the tensor core, which truncates it at each step of 16, holds in one place:
+// 2,048 steps lose 2^-12 at most.  A million terms of one sign in one place lost 0.6%, more than a rounding to
+// bfloat16; a block's eight warps share a sum.
+constexpr int64_t kFfnLong = 32768, kFfnWarpLong = 8 * kFfnLong;
 cudaError_t launch_ffn_rows(const FfnArgs& a, cudaStream_t s);
+// bfloat16: hidden from pre (rows x 2 width, stride ld_pre).
+cudaError_t launch_ffn_gate(const FfnArgs& a, const float* pre, int64_t ld_pre, cudaStream_t s);
 // float32: from dh (stride ld_dh) and pre to the planes of the gradients of both halves
 // (3 x rows x 2 half, zeros from width to half), and of hidden (3 x rows x ld_h) unless null.
 struct FfnSplit {

@@ -359,6 +359,24 @@ cudaError_t rows_of(const Few& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// ---- bfloat16, long rows of x: the activation after the product -------------------------
+//
+// A thread a value: 10 bytes of it, beside 65,536 products and more.
+__global__ void __launch_bounds__(kThreads)
+    ffn_gate_kernel(int act, const float* pre, long long ld_pre, __nv_bfloat16* hidden, long long ld_hidden,
+                    long long rows, int width) {
+  const long long all = rows * width, step = (long long)gridDim.x * kThreads;
+  for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < all; i += step) {
+    const long long n = i / width;
+    const int c = int(i - n * width);
+    const float* p = pre + n * ld_pre + c;
+    float v[1] = {p[0]};
+    const float u[1] = {p[width]};
+    activate<true>(act, v, u);
+    hidden[n * ld_hidden + c] = __float2bfloat16_rn(v[0]);
+  }
+}
+
 // ---- float32: the gradients of gates and factors ----------------------------------
 //
 // The tensor cores' epilogue keeps 128 sums a thread in float32, and fetching pre and three
@@ -629,6 +647,13 @@ cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s) {
     ffn_split_kernel<true><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
   else
     ffn_split_kernel<false><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_ffn_gate(const FfnArgs& a, const float* pre, int64_t ld_pre, cudaStream_t s) {
+  const long long blocks = (a.rows * a.width + kThreads - 1) / kThreads;
+  ffn_gate_kernel<<<unsigned(std::min<long long>(blocks, 8 * device_sms())), kThreads, 0, s>>>(
+      a.act, pre, ld_pre, static_cast<__nv_bfloat16*>(a.hidden), a.ld_hidden, a.rows, int(a.width));
   return cudaGetLastError();
 }
 
