@@ -104,7 +104,8 @@ Shape gate_shape(int dtype, int64_t rows, int64_t width, int64_t cols) {
 // of one K block (0.42 us for 256 columns).  A pair's time is the longest tile's, or its share
 // of all steps and half a tile more; the sums of parts are written and read once more, at
 // 6 TB/s.  Bounds of a part as head_splits has them: no shorter than 8 blocks (float32: 2),
-// bfloat16 no longer than 512.  `whole`: the second one's epilogue needs all of its sums.
+// bfloat16 no longer than 512.  `whole`: the second one's epilogue needs all of its sums
+// (of 512 blocks at most there too: longer ones take a launch more, is_long).
 void choose_splits(int dtype, Shape* a, Shape* b, bool whole = false) {
   constexpr int64_t kPairs = 74;
   const int64_t steps = dtype == kF32 ? 6 : 1, shortest = dtype == kF32 ? 2 : 8;
@@ -137,10 +138,10 @@ void choose_splits(int dtype, Shape* a, Shape* b, bool whole = false) {
 }
 
 struct Plan {
-  Shape y{}, gates{}, dx{}, dw_in{}, dw_out{};  // gates: where cols are long
+  Shape y{}, gates{}, dh{}, dx{}, dw_in{}, dw_out{};  // gates: where cols are long
   // offsets into the workspace, 0 for none: packed operands, sums of parts of K
-  int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, dh = 0, bytes = 0;
-  int64_t part = 0, part_in = 0;     // y's, gates', dw_out's or dx's; dw_in's
+  int64_t x = 0, w_in = 0, w_out = 0, hidden = 0, dy = 0, dpre = 0, dh_at = 0, bytes = 0;
+  int64_t part = 0, part_in = 0;     // y's, gates', dh's, dw_out's or dx's; dw_in's
   int64_t pre = 0;                   // where cols are long and no pre is kept
   int64_t half = 0;                  // columns of each half of dpre: width, up to a whole K block
 };
@@ -177,16 +178,23 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t width, int64_t out
     if (pk.dy) p.dy = packed(rows, outs);
     p.half = up(width, kHeadTileK);
     p.dpre = take(planes * rows * 2 * p.half * 2);
-    if (dtype == kF32) p.dh = take(rows * up(width, 4) * 4);
+    // dh in float32, where a launch of its own goes on with it
+    const bool split = dtype == kF32 || is_long(dtype, outs);
+    if (split) p.dh_at = take(rows * up(width, 4) * 4);
     p.dx = shape(rows, cols, 2 * p.half);
     p.dw_in = shape(p.half + width, cols, rows);
     p.dw_out = shape(outs, width, rows);
     choose_splits(dtype, &p.dx, &p.dw_in);
-    Shape dh = shape(rows, width, outs);
-    choose_splits(dtype, &p.dw_out, dtype == kF32 ? nullptr : &dh, true);
-    // dw_out is done before the others begin
+    p.dh = shape(rows, width, outs);
+    if (split) {
+      choose_splits(dtype, &p.dw_out, nullptr);
+      if (dtype == kBF16) choose_splits(dtype, &p.dh, nullptr);
+    } else {
+      choose_splits(dtype, &p.dw_out, &p.dh, true);
+    }
+    // dh and dw_out are done before the others begin
     const int64_t chunks = is_narrow(dtype, width, outs) ? parts(rows, narrow_rows(rows, p.half)) : 0;
-    p.part = take(std::max({sums(p.dw_out), sums(p.dx), chunks * outs * width * 4}));
+    p.part = take(std::max({sums(p.dh), sums(p.dw_out), sums(p.dx), chunks * outs * width * 4}));
     p.part_in = take(sums(p.dw_in));
   }
   p.bytes = at;
@@ -467,8 +475,9 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
   const bool f32 = a.dtype == kF32, inner = a.dx || a.dw_in;
   // h with the others, unless a launch of its own makes its planes
   const HeadPack none;
-  const bool narrow = is_narrow(a.dtype, a.width, a.outs), split = inner && f32 && !narrow;
-  if (c.pack({narrow ? &none : &pdy, inner && !narrow ? &pout : &none, a.dw_out && !split && !narrow ? &ph : &none,
+  const bool narrow = is_narrow(a.dtype, a.width, a.outs);
+  const bool split = inner && (f32 || is_long(a.dtype, a.outs)) && !narrow;
+  if (c.pack({narrow ? &none : &pdy, inner && !narrow ? &pout : &none, a.dw_out && !(f32 && split) && !narrow ? &ph : &none,
               inner ? &px : &none, a.dx ? &pin : &none}, false))
     return -1;
   if (narrow) {  // dh, dpre and dw_out at once
@@ -498,33 +507,38 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
       ++c.launches;
     }
   }
-  // dh = dy w_out; its epilogue (float32: a launch) makes the gradients of gates and factors of it
-  const Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
+  // dh = dy w_out; its epilogue (float32, and long sums: a launch) makes the gradients of gates and factors of it
+  Shape dh{a.rows, a.width, a.outs, kHeadTileN, 1, 0};
+  if (split && !f32) dh.splits = p.dh.splits;
   if (split) {
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
     q.jobs = 1;
     if (c.job(q.job[0], dy, false, w_out, true, dh)) return -1;
     FfnSplit t{};
+    t.dtype = a.dtype;
     t.act = a.act;
     t.rows = a.rows;
     t.width = int(a.width);
     t.half = int(p.half);
     t.ld_h = int(up(a.width, 8));
-    t.dh = reinterpret_cast<const float*>(c.base() + p.dh);
+    t.dh = reinterpret_cast<const float*>(c.base() + p.dh_at);
     t.ld_dh = up(a.width, 4);
     t.pre = a.pre;
     t.ld_pre = a.ld_pre;
     t.hidden = static_cast<const float*>(a.hidden);
     t.ld_hidden = a.ld_hidden;
     t.dpre = c.base() + p.dpre;
-    t.h = a.dw_out ? c.base() + p.hidden : nullptr;
-    c.target(q.job[0], dh, c.base() + p.dh, t.ld_dh, 0, nullptr, nullptr);
-    if (c.products(kHeadOut, q, kHeadTileN, nullptr, 0)) return -1;
+    t.h = f32 && a.dw_out ? c.base() + p.hidden : nullptr;
+    HeadReduce red[1]{};
+    int reds = 0;
+    c.target(q.job[0], dh, c.base() + p.dh_at, t.ld_dh, kF32, p.part, red, &reds);
+    if (c.products(kHeadOut, q, kHeadTileN, red, reds)) return -1;
     FFN_CUDA(launch_ffn_split(t, s), "block split launch");
     ++c.launches;
   }
-  if ((a.dw_out && !narrow) || (inner && !f32)) {
+  const bool with = inner && !f32 && !split;
+  if ((a.dw_out && !narrow) || with) {
     // dw_out = dy^T h: in bfloat16 in one launch with dh, whose epilogue takes longer than its products
     HeadLaunch q{};
     head_settings(q, a.dtype, a.workspace);
@@ -536,7 +550,6 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
       c.target(j, p.dw_out, a.dw_out, a.ld_dout, p.part, red, &reds);
       j.plain = 1;
     }
-    const bool with = inner && !f32;
     if (with) {
       if (c.job(q.job[q.jobs++], dy, false, w_out, true, dh)) return -1;
       gate(q.g, a);

@@ -72,10 +72,11 @@ constexpr int64_t kFfnLong = 32768, kFfnWarpLong = 8 * kFfnLong;
 cudaError_t launch_ffn_rows(const FfnArgs& a, cudaStream_t s);
 // bfloat16: hidden from pre (rows x 2 width, stride ld_pre).
 cudaError_t launch_ffn_gate(const FfnArgs& a, const float* pre, int64_t ld_pre, cudaStream_t s);
-// float32: from dh (stride ld_dh) and pre to the planes of the gradients of both halves
-// (3 x rows x 2 half, zeros from width to half), and of hidden (3 x rows x ld_h) unless null.
+// From dh (float32, stride ld_dh) and pre to the gradients of both halves, zeros from width to half:
+// float32 in planes (3 x rows x 2 half), and those of hidden (3 x rows x ld_h) unless h is null; bfloat16,
+// whose dh is here where outs are long, rounded (rows x 2 half).
 struct FfnSplit {
-  int act;
+  int dtype, act;
   long long rows;
   int width, half, ld_h;
   const float* dh;

@@ -420,9 +420,18 @@ __device__ __forceinline__ void put_planes(__nv_bfloat16* to, long long plane, c
   }
 }
 
+// The same, rounded once (bfloat16).
+__device__ __forceinline__ void put_rounded(__nv_bfloat16* to, const float (&x)[4]) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+  uint2 w;
+  memcpy(&w.x, &lo, 4);
+  memcpy(&w.y, &hi, 4);
+  *reinterpret_cast<uint2*>(to) = w;
+}
+
 // 128 columns a warp, four adjacent ones a lane.  WIDE: rows of dh, hidden and both halves of pre
 // start on 16 bytes; else they are read side by side and change lanes in shared memory.
-template <bool WIDE>
+template <bool F32, bool WIDE>
 __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, int per) {
   __shared__ float turn[WIDE ? 1 : kWarps][WIDE ? 1 : 128];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -451,13 +460,18 @@ __global__ void __launch_bounds__(kThreads) ffn_split_kernel(const FfnSplit a, i
   if (a.h) get(a.hidden + n * a.ld_hidden, h);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    gate_grad<false>(a.act, x[k], y[k], dh[k], dx[k], dy[k]);
+    gate_grad<!F32>(a.act, x[k], y[k], dh[k], dx[k], dy[k]);
     if (c + k >= a.width) dx[k] = dy[k] = 0.f;
   }
   if (c < a.half) {
     __nv_bfloat16* d = static_cast<__nv_bfloat16*>(a.dpre) + n * 2 * a.half + c;
-    put_planes(d, a.rows * 2 * a.half, dx);
-    put_planes(d + a.half, a.rows * 2 * a.half, dy);
+    if constexpr (F32) {
+      put_planes(d, a.rows * 2 * a.half, dx);
+      put_planes(d + a.half, a.rows * 2 * a.half, dy);
+    } else {
+      put_rounded(d, dx);
+      put_rounded(d + a.half, dy);
+    }
   }
   if (a.h && c < a.ld_h) put_planes(static_cast<__nv_bfloat16*>(a.h) + n * a.ld_h + c, a.rows * a.ld_h, h);
 }
@@ -640,13 +654,17 @@ cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s) {
   const int per = (a.half + 127) / 128;  // warps a row
   const long long blocks = (a.rows * per + kWarps - 1) / kWarps;
   if (blocks > INT_MAX) return cudaErrorInvalidValue;
-  const bool wide = (reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.pre) |
-                     reinterpret_cast<uintptr_t>(a.hidden) | uintptr_t(a.ld_dh) * 4 | uintptr_t(a.ld_pre) * 4 |
-                     uintptr_t(a.ld_hidden) * 4 | uintptr_t(a.width) * 4) % 16 == 0;
-  if (wide)
-    ffn_split_kernel<true><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  const uintptr_t hidden = a.h ? reinterpret_cast<uintptr_t>(a.hidden) | uintptr_t(a.ld_hidden) * 4 : 0;
+  const bool wide = (reinterpret_cast<uintptr_t>(a.dh) | reinterpret_cast<uintptr_t>(a.pre) | hidden |
+                     uintptr_t(a.ld_dh) * 4 | uintptr_t(a.ld_pre) * 4 | uintptr_t(a.width) * 4) % 16 == 0;
+  if (a.dtype != kF32 && wide)
+    ffn_split_kernel<false, true><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  else if (a.dtype != kF32)
+    ffn_split_kernel<false, false><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+  else if (wide)
+    ffn_split_kernel<true, true><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
   else
-    ffn_split_kernel<false><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
+    ffn_split_kernel<true, false><<<unsigned(blocks), kThreads, 0, s>>>(a, per);
   return cudaGetLastError();
 }
 

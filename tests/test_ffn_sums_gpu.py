@@ -52,3 +52,46 @@ def test_long_rows(gpu, torch, rows, cols):
     b.forward(keep=False)
     assert torch.equal(b.results()["y"], y) and torch.equal(b.results()["hidden"], hidden)
     b.intact()
+
+
+@pytest.mark.parametrize("rows,outs,pad", [(5, 2 ** 20 - 8, 0), (100, 2 ** 20 - 8, 0), (300, 40_000, 0), (70, 40_001, 3)])
+def test_long_outputs(gpu, torch, rows, outs, pad):
+    """dh = dy w_out over many outputs, bfloat16.  The gradients of gates and factors are rounded to
+    bfloat16, by 2^-9 of each on average 0: their mean over `width` x rows values is off by what the
+    sums lost, 2^-12, and by eight times 2^-9 / sqrt(rows x width)."""
+    width = cols = 64
+    b = _block(gpu, torch, rows, cols, width, outs, "bfloat16", "silu", pad=pad, seed=7)
+    _positive(torch, b.dy, 8)
+    _positive(torch, b.w_out, 9)
+    b.w_out.mul_(1.0 / outs)
+    b.forward()
+    b.x.zero_()
+    b.x[:, :cols] = 1.0
+    # dw_in of one column is the sum of the rows' gradients; dx of an identity is the gradients themselves
+    b.w_in.zero_()
+    b.w_in[width:2 * width, :width] = torch.eye(width, device="cuda").bfloat16()
+    b.grad()
+    b.check()
+    dy, w_out = b.dy[:, :outs], b.w_out[:, :width]
+    dh = sum(dy[:, i:i + 65_536].double() @ w_out[i:i + 65_536].double() for i in range(0, outs, 65_536))
+    gate = b.results()["pre"][:, :width].double()
+    db = dh * torch.nn.functional.silu(gate)
+    got = b.results()["dx"].double()
+    there = db.abs() > 2.0 ** -60
+    error = (got - db)[there] / db[there]
+    assert float(error.abs().max()) <= 2.0 ** -8 + 2.0 ** -11
+    assert abs(float(error.mean())) <= 2.0 ** -12 + 8 * 2.0 ** -9 / error.numel() ** 0.5
+    first = {k: v.clone() for k, v in b.results().items()}
+    for name in ("dx", "dw_in", "dw_out"):
+        getattr(b, name).fill_(7.0)
+        b.grad((name,))
+        assert torch.equal(b.results()[name], first[name]), name
+    dw_in = torch.cat((dh * b.results()["pre"][:, width:].double() * _silu_slope(torch, gate), db), 1).sum(0)
+    most = torch.cat(((dh * b.results()["pre"][:, width:].double() * _silu_slope(torch, gate)).abs(), db.abs()), 1).sum(0)
+    assert torch.all((first["dw_in"][:, 0].double() - dw_in).abs() <= most * (2.0 ** -8 + 2.0 ** -11) + dw_in.abs() * 2.0 ** -8)
+    b.intact()
+
+
+def _silu_slope(torch, a):
+    p = 1.0 / (1.0 + torch.exp(-a))
+    return p * (1.0 + a * (1.0 - p))
