@@ -92,7 +92,7 @@ cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s);
 // float32 with few outputs (a class margin each, say): y, dh and dw_out are too little for tiles that
 // want planes of h first, and go to the CUDA cores.
 constexpr int64_t kFfnNarrow = 16, kFfnNarrowValues = 16384;  // outs; outs * width
-constexpr int64_t kFfnNarrowWarps = 1184;                     // of the gradient, about: eight a multiprocessor
+constexpr int64_t kFfnNarrowWarps = 1184;                     // of the gradient, at least: eight a multiprocessor
 cudaError_t launch_ffn_narrow(const FfnArgs& a, cudaStream_t s);
 struct FfnNarrow {
   int act, outs;

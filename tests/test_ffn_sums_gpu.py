@@ -95,3 +95,24 @@ def test_long_outputs(gpu, torch, rows, outs, pad):
 def _silu_slope(torch, a):
     p = 1.0 / (1.0 + torch.exp(-a))
     return p * (1.0 + a * (1.0 - p))
+
+
+def test_narrow_gradient_of_many_rows(gpu, torch):
+    """float32 with one output: dw_out of 500,000 rows, each of them 1 + 0.9 x 2^-12.  A sum past 4,096 in
+    steps of 2^-11 leaves all of the 0.9 x 2^-12 behind, term after term.  A warp has at
+    most 256 rows (251 in 27 rounds), and loses at most 2^-24 of what is there with each, half of them on
+    average; eight threads share the 1,993 warps' sums and lose the same with each of theirs, and at most 2^-24
+    of the whole with each of the eight: (251 / 2 + 250 / 2 + 8) x 2^-24 of it."""
+    rows, width = 500_000, 2048
+    b = _block(gpu, torch, rows, 4, width, 1, "float32", "silu", seed=3)
+    b.hidden.fill_(1.0 + 0.9 * 2.0 ** -12)
+    b.dy.fill_(1.0)
+    b.grad(("dw_out",))
+    want = rows * float(b.hidden[0, 0].double())
+    got = b.results()["dw_out"].double()
+    assert float((got - want).abs().max()) <= (251 / 2 + 250 / 2 + 8) * 2.0 ** -24 * want
+    # with dx and dw_in beside it, the same bits
+    first = b.results()["dw_out"].clone()
+    b.pre.fill_(0.25)
+    b.grad()
+    assert torch.equal(b.results()["dw_out"], first)
