@@ -117,19 +117,27 @@ __device__ __forceinline__ double chunk_squares(const T* src, long long left, bo
   return sum;
 }
 
+// The factor, as a product: one below float32's normal numbers would have few bits left, or none (gradients of
+// 1e38 clipped to a norm of 1e-5 came out twice too large).
+struct Factor {
+  float high, low;  // low: 1, or 2^-100
+  __device__ __forceinline__ bool one() const { return high == 1.f && low == 1.f; }
+  __device__ __forceinline__ float operator()(float v) const { return v * high * low; }
+};
+
 template <class T>
-__device__ __forceinline__ uint4 scaled(uint4 u, float factor) {
+__device__ __forceinline__ uint4 scaled(uint4 u, Factor factor) {
   constexpr int N = 16 / int(sizeof(T));
   T v[N];
   memcpy(v, &u, 16);
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = from_float<T>(to_float(v[k]) * factor);
+  for (int k = 0; k < N; ++k) v[k] = from_float<T>(factor(to_float(v[k])));
   memcpy(&u, v, 16);
   return u;
 }
 
 template <class T>
-__device__ __forceinline__ void chunk_scale(const T* src, T* dst, long long left, float factor) {
+__device__ __forceinline__ void chunk_scale(const T* src, T* dst, long long left, Factor factor) {
   // 16 bytes at a time where both sides reach a boundary together
   const bool whole = (reinterpret_cast<uintptr_t>(src) - reinterpret_cast<uintptr_t>(dst)) % 16 == 0;
   const Span<T> c(src, left, whole);
@@ -147,7 +155,7 @@ __device__ __forceinline__ void chunk_scale(const T* src, T* dst, long long left
   for (; n > 0; n -= kThreads, q += kThreads, to += kThreads) __stcs(to, scaled<T>(*q, factor));
   for (int i = threadIdx.x; i < c.head + c.tail; i += kThreads) {
     const int at = i < c.head ? i : i + c.units * N;
-    dst[at] = from_float<T>(to_float(src[at]) * factor);
+    dst[at] = from_float<T>(factor(to_float(src[at])));
   }
 }
 
@@ -202,8 +210,10 @@ __device__ __forceinline__ double norm_of(const ClipState& c, double* shared) {
   return sqrt(block_sum(sum, shared));
 }
 
-__device__ __forceinline__ float factor_of(double norm, double max_norm) {
-  return norm > max_norm ? float(max_norm / norm) : norm == norm ? 1.f : float(norm);
+__device__ __forceinline__ Factor factor_of(double norm, double max_norm) {
+  if (!(norm > max_norm)) return Factor{norm == norm ? 1.f : float(norm), 1.f};
+  const double f = max_norm / norm;
+  return f < 0x1p-126 && f > 0.0 ? Factor{float(f * 0x1p100), 0x1p-100f} : Factor{float(f), 1.f};
 }
 
 template <int N>
@@ -212,8 +222,8 @@ __global__ void __launch_bounds__(kThreads, 4)
   __shared__ double shared[kThreads / 32];
   const double norm = norm_of(c, shared);
   if (c.first == 0 && blockIdx.x == 0 && threadIdx.x == 0) *c.norm = float(norm);
-  const float factor = factor_of(norm, c.max_norm);
-  if (c.in_place && factor == 1.f) return;
+  const Factor factor = factor_of(norm, c.max_norm);
+  if (c.in_place && factor.one()) return;
   for (unsigned k = blockIdx.x; k < t.chunks; k += gridDim.x)
     with_chunk(t, t.chunks - 1 - k, [&](const auto* src, auto* dst, long long left) {
       chunk_scale(src, dst, left, factor);
@@ -249,8 +259,8 @@ __global__ void __cluster_dims__(kClipCluster, 1, 1) __launch_bounds__(kThreads)
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const double norm = sqrt(sum);
   if (blockIdx.x == 0 && threadIdx.x == 0) *c.norm = float(norm);
-  const float factor = factor_of(norm, c.max_norm);
-  if (t.dst && !(c.in_place && factor == 1.f))
+  const Factor factor = factor_of(norm, c.max_norm);
+  if (t.dst && !(c.in_place && factor.one()))
     for (unsigned chunk = blockIdx.x; chunk < t.chunks; chunk += kClipCluster)
       with_chunk(t, chunk, [&](const auto* src, auto* dst, long long left) {
         chunk_scale(src, dst, left, factor);
