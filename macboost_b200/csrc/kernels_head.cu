@@ -601,6 +601,8 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             return q.b_mn ? min(TN / kHeadPair / 64, max(0, (q.N - n0 + 63) / 64)) * 8192
                           : EPI == kHeadGate || n0 < q.N ? q.b_box * 128 : 0;
           };
+          // (read from the job at every block, and in every form of the kernel, the gap cost the head's tiles 2 to 4%)
+          const int b_k0 = q.b_k0, gap = q.b_from / kHeadTileK, skip = q.b_skip;
           const int m0 = t.m * kHeadPair * kHeadTileM, n0 = t.n * TN;
           const uint32_t bytes = kPlanes * uint32_t(bytes_a(m0) + bytes_a(m0 + kHeadTileM) + bytes_b(n0) +
                                           bytes_b(n0 + TN / kHeadPair));
@@ -616,7 +618,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             }
             if (a.stall) continue;
             const int ka = q.a_k0 + kb * kHeadTileK;
-            const int kk = q.b_k0 + kb * kHeadTileK - (kb * kHeadTileK >= q.b_from ? q.b_skip : 0);
+            const int kk = b_k0 + kb * kHeadTileK - (EPI == kHeadOut && kb >= gap ? skip : 0);
             for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
               if (q.a_mn) {
 #pragma unroll
