@@ -106,7 +106,7 @@ Shape gate_shape(int dtype, int64_t rows, int64_t width, int64_t cols) {
 // Parts of K of one or two products of a launch: those that end first by an estimate, in steps
 // of one K block (0.42 us for 256 columns).  A pair's time is the longest tile's, or its share
 // of all steps and half a tile more; the sums of parts are written and read once more, at
-// 6 TB/s.  Bounds of a part as head_splits has them: no shorter than 8 blocks (float32: 2),
+// 6 TB/s.  Bounds of a part as in the head: no shorter than 8 blocks (float32: 2),
 // bfloat16 no longer than 512.  `whole`: the second one's epilogue needs all of its sums
 // (of 512 blocks at most there too: longer ones take a launch more, is_long).
 void choose_splits(int dtype, Shape* a, Shape* b, bool whole = false) {

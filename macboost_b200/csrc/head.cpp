@@ -54,6 +54,19 @@ struct Plan {
   int64_t bytes = 0;
 };
 
+// Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
+// CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
+// blocks (float32: 2, of six products), so that the sums of parts stay few.  bfloat16 sums
+// stay in the tensor core, which truncates them at each step of 16: a sum whose terms have one
+// sign lost 1e-7 of itself a step (dw of 300,000 rows, 0.18%).  So its parts are 512 blocks
+// (2,048 steps, 2^-12) at most, and the parts are added up in float32.
+int splits_for(int64_t kblocks, int64_t all, int dtype) {
+  const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
+  const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
+  const int64_t load = std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100);
+  return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
+}
+
 Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad, bool pack_h,
                bool pack_w, bool want_dh, bool want_dw) {
   Plan p{};
@@ -86,8 +99,8 @@ Plan make_plan(int dtype, int64_t rows, int64_t cols, int64_t classes, bool grad
     const int64_t steps = dtype == kF32 ? 6 : 1;
     const int64_t all = dh_tiles * (dh_blocks * steps + kHeadEpilogue) +
                         dw_tiles * (dw_blocks * steps + kHeadEpilogue);
-    p.dh_splits = head_splits(dh_blocks, all, dtype);
-    p.dw_splits = head_splits(dw_blocks, all, dtype);
+    p.dh_splits = splits_for(dh_blocks, all, dtype);
+    p.dw_splits = splits_for(dw_blocks, all, dtype);
     if (want_dh && p.pieces > 1) p.acc = take(rows * cols * 4);
     if (want_dh && p.dh_splits > 1) p.dh_part = take(p.dh_splits * rows * cols * 4);
     if (want_dw && p.dw_splits > 1) p.dw_part = take(p.dw_splits * p.piece * cols * 4);
@@ -336,19 +349,6 @@ int few(int device, const HeadArgs& a, bool grad, cudaStream_t s, std::string& e
 // TMA reads rows in place when they start on 16 bytes.
 bool head_in_place(int dtype, const void* p, int64_t ld) {
   return dtype == kBF16 && aligned(p, 16) && ld % 8 == 0;
-}
-
-// Parts of K of a product whose tiles walk `kblocks`: none longer than what each pair of
-// CTAs gets of `all` steps in total, so that they end together, and none shorter than 8
-// blocks (float32: 2, of six products), so that the sums of parts stay few.  bfloat16 sums
-// stay in the tensor core, which truncates them at each step of 16: a sum whose terms have one
-// sign lost 1e-7 of itself a step (dw of 300,000 rows, 0.18%).  So its parts are 512 blocks
-// (2,048 steps, 2^-12) at most, and the parts are added up in float32.
-int head_splits(int64_t kblocks, int64_t all, int dtype) {
-  const int64_t least = dtype == kF32 ? 2 : 8, steps = dtype == kF32 ? 6 : 1;
-  const int64_t most = std::max(least, (all / 74 - kHeadEpilogue) / steps);
-  const int64_t load = std::min<int64_t>(std::min(parts(kblocks, most), kblocks / least), 100);
-  return int(std::max<int64_t>({1, load, dtype == kF32 ? 1 : parts(kblocks, 512)}));
 }
 
 int head_encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,

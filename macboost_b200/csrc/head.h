@@ -213,8 +213,6 @@ constexpr int64_t kStatusBytes = 256;
 // Host side of products as tiles, for the blocks that use them (head.cpp).
 // TMA reads rows in place when they start on 16 bytes.
 bool head_in_place(int dtype, const void* p, int64_t ld);
-// Parts of K of a product whose tiles walk `kblocks`, of a launch of `all` steps.
-int head_splits(int64_t kblocks, int64_t all, int dtype);
 // A matrix of planes x outer x inner 16-bit values, stride ld, fetched in boxes of 64
 // inner x `box` outer values into 128-byte swizzled rows; zeros outside.
 int head_encode(CUtensorMap* m, const void* p, int64_t inner, int64_t outer, int64_t ld, int planes,
