@@ -529,11 +529,11 @@ int32_t macboost_head_check_device(int32_t device, const void *workspace, char *
  * allocated, results that do not depend on timing, sums in float32 rounded once. */
 
 /* out[n] = scale * sum over j of table[starts[j] + ids[n, j]], for rows rows of k
- * int32 ids.  table is entries x cols (entries below 2^30, stride ld), out rows x
- * cols (stride ld_out), both of `dtype`.  starts (k int32; NULL: zeros) is the
- * first row of each column of ids, so that one table holds all trees' nodes:
- * starts[j] = j * nodes.  An id that is negative, or that leads to no row of the
- * table, adds nothing; k = 1 is a plain lookup. */
+ * int32 ids, added up in the order of j.  table is entries x cols (entries below
+ * 2^30, stride ld), out rows x cols (stride ld_out), both of `dtype`.  starts (k
+ * int32; NULL: zeros) is the first row of each column of ids, so that one table holds
+ * all trees' nodes: starts[j] = j * nodes.  An id that is negative, or that leads to
+ * no row of the table, adds nothing; k = 1 is a plain lookup. */
 int32_t macboost_embed_device(int32_t device, int32_t dtype, const void *table, int64_t entries,
                               int64_t cols, int64_t ld, const int32_t *ids, int64_t rows,
                               int64_t k, const int32_t *starts, float scale, void *out,
@@ -605,13 +605,14 @@ int64_t macboost_clip_workspace(int64_t count, const int32_t *dtypes, const int6
 
 /* norm (one float32 on the device) = the square root of the sum of squares of all
  * values of `count` gradients; then, unless outs is NULL, outs[i] = grads[i] * (norm
- * > max_norm ? max_norm / norm : 1), rounded once (NaN everywhere for a norm that is
- * NaN).  dtypes, grads, sizes (values, each gradient without gaps) and outs are host
- * arrays, free again when the call returns; grads[i] and outs[i] are device memory,
- * either the same (then a factor of 1 writes nothing) or apart.  Squares are added up
- * so that nothing overflows or vanishes that float32 holds as a norm.  `workspace` is
- * device memory, 8-byte aligned, used until the call's work is done, but for its first
- * 256 bytes, as in macboost_embed_grad_device. */
+ * > max_norm ? max_norm / norm : 1), with 24 bits of the factor, and rounded to the type
+ * (NaN everywhere for a norm that is NaN).  dtypes, grads, sizes (values, each gradient
+ * without gaps) and outs are host arrays, free again when the call returns; grads[i] and
+ * outs[i] are device memory, either the same (then a factor of 1 writes nothing) or
+ * apart; outs are apart from each other and from other gradients.  Squares are added up so
+ * that nothing overflows or vanishes that float32 holds as a norm.  `workspace` is device
+ * memory, 8-byte aligned, used until the call's work is done, but for its first 256 bytes,
+ * as in macboost_embed_grad_device. */
 int32_t macboost_clip_device(int32_t device, int64_t count, const int32_t *dtypes,
                              const void *const *grads, const int64_t *sizes, void *const *outs,
                              double max_norm, float *norm, void *workspace,

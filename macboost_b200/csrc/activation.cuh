@@ -32,7 +32,8 @@ __device__ __forceinline__ float sigmoid(float x) {
 
 // The normal distribution function and its density.  FAST: formula 7.1.26 of Abramowitz and
 // Stegun, "Handbook of Mathematical Functions" (1964), off by less than 1.5e-7 / 2, in its form
-// for the tail, whose exponential is the density's.
+// for the tail, whose exponential is the density's.  Of the tail itself that is 0.16% at -5, where x p is
+// -1.4e-6, and 1% at -8, where it is -5e-15.
 template <bool FAST>
 __device__ __forceinline__ void normal(float x, float& p, float& density) {
   constexpr float kRoot2Pi = 0.3989422804014327f;  // 1 / sqrt(2 pi)

@@ -90,7 +90,11 @@ struct FfnSplit {
 cudaError_t launch_ffn_split(const FfnSplit& a, cudaStream_t s);
 
 // float32 with few outputs (a class margin each, say): y, dh and dw_out are too little for tiles that
-// want planes of h first, and go to the CUDA cores.
+// want planes of h first, and go to the CUDA cores.  Forward passes of 64 columns as graphs, these and tiles, in us
+// at 17, 200, 800 and 6,400 rows: 403 x 10 18, 19, 20, 31 and 27, 29, 29, 46; 1,024 x 16 20, 23, 25, 50 and 26, 27, 28, 60;
+// 4,096 x 1 35, 36, 47, 119 and 39, 40, 53, 185.  Where both limits meet tiles end up to 15% sooner on few rows
+// (4,096 x 4 41, 45, 56, 141 and 40, 41, 53, 186; 16,384 x 1 113, 120, 164, 424 and 103, 108, 186, 647), but the
+// gradient does not: 17 rows of 16,384 x 1 64, of 17 outputs, as tiles, 126.
 constexpr int64_t kFfnNarrow = 16, kFfnNarrowValues = 16384;  // outs; outs * width
 constexpr int64_t kFfnNarrowWarps = 1184;                     // of the gradient, at least: eight a multiprocessor
 cudaError_t launch_ffn_narrow(const FfnArgs& a, cudaStream_t s);

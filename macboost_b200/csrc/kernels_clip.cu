@@ -56,7 +56,8 @@ __device__ __forceinline__ double block_sum(double v, double* shared) {
 
 // Squares of 16 bytes of values.  Sums of squares between 2^-80 and 2^120 lose nothing to
 // float32's range: a square below its smallest normal number, 2^-126, is below 2^-46 of
-// the sum.
+// the sum.  (Units of zeros go the long way too: the norm of 340 MB of them takes 94 us, of noise 77, both with
+// the call.)
 template <class T>
 __device__ __forceinline__ double squares(uint4 u) {
   constexpr int N = 16 / int(sizeof(T));

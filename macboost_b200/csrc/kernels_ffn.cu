@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) ffn_few_kernel(const Few a) {
             activate<sizeof(T) == 2>(a.act, v, u);
             y = v[0];
           }
-          static_cast<T*>(a.out)[n * a.ld_out + o0 + c] = from_float<T>(y);
+          static_cast<T*>(a.out)[n * a.ld_out + o0 + c] = from_float<T>(y);  // h as in the tiles: rounded here
         }
   }
 }
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(WARPS * 32) ffn_rows_kernel(const Few a) {
             }
             float y[1] = {v[i]};
             const float u[1] = {v[2 + i]};
-            activate<true>(a.act, y, u);
+            activate<true>(a.act, y, u);  // h is rounded, as in the tiles
             out[o + g] = __float2bfloat16_rn(y[0]);
           }
         } else {
