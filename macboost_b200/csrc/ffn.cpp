@@ -421,7 +421,7 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
     HeadReduce red[1]{};
     int reds = 0;
     c.target(l.job[0], in, pre, ld, kF32, p.part, red, &reds);
-    if (c.products(kHeadOut, l, in.tile_n, red, reds)) return -1;
+    if (c.products(kHeadBlock, l, in.tile_n, red, reds)) return -1;
     FFN_CUDA(launch_ffn_gate(a, pre, ld, s), "block launch");
   } else {
     gate(l.g, a);
@@ -442,7 +442,7 @@ int ffn_device(int device, const FfnArgs& a, cudaStream_t s, std::string& err) {
   int reds = 0;
   if (c.job(q.job[0], h, false, w_out, false, p.y)) return -1;
   c.target(q.job[0], p.y, a.y, a.ld_y, p.part, red, &reds);
-  if (c.products(kHeadOut, q, p.y.tile_n, red, reds)) return -1;
+  if (c.products(kHeadBlock, q, p.y.tile_n, red, reds)) return -1;
   g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
   return 0;
 }
@@ -536,7 +536,7 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     HeadReduce red[1]{};
     int reds = 0;
     c.target(q.job[0], dh, c.base() + p.dh_at, t.ld_dh, kF32, p.part, red, &reds);
-    if (c.products(kHeadOut, q, kHeadTileN, red, reds)) return -1;
+    if (c.products(kHeadBlock, q, kHeadTileN, red, reds)) return -1;
     FFN_CUDA(launch_ffn_split(t, s), "block split launch");
     ++c.launches;
   }
@@ -566,7 +566,7 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
       q.job[0].tiles_n = int(parts(p.dw_out.n, tile));
       q.job[0].divide();
     }
-    if (c.products(with ? kHeadGateGrad : kHeadOut, q, tile, red, reds)) return -1;
+    if (c.products(with ? kHeadGateGrad : kHeadBlock, q, tile, red, reds)) return -1;
   }
   if (inner) {
     HeadLaunch q{};
@@ -592,7 +592,7 @@ int ffn_grad_device(int device, const FfnArgs& a, cudaStream_t s, std::string& e
     q.jobs = a.dx && a.dw_in ? 2 : 1;
     q.job[0] = dw_first ? dw : dx;
     if (q.jobs == 2) q.job[1] = dw_first ? dx : dw;
-    if (c.products(kHeadOut, q, p.dx.tile_n, red, reds)) return -1;
+    if (c.products(kHeadBlock, q, p.dx.tile_n, red, reds)) return -1;
   }
   g_kernel_launches.fetch_add(c.launches, std::memory_order_relaxed);
   return 0;

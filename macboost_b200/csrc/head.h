@@ -175,7 +175,8 @@ struct HeadFew {
 };
 cudaError_t launch_head_few(const HeadArgs& h, bool grad, const HeadFew& f, cudaStream_t s);
 
-enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2, kHeadGate = 3, kHeadGateGrad = 4 };
+// kHeadOut: the head's sums written out; kHeadBlock: the gated block's.
+enum { kHeadLse = 0, kHeadG = 1, kHeadOut = 2, kHeadGate = 3, kHeadGateGrad = 4, kHeadBlock = 5 };
 cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStream_t s);
 // Source rows (float32 or bfloat16) to planes of bfloat16 (3 or 1), stride ldp; rows
 // whose label (unless null) is none of the classes become zeros.

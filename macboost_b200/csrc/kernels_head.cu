@@ -618,7 +618,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             }
             if (a.stall) continue;
             const int ka = q.a_k0 + kb * kHeadTileK;
-            const int kk = b_k0 + kb * kHeadTileK - (EPI == kHeadOut && kb >= gap ? skip : 0);
+            const int kk = b_k0 + kb * kHeadTileK - (EPI == kHeadBlock && kb >= gap ? skip : 0);
             for (int z = 0; z < kPlanes; ++z, sa += kBytesA, sb += kBytesB) {
               if (q.a_mn) {
 #pragma unroll
@@ -713,7 +713,11 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
     float sums[F32 ? TN / 2 : 1];
     // float32 sums go back to tensor memory, and from there the way of bfloat16's: an epilogue
     // unrolled over 128 registers runs at the speed of instruction fetches (25 us a tile)
-    constexpr bool kBack = F32 && (EPI == kHeadOut || EPI == kHeadGate);
+    constexpr bool kBack = F32 && (EPI == kHeadOut || EPI == kHeadBlock || EPI == kHeadGate);
+    // A gated block's products: rows that move up, and rows side by side whatever their alignment.  The head's
+    // are a form of their own without that: in one form with it they took 1.5 to 2 us longer a launch
+    // (2,048 x 512 x 1,000 dh and dw 15.6, in one form 18.0, now 16.2; 1,000 x 100 x 403 11.9, 13.4, 12.2).
+    constexpr bool kBlock = EPI != kHeadOut;
     while (walk.next(&t)) {
       const HeadJob& q = a.job[t.job];
       int k0, k1;
@@ -795,7 +799,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
             for (int i = 0; i < 32; ++i) v[i] = sums[c + i];
             f(c, v);
           }
-        } else if constexpr (EPI != kHeadLse && EPI != kHeadG) {
+        } else if constexpr (EPI != kHeadLse && EPI != kHeadG && EPI != kHeadOut) {
           // one copy of an epilogue that is long: its instructions come from far
           float v[32];
 #pragma unroll 1
@@ -831,7 +835,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
           return r < q.m_from ? r : r < q.m_to ? -1 : r - (q.m_to - q.m_from);
         };
         each_part([&](int c, float (&v)[32]) {
-          if (q.final && !q.acc_in && q.wide != 1) {
+          if (kBlock && q.final && !q.acc_in && q.wide != 1) {
             // rows that start on 16 bytes of bfloat16, or off four values
             if (q.wide) {
               turn_bf16(stage, v, lane, [&](int rr, int cc, uint4 x) {
@@ -867,7 +871,7 @@ __global__ void __cluster_dims__(kHeadPair, 1, 1) __launch_bounds__(kHeadThreads
                 if (n > 3) x.w += sum[3];
               }
             }
-            const int to = place(row0 + rr);
+            const int to = kBlock ? place(row0 + rr) : row0 + rr;
             if (q.final && to < 0) return;
             const long long at = (long long)to * q.ld_out + col0 + c + cc;
             if (!q.final)
@@ -1853,6 +1857,7 @@ cudaError_t launch_head(int epilogue, int tile_n, const HeadLaunch& a, cudaStrea
   if (epilogue == kHeadGate) return tile_n == 128 ? go<kHeadGate, 128>(a, s) : go<kHeadGate, 256>(a, s);
   if (epilogue == kHeadGateGrad)  // float32: a launch of its own (launch_ffn_split)
     return a.f32 ? cudaErrorInvalidValue : go_type<kHeadGateGrad, 256, false>(a, s);
+  if (epilogue == kHeadBlock) return tile_n == 128 ? go<kHeadBlock, 128>(a, s) : go<kHeadBlock, 256>(a, s);
   return tile_n == 128 ? go<kHeadOut, 128>(a, s) : go<kHeadOut, 256>(a, s);
 }
 
