@@ -116,3 +116,27 @@ def test_narrow_gradient_of_many_rows(gpu, torch):
     b.pre.fill_(0.25)
     b.grad()
     assert torch.equal(b.results()["dw_out"], first)
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+def test_long_rows_apart(gpu, torch, rows):
+    """Rows that start off 16 bytes, odd sizes, a width of more than one tile; a row that is not finite leaves
+    the others as they were."""
+    cols, width = 33_001, 301
+    b = _block(gpu, torch, rows, cols, width, 9, "bfloat16", "gelu_tanh", pad=3, seed=12)
+    _positive(torch, b.x, 13)
+    _positive(torch, b.w_in, 14)
+    b.w_in.mul_(1.0 / cols)
+    b.forward()
+    b.check()
+    b.intact()
+    pre = b.x[:, :cols].double() @ b.w_in[:, :cols].double().t()
+    got = {k: v.clone() for k, v in b.results().items()}
+    assert float((got["pre"].double() / pre - 1).abs().max()) <= 2.0 ** -12 + 2.0 ** -18
+    b.x[1, 5] = float("nan")
+    b.forward()
+    keep = [i for i in range(rows) if i != 1]
+    assert torch.equal(b.results()["y"][keep], got["y"][keep]) and torch.isnan(b.results()["y"][1]).all()
+    b.grad()
+    b.check()
+    b.intact()
